@@ -5,8 +5,9 @@
  * The drop-in boundary is one symbol, the backend's function table, which
  * the TurboEmbed core lists beside its other backends. Everything else here
  * is the host-side checking the core does before it calls a backend (so a
- * harness without the Rust core checks rows as the core does) and hooks for
- * tests and measurement, which the core never calls.
+ * harness without the Rust core checks rows as the core does), operators on
+ * device memory for programs that run layers of their own over a session's
+ * states, and hooks for tests and measurement, which the core never calls.
  */
 #ifndef TURBO_ROCM_H
 #define TURBO_ROCM_H
@@ -112,6 +113,169 @@ int32_t turbo_rocm_rerank_run(void *session, const int32_t *ids, const int32_t *
  * allocations the call made (none) in device_allocs. */
 int32_t turbo_rocm_buffer_quantize_static(void *buffer, uint32_t quantization, const float *int8_ranges, uint32_t rows,
                                           uint32_t dim, turbo_backend_run *run, turbo_error *err);
+
+/* ---- Operators on device memory (no counterpart in the reference) ----
+ *
+ * What a program needs to run layers of its own over a session's states
+ * (taps, hidden states, imported embeddings): an RMS norm with the residual's
+ * addition and int8 codes out, those codes of any rows, the int8 product on
+ * codes and scales, and the attention of its tokens to an encoder's states of
+ * another length. Like buffer_quantize
+ * they work on memory that the caller owns.
+ *
+ * Each takes a context and a call struct whose first field is struct_size
+ * (another size: TURBO_E_INVALID_STRUCT_SIZE). Every argument is checked on
+ * the host before any device work (those that a NULL context could serve
+ * first, then the context: TURBO_E_INVALID_HANDLE); a refused call has written
+ * nothing, and its error's field is the place, from 1, of the array it is
+ * about among the call's arrays, or 0. With
+ * TURBO_ROCM_ENQUEUE in flags the kernels are enqueued on `stream` (a
+ * hipStream_t of the context's device; NULL: that device's default stream)
+ * and the call returns: it allocates nothing, waits for nothing and may be
+ * captured into a graph. A stream of another device is refused. Without the
+ * flag `stream` must be NULL, and the call runs
+ * on the context's own stream and returns when its results are there. Calls
+ * keep no state of their own: any number may run at once, from any threads
+ * and on any streams, when none writes memory that another reads or writes.
+ * The calling thread's current device may be any; it is the caller's again
+ * afterwards. */
+#define TURBO_ROCM_ENQUEUE 1u
+
+/* An array in device-addressable memory: `data` is the address of its first
+ * element on the context's device (a buffer's exported
+ * TURBO_HANDLE_CUDA_PTR, or any memory of that device), and `bytes` what lies
+ * behind it there. ndim 1 to 3; the last axis is contiguous, stride[i] is the
+ * elements from one step of axis i to the next (for i < ndim - 1; the other
+ * strides are ignored). Strides need not keep an order and 0 repeats an input;
+ * an output's elements must not overlap. Every element is checked to lie
+ * within `bytes`; data must be aligned to one element. An absent optional
+ * array is all zeros (ndim 0). An array with an empty axis is never read, and
+ * its data may be NULL. */
+typedef struct turbo_rocm_tensor {
+    void    *data;
+    uint64_t bytes;
+    uint64_t shape[3];
+    uint64_t stride[2];
+    uint32_t ndim;
+    uint32_t dtype;   /* TURBO_DTYPE_* */
+} turbo_rocm_tensor;
+
+/* turbo_rocm_rms_norm: rows of `cols` values, at most 65536. For each row
+ *
+ *   v = x, or x + residual in F32 rounded once to the residual's type
+ *   y = v * weight / sqrt(mean(v^2) + eps)      (64-bit sums and products)
+ *
+ * x [rows, cols] F32, F16 or BF16; residual [rows, cols] (optional) of x's
+ * type or F32; weight [cols], F32 or x's type; eps positive and finite.
+ * Outputs, any of:
+ *   sum [rows, cols], the residual's type: v (only with a residual). It may
+ *     be the residual itself, or x where the types are equal: same address
+ *     and strides.
+ *   out [rows, cols], F32, F16 or BF16: y, rounded once. It may be x, in the
+ *     same way.
+ *   codes [rows, cols] I8 with scales [rows] F32: symmetric int8 codes of y's
+ *     row before any rounding: scale = max|y| / 127 rounded to F32, code =
+ *     the whole number nearest to 127 y / max|y|, ties to even, exactly. A row
+ *     of zeros has scale 0 and codes 0. A row with an infinity or NaN among
+ *     its v * weight has scale NaN and codes 0, so whatever reads the codes
+ *     sees it.
+ * One of out and codes at least; sum, out and codes may not overlap each
+ * other, nor an input except as said. */
+typedef struct turbo_rocm_rms_norm_call {
+    uint32_t struct_size;
+    uint32_t flags;
+    void    *stream;
+    double   eps;
+    turbo_rocm_tensor x, residual, weight, sum, out, codes, scales;
+} turbo_rocm_rms_norm_call;
+int32_t turbo_rocm_rms_norm(void *ctx, const turbo_rocm_rms_norm_call *call, turbo_error *err);
+
+/* turbo_rocm_quantize_tokens: the codes and scales above of the rows of x
+ * [rows, cols] (F32, F16 or BF16; at most 65536 columns) themselves, as an
+ * int8 product takes them. */
+typedef struct turbo_rocm_quantize_tokens_call {
+    uint32_t struct_size;
+    uint32_t flags;
+    void    *stream;
+    turbo_rocm_tensor x, codes, scales;
+} turbo_rocm_quantize_tokens_call;
+int32_t turbo_rocm_quantize_tokens(void *ctx, const turbo_rocm_quantize_tokens_call *call, turbo_error *err);
+
+/* turbo_rocm_linear_i8: out[m, n] = (sum_k codes[m, k] weight[n, k]) *
+ * scales[m] * weight_scales[n] + bias[n], the sum exact in 32-bit integers
+ * (inner width at most 131071, where the largest sum still fits), the rest in
+ * F32, rounded once to out's type. codes [M, K] and weight [N, K] I8, scales
+ * [M], weight_scales [N] and bias [N] (optional) F32, out [M, N] F32, F16 or
+ * BF16. K 0 gives the bias (or zeros, as an empty sum times the scales). out
+ * may not overlap an input. */
+typedef struct turbo_rocm_linear_i8_call {
+    uint32_t struct_size;
+    uint32_t flags;
+    void    *stream;
+    turbo_rocm_tensor codes, scales, weight, weight_scales, bias, out;
+} turbo_rocm_linear_i8_call;
+int32_t turbo_rocm_linear_i8(void *ctx, const turbo_rocm_linear_i8_call *call, turbo_error *err);
+
+/* Cross attention: the queries of each sequence attend to the encoder states
+ * of that sequence, whose number is another. Sequences are packed one after
+ * another: sequence s has q_lens[s] query tokens behind those of the
+ * sequences before it, and k_lens[s] states likewise (both host arrays of
+ * `batch`; 0 is allowed). Query head h reads key and value head h / (heads /
+ * kv_heads); heads must be a multiple of kv_heads. width is the head width, 1
+ * to 128. dtype F32, F16 or BF16.
+ *
+ * turbo_rocm_cross_plan_create works out, for these lengths on the context's
+ * device, which workgroup takes which tokens and keys, and keeps that on the
+ * device. A plan is never written after that: one serves any number of calls
+ * (a decoder's layers and steps) on any streams, at once. It must outlive the
+ * calls and graphs that use it, and its context must outlive it.
+ * *workspace_bytes (may be NULL) is what each call needs beside its operands. */
+typedef struct turbo_rocm_cross_desc {
+    uint32_t struct_size;
+    uint32_t dtype;
+    uint32_t batch;
+    uint32_t heads;
+    uint32_t kv_heads;
+    uint32_t width;
+    const uint32_t *q_lens;
+    const uint32_t *k_lens;
+} turbo_rocm_cross_desc;
+int32_t turbo_rocm_cross_plan_create(void *ctx, const turbo_rocm_cross_desc *desc, uint64_t *workspace_bytes,
+                                     void **out, turbo_error *err);
+void turbo_rocm_cross_plan_release(void *plan);
+
+/* turbo_rocm_cross_attention: for each query token i and head h of a sequence
+ *
+ *   out[i, h] = sum_j p_j v[j, h'],  p = softmax over j of scale * q[i, h] . k[j, h']
+ *
+ * over the sequence's live states j; h' is the head that h reads. q and out
+ * [tokens, heads, width], k and v [states, kv_heads, width], in the plan's
+ * type, with at least the plan's tokens and states (out's rows past the last
+ * sequence are left as they were). mask [states] I32 (optional): a state whose
+ * entry is 0 is not live, and nothing of its key and value is used, whatever
+ * they hold. A query with no live state has a zero output. scale finite.
+ * Scores, probabilities and sums are F32; 16-bit operands round a probability
+ * once, to their type, for the product with V, and the output once. An
+ * infinite or undefined score gives what the formula gives: a NaN. workspace:
+ * `workspace_bytes` of the context's device, 16-byte aligned, at least the
+ * plan's, for this call alone until it has finished (two graphs that may run
+ * at once need one each). It holds nothing between calls. out may not overlap an input
+ * or the workspace. */
+typedef struct turbo_rocm_cross_attention_call {
+    uint32_t struct_size;
+    uint32_t flags;
+    void    *stream;
+    void    *workspace;
+    uint64_t workspace_bytes;
+    double   scale;
+    turbo_rocm_tensor q, k, v, mask, out;
+} turbo_rocm_cross_attention_call;
+int32_t turbo_rocm_cross_attention(void *plan, const turbo_rocm_cross_attention_call *call, turbo_error *err);
+
+/* The checks of a plan's description and of a call with it, as the two
+ * functions above make them (but for the workspace, which the plan sizes), without a device; call may be NULL. */
+int32_t turbo_rocm_cross_check(const turbo_rocm_cross_desc *desc, const turbo_rocm_cross_attention_call *call,
+                               turbo_error *err);
 
 /* ---- Test and measurement hooks (no counterpart in the reference's seam; the
  * reference's CUDA backend keeps similar ones, core/src/cuda.rs:177-499) ---- */

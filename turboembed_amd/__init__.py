@@ -17,8 +17,10 @@ import os
 
 import numpy as np
 
+from . import operators
 from . import seam as S
 from .model import ModelDesc  # noqa: F401  (re-exported)
+from .operators import DeviceArray  # noqa: F401  (re-exported)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libturbo_rocm.so")
@@ -69,11 +71,20 @@ def library():
         "turbo_rocm_fail_variant": [C.c_char_p, E],
         "turbo_rocm_buffer_quantize_static": [P, u32, C.POINTER(C.c_float), u32, u32, C.POINTER(S.turbo_backend_run),
                                               E],
+        # (The operators' call structs come packed as bytes: operators.py.)
+        "turbo_rocm_rms_norm": [P, C.c_char_p, E],
+        "turbo_rocm_quantize_tokens": [P, C.c_char_p, E],
+        "turbo_rocm_linear_i8": [P, C.c_char_p, E],
+        "turbo_rocm_cross_plan_create": [P, C.POINTER(S.turbo_rocm_cross_desc), C.POINTER(C.c_uint64), C.POINTER(P), E],
+        "turbo_rocm_cross_attention": [P, C.c_char_p, E],
+        "turbo_rocm_cross_check": [C.POINTER(S.turbo_rocm_cross_desc), C.c_char_p, E],
     }
     for name, args in protos.items():
         f = getattr(lib, name)
         f.argtypes = args
         f.restype = C.c_int32
+    lib.turbo_rocm_cross_plan_release.argtypes = [P]
+    lib.turbo_rocm_cross_plan_release.restype = None
     _lib = lib
     return lib
 
@@ -149,6 +160,20 @@ class Context:
         """A buffer of the context's device (buffer_alloc): DEVICE, PINNED,
         SHARED or HOST; the last three have a host pointer."""
         return Buffer(self, nbytes, placement)
+
+    # -- operators on device memory (operators.py) ---------------------------------
+    def rms_norm(self, x, weight, eps, residual=None, sum=None, out=None, codes=None, scales=None, stream=None):
+        operators.rms_norm(self, x, weight, eps, residual, sum, out, codes, scales, stream)
+
+    def quantize_tokens(self, x, codes, scales, stream=None):
+        operators.quantize_tokens(self, x, codes, scales, stream)
+
+    def linear_i8(self, codes, scales, weight, weight_scales, out, bias=None, stream=None):
+        operators.linear_i8(self, codes, scales, weight, weight_scales, out, bias, stream)
+
+    def cross_plan(self, q_lens, k_lens, heads, kv_heads, width, dtype):
+        """A CrossPlan: attention of sequences of q_lens tokens to k_lens states."""
+        return operators.CrossPlan(self, q_lens, k_lens, heads, kv_heads, width, dtype)
 
     def close(self):
         if self.h:

@@ -1,0 +1,81 @@
+// Launchers of the operators on device memory (operators.cpp checks their
+// arguments). As the launchers of kernels.h: each enqueues on the given
+// stream and returns the launch's error; none allocates, waits or copies.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kernels.h"
+
+namespace rocm {
+
+// Rows at most this wide are held in one workgroup's registers (row_codes.hip).
+constexpr uint64_t ROW_COLS_MAX = 65536;
+
+// Row strides are in elements. Absent arrays are NULL (codes are wanted where
+// scales is given: rows of no columns have scales alone).
+struct RowArgs {
+    const void *x, *res, *w;
+    void *sum, *out;
+    int8_t *codes;
+    float *scales;
+    uint64_t ldx, ldr, lds, ldo, ldc;
+    Dt xt, rt, wt, ot;   // rt: the residual's, and v's (xt without one)
+    int rows, cols;
+    double eps;
+};
+// rms_norm (with w), or quantize_tokens (w NULL: codes and scales alone).
+hipError_t row_codes(hipStream_t s, const RowArgs &a);
+
+// The widest inner width of an int8 product: 131071 * 128 * 128 < 2^31.
+constexpr uint64_t I8_INNER_MAX = 131071;
+
+struct LinearArgs {
+    const int8_t *a, *w;
+    const float *as, *ws, *bias;
+    void *out;
+    uint64_t lda, ldw, ldo;
+    Dt ot;
+    int m, n, k;
+};
+hipError_t linear_i8(hipStream_t s, const LinearArgs &a);
+
+// Cross attention's work, as a plan holds it on the device. The rows of a
+// (sequence, key head) are its query tokens' heads that read the key head:
+// row r is token r / share of the sequence's, head kv * share + r % share.
+// An item is up to CROSS_ROWS of them against keys k0 .. k0 + nk - 1; where a
+// row's keys are cut over several items, each leaves its part (`part`) in the
+// workspace and a join adds them up; part -1 writes the output itself.
+constexpr int CROSS_ROWS = 128;
+struct CrossItem {
+    int32_t q0;           // the sequence's first token
+    int32_t row0, rows;
+    int32_t k0, nk;
+    int32_t kv;
+    int32_t part;
+    int32_t pad;
+};
+// The rows whose keys were cut: parts part0 .. part0 + parts - 1.
+struct CrossJoin {
+    int32_t q0, row0, rows, kv, part0, parts, pad[2];
+};
+
+struct CrossArgs {
+    const void *q, *k, *v;
+    void *out;
+    const int32_t *mask;
+    float *ws;               // parts
+    const CrossItem *items;
+    const CrossJoin *joins;
+    uint64_t qs[2], ks[2], vs[2], os[2];   // strides of tokens and heads, elements
+    Dt dt;
+    int n_items, n_joins, share, width;
+    float scale;             // of a score, times log2(e)
+};
+hipError_t cross_attention(hipStream_t s, const CrossArgs &a);
+// A part: rows of `width` sums, then each row's maximum (base 2) and sum; a
+// row without a finite maximum leaves 1 for its sum if it had a live key.
+inline uint64_t cross_part_floats(int width) { return (uint64_t)CROSS_ROWS * (width + 2); }
+
+}  // namespace rocm

@@ -1,0 +1,225 @@
+// RMS norm with the residual's addition and int8 codes out, and the codes of
+// rows alone.
+//
+// A row is held in registers by one wave or one workgroup: x (and the
+// residual) are read once, everything else is made from the registers, and
+// the outputs are written once. The weight is read twice, from the caches.
+//
+// The codes are those of the definition, not of a rounded norm: code_i = the
+// whole number nearest to 127 y_i / max|y| = 127 c_i / max|c|, c = v w, as the
+// norm's factor is common to the row. c is exact in 64 bits (24 by 24 bits),
+// so a code can only go wrong next to the border of two codes, where the
+// quotient is decided again without rounding (nearest_code). 64-bit
+// arithmetic runs at the rate of 32-bit on gfx950's vector units, some 20
+// operations a value here, and the kernel waits for memory.
+#include <hip/hip_runtime.h>
+
+#include "devmath.h"
+#include "launch.h"
+#include "operators.h"
+
+namespace rocm {
+
+// Eight consecutive values at p, of which the first n exist (the rest read as
+// 0). Rows may start at any element, so the vectors are read at its alignment.
+template <typename H> __device__ __forceinline__ void read8(const H *p, int n, float (&v)[8]) {
+    typedef H loose8 __attribute__((ext_vector_type(8), aligned(sizeof(H))));
+    if (n >= 8) {
+        const loose8 q = *(const loose8 *)p;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = to_f32(q[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = k < n ? to_f32(p[k]) : 0.0f;
+    }
+}
+
+template <typename H> __device__ __forceinline__ void write8(H *p, int n, const float (&v)[8]) {
+    typedef H loose8 __attribute__((ext_vector_type(8), aligned(sizeof(H))));
+    if (n >= 8) {
+        loose8 q;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[k] = from_f32<H>(v[k]);
+        *(loose8 *)p = q;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < n) p[k] = from_f32<H>(v[k]);
+    }
+}
+
+__device__ __forceinline__ void write8(void *p, Dt t, uint64_t at, int n, const float (&v)[8]) {
+    if (t == Dt::F32) write8((float *)p + at, n, v);
+    else if (t == Dt::F16) write8((_Float16 *)p + at, n, v);
+    else write8((__bf16 *)p + at, n, v);
+}
+
+// The whole number nearest to 127 c / top (ties to even), |c| <= top, from t,
+// that quotient to some 2^-45. Where t is next to a border h + 1/2 the two
+// sides 127 c and (h + 1/2) top are compared as exact sums of two numbers each.
+__device__ __forceinline__ int nearest_code(double t, double c, double top) {
+#pragma clang fp contract(off)
+    double n = rint(t);
+    if (__builtin_expect(fabs(fabs(t - n) - 0.5) < 1e-9, 0)) {
+        const double low = floor(t), half = low + 0.5;
+        const double a = 127.0 * c, b = half * top;
+        const double d = (a - b) + (fma(127.0, c, -a) - fma(half, top, -b));
+        n = d > 0.0 ? low + 1.0 : d < 0.0 ? low : 2.0 * rint(0.5 * half);
+    }
+    return (int)n;
+}
+
+// The sum (or maximum) over the WAVES waves that share a row; red is their
+// LDS. Every lane of them calls it.
+template <int WAVES, bool MAX> __device__ __forceinline__ double row_reduce(double v, double *red) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const double u = __shfl_xor(v, o, 64);
+        v = MAX ? fmax(v, u) : v + u;
+    }
+    if constexpr (WAVES > 1) {
+        __syncthreads();   // the last use of red is over
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = red[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) v = MAX ? fmax(v, red[i]) : v + red[i];
+    }
+    return v;
+}
+
+// X: x's type; R: the residual's (and v's); NORM: rms_norm, else the codes of
+// x. WAVES waves hold a row, lane l of them columns 8 (l + 64 WAVES g) .. + 7
+// of each group g < G; a workgroup is at least four waves.
+template <typename X, typename R, bool NORM, int WAVES, int G>
+__global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel(RowArgs a) {
+    constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1, LANES = 64 * WAVES;
+    __shared__ double red[WAVES];
+    const int lane = threadIdx.x % LANES;
+    for (int row = blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += gridDim.x * ROWS) {
+        float v[G][8];
+        double ss = 0.0, top = 0.0, bad = 0.0;
+        // (A weight of either type, 1 without one.)
+        auto weight = [&](int c, int n, float(&w)[8]) {
+            if constexpr (NORM) {
+                if (a.wt == Dt::F32) read8((const float *)a.w + c, n, w);
+                else read8((const X *)a.w + c, n, w);
+            }
+        };
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int c = 8 * (lane + LANES * g), n = a.cols - c;
+            if (n > 0) {
+                read8((const X *)a.x + row * a.ldx + c, n, v[g]);
+                if (NORM && a.res) {
+                    float r[8];
+                    read8((const R *)a.res + row * a.ldr + c, n, r);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[g][k] = to_f32(from_f32<R>(v[g][k] + r[k]));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[g][k] = 0.0f;
+            }
+        }
+        if (NORM && a.sum)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int c = 8 * (lane + LANES * g), n = a.cols - c;
+                if (n > 0) write8((R *)a.sum + row * a.lds + c, n, v[g]);
+            }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int c = 8 * (lane + LANES * g), n = a.cols - c;
+            if (n <= 0) continue;
+            float w[8];
+            if (a.scales) weight(c, n, w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const double d = v[g][k];
+                if constexpr (NORM) ss = fma(d, d, ss);
+                if (a.scales) {
+                    const double e = NORM ? d * w[k] : d;
+                    top = fmax(top, fabs(e));
+                    bad = fma(e, 0.0, bad);   // not 0: an infinity or a NaN
+                }
+            }
+        }
+        double r = 1.0;
+        if constexpr (NORM) r = 1.0 / sqrt(row_reduce<WAVES, false>(ss, red) / a.cols + a.eps);
+        if (NORM && a.out)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int c = 8 * (lane + LANES * g), n = a.cols - c;
+                if (n <= 0) continue;
+                float w[8], y[8];
+                weight(c, n, w);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = (float)(v[g][k] * r * w[k]);
+                write8(a.out, a.ot, row * a.ldo + c, n, y);
+            }
+        if (!a.scales) continue;
+        top = row_reduce<WAVES, true>(top, red);
+        const bool fine = row_reduce<WAVES, false>(bad, red) == 0.0;
+        const double k127 = fine && top > 0.0 ? 127.0 / top : 0.0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int c = 8 * (lane + LANES * g), n = a.cols - c;
+            if (n <= 0) continue;
+            float w[8];
+            weight(c, n, w);
+            uint32_t q[2] = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const double e = NORM ? (double)v[g][k] * w[k] : (double)v[g][k];
+                const int code = fine ? nearest_code(e * k127, e, top) : 0;
+                q[k >> 2] |= (uint32_t)(uint8_t)(int8_t)code << (8 * (k & 3));
+            }
+            int8_t *p = a.codes + row * a.ldc + c;
+            if (n >= 8) {
+                typedef uint32_t loose2 __attribute__((ext_vector_type(2), aligned(1)));
+                *(loose2 *)p = loose2{q[0], q[1]};
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (k < n) p[k] = (int8_t)(q[k >> 2] >> (8 * (k & 3)));
+            }
+        }
+        if (lane == 0) a.scales[row] = !fine ? __builtin_nanf("") : top > 0.0 ? (float)(top * r / 127.0) : 0.0f;
+    }
+}
+
+template <typename X, typename R, bool NORM> static hipError_t launch_rows(hipStream_t s, const RowArgs &a) {
+    // Workgroups enough for every row, up to a bound past which they take
+    // several (a launch holds less than 2^32 threads).
+    auto go = [&](auto kernel, int waves) {
+        const int per = waves < 4 ? 4 / waves : 1, threads = waves < 4 ? 256 : 64 * waves;
+        const int blocks = (a.rows - 1) / per + 1;
+        enqueue(kernel, dim3(blocks < (1 << 20) ? blocks : 1 << 20), dim3(threads), 0, s, a);
+        return hipGetLastError();
+    };
+#define ROWS(W, G) return go(row_codes_kernel<X, R, NORM, W, G>, W)
+    if (a.cols <= 512) ROWS(1, 1);
+    if (a.cols <= 1024) ROWS(1, 2);
+    if (a.cols <= 2048) ROWS(1, 4);
+    if (a.cols <= 4096) ROWS(4, 2);
+    if (a.cols <= 8192) ROWS(4, 4);
+    if (a.cols <= 16384) ROWS(4, 8);
+    ROWS(16, 8);
+#undef ROWS
+}
+
+hipError_t row_codes(hipStream_t s, const RowArgs &a) {
+    if (a.rows <= 0) return hipSuccess;
+    if (!a.w) {
+        if (a.xt == Dt::F32) return launch_rows<float, float, false>(s, a);
+        if (a.xt == Dt::F16) return launch_rows<_Float16, _Float16, false>(s, a);
+        return launch_rows<__bf16, __bf16, false>(s, a);
+    }
+    if (a.xt == Dt::F32) return launch_rows<float, float, true>(s, a);
+    if (a.xt == Dt::F16)
+        return a.rt == Dt::F32 ? launch_rows<_Float16, float, true>(s, a) : launch_rows<_Float16, _Float16, true>(s, a);
+    return a.rt == Dt::F32 ? launch_rows<__bf16, float, true>(s, a) : launch_rows<__bf16, __bf16, true>(s, a);
+}
+
+}  // namespace rocm

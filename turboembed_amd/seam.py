@@ -10,6 +10,7 @@ import ctypes as C
 TURBO_OK = 0
 TURBO_E_INVALID_ARGUMENT = 256
 TURBO_E_INVALID_STRUCT_SIZE = 257
+TURBO_E_INVALID_HANDLE = 259
 TURBO_E_INVALID_SHAPE = 260
 TURBO_E_INVALID_STATE = 261
 TURBO_E_INVALID_ENUM = 262
@@ -127,6 +128,13 @@ class turbo_native_handle(C.Structure):
 class turbo_buffer_desc(C.Structure):
     _fields_ = [("struct_size", C.c_uint32), ("placement", C.c_uint32), ("dtype", C.c_uint32), ("ndim", C.c_uint32),
                 ("shape", C.c_uint64 * 2), ("bytes", C.c_uint64)]
+
+
+class turbo_rocm_cross_desc(C.Structure):
+    """include/turbo_rocm.h's (the reference has none)."""
+    _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("batch", C.c_uint32), ("heads", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("width", C.c_uint32), ("q_lens", C.POINTER(C.c_uint32)),
+                ("k_lens", C.POINTER(C.c_uint32))]
 
 
 class turbo_token_range(C.Structure):
