@@ -1,4 +1,15 @@
-// The int8 product on the caller's codes and scales.
+// The int8 product on the caller's codes and scales: out[m, n] =
+// (sum_k a[m, k] w[n, k]) as[m] ws[n] + bias[n].
+//
+// The sum is whole, so how it is cut over waves and steps changes nothing, and
+// an inner width that no vector divides costs no copy: the inner width is read
+// in 16-byte chunks, the last of them ending at the row's end and so
+// overlapping the one before; a's bytes that were already counted there are
+// taken as 0 (and all of them in chunks past the end), w's are left as they
+// are. Rows past M or N repeat the last.
+//
+// Every kernel multiplies w by a transposed, so that a lane holds four
+// consecutive columns of one output row.
 #include <hip/hip_runtime.h>
 
 #include "devmath.h"
@@ -6,6 +17,11 @@
 #include "operators.h"
 
 namespace rocm {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int loose4 __attribute__((ext_vector_type(4), aligned(1)));
 
 // An output from its exact sum: both scales, then the bias, each rounded.
 __device__ __forceinline__ float scaled(int sum, float as, float ws, float bias) {
@@ -19,8 +35,20 @@ __device__ __forceinline__ void put(void *out, Dt t, uint64_t at, float v) {
     else ((__bf16 *)out)[at] = (__bf16)v;
 }
 
-// An output a lane, its products one by one.
-__global__ void __launch_bounds__(256) linear_i8_plain(LinearArgs a) {
+// The bytes of a's 16-byte chunk c that count, of an inner width k >= 16.
+__device__ __forceinline__ i32x4 counted(i32x4 v, int c, int k) {
+    const int z = 16 * c - (k - 16);   // bytes from the front that do not
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int zi = z - 4 * i;
+        v[i] = zi <= 0 ? v[i] : zi >= 4 ? 0 : v[i] & (int)(0xffffffffu << (8 * zi));
+    }
+    return v;
+}
+
+// ---- Inner widths below 16: an output a lane, its products one by one ------------
+
+__global__ void __launch_bounds__(256) linear_i8_narrow(LinearArgs a) {
     for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)a.m * a.n; i += (uint64_t)gridDim.x * 256) {
         const uint64_t m = i / a.n, n = i % a.n;
         int sum = 0;
@@ -29,11 +57,252 @@ __global__ void __launch_bounds__(256) linear_i8_plain(LinearArgs a) {
     }
 }
 
+// ---- Few rows: 16 columns a workgroup, its waves cutting the inner width ---------
+//
+// Bound by w's bytes, each read once, straight into the matrix instruction's
+// registers: a lane 16 bytes of a column's row, four lanes 64 consecutive ones.
+// The waves' sums meet in LDS.
+template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linear_i8_rows(LinearArgs a, int tiles) {
+    __shared__ __attribute__((aligned(16))) i32x4 part[WAVES][MT][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, h = lane >> 4;
+    const int m0 = blockIdx.y * 16 * MT;
+    const int chunks = (a.k + 15) / 16, full = a.k / 16;
+    const int8_t *ap[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) ap[t] = a.a + (uint64_t)min(m0 + 16 * t + r, a.m - 1) * a.lda;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const int8_t *wp = a.w + (uint64_t)min(16 * tile + r, a.n - 1) * a.ldw;
+        i32x4 acc[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
+        // A step is 8 chunks of each row (128 bytes), two products.
+        for (int c0 = 8 * wave; c0 < chunks; c0 += 8 * WAVES) {
+            i32x4 w[2], x[2][MT];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int c = c0 + 4 * u + h, k = min(16 * c, a.k - 16);
+                w[u] = *(const loose4 *)(wp + k);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) x[u][t] = *(const loose4 *)(ap[t] + k);
+            }
+            if (c0 + 8 > full)   // uniform
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) x[u][t] = counted(x[u][t], c0 + 4 * u + h, a.k);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x[u][t], acc[t], 0, 0, 0);
+        }
+        if (tile != (int)blockIdx.x) __syncthreads();   // the last tile's sums are read
+#pragma unroll
+        for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+        __syncthreads();
+        for (int i = tid; i < 64 * MT; i += 64 * WAVES) {
+            const int t = i >> 6, l = i & 63;
+            i32x4 s = part[0][t][l];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) s += part[w][t][l];
+            // Columns 4 (l / 16) .. + 3 of row l % 16.
+            const int m = m0 + 16 * t + (l & 15), n = 16 * tile + 4 * (l >> 4);
+            if (m >= a.m) continue;
+            const float as = a.as[m];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < a.n)
+                    put(a.out, a.ot, (uint64_t)m * a.ldo + n + j,
+                        scaled(s[j], as, a.ws[n + j], a.bias ? a.bias[n + j] : 0.0f));
+        }
+    }
+}
+
+// ---- Tiles: both operands through LDS ----------------------------------------------
+//
+// BM rows of a by BN of w a workgroup, WM x WN waves, 128 bytes of the inner
+// width a stage, two stages: the next one's loads run while one is computed.
+// LDS rows are 128 bytes, chunk c of row r at place c ^ (r % 8), so that the 8
+// rows of a read's pass lie in different banks. DIRECT (16-byte aligned
+// operands and strides, K a multiple of 16): memory to LDS without registers.
+template <int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, int grid_n) {
+    constexpr int WAVES = WM * WN, ROWS = BM + BN, STAGE = ROWS * 128;
+    constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    constexpr int LOADS = ROWS / 8 / WAVES;   // a wave's, 8 rows each
+    static_assert(LOADS * 8 * WAVES == ROWS, "whole loads a wave");
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    // XCD-aware numbering: workgroups go to the 8 XCDs in turn, and each XCD
+    // takes tiles that follow one another.
+    const int per = gridDim.x / 8;
+    int b = blockIdx.x;
+    if (b < per * 8) b = (b % 8) * per + b / 8;
+    const int m0 = b / grid_n * BM, n0 = b % grid_n * BN;
+
+    // This lane's place in each load: row (of a, then of w) and chunk.
+    const int8_t *src[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+        const int row = (wave * LOADS + j) * 8 + (lane >> 3);
+        src[j] = row < BM ? a.a + (uint64_t)min(m0 + row, a.m - 1) * a.lda
+                          : a.w + (uint64_t)min(n0 + row - BM, a.n - 1) * a.ldw;
+    }
+    const int my_chunk = (lane & 7) ^ (lane >> 3);   // (the row's number modulo 8 is lane / 8)
+    i32x4 held[DIRECT ? 1 : LOADS];
+    auto load = [&](int stage, int buf) {
+        const int k = min(128 * stage + 16 * my_chunk, a.k - 16);
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            if constexpr (DIRECT) {
+                char *dst = smem + buf * STAGE + (wave * LOADS + j) * 1024;
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[j] + k),
+                                                 (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+            } else {
+                held[j] = *(const loose4 *)(src[j] + k);
+            }
+        }
+    };
+    auto place = [&](int buf) {
+        if constexpr (!DIRECT)
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j)
+                *(i32x4 *)(smem + buf * STAGE + (wave * LOADS + j) * 1024 + lane * 16) = held[j];
+    };
+
+    i32x16 acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = i32x16{};
+    const int r = lane & 31, h = lane >> 5;
+    const int stages = (a.k + 127) / 128;
+    load(0, 0);
+    place(0);
+    for (int s = 0; s < stages; ++s) {
+        const int buf = s & 1;
+        if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this stage is in LDS
+        __syncthreads();
+        if (s + 1 < stages) load(s + 1, buf ^ 1);
+        const char *A = smem + buf * STAGE + wm * (BM / WM) * 128, *W = smem + buf * STAGE + (BM + wn * (BN / WN)) * 128;
+        const bool tail = 128 * (s + 1) > a.k;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const int c = 2 * ks + h, at = r * 128 + ((c ^ (r & 7)) * 16);
+            i32x4 x[TM], w[TN];
+#pragma unroll
+            for (int j = 0; j < TM; ++j) x[j] = *(const i32x4 *)(A + j * 4096 + at);
+#pragma unroll
+            for (int i = 0; i < TN; ++i) w[i] = *(const i32x4 *)(W + i * 4096 + at);
+            if (tail)
+#pragma unroll
+                for (int j = 0; j < TM; ++j) x[j] = counted(x[j], 8 * s + c, a.k);
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[i], x[j], acc[i][j], 0, 0, 0);
+        }
+        place(buf ^ 1);   // (the last stage's held rows go where nobody reads)
+    }
+
+    // Epilogue: a lane's row is m = lane % 32, its columns 8 g + 4 h .. + 3 of
+    // each tile. Staged through LDS 32 rows at a time in the output's type, so
+    // that a store writes a row's columns one after another.
+    __syncthreads();
+    constexpr int COLS = BN / WN, PITCH = COLS * 4 + 16;   // bytes of a staged row, F32's
+    static_assert(WAVES * 32 * PITCH <= 2 * STAGE, "staging fits the stages");
+    char *mine = smem + wave * 32 * PITCH;
+    const int nw = n0 + wn * COLS, mw = m0 + wm * (BM / WM);
+    const bool f32 = a.ot == Dt::F32;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+        const int mb = mw + 32 * j;
+        const float as = a.as[min(mb + r, a.m - 1)];
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int cl = 32 * i + 8 * g + 4 * h;
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int n = min(nw + cl + e, a.n - 1);
+                    y[e] = scaled(acc[i][j][4 * g + e], as, a.ws[n], a.bias ? a.bias[n] : 0.0f);
+                }
+                char *p = mine + r * PITCH + cl * (f32 ? 4 : 2);
+                if (f32) {
+                    *(f32x4 *)p = f32x4{y[0], y[1], y[2], y[3]};
+                } else if (a.ot == Dt::F16) {
+                    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+                    *(h4 *)p = h4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+                } else {
+                    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+                    *(b4 *)p = b4{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]};
+                }
+            }
+        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the wave's rows are in LDS
+        __builtin_amdgcn_wave_barrier();
+        const int size = f32 ? 4 : 2, lanes = COLS * size / 16;   // lanes a row
+        for (int q = lane; q < 32 * lanes; q += 64) {
+            const int row = q / lanes, byte = q % lanes * 16, m = mb + row, n = nw + byte / size;
+            if (m >= a.m || n >= a.n) continue;
+            const i32x4 v = *(const i32x4 *)(mine + row * PITCH + byte);
+            char *o = (char *)a.out + ((uint64_t)m * a.ldo + n) * size;
+            const int left = (a.n - n) * size;
+            if (left >= 16) {
+                *(loose4 *)o = v;
+            } else if (f32) {
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (4 * e < left) ((int *)o)[e] = v[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 7; ++e)
+                    if (2 * e < left) ((short *)o)[e] = (short)(v[e >> 1] >> (16 * (e & 1)));
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);   // read before the next rows overwrite them
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int BM, int BN, int WM, int WN> static hipError_t launch_tiles(hipStream_t s, const LinearArgs &a, bool direct) {
+    const int gn = (a.n - 1) / BN + 1, gm = (a.m - 1) / BM + 1;
+    const dim3 grid((uint32_t)gn * gm), block(64 * WM * WN);
+    constexpr int lds = 2 * (BM + BN) * 128;
+    if (direct) enqueue(linear_i8_tiles<BM, BN, WM, WN, true>, grid, block, lds, s, a, gn);
+    else enqueue(linear_i8_tiles<BM, BN, WM, WN, false>, grid, block, lds, s, a, gn);
+    return hipGetLastError();
+}
+
+template <int MT> static hipError_t launch_rows(hipStream_t s, const LinearArgs &a) {
+    const int tiles = (a.n - 1) / 16 + 1;
+    const dim3 grid(tiles < (1 << 16) ? tiles : 1 << 16, (a.m - 1) / (16 * MT) + 1);
+    enqueue(linear_i8_rows<16, MT>, grid, dim3(1024), 0, s, a, tiles);
+    return hipGetLastError();
+}
+
 hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
     if (a.m <= 0 || a.n <= 0) return hipSuccess;
-    const uint64_t blocks = ((uint64_t)a.m * a.n + 255) / 256;
-    enqueue(linear_i8_plain, dim3((uint32_t)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, s, a);
-    return hipGetLastError();
+    if (a.k < 16) {
+        const uint64_t blocks = ((uint64_t)a.m * a.n + 255) / 256;
+        enqueue(linear_i8_narrow, dim3((uint32_t)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, s, a);
+        return hipGetLastError();
+    }
+    if (a.m <= 64) return a.m <= 16 ? launch_rows<1>(s, a) : a.m <= 32 ? launch_rows<2>(s, a) : launch_rows<4>(s, a);
+    const auto whole = [](const void *p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) | ld) % 16 == 0; };
+    const bool direct = whole(a.a, a.lda) && whole(a.w, a.ldw) && a.k % 16 == 0;
+    // The tile by its rounds over the compute units, at the relative times of
+    // one tile of each.
+    const auto rounds = [&](int bm, int bn) {
+        const uint64_t t = (uint64_t)((a.m - 1) / bm + 1) * ((a.n - 1) / bn + 1);
+        return (double)((t + 255) / 256);
+    };
+    const double wide = 4.3 * rounds(256, 256), mid = 2.1 * rounds(128, 128), small = rounds(64, 64);
+    if (small < mid && small < wide) return launch_tiles<64, 64, 2, 2>(s, a, direct);
+    if (mid < wide) return launch_tiles<128, 128, 2, 2>(s, a, direct);
+    return launch_tiles<256, 256, 2, 4>(s, a, direct);
 }
 
 }  // namespace rocm
