@@ -253,7 +253,7 @@ void turbo_rocm_cross_plan_release(void *plan);
  * type, with at least the plan's tokens and states (out's rows past the last
  * sequence are left as they were). mask [states] I32 (optional): a state whose
  * entry is 0 is not live, and nothing of its key and value is used, whatever
- * they hold. A query with no live state has a zero output. scale finite.
+ * they hold. A query with no live state has a zero output. scale finite in F32.
  * Scores, probabilities and sums are F32; 16-bit operands round a probability
  * once, to their type, for the product with V, and the output once. An
  * infinite or undefined score gives what the formula gives: a NaN. workspace:

@@ -248,6 +248,25 @@ def test_nothing_to_do(context):
     plan.close()
 
 
+def test_a_workspace_too_small_is_refused(context):
+    plan = context.cross_plan((1,), (20000,), 2, 2, 64, torch.float16)
+    assert plan.workspace_bytes > 0     # one token against many states: its keys are cut
+    q, k, v = _operands(0, 1, 20000, 2, 2, 64, "f16")
+    out = torch.empty_like(q)
+    ws = torch.empty(plan.workspace_bytes + 16, dtype=torch.uint8, device="cuda")
+    for bad in (None, ws[:plan.workspace_bytes - 1]):
+        with pytest.raises(T.TurboError) as e:
+            plan.run(q, k, v, out, workspace=bad, stream=_stream())
+        assert e.value.code == S.TURBO_E_CAPACITY
+    for bad in (ws[1:], k.view(torch.uint8).flatten()[:plan.workspace_bytes + 16]):
+        with pytest.raises(T.TurboError) as e:
+            plan.run(q, k, v, out, workspace=bad, stream=_stream())
+        assert e.value.code == S.TURBO_E_INVALID_ARGUMENT
+    plan.run(q, k, v, out, workspace=ws)          # the context's own stream, waited for
+    _check(out, q, k, v, (1,), (20000,))
+    plan.close()
+
+
 @pytest.mark.parametrize("q_lens, k_lens", [((1, 1), (900, 20000)), ((40, 9), (300, 5000)), ((300,), (1000,))])
 def test_captured_and_replayed_beside_another(context, q_lens, k_lens):
     t, heads, kv, d = "bf16", 4, 2, 64

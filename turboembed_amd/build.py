@@ -31,6 +31,8 @@ WRAPPED = ["malloc", "calloc", "realloc", "aligned_alloc", "posix_memalign", "_Z
 # accumulation registers; and no NaN operands (its inputs are finite), so a
 # max of scores is one v_max3_f32 without a quieting v_max_f32 per score.
 EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"] for f in ("attention.hip", "attention_f32p.hip")}
+# (Cross attention's inputs may be anything: the first of the two alone.)
+EXTRA["cross_attention.hip"] = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 
 FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",

@@ -3,11 +3,13 @@
 // cross_attention.hip.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <memory>
 #include <mutex>
 #include <string>
+#include <vector>
 
 #include "turbo_rocm.h"
 #include "operators.h"
@@ -282,7 +284,8 @@ struct CrossPlan {
     Context *ctx = nullptr;
     uint32_t dtype = 0, heads = 0, kv = 0, width = 0;
     uint64_t tokens = 0, states = 0, workspace = 0;
-    int items = 0, joins = 0;
+    int items = 0, joins = 0, part_rows = 0;
+    uint64_t parts = 0;
     DevPtr work;   // the items, then the joins
 };
 
@@ -309,12 +312,15 @@ Totals check_desc(const turbo_rocm_cross_desc *d) {
     return t;
 }
 
+// A score's factor in base 2, as the kernels take it.
+float base2(double scale) { return (float)(scale * 1.4426950408889634); }
+
 void check_cross(const turbo_rocm_cross_attention_call *call, uint32_t dtype, uint32_t heads, uint32_t kv,
                  uint32_t width, const Totals &n) {
     check_call(call);
     const Arg q{&call->q, "q", 1}, k{&call->k, "k", 2}, v{&call->v, "v", 3}, mask{&call->mask, "mask", 4},
         out{&call->out, "out", 5};
-    if (!std::isfinite(call->scale)) refuse(0, "scale must be finite");
+    if (!std::isfinite(base2(call->scale))) refuse(0, "scale must be finite, in F32");
     for (const Arg &a : {q, k, v, out}) {
         check_array(a, 3, bit(dtype), false);
         const bool states = a.field == 2 || a.field == 3;
@@ -330,6 +336,80 @@ void check_cross(const turbo_rocm_cross_attention_call *call, uint32_t dtype, ui
     for (const Arg &a : {q, k, v, mask}) check_clear(out, a);
 }
 
+// The items of a plan, in the order of their workgroups, and the joins.
+//
+// Rows 32 at a time where no sequence has more for a key head, 128 otherwise.
+// Keys are cut where the rows alone would leave compute units idle: into runs
+// of at most `slice` keys, so that about `wanted` workgroups have equal work,
+// but no shorter than a run that outweighs its part's way through memory.
+void lay_out(const turbo_rocm_cross_desc &d, std::vector<CrossItem> &items, std::vector<CrossJoin> &joins,
+             int &part_rows, uint64_t &parts) {
+    const uint64_t share = d.heads / d.kv_heads;
+    uint64_t most = 0;
+    for (uint32_t s = 0; s < d.batch; ++s) most = std::max(most, d.q_lens[s] * share);
+    part_rows = most <= 32 ? 32 : 128;
+    const uint64_t wanted = part_rows == 32 ? 2048 : 512, shortest = part_rows == 32 ? 256 : 512;
+    uint64_t work = 0;   // keys, over all items
+    for (uint32_t s = 0; s < d.batch; ++s)
+        work += (d.q_lens[s] * share + part_rows - 1) / part_rows * d.kv_heads * d.k_lens[s];
+    const uint64_t slice = (std::max(shortest, (work + wanted - 1) / wanted) + 63) / 64 * 64;
+
+    // The row blocks of a (sequence, key head) read the same keys: they go to
+    // one XCD (workgroups go to the 8 in turn), the XCD with the least work so
+    // far, the longest first.
+    struct Group {
+        uint32_t seq, kv;
+        uint64_t q0, k0, work;
+    };
+    std::vector<Group> groups;
+    uint64_t q0 = 0, k0 = 0;
+    for (uint32_t s = 0; s < d.batch; ++s) {
+        const uint64_t rows = d.q_lens[s] * share;
+        for (uint32_t h = 0; h < d.kv_heads && rows; ++h)
+            groups.push_back({s, h, q0, k0, (rows + part_rows - 1) / part_rows * (d.k_lens[s] + 64ull)});
+        q0 += d.q_lens[s], k0 += d.k_lens[s];
+    }
+    std::stable_sort(groups.begin(), groups.end(), [](const Group &a, const Group &b) { return a.work > b.work; });
+    constexpr int XCDS = 8;
+    std::vector<CrossItem> lists[XCDS];
+    uint64_t load[XCDS] = {};
+    parts = 0;
+    for (const Group &g : groups) {
+        const int x = (int)(std::min_element(load, load + XCDS) - load);
+        load[x] += g.work;
+        const uint64_t rows = d.q_lens[g.seq] * share, nk = d.k_lens[g.seq];
+        const uint64_t cuts = std::max<uint64_t>(1, (nk + slice - 1) / slice);
+        // Equal runs, whole 64s but for the last.
+        const uint64_t run = (nk + cuts * 64 - 1) / (cuts * 64) * 64;
+        for (uint64_t r = 0; r < rows; r += part_rows) {
+            CrossItem it{};
+            it.q0 = (int32_t)g.q0, it.kv = (int32_t)g.kv;
+            it.row0 = (int32_t)r, it.rows = (int32_t)std::min<uint64_t>(part_rows, rows - r);
+            const uint64_t pieces = run ? (nk + run - 1) / run : 1;
+            if (pieces > 1)
+                joins.push_back({it.q0, it.row0, it.rows, it.kv, (int32_t)parts, (int32_t)pieces, {0, 0}});
+            for (uint64_t i = 0; i < pieces; ++i) {
+                it.k0 = (int32_t)(g.k0 + i * run);
+                it.nk = (int32_t)std::min(run, nk - i * run);
+                it.part = pieces > 1 ? (int32_t)parts++ : -1;
+                lists[x].push_back(it);
+            }
+        }
+    }
+    size_t total = 0, taken[XCDS] = {};
+    for (const auto &l : lists) total += l.size();
+    // (A launch holds less than 2^32 threads.)
+    if (total > (1u << 23)) fail(TURBO_E_CAPACITY, "rocm: a plan of " + std::to_string(total) + " workgroups");
+    items.reserve(total);
+    for (int x = 0; items.size() < total; x = (x + 1) % XCDS) {
+        int from = x;
+        if (taken[x] == lists[x].size())   // a list at its end: from the one with the most left
+            for (int y = 0; y < XCDS; ++y)
+                if (lists[y].size() - taken[y] > lists[from].size() - taken[from]) from = y;
+        items.push_back(lists[from][taken[from]++]);
+    }
+}
+
 CrossPlan *cross_plan_create(Context *c, const turbo_rocm_cross_desc *d) {
     const Totals t = check_desc(d);
     if (!c) fail(TURBO_E_INVALID_HANDLE, "rocm: no context");
@@ -339,16 +419,8 @@ CrossPlan *cross_plan_create(Context *c, const turbo_rocm_cross_desc *d) {
     p->tokens = t.tokens, p->states = t.states;
     std::vector<CrossItem> items;
     std::vector<CrossJoin> joins;
-    const uint32_t share = d->heads / d->kv_heads;
-    uint64_t q0 = 0, k0 = 0;
-    for (uint32_t s = 0; s < d->batch; ++s) {
-        const uint64_t rows = (uint64_t)d->q_lens[s] * share;
-        for (uint32_t h = 0; h < d->kv_heads; ++h)
-            for (uint64_t r = 0; r < rows; r += CROSS_ROWS)
-                items.push_back({(int32_t)q0, (int32_t)r, (int32_t)std::min<uint64_t>(CROSS_ROWS, rows - r), (int32_t)k0,
-                                 (int32_t)d->k_lens[s], (int32_t)h, -1, 0});
-        q0 += d->q_lens[s], k0 += d->k_lens[s];
-    }
+    lay_out(*d, items, joins, p->part_rows, p->parts);
+    p->workspace = p->parts * cross_part_floats(p->part_rows, (int)d->width) * 4;
     p->items = (int)items.size(), p->joins = (int)joins.size();
     const size_t ib = items.size() * sizeof(CrossItem), jb = joins.size() * sizeof(CrossJoin);
     if (ib + jb) {
@@ -392,8 +464,11 @@ void cross_run(CrossPlan *p, const turbo_rocm_cross_attention_call *call) {
         a.qs[i] = call->q.stride[i], a.ks[i] = call->k.stride[i], a.vs[i] = call->v.stride[i],
         a.os[i] = call->out.stride[i];
     a.dt = dt_of(p->dtype);
-    a.n_items = p->items, a.n_joins = p->joins, a.share = (int)(p->heads / p->kv), a.width = (int)p->width;
-    a.scale = (float)(call->scale * 1.4426950408889634);
+    a.n_items = p->items, a.n_joins = p->joins, a.part_rows = p->part_rows;
+    a.share = (int)(p->heads / p->kv), a.width = (int)p->width;
+    a.scale = base2(call->scale);
+    a.turn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f;
+    a.scale = a.scale == 0 ? 1.0f : std::fabs(a.scale);
     run_call(p->ctx, call, "cross_attention", [&](hipStream_t s) { return cross_attention(s, a); });
 }
 

@@ -44,10 +44,10 @@ hipError_t linear_i8(hipStream_t s, const LinearArgs &a);
 // Cross attention's work, as a plan holds it on the device. The rows of a
 // (sequence, key head) are its query tokens' heads that read the key head:
 // row r is token r / share of the sequence's, head kv * share + r % share.
-// An item is up to CROSS_ROWS of them against keys k0 .. k0 + nk - 1; where a
-// row's keys are cut over several items, each leaves its part (`part`) in the
-// workspace and a join adds them up; part -1 writes the output itself.
-constexpr int CROSS_ROWS = 128;
+// An item is up to part_rows of them (32, a wave's, or 128, four waves')
+// against keys k0 .. k0 + nk - 1; where a row's keys are cut over several
+// items, each leaves its part (`part`) in the workspace and a join adds them
+// up; part -1 writes the output itself.
 struct CrossItem {
     int32_t q0;           // the sequence's first token
     int32_t row0, rows;
@@ -70,12 +70,15 @@ struct CrossArgs {
     const CrossJoin *joins;
     uint64_t qs[2], ks[2], vs[2], os[2];   // strides of tokens and heads, elements
     Dt dt;
-    int n_items, n_joins, share, width;
-    float scale;             // of a score, times log2(e)
+    int n_items, n_joins, part_rows, share, width;
+    float scale;             // of a score, times log2(e); positive...
+    float turn;              // ...with 1, -1 or 0 times q
 };
 hipError_t cross_attention(hipStream_t s, const CrossArgs &a);
-// A part: rows of `width` sums, then each row's maximum (base 2) and sum; a
-// row without a finite maximum leaves 1 for its sum if it had a live key.
-inline uint64_t cross_part_floats(int width) { return (uint64_t)CROSS_ROWS * (width + 2); }
+
+// A part's floats: each row's `width` sums, then each row's maximum (base 2)
+// and sum; a row without a finite maximum leaves 1 for its sum if it had a
+// live key.
+inline uint64_t cross_part_floats(int part_rows, int width) { return (uint64_t)part_rows * (width + 2); }
 
 }  // namespace rocm
