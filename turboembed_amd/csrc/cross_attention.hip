@@ -34,11 +34,7 @@ __device__ __forceinline__ float both_max(float v) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// a b, rounded, less c.
-__device__ __forceinline__ float rounded_less(float a, float b, float c) {
-#pragma clang fp contract(off)
-    return a * b - c;
-}
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Chunk {   // 16 bytes of a row
     static constexpr int N = 16 / sizeof(T);
@@ -57,37 +53,107 @@ template <typename T> __device__ __forceinline__ typename Chunk<T>::vec read_chu
 
 // Where a part of `rows` rows lies in the workspace.
 __device__ __forceinline__ float *part_of(const CrossArgs &a, int part) {
-    return a.ws + (uint64_t)part * a.part_rows * (a.width + 2);
+    return a.ws + (uint64_t)part * cross_part_floats(a.most_rows, a.width);
 }
 
-// DP: the head width rounded up to 32, 64, 96 or 128.
+// DP: the head width rounded up to 32, 64, 96 or 128. A tile's rows are DP
+// elements in LDS, chunk c of key k at place c ^ swap(k), so that what a
+// read's pass reads lies in different banks.
 template <typename T, int DP, int WAVES> struct CrossTile {
     static constexpr bool F32 = std::is_same<T, float>::value;
-    static constexpr int KB = WAVES == 1 || (F32 && DP > 64) ? 32 : 64;
-    static constexpr int PITCH = DP * (int)sizeof(T) + 16;   // 16 bytes more: rows in different banks
+    static constexpr int KB = WAVES == 1 || F32 ? 32 : 64;
+    static constexpr int PITCH = DP * (int)sizeof(T), CPR = PITCH / 16;
     static constexpr int BUF = KB * PITCH;
-    static constexpr int LDS = 4 * BUF;                      // K and V, two tiles of each
+    static constexpr int LDS = 4 * BUF;   // K and V, two tiles of each
+    static constexpr int OCC = F32 ? (WAVES == 4 && DP > 96 ? 2 : 1) : DP <= 64 ? 3 : 2;   // waves a SIMD, at least
+    // LDS serves 256 bytes a cycle: 16 keys of one chunk of K (a 16-byte
+    // read's pass), 4 keys of 4 chunks of V (a transposing read's).
+    static constexpr int PERIOD = CPR % 16 == 0 ? 1 : CPR % 8 == 0 ? 2 : 4;   // keys until the banks repeat
+    static __device__ __forceinline__ int swap_k(int key) { return key / PERIOD % (16 / PERIOD); }
+    static __device__ __forceinline__ int swap_v(int key) {
+        if (F32) return CPR % 16 == 0 ? (key >> 2 & 1) * 8 : 0;   // (a read's pass: 8 chunks of keys k and k + 4)
+        return PERIOD == 1 ? (key & 3) * 4 : PERIOD == 2 ? (key >> 1 & 1) * 4 : 0;
+    }
 };
 
 template <typename T, int DP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) cross_tiles(CrossArgs a) {
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(CrossTile<T, DP, WAVES>::OCC)))
+cross_tiles(CrossArgs a) {
     using C = CrossTile<T, DP, WAVES>;
     constexpr bool F32 = C::F32;
-    constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, DT = DP / 32;
-    constexpr int E = Chunk<T>::N, CPR = DP / E, THREADS = 64 * WAVES, NL = KB * CPR / THREADS;
-    static_assert(NL * THREADS == KB * CPR, "whole loads a thread");
+    constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR, DT = DP / 32;
+    constexpr int E = Chunk<T>::N, NL = KB * CPR / 64 / WAVES;
+    static_assert(NL * 64 * WAVES == KB * CPR, "whole loads a wave");
     constexpr float LAG = 8.0f;
+    constexpr uint64_t FULL = KB == 64 ? ~0ull : 0xffffffffull;
     typedef typename Chunk<T>::vec vec;
     typedef typename Mma<T>::frag frag;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
 
     const CrossItem it = a.items[blockIdx.x];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5, d = a.width;
     const bool work = 32 * wave < it.rows;   // this wave has rows
     const int row = it.row0 + min(32 * wave + r, it.rows - 1);
-    const uint64_t token = (uint64_t)it.q0 + row / a.share, head = (uint64_t)it.kv * a.share + row % a.share;
+    const int of_token = a.share == 1 ? row : row / a.share;
+    const uint64_t token = (uint64_t)it.q0 + of_token, head = (uint64_t)it.kv * a.share + (row - of_token * a.share);
 
+    // This lane's places of a tile: load j of the wave fills 64 chunks in order.
+    const T *K0 = (const T *)a.k + (uint64_t)it.k0 * a.ks[0] + it.kv * a.ks[1];
+    const T *V0 = (const T *)a.v + (uint64_t)it.k0 * a.vs[0] + it.kv * a.vs[1];
+    const auto key_of = [&](int j) { return ((wave * NL + j) * 64 + lane) / CPR; };
+    const auto col_k = [&](int j) { return (((wave * NL + j) * 64 + lane) % CPR ^ C::swap_k(key_of(j))) * E; };
+    const auto col_v = [&](int j) { return (((wave * NL + j) * 64 + lane) % CPR ^ C::swap_v(key_of(j))) * E; };
+    uint64_t ko[NL], vo[NL];
+#pragma unroll
+    for (int j = 0; j < NL; ++j) ko[j] = key_of(j) * a.ks[0] + col_k(j), vo[j] = key_of(j) * a.vs[0] + col_v(j);
+    const int32_t *mask = a.mask ? a.mask + it.k0 : nullptr;
+    int alive = 1;   // of the tile on its way: key `lane` is live
+
+    // Starts a tile on its way to LDS: aligned rows of whole chunks go there by
+    // themselves, others through registers at once. Keys past the last repeat it.
+    const auto load = [&](int kb, int buf) {
+        char *K = smem + buf * 2 * BUF, *V = K + BUF;
+        const T *kt = K0 + kb * a.ks[0], *vt = V0 + kb * a.vs[0];
+        const int last = it.nk - 1 - kb;
+        if (mask || last < KB - 1) {   // uniform
+            const int key = min(lane, last);
+            alive = lane <= last && (!mask || mask[kb + key] != 0);
+        }
+        if (a.direct) {
+#pragma unroll
+            for (int j = 0; j < NL; ++j) {
+                const T *kp = kt + ko[j], *vp = vt + vo[j];
+                if (last < KB - 1) {   // uniform
+                    const int64_t back = min(0, last - key_of(j));
+                    kp += back * (int64_t)a.ks[0], vp += back * (int64_t)a.vs[0];
+                }
+                // (Columns past the width keep the zeros they began with.)
+                if (d == DP || col_k(j) < d)
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)kp,
+                                                     (__attribute__((address_space(3))) void *)(K + (wave * NL + j) * 1024),
+                                                     16, 0, 0);
+                if (d == DP || col_v(j) < d)
+                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)vp,
+                                                     (__attribute__((address_space(3))) void *)(V + (wave * NL + j) * 1024),
+                                                     16, 0, 0);
+            }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+            const int64_t back = min(0, last - key_of(j));
+            const int at = ((wave * NL + j) * 64 + lane) * 16, nk = d - col_k(j), nv = d - col_v(j);
+            *(vec *)(K + at) = nk > 0 ? read_chunk(kt + ko[j] + back * (int64_t)a.ks[0], nk) : vec{};
+            *(vec *)(V + at) = nv > 0 ? read_chunk(vt + vo[j] + back * (int64_t)a.vs[0], nv) : vec{};
+        }
+    };
+
+    if (a.direct && d < DP) {   // uniform
+        for (int i = tid; i < C::LDS / 16; i += 64 * WAVES) *(vec *)(smem + i * 16) = vec{};
+        __syncthreads();
+    }
+    if (it.nk > 0) load(0, 0);
     // This row's q: of each 2 E columns the lane's half's E.
     vec q[CPR / 2];
     {
@@ -96,65 +162,30 @@ __global__ void __launch_bounds__(64 * WAVES) cross_tiles(CrossArgs a) {
         for (int s = 0; s < CPR / 2; ++s) {
             const int c = (2 * s + h) * E;
             q[s] = read_chunk(p + c, d - c);
-#pragma unroll
-            for (int e = 0; e < E; ++e) q[s][e] = from_f32<T>(to_f32(q[s][e]) * a.turn);
         }
+        if (a.turn != 1.0f)   // uniform
+#pragma unroll
+            for (int s = 0; s < CPR / 2; ++s)
+#pragma unroll
+                for (int e = 0; e < E; ++e) q[s][e] = from_f32<T>(to_f32(q[s][e]) * a.turn);
     }
-
-    // This thread's chunks of a tile.
-    const T *kp[NL], *vp[NL];
-    {
-        const T *K = (const T *)a.k + (uint64_t)it.k0 * a.ks[0] + it.kv * a.ks[1];
-        const T *V = (const T *)a.v + (uint64_t)it.k0 * a.vs[0] + it.kv * a.vs[1];
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-            const int i = tid + j * THREADS, key = i / CPR, c = i % CPR * E;
-            kp[j] = K + key * a.ks[0] + c;
-            vp[j] = V + key * a.vs[0] + c;
-        }
-    }
-    const int32_t *mask = a.mask ? a.mask + it.k0 : nullptr;
-    vec kr[NL], vr[NL];
-    int alive = 0;   // of the held tile: key `lane` is live
-    auto load = [&](int kb) {
-        const bool mine = lane < KB && kb + lane < it.nk;
-        alive = mine && mask ? mask[kb + lane] : mine;
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-            const int i = tid + j * THREADS, key = i / CPR, n = d - i % CPR * E;
-            kr[j] = vr[j] = vec{};
-            if (kb + key < it.nk) {
-                kr[j] = read_chunk(kp[j] + kb * a.ks[0], n);
-                // (A masked value weighs 0, but not if it is no number.)
-                if (!mask || mask[kb + key] != 0) vr[j] = read_chunk(vp[j] + kb * a.vs[0], n);
-            }
-        }
-    };
-    auto place = [&](int buf) {
-        char *K = smem + buf * 2 * BUF, *V = K + BUF;
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-            const int i = tid + j * THREADS, at = i / CPR * PITCH + i % CPR * 16;
-            *(vec *)(K + at) = kr[j];
-            *(vec *)(V + at) = vr[j];
-        }
-    };
 
     floatx16 o[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) o[t] = floatx16{};
     float m = -INFINITY, l = 0.0f;
-    bool any = false;   // a live key so far
+    bool any = false, far = false;   // a live key so far; a maximum past 2^24
 
-    auto compute = [&](int buf, uint64_t live) {
-        const char *K = smem + buf * 2 * BUF, *V = K + BUF;
-        floatx16 s[SUB];
+    // S^T of 32 keys. Register i is key 8 (i / 4) + 4 h + i % 4.
+    const int kr = r * PITCH, ks = C::swap_k(r);   // (32 keys on, the swap is the same)
+    const auto scores = [&](const char *K, floatx16 (&s)[SUB]) {
 #pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-            s[u] = floatx16{};
+        for (int u = 0; u < SUB; ++u) s[u] = floatx16{};
 #pragma unroll
-            for (int c = 0; c < CPR / 2; ++c) {
-                const vec k = *(const vec *)(K + (32 * u + r) * PITCH + (2 * c + h) * 16);
+        for (int c = 0; c < CPR / 2; ++c)
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+                const vec k = *(const vec *)(K + 32 * u * PITCH + kr + ((2 * c + h) ^ ks) * 16);
                 if constexpr (F32) {
 #pragma unroll
                     for (int e = 0; e < E; ++e) s[u] = Mma<T>::run(k[e], q[c][e], s[u]);
@@ -162,9 +193,59 @@ __global__ void __launch_bounds__(64 * WAVES) cross_tiles(CrossArgs a) {
                     s[u] = Mma<T>::run(k, q[c], s[u]);
                 }
             }
+    };
+    // O^T += V^T P^T over 32 keys.
+    const auto add_values = [&](const char *V, const floatx16 &p) {
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = 8 * (i >> 2) + 4 * h + (i & 3);
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+                    o[t] = Mma<T>::run(*(const float *)(V + key * PITCH + (((r >> 2) + 8 * t) ^ C::swap_v(key)) * 16 + (r & 3) * 4),
+                                       p[i], o[t]);
+            }
+        } else {
+            // 16 keys a product: registers 8 j .. 8 j + 7. A group of 16 lanes
+            // reads 4 keys by 16 columns, and a lane gets its column's 4.
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            const int g = lane >> 4, n = lane & 15, key = 4 * (g >> 1) + (n >> 2);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                frag f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = from_f32<T>(p[8 * j + e]);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) {
+                    const int c = 4 * t + 2 * (g & 1) + ((n >> 1) & 1);
+                    const auto at = [&](int k) {
+                        return (__attribute__((address_space(3))) s4 *)(V + k * PITCH + (c ^ C::swap_v(k)) * 16 + (n & 1) * 8);
+                    };
+                    struct {
+                        s4 lo, hi;
+                    } v;
+                    v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(16 * j + key));
+                    v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(16 * j + 8 + key));
+                    o[t] = Mma<T>::run(__builtin_bit_cast(frag, v), f, o[t]);
+                }
+            }
         }
-        // Register i is key 8 (i / 4) + 4 h + i % 4 of its 32.
-        if (live != (KB == 64 ? ~0ull : 0xffffffffull))   // uniform
+    };
+    const auto raise = [&](float mx) {   // the maximum so far, where scores pass it by LAG
+        if (__ballot(mx > m + LAG) == 0) return;
+        const float mn = fmaxf(m, mx);
+        // (Equal: both infinite, of one sign.)
+        const float f = __builtin_amdgcn_exp2f(m == mn ? 0.0f : m - mn);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] *= f;
+        l *= f;
+        m = mn;
+        far = __ballot(fabsf(m) > 16777216.0f && m != -INFINITY) != 0;
+    };
+    const auto tile = [&](const char *K, uint64_t live) {
+        floatx16 s[SUB];
+        scores(K, s);
+        if (live != FULL) {   // uniform
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 const uint32_t word = (uint32_t)(live >> (32 * u)) >> (4 * h);
@@ -172,91 +253,50 @@ __global__ void __launch_bounds__(64 * WAVES) cross_tiles(CrossArgs a) {
                 for (int i = 0; i < 16; ++i)
                     s[u][i] = (word >> (8 * (i >> 2) + (i & 3))) & 1u ? s[u][i] : -INFINITY;
             }
+        }
         float mx = s[0][0];
 #pragma unroll
         for (int u = 0; u < SUB; ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-        mx = both_max(mx) * a.scale;
-        if (__ballot(mx > m + LAG) != 0) {
-            const float mn = fmaxf(m, mx);
-            // (Equal: both infinite, of one sign.)
-            const float f = __builtin_amdgcn_exp2f(m == mn ? 0.0f : m - mn);
-#pragma unroll
-            for (int t = 0; t < DT; ++t) o[t] *= f;
-            l *= f;
-            m = mn;
-        }
+        raise(both_max(mx) * a.scale);
         const float base = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f;
         // A score's distance from the maximum in one rounding; where the
         // maximum is so large that its own rounding shows, from the rounded
         // score, which is no larger.
-        if (__ballot(fabsf(base) > 16777216.0f) == 0) {
+        float scale = a.scale;
+        if (far) {   // uniform
 #pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], a.scale, -base));
-                    sum += s[u][i];
-                }
-        } else {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[u][i] = __builtin_amdgcn_exp2f(rounded_less(s[u][i], a.scale, base));
-                    sum += s[u][i];
-                }
+            for (int u = 0; u < SUB; ++u) s[u] *= scale;
+            scale = 1.0f;
         }
-        l += sum;
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
-            if constexpr (F32) {
+            float sum = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const char *at = V + (32 * u + 8 * (i >> 2) + 4 * h + (i & 3)) * PITCH + r * 4;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) o[t] = Mma<T>::run(*(const float *)(at + t * 128), s[u][i], o[t]);
-                }
-            } else {
-                // 16 keys a product: registers 8 b .. 8 b + 7. A group of 16 lanes
-                // reads 4 keys by 16 columns, and a lane gets its column's 4.
-                typedef short s4 __attribute__((ext_vector_type(4)));
-                const int g = lane >> 4, n = lane & 15;
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    frag p;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = from_f32<T>(s[u][8 * b + e]);
-                    const char *at = V + (32 * u + 16 * b + 4 * (g >> 1) + (n >> 2)) * PITCH + (16 * (g & 1) + 4 * (n & 3)) * 2;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) {
-                        struct {
-                            s4 lo, hi;
-                        } v;
-                        v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s4 *)(at + 64 * t));
-                        v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s4 *)(at + 64 * t + 8 * PITCH));
-                        o[t] = Mma<T>::run(__builtin_bit_cast(frag, v), p, o[t]);
-                    }
-                }
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
+                sum += s[u][i];
             }
+            l += sum;
+            add_values(K + BUF + 32 * u * PITCH, s[u]);
         }
     };
 
-    if (it.nk > 0) {
-        load(0);
-        place(0);
-    }
     for (int kb = 0, buf = 0; kb < it.nk; kb += KB, buf ^= 1) {
-        const uint64_t live = __ballot(alive != 0);
-        __syncthreads();   // the tile is in LDS, and the other one read
-        if (kb + KB < it.nk) load(kb + KB);
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
+        const uint64_t live = __ballot(lane < KB && alive);
+        if (live != FULL) {   // uniform
+            // A masked value weighs 0, but not if it is no number.
+#pragma unroll
+            for (int j = 0; j < NL; ++j)
+                if (!((live >> key_of(j)) & 1))
+                    *(vec *)(smem + buf * 2 * BUF + BUF + ((wave * NL + j) * 64 + lane) * 16) = vec{};
+        }
+        __syncthreads();   // the tile is there, and the other one read
+        if (kb + KB < it.nk) load(kb + KB, buf ^ 1);
         any |= live != 0;
-        if (work && live != 0) compute(buf, live);
-        if (kb + KB < it.nk) place(buf ^ 1);
+        if (work && live != 0) tile(smem + buf * 2 * BUF, live);
     }
     if (!work) return;
 
@@ -283,37 +323,54 @@ __global__ void __launch_bounds__(64 * WAVES) cross_tiles(CrossArgs a) {
             }
         return;
     }
-    float *p = part_of(a, it.part), *po = p + (uint64_t)(32 * wave + r) * d;
+    // Four columns of every row, then the next four; then the maxima and sums.
+    f32x4 *p = (f32x4 *)part_of(a, it.part);
+    const int at = 32 * wave + r, groups = (d + 3) / 4;
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int c = 32 * t + 8 * (i >> 2) + 4 * h + (i & 3);
-            if (c < d) po[c] = o[t][i];
+        for (int g = 0; g < 4; ++g) {
+            const int c = 8 * t + 2 * g + h;
+            if (c < groups) p[c * it.rows + at] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
         }
     if (h == 0) {
-        float *ml = p + (uint64_t)a.part_rows * d + 2 * (32 * wave + r);
-        ml[0] = m;
-        ml[1] = any && m == -INFINITY && l == 0.0f ? 1.0f : l;
+        float2 *ml = (float2 *)(p + groups * it.rows);
+        ml[at] = float2{m, any && m == -INFINITY && l == 0.0f ? 1.0f : l};
     }
 }
 
 // The parts of rows whose keys were cut: a wave a row, a lane a column of each 64.
 template <typename T> __global__ void __launch_bounds__(256) cross_join(CrossArgs a) {
     const CrossJoin j = a.joins[blockIdx.x];
-    const int lane = threadIdx.x & 63, d = a.width;
-    for (int i = blockIdx.y * 4 + (threadIdx.x >> 6); i < j.rows; i += gridDim.y * 4) {
+    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, d = a.width, groups = (d + 3) / 4;
+    const uint64_t pitch = cross_part_floats(a.most_rows, d);
+    const float *first = part_of(a, j.part0);
+    for (int i = blockIdx.y * waves + (threadIdx.x >> 6); i < j.rows; i += gridDim.y * waves) {
+        // A lane a part: its maximum and sum.
+        const float *ml = first + 4 * groups * j.rows + 2 * i;
         float m = -INFINITY;
-        for (int p = 0; p < j.parts; ++p) m = fmaxf(m, part_of(a, j.part0 + p)[(uint64_t)a.part_rows * d + 2 * i]);
-        float l = 0.0f, o[2] = {0.0f, 0.0f};
-        for (int p = 0; p < j.parts; ++p) {
-            const float *part = part_of(a, j.part0 + p), *ml = part + (uint64_t)a.part_rows * d + 2 * i;
-            const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ml[0] - m);
-            l = fmaf(w, ml[1], l);
+        for (int p = lane; p < j.parts; p += 64) m = fmaxf(m, ml[p * pitch]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-                if (lane + 64 * u < d) o[u] = fmaf(w, part[(uint64_t)i * d + lane + 64 * u], o[u]);
+        for (int w = 32; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+        float l = 0.0f, o[2] = {0.0f, 0.0f};
+        for (int p0 = 0; p0 < j.parts; p0 += 64) {
+            const int n = min(64, j.parts - p0);
+            float w = 0.0f;
+            if (lane < n) {
+                const float *q = ml + (p0 + lane) * pitch;
+                w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(q[0] - m);
+                l = fmaf(w, q[1], l);
+            }
+            const float *part = first + p0 * pitch + 4 * i + (lane & 3);
+#pragma unroll 4
+            for (int p = 0; p < n; ++p, part += pitch) {
+                const float wp = __shfl(w, p, 64);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+                    if (lane + 64 * u < d) o[u] = fmaf(wp, part[((lane >> 2) + 16 * u) * 4 * j.rows], o[u]);
+            }
         }
+        l = wave_sum(l);
         // No maximum: no live key (0), or scores of minus infinity alone.
         const float inv = m == -INFINITY ? (l == 0.0f ? 0.0f : __builtin_nanf("")) : 1.0f / l;
         const int row = j.row0 + i;
@@ -335,12 +392,21 @@ template <typename T> static hipError_t launch_cross(hipStream_t s, const CrossA
     else if (a.width <= 96) { TILES(96); }
     else { TILES(128); }
 #undef TILES
-    if (a.n_joins) enqueue(cross_join<T>, dim3(a.n_joins, a.part_rows == 32 ? 2 : 8), dim3(256), 0, s, a);
+    if (a.n_joins) {
+        const int waves = a.most_rows < 4 ? a.most_rows : 4;
+        enqueue(cross_join<T>, dim3(a.n_joins, (a.most_rows + 2 * waves - 1) / (2 * waves)), dim3(64 * waves), 0, s, a);
+    }
     return hipGetLastError();
 }
 
-hipError_t cross_attention(hipStream_t s, const CrossArgs &a) {
-    if (a.n_items == 0) return hipSuccess;
+hipError_t cross_attention(hipStream_t s, const CrossArgs &given) {
+    if (given.n_items == 0) return hipSuccess;
+    CrossArgs a = given;
+    const auto whole = [&](const void *p, const uint64_t (&stride)[2]) {
+        const uint64_t size = dt_bytes(a.dt);
+        return (reinterpret_cast<uintptr_t>(p) | stride[0] * size | stride[1] * size) % 16 == 0;
+    };
+    a.direct = a.width * dt_bytes(a.dt) % 16 == 0 && whole(a.k, a.ks) && whole(a.v, a.vs);
     if (a.dt == Dt::F32) return launch_cross<float>(s, a);
     if (a.dt == Dt::F16) return launch_cross<_Float16>(s, a);
     return launch_cross<__bf16>(s, a);

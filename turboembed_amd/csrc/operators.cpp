@@ -284,7 +284,7 @@ struct CrossPlan {
     Context *ctx = nullptr;
     uint32_t dtype = 0, heads = 0, kv = 0, width = 0;
     uint64_t tokens = 0, states = 0, workspace = 0;
-    int items = 0, joins = 0, part_rows = 0;
+    int items = 0, joins = 0, part_rows = 0, most_rows = 0;
     uint64_t parts = 0;
     DevPtr work;   // the items, then the joins
 };
@@ -336,23 +336,63 @@ void check_cross(const turbo_rocm_cross_attention_call *call, uint32_t dtype, ui
     for (const Arg &a : {q, k, v, mask}) check_clear(out, a);
 }
 
+// How a plan's rows and keys are cut: row blocks of 32 (a wave) or 128 (four),
+// and runs of at most `slice` keys. The choice is the least of an estimate of
+// the call's time in us, from what items were measured to take (F16 and F32,
+// widths 32 to 128; 16 calls of 1 to 2048 rows a sequence, at 14 cuts each:
+// its choice is within 15% of the best of the 14 for all but two):
+// - a compute unit's time for 64 keys of an item among others: products and
+//   softmax (32 rows: a quarter, one wave of four), or its keys and values
+//   from memory (18 KB/us a unit), or the caches where several row blocks read
+//   them (40 KB/us); a part's way to memory and back beside it;
+// - the longest item's time when it runs alone, of which the last items leave
+//   about three tenths;
+// - the join's launch.
+struct Cut {
+    int rows;
+    uint64_t slice;
+};
+Cut choose_cut(const turbo_rocm_cross_desc &d) {
+    const uint64_t share = d.heads / d.kv_heads;
+    uint64_t longest = 0;
+    for (uint32_t s = 0; s < d.batch; ++s) longest = std::max<uint64_t>(longest, d.k_lens[s]);
+    const bool f32 = d.dtype == TURBO_DTYPE_F32;
+    const double dp = (d.width + 31) / 32 * 32, bytes = 128.0 * d.width * (f32 ? 4 : 2);
+    Cut best{128, std::max<uint64_t>(64, longest)};
+    double least = INFINITY;
+    for (int rows : {32, 128}) {
+        const double wave = f32 ? 0.072 * dp : 0.36 + 0.0056 * dp, work = rows == 32 ? wave / 4 : wave;
+        const double alone = rows == 32 ? (f32 ? 0.088 * dp : 0.8 + 0.014 * dp) : f32 ? 0.074 * dp : 0.5 + 0.0088 * dp;
+        const double fixed = f32 && rows == 32 ? 4 : 1;   // (one such wave a SIMD: nothing beside its start)
+        for (uint64_t slice = 64;; slice *= 2) {
+            double total = 0, most = 0;
+            bool joined = false;
+            for (uint32_t s = 0; s < d.batch; ++s) {
+                const uint64_t r = d.q_lens[s] * share, blocks = (r + rows - 1) / rows;
+                if (!blocks) continue;
+                const uint64_t pieces = std::max<uint64_t>(1, (d.k_lens[s] + slice - 1) / slice);
+                const double tiles = std::ceil((double)d.k_lens[s] / pieces / 64);
+                const double part = pieces > 1 ? 8.0 * std::min<uint64_t>(r, rows) * (d.width + 2) / 18000 : 0;
+                total += (double)(blocks * d.kv_heads * pieces) *
+                         (fixed + part + tiles * std::max(work, bytes / (blocks > 1 ? 40000 : 18000)));
+                most = std::max(most, tiles * alone + 6);
+                joined |= pieces > 1;
+            }
+            const double time = std::max(total / 256 + 0.3 * most, most) + (joined ? 4 : 0);
+            if (time < least) least = time, best = {rows, slice};
+            if (slice >= longest) break;
+        }
+    }
+    return best;
+}
+
 // The items of a plan, in the order of their workgroups, and the joins.
-//
-// Rows 32 at a time where no sequence has more for a key head, 128 otherwise.
-// Keys are cut where the rows alone would leave compute units idle: into runs
-// of at most `slice` keys, so that about `wanted` workgroups have equal work,
-// but no shorter than a run that outweighs its part's way through memory.
 void lay_out(const turbo_rocm_cross_desc &d, std::vector<CrossItem> &items, std::vector<CrossJoin> &joins,
              int &part_rows, uint64_t &parts) {
     const uint64_t share = d.heads / d.kv_heads;
-    uint64_t most = 0;
-    for (uint32_t s = 0; s < d.batch; ++s) most = std::max(most, d.q_lens[s] * share);
-    part_rows = most <= 32 ? 32 : 128;
-    const uint64_t wanted = part_rows == 32 ? 2048 : 512, shortest = part_rows == 32 ? 256 : 512;
-    uint64_t work = 0;   // keys, over all items
-    for (uint32_t s = 0; s < d.batch; ++s)
-        work += (d.q_lens[s] * share + part_rows - 1) / part_rows * d.kv_heads * d.k_lens[s];
-    const uint64_t slice = (std::max(shortest, (work + wanted - 1) / wanted) + 63) / 64 * 64;
+    const Cut cut = choose_cut(d);
+    part_rows = cut.rows;
+    const uint64_t slice = cut.slice;
 
     // The row blocks of a (sequence, key head) read the same keys: they go to
     // one XCD (workgroups go to the 8 in turn), the XCD with the least work so
@@ -420,7 +460,8 @@ CrossPlan *cross_plan_create(Context *c, const turbo_rocm_cross_desc *d) {
     std::vector<CrossItem> items;
     std::vector<CrossJoin> joins;
     lay_out(*d, items, joins, p->part_rows, p->parts);
-    p->workspace = p->parts * cross_part_floats(p->part_rows, (int)d->width) * 4;
+    for (const CrossJoin &j : joins) p->most_rows = std::max(p->most_rows, j.rows);
+    p->workspace = p->parts * cross_part_floats(p->most_rows, (int)d->width) * 4;
     p->items = (int)items.size(), p->joins = (int)joins.size();
     const size_t ib = items.size() * sizeof(CrossItem), jb = joins.size() * sizeof(CrossJoin);
     if (ib + jb) {
@@ -464,7 +505,7 @@ void cross_run(CrossPlan *p, const turbo_rocm_cross_attention_call *call) {
         a.qs[i] = call->q.stride[i], a.ks[i] = call->k.stride[i], a.vs[i] = call->v.stride[i],
         a.os[i] = call->out.stride[i];
     a.dt = dt_of(p->dtype);
-    a.n_items = p->items, a.n_joins = p->joins, a.part_rows = p->part_rows;
+    a.n_items = p->items, a.n_joins = p->joins, a.part_rows = p->part_rows, a.most_rows = p->most_rows;
     a.share = (int)(p->heads / p->kv), a.width = (int)p->width;
     a.scale = base2(call->scale);
     a.turn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f;

@@ -70,15 +70,18 @@ struct CrossArgs {
     const CrossJoin *joins;
     uint64_t qs[2], ks[2], vs[2], os[2];   // strides of tokens and heads, elements
     Dt dt;
-    int n_items, n_joins, part_rows, share, width;
+    int n_items, n_joins, part_rows, most_rows, share, width;   // (most_rows: of one join)
+    bool direct;             // (the launcher's) keys and values in aligned whole chunks
     float scale;             // of a score, times log2(e); positive...
     float turn;              // ...with 1, -1 or 0 times q
 };
 hipError_t cross_attention(hipStream_t s, const CrossArgs &a);
 
-// A part's floats: each row's `width` sums, then each row's maximum (base 2)
-// and sum; a row without a finite maximum leaves 1 for its sum if it had a
-// live key.
-inline uint64_t cross_part_floats(int part_rows, int width) { return (uint64_t)part_rows * (width + 2); }
+// A part's floats, of the most rows that a join has: its rows' sums, four columns of every row after another,
+// then each row's maximum (base 2) and sum of weights; a row without a finite
+// maximum leaves 1 for that sum if it had a live key.
+inline __host__ __device__ uint64_t cross_part_floats(int most_rows, int width) {
+    return ((uint64_t)most_rows * ((width + 3) / 4 * 4 + 2) + 3) / 4 * 4;   // (16-byte stores)
+}
 
 }  // namespace rocm
