@@ -23,10 +23,10 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int loose4 __attribute__((ext_vector_type(4), aligned(1)));
 
-// An output from its exact sum: both scales, then the bias, each rounded.
+// An output from its exact sum: both scales and the bias in F32 (the sum's
+// conversion and its product with a's scale round, then the rest once).
 __device__ __forceinline__ float scaled(int sum, float as, float ws, float bias) {
-#pragma clang fp contract(off)
-    return (float)sum * as * ws + bias;
+    return fmaf((float)sum * as, ws, bias);
 }
 
 __device__ __forceinline__ void put(void *out, Dt t, uint64_t at, float v) {
@@ -122,8 +122,9 @@ template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linea
 //
 // BM rows of a by BN of w a workgroup, WM x WN waves, 128 bytes of the inner
 // width a stage, two stages: the next one's loads run while one is computed.
-// LDS rows are 128 bytes, chunk c of row r at place c ^ (r % 8), so that the 8
-// rows of a read's pass lie in different banks. DIRECT (16-byte aligned
+// LDS rows are 128 bytes, chunk c of row r at place c ^ (r / 2 % 8), so that
+// the 16 rows of a read's pass (256 bytes, two rows a bank round) lie in
+// different banks. DIRECT (16-byte aligned
 // operands and strides, K a multiple of 16): memory to LDS without registers.
 template <int BM, int BN, int WM, int WN, bool DIRECT>
 __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, int grid_n) {
@@ -139,7 +140,12 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
     const int per = gridDim.x / 8;
     int b = blockIdx.x;
     if (b < per * 8) b = (b % 8) * per + b / 8;
-    const int m0 = b / grid_n * BM, n0 = b % grid_n * BN;
+    // GROUP rows of tiles at a time, column by column: the tiles at work in an
+    // XCD share more of a and w than a row of them would.
+    constexpr int GROUP = 4;
+    const int grid_m = gridDim.x / grid_n, g0 = b / (GROUP * grid_n) * GROUP, gm = min(GROUP, grid_m - g0);
+    const int in = b - g0 * grid_n;
+    const int m0 = (g0 + in % gm) * BM, n0 = in / gm * BN;
 
     // This lane's place in each load: row (of a, then of w) and chunk.
     const int8_t *src[LOADS];
@@ -149,12 +155,15 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
         src[j] = row < BM ? a.a + (uint64_t)min(m0 + row, a.m - 1) * a.lda
                           : a.w + (uint64_t)min(n0 + row - BM, a.n - 1) * a.ldw;
     }
-    const int my_chunk = (lane & 7) ^ (lane >> 3);   // (the row's number modulo 8 is lane / 8)
+    // (Half the row's number: 4 for every other load, and lane / 16.)
+    static_assert(LOADS % 2 == 0, "a load's parity is its number's");
+    const int chunk[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};
     i32x4 held[DIRECT ? 1 : LOADS];
     auto load = [&](int stage, int buf) {
-        const int k = min(128 * stage + 16 * my_chunk, a.k - 16);
+        const int at[2] = {min(128 * stage + 16 * chunk[0], a.k - 16), min(128 * stage + 16 * chunk[1], a.k - 16)};
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
+            const int k = at[j & 1];
             if constexpr (DIRECT) {
                 char *dst = smem + buf * STAGE + (wave * LOADS + j) * 1024;
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[j] + k),
@@ -164,107 +173,146 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
             }
         }
     };
-    auto place = [&](int buf) {
-        if constexpr (!DIRECT)
+    const int stages = (a.k + 127) / 128, r = lane & 31, h = lane >> 5;
+    // A stage's loads are over and in LDS, and every wave is done with the
+    // stage before; where the inner width ends in it, a's bytes that do not
+    // count are 0.
+    auto arrive = [&](int stage) {
+        char *at = smem + (stage & 1) * STAGE + wave * LOADS * 1024 + lane * 16;
+        const bool tail = 128 * (stage + 1) > a.k;   // uniform
+        if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
 #pragma unroll
-            for (int j = 0; j < LOADS; ++j)
-                *(i32x4 *)(smem + buf * STAGE + (wave * LOADS + j) * 1024 + lane * 16) = held[j];
+        for (int j = 0; j < LOADS; ++j) {
+            const bool rows = (wave * LOADS + j) * 8 < BM;   // (uniform: of a)
+            if constexpr (DIRECT) {
+                if (tail && rows) *(i32x4 *)(at + j * 1024) = counted(*(i32x4 *)(at + j * 1024), 8 * stage + chunk[j & 1], a.k);
+            } else {
+                *(i32x4 *)(at + j * 1024) = tail && rows ? counted(held[j], 8 * stage + chunk[j & 1], a.k) : held[j];
+            }
+        }
+        __syncthreads();
     };
 
+    // What the epilogue multiplies by, read now: this lane's rows' scales, and
+    // columns 64 i + lane of the wave's.
+    constexpr int COLS = BN / WN, PITCH = COLS * 4 + 16;   // bytes of a staged row, F32's
+    static_assert(WAVES * (32 * PITCH + 8 * COLS) <= 2 * STAGE, "staging fits the stages");
+    const int nw = n0 + wn * COLS, mw = m0 + wm * (BM / WM);
+    float ascale[TM], wscale[(COLS + 63) / 64], wbias[(COLS + 63) / 64];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) ascale[j] = a.as[min(mw + 32 * j + r, a.m - 1)];
+#pragma unroll
+    for (int i = 0; i < (COLS + 63) / 64; ++i) {
+        const int n = min(nw + 64 * i + lane, a.n - 1);
+        wscale[i] = a.ws[n], wbias[i] = a.bias ? a.bias[n] : 0.0f;
+    }
     i32x16 acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = i32x16{};
-    const int r = lane & 31, h = lane >> 5;
-    const int stages = (a.k + 127) / 128;
+    // A quarter of a stage (32 bytes of the inner width) as the matrix
+    // instruction takes it, read while the quarter before is multiplied.
+    struct Quarter {
+        i32x4 x[TM], w[TN];
+    };
+    const auto read = [&](Quarter &f, int stage, int ks) {
+        const char *A = smem + (stage & 1) * STAGE + wm * (BM / WM) * 128,
+                   *W = smem + (stage & 1) * STAGE + (BM + wn * (BN / WN)) * 128;
+        const int at = r * 128 + (((2 * ks + h) ^ (r >> 1 & 7)) * 16);
+        // lgkmcnt(0): the quarter read before the last products; so the next
+        // ones wait for it alone, not for this one.
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) f.w[i] = *(const i32x4 *)(W + i * 4096 + at);
+#pragma unroll
+        for (int j = 0; j < TM; ++j) f.x[j] = *(const i32x4 *)(A + j * 4096 + at);
+    };
+    const auto multiply = [&](const Quarter &f) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    Quarter f0, f1;
     load(0, 0);
-    place(0);
-    for (int s = 0; s < stages; ++s) {
-        const int buf = s & 1;
-        if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this stage is in LDS
-        __syncthreads();
-        if (s + 1 < stages) load(s + 1, buf ^ 1);
-        const char *A = smem + buf * STAGE + wm * (BM / WM) * 128, *W = smem + buf * STAGE + (BM + wn * (BN / WN)) * 128;
-        const bool tail = 128 * (s + 1) > a.k;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            const int c = 2 * ks + h, at = r * 128 + ((c ^ (r & 7)) * 16);
-            i32x4 x[TM], w[TN];
-#pragma unroll
-            for (int j = 0; j < TM; ++j) x[j] = *(const i32x4 *)(A + j * 4096 + at);
-#pragma unroll
-            for (int i = 0; i < TN; ++i) w[i] = *(const i32x4 *)(W + i * 4096 + at);
-            if (tail)
-#pragma unroll
-                for (int j = 0; j < TM; ++j) x[j] = counted(x[j], 8 * s + c, a.k);
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-                for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[i], x[j], acc[i][j], 0, 0, 0);
+    arrive(0);
+    if (stages > 1) load(1, 1);
+    read(f0, 0, 0);
+    for (int s = 0; s + 1 < stages; ++s) {
+            read(f1, s, 1);
+        multiply(f0);
+        read(f0, s, 2);
+        multiply(f1);
+        read(f1, s, 3);
+        multiply(f0);
+        arrive(s + 1);
+        if (s + 2 < stages) load(s + 2, s & 1);
+        read(f0, s + 1, 0);
+        multiply(f1);
         }
-        place(buf ^ 1);   // (the last stage's held rows go where nobody reads)
-    }
+    read(f1, stages - 1, 1);
+    multiply(f0);
+    read(f0, stages - 1, 2);
+    multiply(f1);
+    read(f1, stages - 1, 3);
+    multiply(f0);
+    multiply(f1);
 
     // Epilogue: a lane's row is m = lane % 32, its columns 8 g + 4 h .. + 3 of
     // each tile. Staged through LDS 32 rows at a time in the output's type, so
     // that a store writes a row's columns one after another.
     __syncthreads();
-    constexpr int COLS = BN / WN, PITCH = COLS * 4 + 16;   // bytes of a staged row, F32's
-    static_assert(WAVES * 32 * PITCH <= 2 * STAGE, "staging fits the stages");
-    char *mine = smem + wave * 32 * PITCH;
-    const int nw = n0 + wn * COLS, mw = m0 + wm * (BM / WM);
-    const bool f32 = a.ot == Dt::F32;
+    char *mine = smem + wave * (32 * PITCH + 8 * COLS);
+    float *cols = (float *)(mine + 32 * PITCH);   // the wave's columns' scales, then their biases
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-        const int mb = mw + 32 * j;
-        const float as = a.as[min(mb + r, a.m - 1)];
+    for (int i = 0; i < (COLS + 63) / 64; ++i)
+        if (COLS >= 64 || lane < COLS) cols[64 * i + lane] = wscale[i], cols[COLS + 64 * i + lane] = wbias[i];
+    const auto finish = [&](auto zero) {
+        typedef decltype(zero) O;
+        typedef O out4 __attribute__((ext_vector_type(4)));
+        constexpr int PER = 16 / sizeof(O), LANES = COLS / PER;   // a store's columns, a row's stores
 #pragma unroll
-        for (int i = 0; i < TN; ++i)
+        for (int j = 0; j < TM; ++j) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int cl = 32 * i + 8 * g + 4 * h;
-                float y[4];
+            for (int i = 0; i < TN; ++i) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int n = min(nw + cl + e, a.n - 1);
-                    y[e] = scaled(acc[i][j][4 * g + e], as, a.ws[n], a.bias ? a.bias[n] : 0.0f);
+                for (int g = 0; g < 4; ++g) {
+                    const int c = 32 * i + 8 * g + 4 * h;
+                    const f32x4 ws = *(const f32x4 *)(cols + c), bias = *(const f32x4 *)(cols + COLS + c);
+                    out4 y;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) y[e] = from_f32<O>(scaled(acc[i][j][4 * g + e], ascale[j], ws[e], bias[e]));
+                    *(out4 *)(mine + r * PITCH + c * sizeof(O)) = y;
                 }
-                char *p = mine + r * PITCH + cl * (f32 ? 4 : 2);
-                if (f32) {
-                    *(f32x4 *)p = f32x4{y[0], y[1], y[2], y[3]};
-                } else if (a.ot == Dt::F16) {
-                    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-                    *(h4 *)p = h4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+                __builtin_amdgcn_sched_barrier(0);   // (one tile's sums out of the accumulators at a time)
+            }
+            __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the wave's rows are in LDS
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < 32 * LANES / 64; ++q) {
+                const int at = 64 * q + lane, row = at / LANES, c = at % LANES * PER;
+                const int m = mw + 32 * j + row, n = nw + c;
+                const i32x4 v = *(const i32x4 *)(mine + row * PITCH + c * sizeof(O));
+                if (m >= a.m || n >= a.n) continue;
+                O *o = (O *)a.out + (uint64_t)m * a.ldo + n;
+                if (n + PER <= a.n) {
+                    *(loose4 *)o = v;
                 } else {
-                    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-                    *(b4 *)p = b4{(__bf16)y[0], (__bf16)y[1], (__bf16)y[2], (__bf16)y[3]};
+#pragma unroll
+                    for (int e = 0; e < PER - 1; ++e)
+                        if (n + e < a.n) o[e] = *(const O *)(mine + row * PITCH + (c + e) * sizeof(O));
                 }
             }
-        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): the wave's rows are in LDS
-        __builtin_amdgcn_wave_barrier();
-        const int size = f32 ? 4 : 2, lanes = COLS * size / 16;   // lanes a row
-        for (int q = lane; q < 32 * lanes; q += 64) {
-            const int row = q / lanes, byte = q % lanes * 16, m = mb + row, n = nw + byte / size;
-            if (m >= a.m || n >= a.n) continue;
-            const i32x4 v = *(const i32x4 *)(mine + row * PITCH + byte);
-            char *o = (char *)a.out + ((uint64_t)m * a.ldo + n) * size;
-            const int left = (a.n - n) * size;
-            if (left >= 16) {
-                *(loose4 *)o = v;
-            } else if (f32) {
-#pragma unroll
-                for (int e = 0; e < 3; ++e)
-                    if (4 * e < left) ((int *)o)[e] = v[e];
-            } else {
-#pragma unroll
-                for (int e = 0; e < 7; ++e)
-                    if (2 * e < left) ((short *)o)[e] = (short)(v[e >> 1] >> (16 * (e & 1)));
-            }
+            __builtin_amdgcn_s_waitcnt(0xc07f);   // read before the next rows overwrite them
+            __builtin_amdgcn_wave_barrier();
         }
-        __builtin_amdgcn_s_waitcnt(0xc07f);   // read before the next rows overwrite them
-        __builtin_amdgcn_wave_barrier();
-    }
+    };
+    if (a.ot == Dt::F32) finish(0.0f);
+    else if (a.ot == Dt::F16) finish((_Float16)0.0f);
+    else finish((__bf16)0.0f);
 }
 
 template <int BM, int BN, int WM, int WN> static hipError_t launch_tiles(hipStream_t s, const LinearArgs &a, bool direct) {
@@ -272,7 +320,8 @@ template <int BM, int BN, int WM, int WN> static hipError_t launch_tiles(hipStre
     const dim3 grid((uint32_t)gn * gm), block(64 * WM * WN);
     constexpr int lds = 2 * (BM + BN) * 128;
     if (direct) enqueue(linear_i8_tiles<BM, BN, WM, WN, true>, grid, block, lds, s, a, gn);
-    else enqueue(linear_i8_tiles<BM, BN, WM, WN, false>, grid, block, lds, s, a, gn);
+    else if constexpr (BM < 256) enqueue(linear_i8_tiles<BM, BN, WM, WN, false>, grid, block, lds, s, a, gn);
+    else return hipErrorInvalidValue;
     return hipGetLastError();
 }
 
@@ -301,7 +350,7 @@ hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
     };
     const double wide = 4.3 * rounds(256, 256), mid = 2.1 * rounds(128, 128), small = rounds(64, 64);
     if (small < mid && small < wide) return launch_tiles<64, 64, 2, 2>(s, a, direct);
-    if (mid < wide) return launch_tiles<128, 128, 2, 2>(s, a, direct);
+    if (mid < wide || !direct) return launch_tiles<128, 128, 2, 2>(s, a, direct);   // (256: no registers to hold a stage)
     return launch_tiles<256, 256, 2, 4>(s, a, direct);
 }
 
