@@ -12,6 +12,8 @@
 // consecutive columns of one output row.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
+
 #include "devmath.h"
 #include "launch.h"
 #include "operators.h"
@@ -76,25 +78,42 @@ template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linea
         i32x4 acc[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) acc[t] = i32x4{0, 0, 0, 0};
-        // A step is 8 chunks of each row (128 bytes), two products.
-        for (int c0 = 8 * wave; c0 < chunks; c0 += 8 * WAVES) {
+        // A step is 8 chunks of each row (128 bytes), two products; the next
+        // step's reads go out before this one's products.
+        struct Step {
             i32x4 w[2], x[2][MT];
+        };
+        const auto read = [&](Step &f, int c0) {
+            if (c0 >= chunks) return;   // uniform
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int c = c0 + 4 * u + h, k = min(16 * c, a.k - 16);
-                w[u] = *(const loose4 *)(wp + k);
+                const int k = min(16 * (c0 + 4 * u + h), a.k - 16);
+                f.w[u] = *(const loose4 *)(wp + k);
 #pragma unroll
-                for (int t = 0; t < MT; ++t) x[u][t] = *(const loose4 *)(ap[t] + k);
+                for (int t = 0; t < MT; ++t) f.x[u][t] = *(const loose4 *)(ap[t] + k);
             }
-            if (c0 + 8 > full)   // uniform
+        };
+        const auto multiply = [&](Step &f, int c0) {
+            if (c0 >= chunks) return;
+            if (c0 + 8 > full)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) x[u][t] = counted(x[u][t], c0 + 4 * u + h, a.k);
+                    for (int t = 0; t < MT; ++t) f.x[u][t] = counted(f.x[u][t], c0 + 4 * u + h, a.k);
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u], x[u][t], acc[t], 0, 0, 0);
+                for (int t = 0; t < MT; ++t)
+                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f.w[u], f.x[u][t], acc[t], 0, 0, 0);
+        };
+        Step f0, f1;
+        constexpr int STEP = 8 * WAVES;
+        read(f0, 8 * wave);
+        for (int c0 = 8 * wave; c0 < chunks; c0 += 2 * STEP) {
+            read(f1, c0 + STEP);
+            multiply(f0, c0);
+            read(f0, c0 + 2 * STEP);
+            multiply(f1, c0 + STEP);
         }
         if (tile != (int)blockIdx.x) __syncthreads();   // the last tile's sums are read
 #pragma unroll
@@ -121,7 +140,11 @@ template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linea
 // ---- Tiles: both operands through LDS ----------------------------------------------
 //
 // BM rows of a by BN of w a workgroup, WM x WN waves, 128 bytes of the inner
-// width a stage, two stages: the next one's loads run while one is computed.
+// width a stage, two stages: the next one is on its way while one is computed.
+// (Three and four stages were no faster: a compute unit reads some 20 to 27
+// bytes a clock, and the stages wait for that. A 256 x 256 tile asks for 32;
+// on random operands the chip's power holds the clock at 1.9 GHz besides:
+// 32768 x 4096 x 4096 takes 540 us, 433 on zeros.)
 // LDS rows are 128 bytes, chunk c of row r at place c ^ (r / 2 % 8), so that
 // the 16 rows of a read's pass (256 bytes, two rows a bank round) lie in
 // different banks. DIRECT (16-byte aligned
@@ -159,13 +182,13 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
     static_assert(LOADS % 2 == 0, "a load's parity is its number's");
     const int chunk[2] = {(lane & 7) ^ (lane >> 4), (lane & 7) ^ (4 + (lane >> 4))};
     i32x4 held[DIRECT ? 1 : LOADS];
-    auto load = [&](int stage, int buf) {
+    auto load = [&](int stage) {
         const int at[2] = {min(128 * stage + 16 * chunk[0], a.k - 16), min(128 * stage + 16 * chunk[1], a.k - 16)};
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int k = at[j & 1];
             if constexpr (DIRECT) {
-                char *dst = smem + buf * STAGE + (wave * LOADS + j) * 1024;
+                char *dst = smem + stage % 2 * STAGE + (wave * LOADS + j) * 1024;
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src[j] + k),
                                                  (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
             } else {
@@ -178,7 +201,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
     // stage before; where the inner width ends in it, a's bytes that do not
     // count are 0.
     auto arrive = [&](int stage) {
-        char *at = smem + (stage & 1) * STAGE + wave * LOADS * 1024 + lane * 16;
+        char *at = smem + stage % 2 * STAGE + wave * LOADS * 1024 + lane * 16;
         const bool tail = 128 * (stage + 1) > a.k;   // uniform
         if constexpr (DIRECT) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
 #pragma unroll
@@ -190,7 +213,10 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
                 *(i32x4 *)(at + j * 1024) = tail && rows ? counted(held[j], 8 * stage + chunk[j & 1], a.k) : held[j];
             }
         }
-        __syncthreads();
+        __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): this wave's reads and writes of LDS
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
 
     // What the epilogue multiplies by, read now: this lane's rows' scales, and
@@ -217,8 +243,8 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
         i32x4 x[TM], w[TN];
     };
     const auto read = [&](Quarter &f, int stage, int ks) {
-        const char *A = smem + (stage & 1) * STAGE + wm * (BM / WM) * 128,
-                   *W = smem + (stage & 1) * STAGE + (BM + wn * (BN / WN)) * 128;
+        const char *A = smem + stage % 2 * STAGE + wm * (BM / WM) * 128,
+                   *W = smem + stage % 2 * STAGE + (BM + wn * (BN / WN)) * 128;
         const int at = r * 128 + (((2 * ks + h) ^ (r >> 1 & 7)) * 16);
         // lgkmcnt(0): the quarter read before the last products; so the next
         // ones wait for it alone, not for this one.
@@ -237,9 +263,9 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
         __builtin_amdgcn_sched_barrier(0);
     };
     Quarter f0, f1;
-    load(0, 0);
+    load(0);
     arrive(0);
-    if (stages > 1) load(1, 1);
+    if (stages > 1) load(1);
     read(f0, 0, 0);
     for (int s = 0; s + 1 < stages; ++s) {
             read(f1, s, 1);
@@ -249,7 +275,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
         read(f1, s, 3);
         multiply(f0);
         arrive(s + 1);
-        if (s + 2 < stages) load(s + 2, s & 1);
+        if (s + 2 < stages) load(s + 2);
         read(f0, s + 1, 0);
         multiply(f1);
         }
@@ -326,9 +352,10 @@ template <int BM, int BN, int WM, int WN> static hipError_t launch_tiles(hipStre
 }
 
 template <int MT> static hipError_t launch_rows(hipStream_t s, const LinearArgs &a) {
+    constexpr int WAVES = 8;   // (4 to 16 take the same time within 5%)
     const int tiles = (a.n - 1) / 16 + 1;
     const dim3 grid(tiles < (1 << 16) ? tiles : 1 << 16, (a.m - 1) / (16 * MT) + 1);
-    enqueue(linear_i8_rows<16, MT>, grid, dim3(1024), 0, s, a, tiles);
+    enqueue(linear_i8_rows<WAVES, MT>, grid, dim3(64 * WAVES), 0, s, a, tiles);
     return hipGetLastError();
 }
 
@@ -339,19 +366,39 @@ hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
         enqueue(linear_i8_narrow, dim3((uint32_t)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, s, a);
         return hipGetLastError();
     }
-    if (a.m <= 64) return a.m <= 16 ? launch_rows<1>(s, a) : a.m <= 32 ? launch_rows<2>(s, a) : launch_rows<4>(s, a);
     const auto whole = [](const void *p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) | ld) % 16 == 0; };
     const bool direct = whole(a.a, a.lda) && whole(a.w, a.ldw) && a.k % 16 == 0;
-    // The tile by its rounds over the compute units, at the relative times of
-    // one tile of each.
-    const auto rounds = [&](int bm, int bn) {
-        const uint64_t t = (uint64_t)((a.m - 1) / bm + 1) * ((a.n - 1) / bn + 1);
-        return (double)((t + 255) / 256);
+    // The kernel by its estimated time in us, fitted to 26 shapes of 1 to 4096
+    // rows, N and K of 768 to 8192 (its choice is the fastest measured or
+    // within 10% of it). What a compute unit reads sets the pace: 36 KB/us of
+    // 16-row pieces, or a stage of a tile in 0.25 to 1.75 us (64 x 64: 16 KB;
+    // 128 x 128: 32 KB, slower with every unit at work; 256 x 256: 64 KB).
+    // us measured, rows kernel / 64 / 128 / 256: 48 x 1024 x 4096 6.6, 11.3,
+    // 23.7, 51; 256 x 1024 x 1024 6.1, 5.2, 10.0, 19; 2048 x 4096 x 1024 -,
+    // 18.8, 16.2, 21.9; 8192 x 4096 x 4096 -, -, -, 134.
+    const double stages = (a.k + 127) / 128;
+    const auto blocks = [&](double bm, double bn) { return std::ceil(a.m / bm) * std::ceil(a.n / bn); };
+    const auto rounds = [](double n) { return std::ceil(n / 256); };
+    double least = INFINITY;
+    int best = 0;
+    const auto offer = [&](int which, double time) {
+        if (time < least) least = time, best = which;
     };
-    const double wide = 4.3 * rounds(256, 256), mid = 2.1 * rounds(128, 128), small = rounds(64, 64);
-    if (small < mid && small < wide) return launch_tiles<64, 64, 2, 2>(s, a, direct);
-    if (mid < wide || !direct) return launch_tiles<128, 128, 2, 2>(s, a, direct);   // (256: no registers to hold a stage)
-    return launch_tiles<256, 256, 2, 4>(s, a, direct);
+    for (int mt = 1; mt <= 4; ++mt)
+        if (a.m > 16 * (mt - 1)) offer(mt, rounds(blocks(16.0 * mt, 16)) * a.k * (1 + mt) * 16 / 36000);
+    offer(64, std::fmax(1, blocks(64, 64) / 256) * (stages * 0.25 + 0.3));
+    const double n128 = blocks(128, 128);
+    offer(128, rounds(n128) * (stages * (n128 < 256 ? 0.63 : 0.83) + 2));
+    if (direct) offer(256, rounds(blocks(256, 256)) * (stages * 1.75 + 4));   // (no registers to hold a stage)
+    switch (best) {
+    case 1: return launch_rows<1>(s, a);
+    case 2: return launch_rows<2>(s, a);
+    case 3: return launch_rows<3>(s, a);
+    case 4: return launch_rows<4>(s, a);
+    case 64: return launch_tiles<64, 64, 2, 2>(s, a, direct);
+    case 128: return launch_tiles<128, 128, 2, 2>(s, a, direct);
+    default: return launch_tiles<256, 256, 2, 4>(s, a, direct);
+    }
 }
 
 }  // namespace rocm
