@@ -8,10 +8,10 @@
 // The codes are those of the definition, not of a rounded norm: code_i = the
 // whole number nearest to 127 y_i / max|y| = 127 c_i / max|c|, c = v w, as the
 // norm's factor is common to the row. c is exact in 64 bits (24 by 24 bits),
-// so a code can only go wrong next to the border of two codes, where the
-// quotient is decided again without rounding (nearest_code). 64-bit
-// arithmetic runs at the rate of 32-bit on gfx950's vector units, some 20
-// operations a value here, and the kernel waits for memory.
+// so a code can only go wrong next to the border of two codes: F32 products
+// give the quotient to 3 2^-24 of it, 2.3e-5, and where a border is nearer than
+// 2.5e-5 (one value in 20,000) it is decided again without rounding
+// (nearest_code).
 #include <hip/hip_runtime.h>
 
 #include "devmath.h"
@@ -54,36 +54,40 @@ __device__ __forceinline__ void write8(void *p, Dt t, uint64_t at, int n, const 
     else write8((__bf16 *)p + at, n, v);
 }
 
-// The whole number nearest to 127 c / top (ties to even), |c| <= top, from t,
-// that quotient to some 2^-45. Where t is next to a border h + 1/2 the two
-// sides 127 c and (h + 1/2) top are compared as exact sums of two numbers each.
-__device__ __forceinline__ int nearest_code(double t, double c, double top) {
+// The whole number nearest to 127 c / top (ties to even), |c| <= top, without
+// rounding: low, the whole number below it, and a half are compared with it as
+// exact sums of two numbers each.
+__device__ __forceinline__ int nearest_code(double c, double top, double low) {
 #pragma clang fp contract(off)
-    double n = rint(t);
-    if (__builtin_expect(fabs(fabs(t - n) - 0.5) < 1e-9, 0)) {
-        const double low = floor(t), half = low + 0.5;
-        const double a = 127.0 * c, b = half * top;
-        const double d = (a - b) + (fma(127.0, c, -a) - fma(half, top, -b));
-        n = d > 0.0 ? low + 1.0 : d < 0.0 ? low : 2.0 * rint(0.5 * half);
-    }
-    return (int)n;
+    const double half = low + 0.5, a = 127.0 * c, b = half * top;
+    const double d = (a - b) + (fma(127.0, c, -a) - fma(half, top, -b));
+    return (int)(d > 0.0 ? low + 1.0 : d < 0.0 ? low : 2.0 * rint(0.5 * half));
 }
 
-// The sum (or maximum) over the WAVES waves that share a row; red is their
-// LDS. Every lane of them calls it.
-template <int WAVES, bool MAX> __device__ __forceinline__ double row_reduce(double v, double *red) {
+// A row's sum of squares, largest magnitude and sign of what is no number.
+struct Stats {
+    double ss, top;
+    float bad;
+};
+
+// Over the WAVES waves that share a row; red is their LDS, another for the next
+// row. Every lane of them calls it.
+template <int WAVES> __device__ __forceinline__ Stats row_stats(Stats v, Stats *red) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-        const double u = __shfl_xor(v, o, 64);
-        v = MAX ? fmax(v, u) : v + u;
+        v.ss += __shfl_xor(v.ss, o, 64);
+        v.top = fmax(v.top, __shfl_xor(v.top, o, 64));
+        v.bad += __shfl_xor(v.bad, o, 64);
     }
     if constexpr (WAVES > 1) {
-        __syncthreads();   // the last use of red is over
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
         __syncthreads();
         v = red[0];
 #pragma unroll
-        for (int i = 1; i < WAVES; ++i) v = MAX ? fmax(v, red[i]) : v + red[i];
+        for (int i = 1; i < WAVES; ++i) {
+            const Stats u = red[i];
+            v.ss += u.ss, v.top = fmax(v.top, u.top), v.bad += u.bad;
+        }
     }
     return v;
 }
@@ -94,11 +98,14 @@ template <int WAVES, bool MAX> __device__ __forceinline__ double row_reduce(doub
 template <typename X, typename R, bool NORM, int WAVES, int G>
 __global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel(RowArgs a) {
     constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1, LANES = 64 * WAVES;
-    __shared__ double red[WAVES];
+    // (Two rows' worth: a wave may be a row ahead of the slowest.)
+    __shared__ Stats red[2][WAVES];
     const int lane = threadIdx.x % LANES;
+    int turn = 0;
     for (int row = blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += gridDim.x * ROWS) {
         float v[G][8];
-        double ss = 0.0, top = 0.0, bad = 0.0;
+        double ss = 0.0, top = 0.0;
+        float top32 = 0.0f, bad = 0.0f;   // bad is not 0: an infinity or a NaN among the values
         // (A weight of either type, 1 without one.)
         auto weight = [&](int c, int n, float(&w)[8]) {
             if constexpr (NORM) {
@@ -139,14 +146,20 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel
                 const double d = v[g][k];
                 if constexpr (NORM) ss = fma(d, d, ss);
                 if (a.scales) {
-                    const double e = NORM ? d * w[k] : d;
-                    top = fmax(top, fabs(e));
-                    bad = fma(e, 0.0, bad);   // not 0: an infinity or a NaN
+                    if constexpr (NORM) {
+                        top = fmax(top, fabs(d * w[k]));
+                        bad = fmaf(v[g][k] * 0.0f, w[k], bad);
+                    } else {
+                        top32 = fmaxf(top32, fabsf(v[g][k]));
+                        bad = fmaf(v[g][k], 0.0f, bad);
+                    }
                 }
             }
         }
+        const Stats all = row_stats<WAVES>(Stats{ss, NORM ? top : (double)top32, bad}, red[turn]);
+        turn ^= 1;
         double r = 1.0;
-        if constexpr (NORM) r = 1.0 / sqrt(row_reduce<WAVES, false>(ss, red) / a.cols + a.eps);
+        if constexpr (NORM) r = 1.0 / sqrt(all.ss / a.cols + a.eps);
         if (NORM && a.out)
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -159,22 +172,38 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel
                 write8(a.out, a.ot, row * a.ldo + c, n, y);
             }
         if (!a.scales) continue;
-        top = row_reduce<WAVES, true>(top, red);
-        const bool fine = row_reduce<WAVES, false>(bad, red) == 0.0;
+        top = all.top;
+        const bool fine = all.bad == 0.0f;
         const double k127 = fine && top > 0.0 ? 127.0 / top : 0.0;
+        const float factor = (float)k127;
+        // (Rows so large or small that F32 does not hold the steps.)
+        const bool far = k127 > 1e30 || (k127 > 0.0 && k127 < 1e-30);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const int c = 8 * (lane + LANES * g), n = a.cols - c;
             if (n <= 0) continue;
-            float w[8];
+            float w[8], t[8];
             weight(c, n, w);
-            uint32_t q[2] = {0, 0};
+            float near = 0.0f;   // the largest distance from a whole number
+            int code[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const double e = NORM ? (double)v[g][k] * w[k] : (double)v[g][k];
-                const int code = fine ? nearest_code(e * k127, e, top) : 0;
-                q[k >> 2] |= (uint32_t)(uint8_t)(int8_t)code << (8 * (k & 3));
+                t[k] = (NORM ? v[g][k] * w[k] : v[g][k]) * factor;
+                const float whole = rintf(t[k]);
+                near = fmaxf(near, fabsf(t[k] - whole));
+                code[k] = fine ? (int)whole : 0;
             }
+            if (near > 0.5f - 2.5e-5f || far) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const double e = NORM ? (double)v[g][k] * w[k] : (double)v[g][k];
+                    code[k] = nearest_code(e, top, far ? floor(127.0 * e / top) : (double)floorf(t[k]));
+                    if (!fine) code[k] = 0;
+                }
+            }
+            uint32_t q[2] = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) q[k >> 2] |= (uint32_t)(uint8_t)(int8_t)code[k] << (8 * (k & 3));
             int8_t *p = a.codes + row * a.ldc + c;
             if (n >= 8) {
                 typedef uint32_t loose2 __attribute__((ext_vector_type(2), aligned(1)));
@@ -190,6 +219,9 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel
 }
 
 template <typename X, typename R, bool NORM> static hipError_t launch_rows(hipStream_t s, const RowArgs &a) {
+    // (Waves and values a lane as measured, GB/s of norm and codes, F16 or BF16:
+    // 4096 columns 4 x 16 4140, 1 x 64 3371, 2 x 32 3751, 8 x 16 2985; 8192:
+    // 4 x 32 3740, 8 x 16 3520; 16384: 8 x 32 3784, 4 x 64 2698, 16 x 32 2153.)
     // Workgroups enough for every row, up to a bound past which they take
     // several (a launch holds less than 2^32 threads).
     auto go = [&](auto kernel, int waves) {
@@ -204,7 +236,8 @@ template <typename X, typename R, bool NORM> static hipError_t launch_rows(hipSt
     if (a.cols <= 2048) ROWS(1, 4);
     if (a.cols <= 4096) ROWS(4, 2);
     if (a.cols <= 8192) ROWS(4, 4);
-    if (a.cols <= 16384) ROWS(4, 8);
+    if (a.cols <= 16384) ROWS(8, 4);
+    if (a.cols <= 32768) ROWS(8, 8);
     ROWS(16, 8);
 #undef ROWS
 }

@@ -73,27 +73,33 @@ def _tensor(t):
     if t is None:
         return _ABSENT
     shape, stride = t.shape, t.stride()
-    n = len(shape)
     dtype = _known.get(t.dtype) or dtype_code(t.dtype)
-    if n == 0 or n > 3:
-        raise ValueError(f"an array of {n} axes")
-    if stride[-1] != 1 and shape[-1] > 1:
-        raise ValueError("the last axis of an array must be contiguous")
-    if isinstance(t, DeviceArray):
-        nbytes = t.bytes
-    else:
-        if not t.is_cuda:
-            raise ValueError("a tensor that is not on the GPU")
-        # What its strides reach: a tensor lies within its own storage.
-        nbytes = shape[-1]
-        for i in range(n - 1):
-            nbytes += (shape[i] - 1) * stride[i]
-        nbytes = nbytes * _SIZES[dtype] if 0 not in shape else 0
-    if n == 1:
-        return t.data_ptr(), nbytes, shape[0], 0, 0, 0, 0, 1, dtype
+    n = len(shape)
+    # reach: what the strides reach, in elements (a tensor lies within its own storage).
     if n == 2:
-        return t.data_ptr(), nbytes, shape[0], shape[1], 0, stride[0], 0, 2, dtype
-    return t.data_ptr(), nbytes, shape[0], shape[1], shape[2], stride[0], stride[1], 3, dtype
+        a, b = shape
+        step, last = stride
+        reach = (a - 1) * step + b if a and b else 0
+        rest = a, b, 0, step, 0, 2, dtype
+    elif n == 1:
+        b, = shape
+        last, = stride
+        reach = b
+        rest = b, 0, 0, 0, 0, 1, dtype
+    elif n == 3:
+        a, c, b = shape
+        step, inner, last = stride
+        reach = (a - 1) * step + (c - 1) * inner + b if a and c and b else 0
+        rest = a, c, b, step, inner, 3, dtype
+    else:
+        raise ValueError(f"an array of {n} axes")
+    if last != 1 and b > 1:
+        raise ValueError("the last axis of an array must be contiguous")
+    if type(t) is DeviceArray:
+        return (t.address, t.bytes) + rest
+    if not t.is_cuda:
+        raise ValueError("a tensor that is not on the GPU")
+    return (t.data_ptr(), reach * _SIZES[dtype]) + rest
 
 
 _T = "QQQQQQQII"
@@ -103,13 +109,22 @@ _LINEAR = struct.Struct("=IIQ" + 6 * _T)
 _CROSS = struct.Struct("=IIQQQd" + 5 * _T)
 
 
+_functions = {}   # the library's, once looked up
+_byref, _error, _ERROR = C.byref, S.turbo_error, C.sizeof(S.turbo_error)
+
+
 def _on(stream):
     return (0, 0) if stream is None else (ENQUEUE, stream)
 
 
-def _call(f, handle, packed):
-    err = S.new_error()
-    rc = f(handle, packed, C.byref(err))
+def _call(name, handle, packed):
+    f = _functions.get(name)
+    if f is None:
+        from . import library
+        f = _functions[name] = getattr(library(), name)
+    err = _error()
+    err.struct_size = _ERROR
+    rc = f(handle, packed, _byref(err))
     if rc != S.TURBO_OK:
         from . import TurboError
         raise TurboError(rc, err.field, err.message.decode(errors="replace"))
@@ -118,20 +133,20 @@ def _call(f, handle, packed):
 def rms_norm(ctx, x, weight, eps, residual=None, sum=None, out=None, codes=None, scales=None, stream=None):
     """v = x (+ residual), y = v * weight / sqrt(mean(v^2) + eps): v into
     sum, y into out, y's int8 codes and scales into codes and scales."""
-    _call(_lib().turbo_rocm_rms_norm, None if ctx is None else ctx.h,
+    _call("turbo_rocm_rms_norm", None if ctx is None else ctx.h,
           _NORM.pack(_NORM.size, *_on(stream), eps, *_tensor(x), *_tensor(residual), *_tensor(weight), *_tensor(sum),
                      *_tensor(out), *_tensor(codes), *_tensor(scales)))
 
 
 def quantize_tokens(ctx, x, codes, scales, stream=None):
     """The int8 codes and scales of x's rows, as linear_i8 takes them."""
-    _call(_lib().turbo_rocm_quantize_tokens, None if ctx is None else ctx.h,
+    _call("turbo_rocm_quantize_tokens", None if ctx is None else ctx.h,
           _CODES.pack(_CODES.size, *_on(stream), *_tensor(x), *_tensor(codes), *_tensor(scales)))
 
 
 def linear_i8(ctx, codes, scales, weight, weight_scales, out, bias=None, stream=None):
     """out = (codes weight^T) * scales[:, None] * weight_scales + bias."""
-    _call(_lib().turbo_rocm_linear_i8, None if ctx is None else ctx.h,
+    _call("turbo_rocm_linear_i8", None if ctx is None else ctx.h,
           _LINEAR.pack(_LINEAR.size, *_on(stream), *_tensor(codes), *_tensor(scales), *_tensor(weight),
                        *_tensor(weight_scales), *_tensor(bias), *_tensor(out)))
 
@@ -162,7 +177,7 @@ def check_cross(q_lens, k_lens, heads, kv_heads, width, dtype, q=None, k=None, v
     """A plan's and (with q) a call's checks without a device (turbo_rocm_cross_check)."""
     d = _cross_desc(q_lens, k_lens, heads, kv_heads, width, dtype)
     packed = None if q is None else _cross_call(q, k, v, out, mask, scale, None, stream, width)
-    _call(_lib().turbo_rocm_cross_check, C.byref(d), packed)
+    _call("turbo_rocm_cross_check", C.byref(d), packed)
 
 
 class CrossPlan:
@@ -184,7 +199,7 @@ class CrossPlan:
         states whose mask entry is not 0; scale 1 / sqrt(width) by default.
         workspace: a 1-d tensor (or DeviceArray) of workspace_bytes I8 or U8
         (none needed where that is 0), this call's own until it is done."""
-        _call(_lib().turbo_rocm_cross_attention, self.h,
+        _call("turbo_rocm_cross_attention", self.h,
               _cross_call(q, k, v, out, mask, scale, workspace, stream, self.width))
 
     def close(self):
