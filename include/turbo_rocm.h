@@ -229,7 +229,9 @@ int32_t turbo_rocm_linear_i8(void *ctx, const turbo_rocm_linear_i8_call *call, t
  * device. A plan is never written after that: one serves any number of calls
  * (a decoder's layers and steps) on any streams, at once. It must outlive the
  * calls and graphs that use it, and its context must outlive it.
- * *workspace_bytes (may be NULL) is what each call needs beside its operands. */
+ * *workspace_bytes (may be NULL) is what each call needs beside its operands.
+ * More than 2^31 rows (query tokens times heads) or states, or 2^23
+ * workgroups, are TURBO_E_CAPACITY. */
 typedef struct turbo_rocm_cross_desc {
     uint32_t struct_size;
     uint32_t dtype;

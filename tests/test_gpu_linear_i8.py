@@ -138,3 +138,17 @@ def test_many_columns_of_one_row(context):
     one, out = torch.ones(n, device="cuda"), torch.empty(1, n, device="cuda")
     context.linear_i8(a, one[:1], w, one, out, stream=_stream())
     assert torch.equal(out[0].double(), (w.double() @ a[0].double()))
+
+
+@pytest.mark.parametrize("m, n, k", [(5_000_003, 3, 16), (5_000_003, 17, 64), (270_000_001, 1, 16), (3, 9_000_001, 32)])
+def test_more_rows_or_columns_than_one_launch_takes(context, m, n, k):
+    g = torch.Generator(device="cuda").manual_seed(m % 97)
+    a = torch.randint(-127, 128, (m, k), generator=g, device="cuda", dtype=torch.int8)
+    w = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    a_s, w_s = torch.rand(m, generator=g, device="cuda"), torch.rand(n, generator=g, device="cuda")
+    b = torch.randn(n, generator=g, device="cuda")
+    out = torch.full((m, n), 7.0, device="cuda")
+    context.linear_i8(a, a_s, w, w_s, out, bias=b, stream=_stream())
+    for at in range(0, max(m, n), 10_000_000):
+        rows = slice(at, at + 10_000_000) if m > n else slice(None)
+        _check(out[rows], a[rows], a_s[rows], w, w_s, b)

@@ -64,16 +64,17 @@ __global__ void __launch_bounds__(256) linear_i8_narrow(LinearArgs a) {
 // Bound by w's bytes, each read once, straight into the matrix instruction's
 // registers: a lane 16 bytes of a column's row, four lanes 64 consecutive ones.
 // The waves' sums meet in LDS.
-template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linear_i8_rows(LinearArgs a, int tiles) {
+template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linear_i8_rows(LinearArgs a, uint64_t blocks) {
     __shared__ __attribute__((aligned(16))) i32x4 part[WAVES][MT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, h = lane >> 4;
-    const int m0 = blockIdx.y * 16 * MT;
     const int chunks = (a.k + 15) / 16, full = a.k / 16;
-    const int8_t *ap[MT];
+    const uint32_t tiles = (a.n - 1) / 16 + 1;
+    for (uint64_t i = blockIdx.x; i < blocks; i += gridDim.x) {
+        const int tile = (int)(i % tiles), m0 = (int)(i / tiles) * 16 * MT;
+        const int8_t *ap[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) ap[t] = a.a + (uint64_t)min(m0 + 16 * t + r, a.m - 1) * a.lda;
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        for (int t = 0; t < MT; ++t) ap[t] = a.a + (uint64_t)min(m0 + 16 * t + r, a.m - 1) * a.lda;
         const int8_t *wp = a.w + (uint64_t)min(16 * tile + r, a.n - 1) * a.ldw;
         i32x4 acc[MT];
 #pragma unroll
@@ -115,12 +116,12 @@ template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linea
             read(f0, c0 + 2 * STEP);
             multiply(f1, c0 + STEP);
         }
-        if (tile != (int)blockIdx.x) __syncthreads();   // the last tile's sums are read
+        if (i != blockIdx.x) __syncthreads();   // the last block's sums are read
 #pragma unroll
         for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
         __syncthreads();
-        for (int i = tid; i < 64 * MT; i += 64 * WAVES) {
-            const int t = i >> 6, l = i & 63;
+        for (int e = tid; e < 64 * MT; e += 64 * WAVES) {
+            const int t = e >> 6, l = e & 63;
             i32x4 s = part[0][t][l];
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) s += part[w][t][l];
@@ -353,9 +354,10 @@ template <int BM, int BN, int WM, int WN> static hipError_t launch_tiles(hipStre
 
 template <int MT> static hipError_t launch_rows(hipStream_t s, const LinearArgs &a) {
     constexpr int WAVES = 8;   // (4 to 16 take the same time within 5%)
-    const int tiles = (a.n - 1) / 16 + 1;
-    const dim3 grid(tiles < (1 << 16) ? tiles : 1 << 16, (a.m - 1) / (16 * MT) + 1);
-    enqueue(linear_i8_rows<WAVES, MT>, grid, dim3(64 * WAVES), 0, s, a, tiles);
+    const uint64_t blocks = ((uint64_t)(a.n - 1) / 16 + 1) * ((a.m - 1) / (16 * MT) + 1);
+    // (A launch holds less than 2^32 threads; past a bound workgroups take several blocks.)
+    const dim3 grid((uint32_t)(blocks < (1 << 16) ? blocks : 1 << 16));
+    enqueue(linear_i8_rows<WAVES, MT>, grid, dim3(64 * WAVES), 0, s, a, blocks);
     return hipGetLastError();
 }
 
@@ -365,6 +367,24 @@ hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
         const uint64_t blocks = ((uint64_t)a.m * a.n + 255) / 256;
         enqueue(linear_i8_narrow, dim3((uint32_t)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, s, a);
         return hipGetLastError();
+    }
+    // A launch holds less than 2^32 threads: a product of more than 2^22 of the
+    // smallest tiles goes by halves.
+    if (((uint64_t)(a.m - 1) / 64 + 1) * ((a.n - 1) / 64 + 1) > 1 << 22) {
+        LinearArgs first = a, second = a;
+        const uint64_t size = dt_bytes(a.ot);
+        if (a.m >= a.n) {
+            first.m = (a.m / 2 + 255) / 256 * 256, second.m = a.m - first.m;
+            second.a += first.m * a.lda, second.as += first.m;
+            second.out = (char *)a.out + first.m * a.ldo * size;
+        } else {
+            first.n = (a.n / 2 + 255) / 256 * 256, second.n = a.n - first.n;
+            second.w += first.n * a.ldw, second.ws += first.n;
+            if (a.bias) second.bias += first.n;
+            second.out = (char *)a.out + first.n * size;
+        }
+        const hipError_t e = linear_i8(s, first);
+        return e != hipSuccess ? e : linear_i8(s, second);
     }
     const auto whole = [](const void *p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) | ld) % 16 == 0; };
     const bool direct = whole(a.a, a.lda) && whole(a.w, a.ldw) && a.k % 16 == 0;

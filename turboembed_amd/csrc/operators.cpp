@@ -393,6 +393,13 @@ void lay_out(const turbo_rocm_cross_desc &d, std::vector<CrossItem> &items, std:
     const Cut cut = choose_cut(d);
     part_rows = cut.rows;
     const uint64_t slice = cut.slice;
+    // (A launch holds less than 2^32 threads.)
+    u128 workgroups = 0;
+    for (uint32_t s = 0; s < d.batch; ++s)
+        workgroups += (u128)((d.q_lens[s] * share + part_rows - 1) / part_rows) * d.kv_heads *
+                      std::max<uint64_t>(1, (d.k_lens[s] + slice - 1) / slice);
+    if (workgroups > 1u << 23)
+        fail(TURBO_E_CAPACITY, "rocm: a plan of " + std::to_string((uint64_t)workgroups) + " workgroups, past 2^23");
 
     // The row blocks of a (sequence, key head) read the same keys: they go to
     // one XCD (workgroups go to the 8 in turn), the XCD with the least work so
@@ -438,8 +445,6 @@ void lay_out(const turbo_rocm_cross_desc &d, std::vector<CrossItem> &items, std:
     }
     size_t total = 0, taken[XCDS] = {};
     for (const auto &l : lists) total += l.size();
-    // (A launch holds less than 2^32 threads.)
-    if (total > (1u << 23)) fail(TURBO_E_CAPACITY, "rocm: a plan of " + std::to_string(total) + " workgroups");
     items.reserve(total);
     for (int x = 0; items.size() < total; x = (x + 1) % XCDS) {
         int from = x;

@@ -102,7 +102,8 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel
     __shared__ Stats red[2][WAVES];
     const int lane = threadIdx.x % LANES;
     int turn = 0;
-    for (int row = blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += gridDim.x * ROWS) {
+    // (Unsigned: the last step passes 31 bits.)
+    for (uint32_t row = blockIdx.x * ROWS + threadIdx.x / LANES; row < (uint32_t)a.rows; row += gridDim.x * ROWS) {
         float v[G][8];
         double ss = 0.0, top = 0.0;
         float top32 = 0.0f, bad = 0.0f;   // bad is not 0: an infinity or a NaN among the values
