@@ -120,8 +120,8 @@ int32_t turbo_rocm_buffer_quantize_static(void *buffer, uint32_t quantization, c
  * (taps, hidden states, imported embeddings): an RMS norm with the residual's
  * addition and int8 codes out, those codes of any rows, the int8 product on
  * codes and scales, and the attention of its tokens to an encoder's states of
- * another length. Like buffer_quantize
- * they work on memory that the caller owns.
+ * another length. Like buffer_quantize they work on memory that the caller
+ * owns.
  *
  * Each takes a context and a call struct whose first field is struct_size
  * (another size: TURBO_E_INVALID_STRUCT_SIZE). Every argument is checked on
@@ -133,13 +133,17 @@ int32_t turbo_rocm_buffer_quantize_static(void *buffer, uint32_t quantization, c
  * hipStream_t of the context's device; NULL: that device's default stream)
  * and the call returns: it allocates nothing, waits for nothing and may be
  * captured into a graph. A stream of another device is refused. Without the
- * flag `stream` must be NULL, and the call runs
- * on the context's own stream and returns when its results are there. Calls
+ * flag `stream` must be NULL, and the call runs on the context's own stream
+ * and returns when its results are there. Calls
  * keep no state of their own: any number may run at once, from any threads
  * and on any streams, when none writes memory that another reads or writes.
  * The calling thread's current device may be any; it is the caller's again
  * afterwards. */
 #define TURBO_ROCM_ENQUEUE 1u
+
+/* HIP's number of a context's device (the table's ordinals count the devices
+ * that the backend lists), for a caller to see where an array has to be. */
+int32_t turbo_rocm_context_device(void *ctx, uint32_t *device, turbo_error *err);
 
 /* An array in device-addressable memory: `data` is the address of its first
  * element on the context's device (a buffer's exported
@@ -228,7 +232,7 @@ int32_t turbo_rocm_linear_i8(void *ctx, const turbo_rocm_linear_i8_call *call, t
  * device, which workgroup takes which tokens and keys, and keeps that on the
  * device. A plan is never written after that: one serves any number of calls
  * (a decoder's layers and steps) on any streams, at once. It must outlive the
- * calls and graphs that use it, and its context must outlive it.
+ * calls and graphs that use it, and its context the calls.
  * *workspace_bytes (may be NULL) is what each call needs beside its operands.
  * More than 2^31 rows (query tokens times heads) or states, or 2^23
  * workgroups, are TURBO_E_CAPACITY. */
@@ -261,8 +265,8 @@ void turbo_rocm_cross_plan_release(void *plan);
  * infinite or undefined score gives what the formula gives: a NaN. workspace:
  * `workspace_bytes` of the context's device, 16-byte aligned, at least the
  * plan's, for this call alone until it has finished (two graphs that may run
- * at once need one each). It holds nothing between calls. out may not overlap an input
- * or the workspace. */
+ * at once need one each). It holds nothing between calls. out may not overlap an
+ * input or the workspace. */
 typedef struct turbo_rocm_cross_attention_call {
     uint32_t struct_size;
     uint32_t flags;
@@ -275,7 +279,8 @@ typedef struct turbo_rocm_cross_attention_call {
 int32_t turbo_rocm_cross_attention(void *plan, const turbo_rocm_cross_attention_call *call, turbo_error *err);
 
 /* The checks of a plan's description and of a call with it, as the two
- * functions above make them (but for the workspace, which the plan sizes), without a device; call may be NULL. */
+ * functions above make them (but for the workspace, which the plan sizes),
+ * without a device; call may be NULL. */
 int32_t turbo_rocm_cross_check(const turbo_rocm_cross_desc *desc, const turbo_rocm_cross_attention_call *call,
                                turbo_error *err);
 

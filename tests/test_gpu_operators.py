@@ -1,0 +1,99 @@
+"""The operators' handles and arrays on a device: arrays of another device, of closed buffers and on the host, and
+plans that outlive their contexts, are refused before any kernel."""
+import ctypes as C
+
+import pytest
+import torch
+
+import turboembed_amd as T
+from turboembed_amd import seam as S
+
+pytestmark = pytest.mark.gpu
+
+
+class Elsewhere:
+    """A tensor's twin that says it is on another GPU: nothing may read it."""
+    def __init__(self, t):
+        self.t, self.shape, self.dtype = t, t.shape, t.dtype
+
+    def data_ptr(self):
+        return self.t.data_ptr()
+
+    def stride(self):
+        return self.t.stride()
+
+    def get_device(self):
+        return 7
+
+
+def _norm(context, **kw):
+    a = dict(x=torch.ones(3, 40, device="cuda"), weight=torch.ones(40, device="cuda"), eps=1e-6,
+             out=torch.full((3, 40), 5.0, device="cuda"))
+    a.update(kw)
+    torch.cuda.synchronize()
+    context.rms_norm(**a)
+    return a["out"]
+
+
+def test_a_context_names_its_device(context):
+    assert context.device == torch.cuda.current_device()
+    device = C.c_uint32(99)
+    err = S.new_error()
+    assert T.library().turbo_rocm_context_device(None, C.byref(device), C.byref(err)) == S.TURBO_E_INVALID_HANDLE
+    assert T.library().turbo_rocm_context_device(context.h, None, C.byref(err)) == S.TURBO_E_INVALID_ARGUMENT
+    assert device.value == 99
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "out"])
+def test_an_array_of_another_device_is_refused(context, name):
+    arrays = dict(x=torch.ones(3, 40, device="cuda"), weight=torch.ones(40, device="cuda"),
+                  out=torch.full((3, 40), 5.0, device="cuda"))
+    for wrong in (Elsewhere(arrays[name]), arrays[name].cpu()):
+        with pytest.raises(ValueError, match="GPU 0"):
+            _norm(context, **{**arrays, name: wrong})
+    assert (arrays["out"] == 5).all()
+
+
+def test_a_workspace_of_another_device_is_refused(context):
+    plan = context.cross_plan((1,), (4096,), 1, 1, 64, S.TURBO_DTYPE_F16)
+    assert plan.workspace_bytes > 0
+    q, k = torch.zeros(1, 1, 64, device="cuda").half(), torch.zeros(4096, 1, 64, device="cuda").half()
+    ws = torch.zeros(plan.workspace_bytes, device="cuda", dtype=torch.int8)
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="GPU 0"):
+        plan.run(q, k, k, torch.empty_like(q), workspace=Elsewhere(ws))
+    plan.close()
+
+
+def test_an_array_of_a_closed_buffer_is_refused(context):
+    buf = context.buffer(480)
+    x = T.DeviceArray(buf, (3, 40), S.TURBO_DTYPE_F32)
+    for offset in (-4, 484):
+        with pytest.raises(ValueError):
+            T.DeviceArray(buf, (1,), S.TURBO_DTYPE_F32, offset=offset)
+    buf.view()[:] = 0
+    assert (_norm(context, x=x) == 0).all()
+    buf.close()
+    with pytest.raises(ValueError, match="closed"):
+        _norm(context, x=x)
+
+
+def test_a_plan_after_its_context(runtime):
+    ctx = runtime.context(0)
+    q, k = torch.ones(2, 3, 16, device="cuda"), torch.ones(5, 3, 16, device="cuda")
+    out = torch.full_like(q, 5.0)
+    plan = ctx.cross_plan((2,), (5,), 3, 3, 16, torch.float32)
+    assert plan.workspace_bytes == 0
+    torch.cuda.synchronize()
+    plan.run(q, k, k, out)
+    assert (out == 1).all()
+    out.fill_(5.0)
+    torch.cuda.synchronize()
+    ctx.close()
+    with pytest.raises(T.TurboError) as e:
+        plan.run(q, k, k, out)
+    assert e.value.code == S.TURBO_E_INVALID_HANDLE and (out == 5).all()
+    with pytest.raises(T.TurboError) as e:
+        ctx.rms_norm(q[0], q[0, 0], 1e-6, out=out[0])
+    assert e.value.code == S.TURBO_E_INVALID_HANDLE
+    plan.close()

@@ -74,6 +74,7 @@ def library():
         # (The operators' call structs come packed as bytes: operators.py.)
         "turbo_rocm_rms_norm": [P, C.c_char_p, E],
         "turbo_rocm_quantize_tokens": [P, C.c_char_p, E],
+        "turbo_rocm_context_device": [P, C.POINTER(u32), E],
         "turbo_rocm_linear_i8": [P, C.c_char_p, E],
         "turbo_rocm_cross_plan_create": [P, C.POINTER(S.turbo_rocm_cross_desc), C.POINTER(C.c_uint64), C.POINTER(P), E],
         "turbo_rocm_cross_attention": [P, C.c_char_p, E],
@@ -142,6 +143,9 @@ class Context:
         err = S.new_error()
         _ok(self.t.context_create(ordinal, rt._log, None, C.byref(h), C.byref(err)), err)
         self.h = h
+        device = C.c_uint32()
+        _ok(library().turbo_rocm_context_device(h, C.byref(device), C.byref(err)), err)
+        self.device = device.value   # HIP's number of it
 
     def load(self, desc: ModelDesc):
         return Model(self, desc)

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
     if (stages > 1) load(1);
     read(f0, 0, 0);
     for (int s = 0; s + 1 < stages; ++s) {
-            read(f1, s, 1);
+        read(f1, s, 1);
         multiply(f0);
         read(f0, s, 2);
         multiply(f1);
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, in
         if (s + 2 < stages) load(s + 2);
         read(f0, s + 1, 0);
         multiply(f1);
-        }
+    }
     read(f1, stages - 1, 1);
     multiply(f0);
     read(f0, stages - 1, 2);

@@ -282,6 +282,7 @@ void linear(Context *c, const turbo_rocm_linear_i8_call *call) {
 
 struct CrossPlan {
     Context *ctx = nullptr;
+    int ordinal = 0;   // (the context's, which may be gone when the plan is released)
     uint32_t dtype = 0, heads = 0, kv = 0, width = 0;
     uint64_t tokens = 0, states = 0, workspace = 0;
     int items = 0, joins = 0, part_rows = 0, most_rows = 0;
@@ -459,7 +460,7 @@ CrossPlan *cross_plan_create(Context *c, const turbo_rocm_cross_desc *d) {
     const Totals t = check_desc(d);
     if (!c) fail(TURBO_E_INVALID_HANDLE, "rocm: no context");
     auto p = std::make_unique<CrossPlan>();
-    p->ctx = c;
+    p->ctx = c, p->ordinal = c->ordinal;
     p->dtype = d->dtype, p->heads = d->heads, p->kv = d->kv_heads, p->width = d->width;
     p->tokens = t.tokens, p->states = t.states;
     std::vector<CrossItem> items;
@@ -523,6 +524,15 @@ void cross_run(CrossPlan *p, const turbo_rocm_cross_attention_call *call) {
 
 extern "C" {
 
+int32_t turbo_rocm_context_device(void *ctx, uint32_t *device, turbo_error *err) {
+    return guarded(err, [&] {
+        if (!ctx) fail(TURBO_E_INVALID_HANDLE, "rocm: no context");
+        if (!device) refuse(0, "nowhere to leave the device");
+        *device = (uint32_t)static_cast<Context *>(ctx)->ordinal;
+        return TURBO_OK;
+    });
+}
+
 int32_t turbo_rocm_cross_plan_create(void *ctx, const turbo_rocm_cross_desc *desc, uint64_t *workspace_bytes,
                                      void **out, turbo_error *err) {
     return guarded(err, [&] {
@@ -537,7 +547,7 @@ int32_t turbo_rocm_cross_plan_create(void *ctx, const turbo_rocm_cross_desc *des
 void turbo_rocm_cross_plan_release(void *plan) {
     if (!plan) return;
     CrossPlan *p = static_cast<CrossPlan *>(plan);
-    OnDevice on(p->ctx->ordinal);
+    OnDevice on(p->ordinal);
     delete p;   // (hipFree waits for the device's work.)
 }
 

@@ -2,9 +2,9 @@
 
 rms_norm, quantize_tokens, linear_i8 and CrossPlan.run call the entry points
 of the same names in turbo_rocm.h, which say what each computes, what it
-checks and how it runs. Their arrays are GPU tensors that answer data_ptr(),
-shape, stride() and dtype as torch's do (this package imports no torch), or a
-`DeviceArray` over one of the context's buffers. Outputs are the caller's:
+checks and how it runs. Their arrays are tensors on the context's GPU that
+answer data_ptr(), shape, stride(), dtype and get_device() as torch's do (this
+package imports no torch), or a `DeviceArray` over one of that GPU's buffers. Outputs are the caller's:
 nothing is allocated.
 
 `stream` is a HIP stream's handle (torch.cuda.current_stream().cuda_stream):
@@ -51,6 +51,8 @@ class DeviceArray:
                 strides.insert(0, n)
                 n *= k
         self.strides = tuple(strides)
+        if not 0 <= offset <= buffer.nbytes:
+            raise ValueError(f"an array from byte {offset} of a buffer of {buffer.nbytes}")
         h = S.turbo_native_handle()
         h.struct_size = C.sizeof(h)
         from . import _ok
@@ -69,7 +71,8 @@ class DeviceArray:
 _ABSENT = (0,) * 9
 
 
-def _tensor(t):
+def _tensor(t, device=None):
+    # (device: the HIP device it has to be on, None without a context.)
     if t is None:
         return _ABSENT
     shape, stride = t.shape, t.stride()
@@ -96,9 +99,16 @@ def _tensor(t):
     if last != 1 and b > 1:
         raise ValueError("the last axis of an array must be contiguous")
     if type(t) is DeviceArray:
+        if not t.buffer.h:
+            raise ValueError("an array of a buffer that is closed")
+        if device is not None and t.buffer.ctx.device != device:
+            raise ValueError(f"an array on GPU {t.buffer.ctx.device}, not the context's {device}")
         return (t.address, t.bytes) + rest
-    if not t.is_cuda:
-        raise ValueError("a tensor that is not on the GPU")
+    if device is None:
+        if not t.is_cuda:
+            raise ValueError("a tensor that is not on the GPU")
+    elif t.get_device() != device:
+        raise ValueError(f"a tensor that is not on GPU {device}, the context's")
     return (t.data_ptr(), reach * _SIZES[dtype]) + rest
 
 
@@ -111,6 +121,10 @@ _CROSS = struct.Struct("=IIQQQd" + 5 * _T)
 
 _functions = {}   # the library's, once looked up
 _byref, _error, _ERROR = C.byref, S.turbo_error, C.sizeof(S.turbo_error)
+
+
+def _handle(ctx):
+    return (None, None) if ctx is None else (ctx.h, ctx.device)
 
 
 def _on(stream):
@@ -133,22 +147,25 @@ def _call(name, handle, packed):
 def rms_norm(ctx, x, weight, eps, residual=None, sum=None, out=None, codes=None, scales=None, stream=None):
     """v = x (+ residual), y = v * weight / sqrt(mean(v^2) + eps): v into
     sum, y into out, y's int8 codes and scales into codes and scales."""
-    _call("turbo_rocm_rms_norm", None if ctx is None else ctx.h,
-          _NORM.pack(_NORM.size, *_on(stream), eps, *_tensor(x), *_tensor(residual), *_tensor(weight), *_tensor(sum),
-                     *_tensor(out), *_tensor(codes), *_tensor(scales)))
+    h, on = _handle(ctx)
+    _call("turbo_rocm_rms_norm", h,
+          _NORM.pack(_NORM.size, *_on(stream), eps, *_tensor(x, on), *_tensor(residual, on), *_tensor(weight, on),
+                     *_tensor(sum, on), *_tensor(out, on), *_tensor(codes, on), *_tensor(scales, on)))
 
 
 def quantize_tokens(ctx, x, codes, scales, stream=None):
     """The int8 codes and scales of x's rows, as linear_i8 takes them."""
-    _call("turbo_rocm_quantize_tokens", None if ctx is None else ctx.h,
-          _CODES.pack(_CODES.size, *_on(stream), *_tensor(x), *_tensor(codes), *_tensor(scales)))
+    h, on = _handle(ctx)
+    _call("turbo_rocm_quantize_tokens", h,
+          _CODES.pack(_CODES.size, *_on(stream), *_tensor(x, on), *_tensor(codes, on), *_tensor(scales, on)))
 
 
 def linear_i8(ctx, codes, scales, weight, weight_scales, out, bias=None, stream=None):
     """out = (codes weight^T) * scales[:, None] * weight_scales + bias."""
-    _call("turbo_rocm_linear_i8", None if ctx is None else ctx.h,
-          _LINEAR.pack(_LINEAR.size, *_on(stream), *_tensor(codes), *_tensor(scales), *_tensor(weight),
-                       *_tensor(weight_scales), *_tensor(bias), *_tensor(out)))
+    h, on = _handle(ctx)
+    _call("turbo_rocm_linear_i8", h,
+          _LINEAR.pack(_LINEAR.size, *_on(stream), *_tensor(codes, on), *_tensor(scales, on), *_tensor(weight, on),
+                       *_tensor(weight_scales, on), *_tensor(bias, on), *_tensor(out, on)))
 
 
 def _lengths(q_lens, k_lens):
@@ -166,10 +183,10 @@ def _cross_desc(q_lens, k_lens, heads, kv_heads, width, dtype):
     return d
 
 
-def _cross_call(q, k, v, out, mask, scale, workspace, stream, width):
-    w, wn = (0, 0) if workspace is None else (workspace.data_ptr(), _tensor(workspace)[1])
-    return _CROSS.pack(_CROSS.size, *_on(stream), w, wn, max(1, width) ** -0.5 if scale is None else scale, *_tensor(q),
-                       *_tensor(k), *_tensor(v), *_tensor(mask), *_tensor(out))
+def _cross_call(q, k, v, out, mask, scale, workspace, stream, width, on=None):
+    w, wn = (0, 0) if workspace is None else _tensor(workspace, on)[:2]
+    return _CROSS.pack(_CROSS.size, *_on(stream), w, wn, max(1, width) ** -0.5 if scale is None else scale,
+                       *_tensor(q, on), *_tensor(k, on), *_tensor(v, on), *_tensor(mask, on), *_tensor(out, on))
 
 
 def check_cross(q_lens, k_lens, heads, kv_heads, width, dtype, q=None, k=None, v=None, out=None, mask=None, scale=None,
@@ -199,8 +216,9 @@ class CrossPlan:
         states whose mask entry is not 0; scale 1 / sqrt(width) by default.
         workspace: a 1-d tensor (or DeviceArray) of workspace_bytes I8 or U8
         (none needed where that is 0), this call's own until it is done."""
-        _call("turbo_rocm_cross_attention", self.h,
-              _cross_call(q, k, v, out, mask, scale, workspace, stream, self.width))
+        # (A plan works for as long as its context.)
+        _call("turbo_rocm_cross_attention", self.h if self.ctx.h else None,
+              _cross_call(q, k, v, out, mask, scale, workspace, stream, self.width, self.ctx.device))
 
     def close(self):
         if self.h:
