@@ -15,6 +15,7 @@
 // scale is positive here (the launcher turns q around for a negative one).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "devmath.h"
@@ -59,13 +60,13 @@ __device__ __forceinline__ float *part_of(const CrossArgs &a, int part) {
 // DP: the head width rounded up to 32, 64, 96 or 128. A tile's rows are DP
 // elements in LDS, chunk c of key k at place c ^ swap(k), so that what a
 // read's pass reads lies in different banks.
-template <typename T, int DP, int WAVES> struct CrossTile {
+template <typename T, int DP, int WAVES, bool DIRECT> struct CrossTile {
     static constexpr bool F32 = std::is_same<T, float>::value;
     static constexpr int KB = WAVES == 1 || F32 ? 32 : 64;
     static constexpr int PITCH = DP * (int)sizeof(T), CPR = PITCH / 16;
     static constexpr int BUF = KB * PITCH;
     static constexpr int LDS = 4 * BUF;   // K and V, two tiles of each
-    static constexpr int OCC = F32 ? (WAVES == 4 && DP > 96 ? 2 : 1) : DP <= 64 ? 3 : 2;   // waves a SIMD, at least
+    static constexpr int OCC = F32 ? (DP <= (DIRECT ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;   // waves a SIMD, at least
     // LDS serves 256 bytes a cycle: 16 keys of one chunk of K (a 16-byte
     // read's pass), 4 keys of 4 chunks of V (a transposing read's).
     static constexpr int PERIOD = CPR % 16 == 0 ? 1 : CPR % 8 == 0 ? 2 : 4;   // keys until the banks repeat
@@ -76,10 +77,10 @@ template <typename T, int DP, int WAVES> struct CrossTile {
     }
 };
 
-template <typename T, int DP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(CrossTile<T, DP, WAVES>::OCC)))
+template <typename T, int DP, int WAVES, bool DIRECT>
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(CrossTile<T, DP, WAVES, DIRECT>::OCC)))
 cross_tiles(CrossArgs a) {
-    using C = CrossTile<T, DP, WAVES>;
+    using C = CrossTile<T, DP, WAVES, DIRECT>;
     constexpr bool F32 = C::F32;
     constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR, DT = DP / 32;
     constexpr int E = Chunk<T>::N, NL = KB * CPR / 64 / WAVES;
@@ -104,9 +105,14 @@ cross_tiles(CrossArgs a) {
     const auto key_of = [&](int j) { return ((wave * NL + j) * 64 + lane) / CPR; };
     const auto col_k = [&](int j) { return (((wave * NL + j) * 64 + lane) % CPR ^ C::swap_k(key_of(j))) * E; };
     const auto col_v = [&](int j) { return (((wave * NL + j) * 64 + lane) % CPR ^ C::swap_v(key_of(j))) * E; };
-    uint64_t ko[NL], vo[NL];
+    // (DIRECT: bytes from a tile's first key, which 31 bits hold; else elements.)
+    typedef typename std::conditional<DIRECT, uint32_t, uint64_t>::type place;
+    place ko[NL], vo[NL];
 #pragma unroll
-    for (int j = 0; j < NL; ++j) ko[j] = key_of(j) * a.ks[0] + col_k(j), vo[j] = key_of(j) * a.vs[0] + col_v(j);
+    for (int j = 0; j < NL; ++j) {
+        constexpr place size = DIRECT ? sizeof(T) : 1;
+        ko[j] = (key_of(j) * (place)a.ks[0] + col_k(j)) * size, vo[j] = (key_of(j) * (place)a.vs[0] + col_v(j)) * size;
+    }
     const int32_t *mask = a.mask ? a.mask + it.k0 : nullptr;
     int alive = 1;   // of the tile on its way: key `lane` is live
 
@@ -120,36 +126,43 @@ cross_tiles(CrossArgs a) {
             const int key = min(lane, last);
             alive = lane <= last && (!mask || mask[kb + key] != 0);
         }
-        if (a.direct) {
+        if constexpr (DIRECT) {
+            // (As buffer loads: those count as vector memory alone, so the reads
+            // of LDS below wait for no load.)
+            typedef __attribute__((address_space(3))) void *to;
+            const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *)kt, (short)0, -1, 0x00020000);
+            const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *)vt, (short)0, -1, 0x00020000);
+            const auto send = [&](__amdgpu_buffer_rsrc_t tile, uint32_t at, char *dst) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(tile, (to)dst, 16, (int)at, 0, 0, 0);
+            };
+            if (last >= KB - 1 && d == DP) {   // uniform
+#pragma unroll
+                for (int j = 0; j < NL; ++j)
+                    send(kr, ko[j], K + (wave * NL + j) * 1024);
+#pragma unroll
+                for (int j = 0; j < NL; ++j)
+                    send(vr, vo[j], V + (wave * NL + j) * 1024);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NL; ++j) {
+                    const uint32_t back = max(0, key_of(j) - last) * (uint32_t)sizeof(T);
+                    // (Columns past the width keep the zeros they began with.)
+                    if (col_k(j) < d) send(kr, ko[j] - back * (uint32_t)a.ks[0], K + (wave * NL + j) * 1024);
+                    if (col_v(j) < d) send(vr, vo[j] - back * (uint32_t)a.vs[0], V + (wave * NL + j) * 1024);
+                }
+            }
+        } else {
 #pragma unroll
             for (int j = 0; j < NL; ++j) {
-                const T *kp = kt + ko[j], *vp = vt + vo[j];
-                if (last < KB - 1) {   // uniform
-                    const int64_t back = min(0, last - key_of(j));
-                    kp += back * (int64_t)a.ks[0], vp += back * (int64_t)a.vs[0];
-                }
-                // (Columns past the width keep the zeros they began with.)
-                if (d == DP || col_k(j) < d)
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)kp,
-                                                     (__attribute__((address_space(3))) void *)(K + (wave * NL + j) * 1024),
-                                                     16, 0, 0);
-                if (d == DP || col_v(j) < d)
-                    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)vp,
-                                                     (__attribute__((address_space(3))) void *)(V + (wave * NL + j) * 1024),
-                                                     16, 0, 0);
+                const int64_t back = min(0, last - key_of(j));
+                const int at = ((wave * NL + j) * 64 + lane) * 16, nk = d - col_k(j), nv = d - col_v(j);
+                *(vec *)(K + at) = nk > 0 ? read_chunk(kt + ko[j] + back * (int64_t)a.ks[0], nk) : vec{};
+                *(vec *)(V + at) = nv > 0 ? read_chunk(vt + vo[j] + back * (int64_t)a.vs[0], nv) : vec{};
             }
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < NL; ++j) {
-            const int64_t back = min(0, last - key_of(j));
-            const int at = ((wave * NL + j) * 64 + lane) * 16, nk = d - col_k(j), nv = d - col_v(j);
-            *(vec *)(K + at) = nk > 0 ? read_chunk(kt + ko[j] + back * (int64_t)a.ks[0], nk) : vec{};
-            *(vec *)(V + at) = nv > 0 ? read_chunk(vt + vo[j] + back * (int64_t)a.vs[0], nv) : vec{};
         }
     };
 
-    if (a.direct && d < DP) {   // uniform
+    if (DIRECT && d < DP) {   // uniform
         for (int i = tid; i < C::LDS / 16; i += 64 * WAVES) *(vec *)(smem + i * 16) = vec{};
         __syncthreads();
     }
@@ -181,18 +194,23 @@ cross_tiles(CrossArgs a) {
     const auto scores = [&](const char *K, floatx16 (&s)[SUB]) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) s[u] = floatx16{};
+        const auto chunk = [&](int c, int u) { return *(const vec *)(K + 32 * u * PITCH + kr + ((2 * c + h) ^ ks) * 16); };
+        if constexpr (F32) {
+            // (A chunk read two ahead of its products, which are slow enough to hide it.)
+            vec k[3] = {chunk(0, 0), chunk(1, 0)};
 #pragma unroll
-        for (int c = 0; c < CPR / 2; ++c)
+            for (int c = 0; c < CPR / 2; ++c) {
+                if (c + 2 < CPR / 2) k[(c + 2) % 3] = chunk(c + 2, 0);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) {
-                const vec k = *(const vec *)(K + 32 * u * PITCH + kr + ((2 * c + h) ^ ks) * 16);
-                if constexpr (F32) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e) s[u] = Mma<T>::run(k[e], q[c][e], s[u]);
-                } else {
-                    s[u] = Mma<T>::run(k, q[c], s[u]);
-                }
+                for (int e = 0; e < E; ++e) s[0] = Mma<T>::run(k[c % 3][e], q[c][e], s[0]);
             }
+        } else {
+#pragma unroll
+            for (int c = 0; c < CPR / 2; ++c)
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) s[u] = Mma<T>::run(chunk(c, u), q[c], s[u]);
+        }
     };
     // O^T += V^T P^T over 32 keys.
     const auto add_values = [&](const char *V, const floatx16 &p) {
@@ -382,16 +400,18 @@ template <typename T> __global__ void __launch_bounds__(256) cross_join(CrossArg
     }
 }
 
-template <typename T> static hipError_t launch_cross(hipStream_t s, const CrossArgs &a) {
+template <typename T, bool DIRECT> static hipError_t launch_cross(hipStream_t s, const CrossArgs &a) {
     const dim3 grid(a.n_items);
-#define TILES(DP)                                                                                                \
-    if (a.part_rows == 32) enqueue(cross_tiles<T, DP, 1>, grid, dim3(64), CrossTile<T, DP, 1>::LDS, s, a);        \
-    else enqueue(cross_tiles<T, DP, 4>, grid, dim3(256), CrossTile<T, DP, 4>::LDS, s, a)
+#define WAVES(DP, W) enqueue(cross_tiles<T, DP, W, DIRECT>, grid, dim3(64 * W), CrossTile<T, DP, W, DIRECT>::LDS, s, a)
+#define TILES(DP)                       \
+    if (a.part_rows == 32) WAVES(DP, 1); \
+    else WAVES(DP, 4)
     if (a.width <= 32) { TILES(32); }
     else if (a.width <= 64) { TILES(64); }
     else if (a.width <= 96) { TILES(96); }
     else { TILES(128); }
 #undef TILES
+#undef WAVES
     if (a.n_joins) {
         const int waves = a.most_rows < 4 ? a.most_rows : 4;
         enqueue(cross_join<T>, dim3(a.n_joins, (a.most_rows + 2 * waves - 1) / (2 * waves)), dim3(64 * waves), 0, s, a);
@@ -399,17 +419,22 @@ template <typename T> static hipError_t launch_cross(hipStream_t s, const CrossA
     return hipGetLastError();
 }
 
-hipError_t cross_attention(hipStream_t s, const CrossArgs &given) {
-    if (given.n_items == 0) return hipSuccess;
-    CrossArgs a = given;
+hipError_t cross_attention(hipStream_t s, const CrossArgs &a) {
+    if (a.n_items == 0) return hipSuccess;
     const auto whole = [&](const void *p, const uint64_t (&stride)[2]) {
         const uint64_t size = dt_bytes(a.dt);
         return (reinterpret_cast<uintptr_t>(p) | stride[0] * size | stride[1] * size) % 16 == 0;
     };
-    a.direct = a.width * dt_bytes(a.dt) % 16 == 0 && whole(a.k, a.ks) && whole(a.v, a.vs);
-    if (a.dt == Dt::F32) return launch_cross<float>(s, a);
-    if (a.dt == Dt::F16) return launch_cross<_Float16>(s, a);
-    return launch_cross<__bf16>(s, a);
+    // (Keys and values in aligned whole chunks, a tile of them within 31 bits.)
+    const bool direct = a.width * dt_bytes(a.dt) % 16 == 0 && whole(a.k, a.ks) && whole(a.v, a.vs) &&
+                        std::max(a.ks[0], a.vs[0]) < (1u << 31) / 64 / 4;
+    const auto go = [&](auto zero) {
+        typedef decltype(zero) T;
+        return direct ? launch_cross<T, true>(s, a) : launch_cross<T, false>(s, a);
+    };
+    if (a.dt == Dt::F32) return go(0.0f);
+    if (a.dt == Dt::F16) return go((_Float16)0.0f);
+    return go((__bf16)0.0f);
 }
 
 }  // namespace rocm

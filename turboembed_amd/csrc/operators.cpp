@@ -339,15 +339,15 @@ void check_cross(const turbo_rocm_cross_attention_call *call, uint32_t dtype, ui
 
 // How a plan's rows and keys are cut: row blocks of 32 (a wave) or 128 (four),
 // and runs of at most `slice` keys. The choice is the least of an estimate of
-// the call's time in us, from what items were measured to take (F16 and F32,
-// widths 32 to 128; 16 calls of 1 to 2048 rows a sequence, at 14 cuts each:
-// its choice is within 15% of the best of the 14 for all but two):
+// the call's time in us, fitted to what 23 calls took (F16, BF16 and F32, widths
+// 32 to 128, 1 to 2048 rows a sequence) at 14 cuts each: its choice is within 9%
+// of the best of the 14 for all but one (20%). The terms:
 // - a compute unit's time for 64 keys of an item among others: products and
-//   softmax (32 rows: a quarter, one wave of four), or its keys and values
-//   from memory (18 KB/us a unit), or the caches where several row blocks read
-//   them (40 KB/us); a part's way to memory and back beside it;
+//   softmax, or its keys and values from memory (20.6 KB/us a unit), or the
+//   caches where several row blocks read them (42 KB/us); a part's way to
+//   memory and back beside it;
 // - the longest item's time when it runs alone, of which the last items leave
-//   about three tenths;
+//   a quarter;
 // - the join's launch.
 struct Cut {
     int rows;
@@ -362,9 +362,9 @@ Cut choose_cut(const turbo_rocm_cross_desc &d) {
     Cut best{128, std::max<uint64_t>(64, longest)};
     double least = INFINITY;
     for (int rows : {32, 128}) {
-        const double wave = f32 ? 0.072 * dp : 0.36 + 0.0056 * dp, work = rows == 32 ? wave / 4 : wave;
-        const double alone = rows == 32 ? (f32 ? 0.088 * dp : 0.8 + 0.014 * dp) : f32 ? 0.074 * dp : 0.5 + 0.0088 * dp;
-        const double fixed = f32 && rows == 32 ? 4 : 1;   // (one such wave a SIMD: nothing beside its start)
+        const double wave = f32 ? 0.045 * dp : 0.33 + 0.0077 * dp, work = rows == 32 ? wave / 2.6 : wave;
+        const double alone = f32 ? 0.076 * dp : rows == 32 ? 0.97 + 0.0046 * dp : 0.57 + 0.0064 * dp;
+        const double fixed = f32 && rows == 32 ? 2.8 : 0.36;   // (few such waves a unit: little beside its start)
         for (uint64_t slice = 64;; slice *= 2) {
             double total = 0, most = 0;
             bool joined = false;
@@ -373,13 +373,13 @@ Cut choose_cut(const turbo_rocm_cross_desc &d) {
                 if (!blocks) continue;
                 const uint64_t pieces = std::max<uint64_t>(1, (d.k_lens[s] + slice - 1) / slice);
                 const double tiles = std::ceil((double)d.k_lens[s] / pieces / 64);
-                const double part = pieces > 1 ? 8.0 * std::min<uint64_t>(r, rows) * (d.width + 2) / 18000 : 0;
+                const double part = pieces > 1 ? 8.0 * std::min<uint64_t>(r, rows) * (d.width + 2) / 14800 : 0;
                 total += (double)(blocks * d.kv_heads * pieces) *
-                         (fixed + part + tiles * std::max(work, bytes / (blocks > 1 ? 40000 : 18000)));
-                most = std::max(most, tiles * alone + 6);
+                         (fixed + part + tiles * std::max(work, bytes / (blocks > 1 ? 42200 : 20600)));
+                most = std::max(most, tiles * alone + 2.6);
                 joined |= pieces > 1;
             }
-            const double time = std::max(total / 256 + 0.3 * most, most) + (joined ? 4 : 0);
+            const double time = std::max(total / 256 + 0.25 * most, most) + (joined ? 6.1 : 0);
             if (time < least) least = time, best = {rows, slice};
             if (slice >= longest) break;
         }

@@ -71,7 +71,6 @@ struct CrossArgs {
     uint64_t qs[2], ks[2], vs[2], os[2];   // strides of tokens and heads, elements
     Dt dt;
     int n_items, n_joins, part_rows, most_rows, share, width;   // (most_rows: of one join)
-    bool direct;             // (the launcher's) keys and values in aligned whole chunks
     float scale;             // of a score, times log2(e); positive...
     float turn;              // ...with 1, -1 or 0 times q
 };
