@@ -152,3 +152,14 @@ def test_more_rows_or_columns_than_one_launch_takes(context, m, n, k):
     for at in range(0, max(m, n), 10_000_000):
         rows = slice(at, at + 10_000_000) if m > n else slice(None)
         _check(out[rows], a[rows], a_s[rows], w, w_s, b)
+
+
+@pytest.mark.parametrize("m, n", [(4000, 4103), (4001, 4096), (130, 20000), (20001, 70)])
+@pytest.mark.parametrize("k", [16, 37, 64, 127, 144])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_many_outputs_of_narrow_rows(context, m, n, k, t):
+    """Tiles of one or two stages, the last of them partial: what is not of the rows counts for nothing."""
+    a, a_s, w, w_s, b = _operands(m + n + k, m, n, k, bias=k % 2 == 0)
+    out = torch.full((m, n), 7.0, dtype=TYPES[t], device="cuda")
+    context.linear_i8(a, a_s, w, w_s, out, bias=b, stream=_stream())
+    _check(out, a, a_s, w, w_s, b)

@@ -388,14 +388,15 @@ hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
     }
     const auto whole = [](const void *p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) | ld) % 16 == 0; };
     const bool direct = whole(a.a, a.lda) && whole(a.w, a.ldw) && a.k % 16 == 0;
-    // The kernel by its estimated time in us, fitted to 26 shapes of 1 to 4096
-    // rows, N and K of 768 to 8192 (its choice is the fastest measured or
-    // within 10% of it). What a compute unit reads sets the pace: 36 KB/us of
-    // 16-row pieces, or a stage of a tile in 0.25 to 1.75 us (64 x 64: 16 KB;
-    // 128 x 128: 32 KB, slower with every unit at work; 256 x 256: 64 KB).
+    // The kernel by its estimated time in us, fitted to 52 shapes of 1 to 30000
+    // rows, N of 100 to 30000 and K of 32 to 8192 (its choice is the fastest
+    // measured or within 10% of it). What a compute unit reads sets the pace: 36
+    // KB/us of 16-row pieces and 0.4 us for each one's sums, or a stage of a tile
+    // in 0.25 to 1.75 us (64 x 64: 16 KB; 128 x 128: 32 KB, slower with every
+    // unit at work; 256 x 256: 64 KB) and its start and end.
     // us measured, rows kernel / 64 / 128 / 256: 48 x 1024 x 4096 6.6, 11.3,
     // 23.7, 51; 256 x 1024 x 1024 6.1, 5.2, 10.0, 19; 2048 x 4096 x 1024 -,
-    // 18.8, 16.2, 21.9; 8192 x 4096 x 4096 -, -, -, 134.
+    // 18.8, 16.2, 21.9; 6532 x 7168 x 64 312, 39, 42, 33.
     const double stages = (a.k + 127) / 128;
     const auto blocks = [&](double bm, double bn) { return std::ceil(a.m / bm) * std::ceil(a.n / bn); };
     const auto rounds = [](double n) { return std::ceil(n / 256); };
@@ -405,11 +406,14 @@ hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
         if (time < least) least = time, best = which;
     };
     for (int mt = 1; mt <= 4; ++mt)
-        if (a.m > 16 * (mt - 1)) offer(mt, rounds(blocks(16.0 * mt, 16)) * a.k * (1 + mt) * 16 / 36000);
-    offer(64, std::fmax(1, blocks(64, 64) / 256) * (stages * 0.25 + 0.3));
+        if (a.m > 16 * (mt - 1)) {
+            const double n = blocks(16.0 * mt, 16);
+            offer(mt, rounds(n) * a.k * (1 + mt) * 16 / 36000 + n / 256 * mt * 0.4);
+        }
+    offer(64, std::fmax(1, blocks(64, 64) / 256) * (stages * 0.25 + 0.8));
     const double n128 = blocks(128, 128);
-    offer(128, rounds(n128) * (stages * (n128 < 256 ? 0.63 : 0.83) + 2));
-    if (direct) offer(256, rounds(blocks(256, 256)) * (stages * 1.75 + 4));   // (no registers to hold a stage)
+    offer(128, rounds(n128) * (stages * (n128 < 256 ? 0.63 : 0.83) + 4));
+    if (direct) offer(256, rounds(blocks(256, 256)) * (stages * 1.75 + 8));   // (no registers to hold a stage)
     switch (best) {
     case 1: return launch_rows<1>(s, a);
     case 2: return launch_rows<2>(s, a);
