@@ -272,3 +272,53 @@ def test_captured_and_replayed(context):
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, (s, q, k)))
+
+
+# Rows that share a wave: up to 64, 128 and 256 columns, and one past each; rows that fill no workgroup, and that
+# leave a part of the last one.
+NARROW = [(1, 3), (31, 1), (33, 8), (1000, 53), (257, 64), (70, 65), (333, 100), (17, 128), (16, 129), (99, 200),
+          (9, 256), (41, 257)]
+
+
+@pytest.mark.parametrize("rows, cols", NARROW)
+@pytest.mark.parametrize("x, res, out", [("f32", "f32", "f32"), ("f16", None, "bf16"), ("bf16", "f32", "f16")])
+def test_norms_of_narrow_rows(context, rows, cols, x, res, out):
+    a = _rows(rows * 7919 + cols, rows, cols, x)
+    r = None if res is None else _rows(cols, rows, cols, res)
+    weight = 1 + 0.3 * _rows(3, 1, cols, "f32", 0)[0]
+    s, o, q, k = _norm(context, a, weight, res=r, sum=res is not None, out=out)
+    total, y, c, rr = _want(a, weight, r, 1e-6)
+    if res is not None:
+        assert torch.equal(s, total)
+    _close(o, y, out)
+    _check_codes(q, k, c, rr)
+    # In place, in rows of a wider array.
+    wide = torch.zeros(rows, cols + 9, dtype=a.dtype, device="cuda")
+    wide[:, 4:4 + cols] = a
+    own = wide[:, 4:4 + cols]
+    context.rms_norm(own, weight, 1e-6, out=own, stream=_stream())
+    _close(own, _want(a, weight, None, 1e-6)[1], x)
+    assert (wide[:, :4] == 0).all() and (wide[:, 4 + cols:] == 0).all()
+
+
+@pytest.mark.parametrize("cols", [1, 53, 64, 100, 250])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_narrow_rows_beside_rows_of_no_numbers(context, cols, t):
+    x = _rows(cols, 100, cols, t)
+    x[3::7], x[5::11, cols // 2], x[6::13, 0] = 0, float("inf"), float("nan")
+    q, k = torch.full((100, cols), 77, dtype=torch.int8, device="cuda"), torch.empty(100, device="cuda")
+    context.quantize_tokens(x, q, k, stream=_stream())
+    fine = torch.isfinite(x).all(1)
+    assert torch.equal(torch.isnan(k), ~fine) and (q[~fine] == 0).all()
+    _check_codes(q[fine], k[fine], x[fine].double().cpu().numpy(), np.ones(int(fine.sum())))
+
+
+def test_more_rows_than_a_launch_s_workgroups_take_at_once(context):
+    rows = 4 * (1 << 20) + 5
+    x = _rows(0, 64, 260, "f16").repeat((rows + 63) // 64, 1)[:rows].contiguous()
+    q, k = torch.empty(rows, 260, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    context.quantize_tokens(x, q, k, stream=_stream())
+    want, top = _nearest(x[:64].double().cpu().numpy())
+    assert torch.equal(q[:64].cpu(), torch.from_numpy(want).to(torch.int8))
+    assert torch.equal(q, q[:64].repeat((rows + 63) // 64, 1)[:rows])
+    assert torch.equal(k, k[:64].repeat((rows + 63) // 64)[:rows])

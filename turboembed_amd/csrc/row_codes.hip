@@ -1,9 +1,13 @@
 // RMS norm with the residual's addition and int8 codes out, and the codes of
 // rows alone.
 //
-// A row is held in registers by one wave or one workgroup: x (and the
+// A row is held in registers by a few lanes, a wave or a workgroup: x (and the
 // residual) are read once, everything else is made from the registers, and
 // the outputs are written once. The weight is read twice, from the caches.
+// Bound by those bytes: 4807 x 1023 F32 rows and their norm take 15.4 us (5.1
+// TB/s, a large copy's rate), 65536 x 1024 F16 rows to codes 42 (4.8), 65536 x
+// 4096 BF16 rows with a residual to codes 453 (4.1, as the norm alone does: a
+// workgroup reads its row, exchanges sums and writes in turn).
 //
 // The codes are those of the definition, not of a rounded norm: code_i = the
 // whole number nearest to 127 y_i / max|y| = 127 c_i / max|c|, c = v w, as the
@@ -70,11 +74,13 @@ struct Stats {
     float bad;
 };
 
-// Over the WAVES waves that share a row; red is their LDS, another for the next
-// row. Every lane of them calls it.
-template <int WAVES> __device__ __forceinline__ Stats row_stats(Stats v, Stats *red) {
+// Over the LANES lanes that share a row (a power of 2 of a wave's, or whole
+// waves); red is the waves' LDS, another for the next row. Every lane of them
+// calls it.
+template <int LANES> __device__ __forceinline__ Stats row_stats(Stats v, Stats *red) {
+    constexpr int WAVES = LANES / 64;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
+    for (int o = LANES < 64 ? LANES / 2 : 32; o > 0; o >>= 1) {
         v.ss += __shfl_xor(v.ss, o, 64);
         v.top = fmax(v.top, __shfl_xor(v.top, o, 64));
         v.bad += __shfl_xor(v.bad, o, 64);
@@ -93,13 +99,13 @@ template <int WAVES> __device__ __forceinline__ Stats row_stats(Stats v, Stats *
 }
 
 // X: x's type; R: the residual's (and v's); NORM: rms_norm, else the codes of
-// x. WAVES waves hold a row, lane l of them columns 8 (l + 64 WAVES g) .. + 7
-// of each group g < G; a workgroup is at least four waves.
-template <typename X, typename R, bool NORM, int WAVES, int G>
-__global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel(RowArgs a) {
-    constexpr int ROWS = WAVES < 4 ? 4 / WAVES : 1, LANES = 64 * WAVES;
+// x. LANES lanes hold a row, lane l of them columns 8 (l + LANES g) .. + 7 of
+// each group g < G; a workgroup is at least 256.
+template <typename X, typename R, bool NORM, int LANES, int G>
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) row_codes_kernel(RowArgs a) {
+    constexpr int ROWS = LANES < 256 ? 256 / LANES : 1;
     // (Two rows' worth: a wave may be a row ahead of the slowest.)
-    __shared__ Stats red[2][WAVES];
+    __shared__ Stats red[2][LANES < 64 ? 1 : LANES / 64];
     const int lane = threadIdx.x % LANES;
     int turn = 0;
     // (Unsigned: the last step passes 31 bits.)
@@ -157,7 +163,7 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel
                 }
             }
         }
-        const Stats all = row_stats<WAVES>(Stats{ss, NORM ? top : (double)top32, bad}, red[turn]);
+        const Stats all = row_stats<LANES>(Stats{ss, NORM ? top : (double)top32, bad}, red[turn]);
         turn ^= 1;
         double r = 1.0;
         if constexpr (NORM) r = 1.0 / sqrt(all.ss / a.cols + a.eps);
@@ -220,26 +226,32 @@ __global__ void __launch_bounds__(WAVES < 4 ? 256 : 64 * WAVES) row_codes_kernel
 }
 
 template <typename X, typename R, bool NORM> static hipError_t launch_rows(hipStream_t s, const RowArgs &a) {
-    // (Waves and values a lane as measured, GB/s of norm and codes, F16 or BF16:
-    // 4096 columns 4 x 16 4140, 1 x 64 3371, 2 x 32 3751, 8 x 16 2985; 8192:
-    // 4 x 32 3740, 8 x 16 3520; 16384: 8 x 32 3784, 4 x 64 2698, 16 x 32 2153.)
+    // Lanes a row and values a lane as measured, GB/s of norm, residual and
+    // codes, F16 or BF16: 4096 columns 256 x 16 4140, 64 x 64 3371, 128 x 32
+    // 3751, 512 x 16 2985; 8192: 256 x 32 3740, 512 x 16 3520; 16384: 512 x 32
+    // 3784, 256 x 64 2698, 1024 x 32 2153. Narrow rows share a wave, or most of
+    // it holds nothing: 2^20 rows of 64 in 8 lanes 4112, in 64 665; 2^18 of 256
+    // in 32 lanes 3981, in 64 2319.
     // Workgroups enough for every row, up to a bound past which they take
     // several (a launch holds less than 2^32 threads).
-    auto go = [&](auto kernel, int waves) {
-        const int per = waves < 4 ? 4 / waves : 1, threads = waves < 4 ? 256 : 64 * waves;
+    auto go = [&](auto kernel, int lanes) {
+        const int per = lanes < 256 ? 256 / lanes : 1, threads = lanes < 256 ? 256 : lanes;
         const int blocks = (a.rows - 1) / per + 1;
         enqueue(kernel, dim3(blocks < (1 << 20) ? blocks : 1 << 20), dim3(threads), 0, s, a);
         return hipGetLastError();
     };
-#define ROWS(W, G) return go(row_codes_kernel<X, R, NORM, W, G>, W)
-    if (a.cols <= 512) ROWS(1, 1);
-    if (a.cols <= 1024) ROWS(1, 2);
-    if (a.cols <= 2048) ROWS(1, 4);
-    if (a.cols <= 4096) ROWS(4, 2);
-    if (a.cols <= 8192) ROWS(4, 4);
-    if (a.cols <= 16384) ROWS(8, 4);
-    if (a.cols <= 32768) ROWS(8, 8);
-    ROWS(16, 8);
+#define ROWS(L, G) return go(row_codes_kernel<X, R, NORM, L, G>, L)
+    if (a.cols <= 64) ROWS(8, 1);
+    if (a.cols <= 128) ROWS(16, 1);
+    if (a.cols <= 256) ROWS(32, 1);
+    if (a.cols <= 512) ROWS(64, 1);
+    if (a.cols <= 1024) ROWS(64, 2);
+    if (a.cols <= 2048) ROWS(64, 4);
+    if (a.cols <= 4096) ROWS(256, 2);
+    if (a.cols <= 8192) ROWS(256, 4);
+    if (a.cols <= 16384) ROWS(512, 4);
+    if (a.cols <= 32768) ROWS(512, 8);
+    ROWS(1024, 8);
 #undef ROWS
 }
 
