@@ -407,3 +407,23 @@ def test_a_sublayer_over_a_session_s_states(context):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(first, (total, c1, q, kv, ctx, c2, o, total2, y)))
     plan.close()
+
+
+@pytest.mark.parametrize("step", [(1 << 23) - 8, 1 << 23])
+@pytest.mark.parametrize("t", ["f16", "f32"])
+def test_states_far_apart(context, step, t):
+    """The longest strides that a tile's 32-bit offsets take, and the first that go another way."""
+    heads, d, nk = 1, 64, 70
+    wide = torch.empty(nk * step, dtype=TYPES[t], device="cuda")
+    k = wide.as_strided((nk, heads, d), (step, d, 1))
+    v = wide.as_strided((nk, heads, d), (step, d, 1), 128)
+    kk, vv = _operands(8, 1, nk, heads, heads, d, t)[1:]
+    k.copy_(kk)
+    v.copy_(vv)
+    for nq in (1, 64):
+        q = _operands(9, nq, 1, heads, heads, d, t)[0]
+        out = torch.empty_like(q)
+        plan = context.cross_plan((nq,), (nk,), heads, heads, d, TYPES[t])
+        plan.run(q, k, v, out, workspace=_workspace(plan), stream=_stream())
+        _check(out, q, kk, vv, (nq,), (nk,))
+        plan.close()
