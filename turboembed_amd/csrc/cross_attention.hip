@@ -222,16 +222,25 @@ cross_tiles(CrossArgs a) {
                 for (int u = 0; u < SUB; ++u) s[u] = Mma<T>::run(chunk(c, u), q[c], s[u]);
         }
     };
-    // O^T += V^T P^T over 32 keys.
-    const auto add_values = [&](const char *V, const floatx16 &p) {
+    // O^T += V^T P^T over 32 keys; weight(i) is register i's, in order.
+    const auto add_values = [&](const char *V, auto weight) {
         if constexpr (F32) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            // (Values and weights two keys ahead of their products.)
+            float v[3][DT], p[3];
+            const auto ahead = [&](int i) {
                 const int key = 8 * (i >> 2) + 4 * h + (i & 3);
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
-                    o[t] = Mma<T>::run(*(const float *)(V + key * PITCH + (((r >> 2) + 8 * t) ^ C::swap_v(key)) * 16 + (r & 3) * 4),
-                                       p[i], o[t]);
+                    v[i % 3][t] = *(const float *)(V + key * PITCH + (((r >> 2) + 8 * t) ^ C::swap_v(key)) * 16 + (r & 3) * 4);
+                p[i % 3] = weight(i);
+            };
+            ahead(0), ahead(1);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (i + 2 < 16) ahead(i + 2);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[t] = Mma<T>::run(v[i % 3][t], p[i % 3], o[t]);
             }
         } else {
             // 16 keys a product: registers 8 j .. 8 j + 7. A group of 16 lanes
@@ -242,7 +251,7 @@ cross_tiles(CrossArgs a) {
             for (int j = 0; j < 2; ++j) {
                 frag f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = from_f32<T>(p[8 * j + e]);
+                for (int e = 0; e < 8; ++e) f[e] = from_f32<T>(weight(8 * j + e));
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
                     const int c = 4 * t + 2 * (g & 1) + ((n >> 1) & 1);
@@ -301,13 +310,12 @@ cross_tiles(CrossArgs a) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
             float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
-                sum += s[u][i];
-            }
+            add_values(K + BUF + 32 * u * PITCH, [&](int i) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
+                sum += w;
+                return w;
+            });
             l += sum;
-            add_values(K + BUF + 32 * u * PITCH, s[u]);
         }
     };
 
