@@ -4,11 +4,11 @@
 // token's head; those that share a key head are rows of one item, so that its
 // keys and values are read once for them) against a run of keys. K and V
 // pass through LDS in tiles of KB keys, two of each: the next tile is on its
-// way while one is computed. Scores are computed transposed, S^T =
-// K Q^T, so that a lane holds one row (lane % 32) and 16 of 32 keys, the other
-// 16 in the lane 32 away; O^T += V^T P^T then takes P as the score registers
-// hold it, against V's columns for the same keys in that order (16-bit values
-// by LDS reads that transpose, F32 values one by one).
+// way while one is computed. Scores are computed transposed, S^T = K Q^T, so
+// that a lane holds one row (lane % 32) and 16 of 32 keys, the other 16 in the
+// lane 32 away; O^T += V^T P^T then takes P as the score registers hold it,
+// against V's columns for the same keys in that order (16-bit values by LDS
+// reads that transpose, F32 values one by one).
 //
 // The softmax is the running one, in base 2 and F32; its maximum moves only
 // when a score passes it by more than 2^8, so most tiles rescale nothing. The
@@ -70,13 +70,16 @@ __device__ __forceinline__ float *part_of(const CrossArgs &a, int part) {
 // DP: the head width rounded up to 32, 64, 96 or 128. A tile's rows are DP
 // elements in LDS, chunk c of key k at place c ^ swap(k), so that what a
 // read's pass reads lies in different banks.
+// DIRECT: keys and values in aligned whole chunks, which go to LDS by themselves
+// (a kernel of its own: the other's registers cost it a wave a SIMD).
 template <typename T, int DP, int WAVES, bool DIRECT> struct CrossTile {
     static constexpr bool F32 = std::is_same<T, float>::value;
     static constexpr int KB = WAVES == 1 || F32 ? 32 : 64;
     static constexpr int PITCH = DP * (int)sizeof(T), CPR = PITCH / 16;
     static constexpr int BUF = KB * PITCH;
     static constexpr int LDS = 4 * BUF;   // K and V, two tiles of each
-    static constexpr int OCC = F32 ? (DP <= (DIRECT ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;   // waves a SIMD, at least
+    // Waves a SIMD, at least.
+    static constexpr int OCC = F32 ? (DP <= (DIRECT ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;
     // LDS serves 256 bytes a cycle: 16 keys of one chunk of K (a 16-byte
     // read's pass), 4 keys of 4 chunks of V (a transposing read's).
     static constexpr int PERIOD = CPR % 16 == 0 ? 1 : CPR % 8 == 0 ? 2 : 4;   // keys until the banks repeat
@@ -204,7 +207,9 @@ cross_tiles(CrossArgs a) {
     const auto scores = [&](const char *K, floatx16 (&s)[SUB]) {
 #pragma unroll
         for (int u = 0; u < SUB; ++u) s[u] = floatx16{};
-        const auto chunk = [&](int c, int u) { return *(const vec *)(K + 32 * u * PITCH + kr + ((2 * c + h) ^ ks) * 16); };
+        const auto chunk = [&](int c, int u) {
+            return *(const vec *)(K + 32 * u * PITCH + kr + ((2 * c + h) ^ ks) * 16);
+        };
         if constexpr (F32) {
             // (A chunk read two ahead of its products, which are slow enough to hide it.)
             vec k[3] = {chunk(0, 0), chunk(1, 0)};
@@ -231,7 +236,8 @@ cross_tiles(CrossArgs a) {
                 const int key = 8 * (i >> 2) + 4 * h + (i & 3);
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
-                    v[i % 3][t] = *(const float *)(V + key * PITCH + (((r >> 2) + 8 * t) ^ C::swap_v(key)) * 16 + (r & 3) * 4);
+                    v[i % 3][t] =
+                        *(const float *)(V + key * PITCH + (((r >> 2) + 8 * t) ^ C::swap_v(key)) * 16 + (r & 3) * 4);
                 p[i % 3] = weight(i);
             };
             ahead(0), ahead(1);

@@ -6,8 +6,9 @@
 // the outputs are written once. The weight is read twice, from the caches.
 // Bound by those bytes: 4807 x 1023 F32 rows and their norm take 15.4 us (5.1
 // TB/s, a large copy's rate), 65536 x 1024 F16 rows to codes 42 (4.8), 65536 x
-// 4096 BF16 rows with a residual to codes 453 (4.1, as the norm alone does: a
-// workgroup reads its row, exchanges sums and writes in turn).
+// 4096 BF16 rows with a residual to codes 442 (4.25, as the norm alone does: a
+// workgroup reads its row, exchanges sums and writes in turn). 16-bit rows that
+// no vector's alignment divides reach two thirds of that.
 //
 // The codes are those of the definition, not of a rounded norm: code_i = the
 // whole number nearest to 127 y_i / max|y| = 127 c_i / max|c|, c = v w, as the
@@ -233,11 +234,14 @@ template <typename X, typename R, bool NORM> static hipError_t launch_rows(hipSt
     // it holds nothing: 2^20 rows of 64 in 8 lanes 4112, in 64 665; 2^18 of 256
     // in 32 lanes 3981, in 64 2319.
     // Workgroups enough for every row, up to a bound past which they take
-    // several (a launch holds less than 2^32 threads).
+    // several (a launch holds less than 2^32 threads; and a row a workgroup
+    // spends a fortieth of its time on starting one: 65536 x 4096 452 us, 440 in
+    // 2^14 of them).
     auto go = [&](auto kernel, int lanes) {
         const int per = lanes < 256 ? 256 / lanes : 1, threads = lanes < 256 ? 256 : lanes;
         const int blocks = (a.rows - 1) / per + 1;
-        enqueue(kernel, dim3(blocks < (1 << 20) ? blocks : 1 << 20), dim3(threads), 0, s, a);
+        const int most = lanes < 256 ? 1 << 20 : 1 << 14;
+        enqueue(kernel, dim3(blocks < most ? blocks : most), dim3(threads), 0, s, a);
         return hipGetLastError();
     };
 #define ROWS(L, G) return go(row_codes_kernel<X, R, NORM, L, G>, L)
