@@ -97,3 +97,55 @@ def test_a_plan_after_its_context(runtime):
         ctx.rms_norm(q[0], q[0, 0], 1e-6, out=out[0])
     assert e.value.code == S.TURBO_E_INVALID_HANDLE
     plan.close()
+
+
+def test_calls_at_once_from_threads(context):
+    """One plan and one context, every thread on a stream of its own with its own arrays, or waiting on the
+    context's: each gets what it gets alone."""
+    import threading
+    plan = context.cross_plan((3, 1), (2100, 700), 4, 2, 64, torch.float16)
+    assert plan.workspace_bytes > 0
+    kv = torch.randn(2800, 2, 2, 64, generator=torch.Generator().manual_seed(0)).half().cuda()
+    w = torch.randint(-127, 128, (80, 256), generator=torch.Generator().manual_seed(1), dtype=torch.int8).cuda()
+    ones = torch.ones(256, device="cuda")
+
+    def arrays(seed):
+        q = torch.randn(4, 4, 64, generator=torch.Generator().manual_seed(seed)).half().cuda()
+        return dict(q=q, o=torch.zeros_like(q), c=torch.zeros(4, 256, dtype=torch.int8, device="cuda"),
+                    s=torch.zeros(4, device="cuda"), y=torch.zeros(4, 80, device="cuda"),
+                    ws=torch.empty(plan.workspace_bytes, dtype=torch.uint8, device="cuda"))
+
+    def layer(a, stream):
+        plan.run(a["q"], kv[:, 0], kv[:, 1], a["o"], workspace=a["ws"], stream=stream)
+        context.rms_norm(a["o"].view(4, 256), ones, 1e-6, codes=a["c"], scales=a["s"], stream=stream)
+        context.linear_i8(a["c"], a["s"], w, ones[:80], a["y"], stream=stream)
+    sets = [arrays(10 + i) for i in range(6)]
+    torch.cuda.synchronize()
+    want = []
+    for a in sets:
+        layer(a, None)
+        want.append({k: a[k].clone() for k in "ocsy"})
+    torch.cuda.synchronize()
+    failures = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream() if i % 3 else None
+            for _ in range(20):
+                if stream is None:
+                    layer(sets[i], None)
+                else:
+                    layer(sets[i], stream.cuda_stream)
+            if stream is not None:
+                stream.synchronize()
+            assert all(torch.equal(sets[i][k], want[i][k]) for k in "ocsy")
+        except Exception as e:   # noqa: BLE001
+            failures.append((i, e))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failures, failures
+    plan.close()

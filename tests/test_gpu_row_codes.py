@@ -322,3 +322,18 @@ def test_more_rows_than_a_launch_s_workgroups_take_at_once(context):
     assert torch.equal(q[:64].cpu(), torch.from_numpy(want).to(torch.int8))
     assert torch.equal(q, q[:64].repeat((rows + 63) // 64, 1)[:rows])
     assert torch.equal(k, k[:64].repeat((rows + 63) // 64)[:rows])
+
+
+@pytest.mark.parametrize("cols", [2050, 4096, 9000])
+def test_wide_rows_that_share_a_workgroup(context, cols):
+    # (61 rows over and over: a workgroup's rows, 2^14 apart, are others.)
+    rows, part = (1 << 14) * 2 + 77, 61
+    x, r = _rows(1, part, cols, "bf16"), _rows(2, part, cols, "bf16")
+    weight = 1 + 0.3 * _rows(3, 1, cols, "f32", 0)[0]
+    total, y, c, rr = _want(x, weight, r, 1e-6)
+    many = lambda t: t.repeat(rows // part + 1, *[1] * (t.dim() - 1))[:rows]  # noqa: E731
+    s, o, q, k = _norm(context, many(x), weight, res=many(r), sum=True, out="f16")
+    _close(o[:part], y, "f16")
+    _check_codes(q[:part], k[:part], c, rr)
+    for got, want in ((s, total), (o, o[:part].clone()), (q, q[:part].clone()), (k, k[:part].clone())):
+        assert torch.equal(got, many(want))
