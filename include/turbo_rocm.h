@@ -261,8 +261,8 @@ void turbo_rocm_cross_plan_release(void *plan);
  * entry is 0 is not live, and nothing of its key and value is used, whatever
  * they hold. A query with no live state has a zero output. scale finite in F32.
  * Scores, probabilities and sums are F32; 16-bit operands round a probability
- * once, to their type, for the product with V, and the output once. An
- * infinite or undefined score gives what the formula gives: a NaN. workspace:
+ * for the product with V, to their type or, in calls of few rows, to the sum of
+ * two numbers of it, and the output once. An infinite or undefined score gives what the formula gives: a NaN. workspace:
  * `workspace_bytes` of the context's device, 16-byte aligned, at least the
  * plan's, for this call alone until it has finished (two graphs that may run
  * at once need one each). It holds nothing between calls. out may not overlap an

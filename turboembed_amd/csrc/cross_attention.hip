@@ -62,6 +62,19 @@ template <typename T> __device__ __forceinline__ typename Chunk<T>::vec read_chu
     return v;
 }
 
+// Of each of two weights (0 or more) a number of T one to two of its steps
+// below, so that what is left of it is at least a step: both terms of a weight
+// are positive, and an infinite value stays what its product gives.
+template <typename T>
+__device__ __forceinline__ auto below(float w0, float w1) {
+    typedef unsigned short bits2 __attribute__((ext_vector_type(2)));
+    typedef T two __attribute__((ext_vector_type(2)));
+    bits2 b;
+    if constexpr (std::is_same<T, _Float16>::value) b = __builtin_bit_cast(bits2, __builtin_amdgcn_cvt_pkrtz(w0, w1));
+    else b = bits2{(unsigned short)(__float_as_uint(w0) >> 16), (unsigned short)(__float_as_uint(w1) >> 16)};
+    return __builtin_bit_cast(two, __builtin_elementwise_sub_sat(b, bits2{1, 1}));
+}
+
 // Where a part of `rows` rows lies in the workspace.
 __device__ __forceinline__ float *part_of(const CrossArgs &a, int part) {
     return a.ws + (uint64_t)part * cross_part_floats(a.most_rows, a.width);
@@ -90,7 +103,16 @@ template <typename T, int DP, int WAVES, bool DIRECT> struct CrossTile {
     }
 };
 
-template <typename T, int DP, int WAVES, bool DIRECT>
+// TWO: 16-bit weights are two numbers of T each for the product with V, not one.
+// That is so where no item has more than a wave's rows: the keys' and values'
+// bytes bound it, and the second product mostly hides behind them (48 x 1 by
+// 200-4096, BF16: heads of 64 93.0 us for 92.4, of 128 165.7 for 162.7; 64 x 4
+// by 1024, four heads of 80 a key head, where one wave computes and three
+// load, 31.8 for 27.6; the first's error 2.3e-3 with one, 1.7e-3, the output's
+// own rounding, with two). Where four waves compute, the vector instructions
+// bound it: two numbers would take 407 us for 290 (8 x 1024-2048 by 2048-8192,
+// F16; errors 2.1e-4 and 2.9e-4), so a weight is rounded once.
+template <typename T, int DP, int WAVES, bool DIRECT, bool TWO>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(CrossTile<T, DP, WAVES, DIRECT>::OCC)))
 cross_tiles(CrossArgs a) {
     using C = CrossTile<T, DP, WAVES, DIRECT>;
@@ -255,9 +277,18 @@ cross_tiles(CrossArgs a) {
             const int g = lane >> 4, n = lane & 15, key = 4 * (g >> 1) + (n >> 2);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                frag f;
+                frag f, rest, vt[DT];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = from_f32<T>(weight(8 * j + e));
+                for (int e = 0; e < 8; e += 2) {
+                    const float w0 = weight(8 * j + e), w1 = weight(8 * j + e + 1);
+                    if constexpr (TWO) {
+                        const auto hi = below<T>(w0, w1);
+                        f[e] = hi[0], f[e + 1] = hi[1];
+                        rest[e] = from_f32<T>(w0 - to_f32(hi[0])), rest[e + 1] = from_f32<T>(w1 - to_f32(hi[1]));
+                    } else {
+                        f[e] = from_f32<T>(w0), f[e + 1] = from_f32<T>(w1);
+                    }
+                }
 #pragma unroll
                 for (int t = 0; t < DT; ++t) {
                     const int c = 4 * t + 2 * (g & 1) + ((n >> 1) & 1);
@@ -269,8 +300,12 @@ cross_tiles(CrossArgs a) {
                     } v;
                     v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(16 * j + key));
                     v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(at(16 * j + 8 + key));
-                    o[t] = Mma<T>::run(__builtin_bit_cast(frag, v), f, o[t]);
+                    vt[t] = __builtin_bit_cast(frag, v);
+                    o[t] = Mma<T>::run(vt[t], f, o[t]);
                 }
+                if constexpr (TWO)
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) o[t] = Mma<T>::run(vt[t], rest, o[t]);
             }
         }
     };
@@ -426,10 +461,12 @@ template <typename T> __global__ void __launch_bounds__(256) cross_join(CrossArg
 
 template <typename T, bool DIRECT> static hipError_t launch_cross(hipStream_t s, const CrossArgs &a) {
     const dim3 grid(a.n_items);
-#define WAVES(DP, W) enqueue(cross_tiles<T, DP, W, DIRECT>, grid, dim3(64 * W), CrossTile<T, DP, W, DIRECT>::LDS, s, a)
-#define TILES(DP)                       \
-    if (a.part_rows == 32) WAVES(DP, 1); \
-    else WAVES(DP, 4)
+    constexpr bool F32 = std::is_same<T, float>::value;
+#define WAVES(DP, W, TWO) enqueue(cross_tiles<T, DP, W, DIRECT, TWO>, grid, dim3(64 * W), CrossTile<T, DP, W, DIRECT>::LDS, s, a)
+#define TILES(DP)                                   \
+    if (a.part_rows == 32) WAVES(DP, 1, !F32);      \
+    else if (a.one_wave) WAVES(DP, 4, !F32);        \
+    else WAVES(DP, 4, false)
     if (a.width <= 32) { TILES(32); }
     else if (a.width <= 64) { TILES(64); }
     else if (a.width <= 96) { TILES(96); }

@@ -286,6 +286,7 @@ struct CrossPlan {
     uint32_t dtype = 0, heads = 0, kv = 0, width = 0;
     uint64_t tokens = 0, states = 0, workspace = 0;
     int items = 0, joins = 0, part_rows = 0, most_rows = 0;
+    bool one_wave = true;
     uint64_t parts = 0;
     DevPtr work;   // the items, then the joins
 };
@@ -466,6 +467,7 @@ CrossPlan *cross_plan_create(Context *c, const turbo_rocm_cross_desc *d) {
     std::vector<CrossItem> items;
     std::vector<CrossJoin> joins;
     lay_out(*d, items, joins, p->part_rows, p->parts);
+    for (const CrossItem &it : items) p->one_wave &= it.rows <= 32;
     for (const CrossJoin &j : joins) p->most_rows = std::max(p->most_rows, j.rows);
     p->workspace = p->parts * cross_part_floats(p->most_rows, (int)d->width) * 4;
     p->items = (int)items.size(), p->joins = (int)joins.size();
@@ -512,6 +514,7 @@ void cross_run(CrossPlan *p, const turbo_rocm_cross_attention_call *call) {
         a.os[i] = call->out.stride[i];
     a.dt = dt_of(p->dtype);
     a.n_items = p->items, a.n_joins = p->joins, a.part_rows = p->part_rows, a.most_rows = p->most_rows;
+    a.one_wave = p->one_wave;
     a.share = (int)(p->heads / p->kv), a.width = (int)p->width;
     a.scale = base2(call->scale);
     a.turn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f;

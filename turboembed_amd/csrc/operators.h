@@ -71,6 +71,7 @@ struct CrossArgs {
     uint64_t qs[2], ks[2], vs[2], os[2];   // strides of tokens and heads, elements
     Dt dt;
     int n_items, n_joins, part_rows, most_rows, share, width;   // (most_rows: of one join)
+    bool one_wave;           // no item has more than 32 rows, a wave's
     float scale;             // of a score, times log2(e); positive...
     float turn;              // ...with 1, -1 or 0 times q
 };
