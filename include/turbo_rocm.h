@@ -175,8 +175,8 @@ typedef struct turbo_rocm_tensor {
  *   sum [rows, cols], the residual's type: v (only with a residual). It may
  *     be the residual itself, or x where the types are equal: same address
  *     and strides.
- *   out [rows, cols], F32, F16 or BF16: y, rounded once. It may be x, in the
- *     same way.
+ *   out [rows, cols], F32, F16 or BF16: y, rounded once (BF16 below F32's
+ *     smallest normal number: to F32 first). It may be x, in the same way.
  *   codes [rows, cols] I8 with scales [rows] F32: symmetric int8 codes of y's
  *     row before any rounding: scale = max|y| / 127 rounded to F32, code =
  *     the whole number nearest to 127 y / max|y|, ties to even, exactly. A row

@@ -337,3 +337,20 @@ def test_wide_rows_that_share_a_workgroup(context, cols):
     _check_codes(q[:part], k[:part], c, rr)
     for got, want in ((s, total), (o, o[:part].clone()), (q, q[:part].clone()), (k, k[:part].clone())):
         assert torch.equal(got, many(want))
+
+
+@pytest.mark.parametrize("cols", [40, 1024])
+@pytest.mark.parametrize("x, out", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "bf16")])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -16])
+def test_an_output_is_rounded_once(context, cols, x, out, size):
+    """At most half a step from the 64-bit result, its own roundings (some n 2^-53) aside: a rounding to F32 on the
+    way, which is up to 2^-25 more next to the middle of two steps, would show. The smaller size gives F16 outputs
+    below the smallest normal number."""
+    rows = (1 << 21) // cols
+    a = _rows(cols, rows, cols, x)
+    weight = (1 + 0.3 * _rows(4, 1, cols, "f32", 0)[0]) * size
+    y = _norm(context, a, weight, out=out, codes=False)[1].double().cpu().numpy()
+    want = _want(a, weight, None, 1e-6)[1]
+    info = torch.finfo(TYPES[out])
+    step = np.ldexp(info.eps, np.frexp(np.maximum(np.abs(want), info.tiny))[1] - 1)
+    assert (np.abs(y - want) <= step / 2 + np.abs(want) * 2.0 ** -40).all()
