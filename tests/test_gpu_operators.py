@@ -149,3 +149,39 @@ def test_calls_at_once_from_threads(context):
     torch.cuda.synchronize()
     assert not failures, failures
     plan.close()
+
+
+@pytest.mark.parametrize("waits", [False, True])
+def test_an_error_of_the_caller_s_own_is_the_caller_s(context, waits):
+    """A HIP call of the program's has failed on this thread, and nobody has asked why yet: an operator after it says
+    how its own launches went, and leaves the program its error."""
+    lib = T.library()
+    x, w = torch.randn(3, 256, device="cuda"), torch.ones(256, device="cuda")
+    y, c, s = torch.zeros(3, 256, device="cuda"), torch.zeros(3, 256, dtype=torch.int8, device="cuda"), torch.zeros(3, device="cuda")
+    w8, o = torch.ones(40, 256, dtype=torch.int8, device="cuda"), torch.zeros(3, 40, device="cuda")
+    k = torch.randn(2000, 4, 64, device="cuda")
+    a = torch.zeros(3, 4, 64, device="cuda")
+    plan = context.cross_plan((3,), (2000,), 4, 4, 64, torch.float32)
+    assert plan.workspace_bytes > 0     # (two launches)
+    ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device="cuda")
+    stream = None if waits else torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+
+    def calls():
+        context.rms_norm(x, w, 1e-6, out=y, stream=stream)
+        context.quantize_tokens(x, c, s, stream=stream)
+        context.linear_i8(c, s, w8, w[:40], o, stream=stream)
+        plan.run(x.view(3, 4, 64), k, k, a, workspace=ws, stream=stream)
+    try:
+        wrong = lib.hipSetDevice(4096)
+        assert wrong != 0 and lib.hipPeekAtLastError() == wrong
+        calls()
+        assert lib.hipPeekAtLastError() == wrong
+    finally:
+        lib.hipGetLastError()
+    torch.cuda.synchronize()
+    got = [t.clone() for t in (y, c, s, o, a)]
+    calls()
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, t) and (g != 0).any() for g, t in zip(got, (y, c, s, o, a)))
+    plan.close()

@@ -462,7 +462,9 @@ template <typename T> __global__ void __launch_bounds__(256) cross_join(CrossArg
 template <typename T, bool DIRECT> static hipError_t launch_cross(hipStream_t s, const CrossArgs &a) {
     const dim3 grid(a.n_items);
     constexpr bool F32 = std::is_same<T, float>::value;
-#define WAVES(DP, W, TWO) enqueue(cross_tiles<T, DP, W, DIRECT, TWO>, grid, dim3(64 * W), CrossTile<T, DP, W, DIRECT>::LDS, s, a)
+    hipError_t e;
+#define WAVES(DP, W, TWO) \
+    e = enqueue(cross_tiles<T, DP, W, DIRECT, TWO>, grid, dim3(64 * W), CrossTile<T, DP, W, DIRECT>::LDS, s, a)
 #define TILES(DP)                                   \
     if (a.part_rows == 32) WAVES(DP, 1, !F32);      \
     else if (a.one_wave) WAVES(DP, 4, !F32);        \
@@ -473,11 +475,9 @@ template <typename T, bool DIRECT> static hipError_t launch_cross(hipStream_t s,
     else { TILES(128); }
 #undef TILES
 #undef WAVES
-    if (a.n_joins) {
-        const int waves = a.most_rows < 4 ? a.most_rows : 4;
-        enqueue(cross_join<T>, dim3(a.n_joins, (a.most_rows + 2 * waves - 1) / (2 * waves)), dim3(64 * waves), 0, s, a);
-    }
-    return hipGetLastError();
+    if (e != hipSuccess || a.n_joins == 0) return e;
+    const int waves = a.most_rows < 4 ? a.most_rows : 4;
+    return enqueue(cross_join<T>, dim3(a.n_joins, (a.most_rows + 2 * waves - 1) / (2 * waves)), dim3(64 * waves), 0, s, a);
 }
 
 hipError_t cross_attention(hipStream_t s, const CrossArgs &a) {

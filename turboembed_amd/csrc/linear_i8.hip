@@ -348,10 +348,9 @@ template <int BM, int BN, int WM, int WN> static hipError_t launch_tiles(hipStre
     const int gn = (a.n - 1) / BN + 1, gm = (a.m - 1) / BM + 1;
     const dim3 grid((uint32_t)gn * gm), block(64 * WM * WN);
     constexpr int lds = 2 * (BM + BN) * 128;
-    if (direct) enqueue(linear_i8_tiles<BM, BN, WM, WN, true>, grid, block, lds, s, a, gn);
-    else if constexpr (BM < 256) enqueue(linear_i8_tiles<BM, BN, WM, WN, false>, grid, block, lds, s, a, gn);
-    else return hipErrorInvalidValue;
-    return hipGetLastError();
+    if (direct) return enqueue(linear_i8_tiles<BM, BN, WM, WN, true>, grid, block, lds, s, a, gn);
+    if constexpr (BM < 256) return enqueue(linear_i8_tiles<BM, BN, WM, WN, false>, grid, block, lds, s, a, gn);
+    return hipErrorInvalidValue;
 }
 
 template <int MT> static hipError_t launch_rows(hipStream_t s, const LinearArgs &a) {
@@ -359,16 +358,14 @@ template <int MT> static hipError_t launch_rows(hipStream_t s, const LinearArgs 
     const uint64_t blocks = ((uint64_t)(a.n - 1) / 16 + 1) * ((a.m - 1) / (16 * MT) + 1);
     // (A launch holds less than 2^32 threads; past a bound workgroups take several blocks.)
     const dim3 grid((uint32_t)(blocks < (1 << 16) ? blocks : 1 << 16));
-    enqueue(linear_i8_rows<WAVES, MT>, grid, dim3(64 * WAVES), 0, s, a, blocks);
-    return hipGetLastError();
+    return enqueue(linear_i8_rows<WAVES, MT>, grid, dim3(64 * WAVES), 0, s, a, blocks);
 }
 
 hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
     if (a.m <= 0 || a.n <= 0) return hipSuccess;
     if (a.k < 16) {
         const uint64_t blocks = ((uint64_t)a.m * a.n + 255) / 256;
-        enqueue(linear_i8_narrow, dim3((uint32_t)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, s, a);
-        return hipGetLastError();
+        return enqueue(linear_i8_narrow, dim3((uint32_t)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, s, a);
     }
     // A launch holds less than 2^32 threads: a product of more than 2^22 of the
     // smallest tiles goes by halves.

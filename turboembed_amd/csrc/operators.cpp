@@ -168,8 +168,10 @@ template <class Call, class Launch> void run_call(Context *c, const Call *call, 
         return;
     }
     std::lock_guard<std::recursive_mutex> g(c->lock);
-    check(launch(c->stream), what);
-    check(hipStreamSynchronize(c->stream), what);
+    // (Waited for even where a launch failed: one before it may be running.)
+    const hipError_t launched = launch(c->stream), waited = hipStreamSynchronize(c->stream);
+    check(launched, what);
+    check(waited, what);
 }
 
 void *address(const Tensor &t) { return t.ndim == 0 || empty(t) ? nullptr : t.data; }

@@ -253,8 +253,7 @@ template <typename X, typename R, bool NORM> static hipError_t launch_rows(hipSt
         const int per = lanes < 256 ? 256 / lanes : 1, threads = lanes < 256 ? 256 : lanes;
         const int blocks = (a.rows - 1) / per + 1;
         const int most = lanes < 256 ? 1 << 20 : 1 << 14;
-        enqueue(kernel, dim3(blocks < most ? blocks : most), dim3(threads), 0, s, a);
-        return hipGetLastError();
+        return enqueue(kernel, dim3(blocks < most ? blocks : most), dim3(threads), 0, s, a);
     };
 #define ROWS(L, G) return go(row_codes_kernel<X, R, NORM, L, G>, L)
     if (a.cols <= 64) ROWS(8, 1);
