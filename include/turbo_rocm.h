@@ -262,11 +262,14 @@ void turbo_rocm_cross_plan_release(void *plan);
  * they hold. A query with no live state has a zero output. scale finite in F32.
  * Scores, probabilities and sums are F32; 16-bit operands round a probability
  * for the product with V, to their type or, in calls of few rows, to the sum of
- * two numbers of it, and the output once. An infinite or undefined score gives what the formula gives: a NaN. workspace:
- * `workspace_bytes` of the context's device, 16-byte aligned, at least the
- * plan's, for this call alone until it has finished (two graphs that may run
- * at once need one each). It holds nothing between calls. out may not overlap an
- * input or the workspace. */
+ * two numbers of it, and the output once. Values are summed with weights of at
+ * most 1 (256 for F16) and divided at the end: outputs are finite where the
+ * largest |v| times the number of live states is, in F32. A score of plus
+ * infinity or one that is undefined gives what the formula gives, a NaN; one of
+ * minus infinity weighs nothing. workspace: `workspace_bytes` of the context's
+ * device, 16-byte aligned, at least the plan's, for this call alone until it has
+ * finished (two graphs that may run at once need one each). It holds nothing
+ * between calls. out may not overlap an input or the workspace. */
 typedef struct turbo_rocm_cross_attention_call {
     uint32_t struct_size;
     uint32_t flags;

@@ -72,3 +72,46 @@ def test_one_token_s_probabilities_are_two_numbers(context, t, d, spread):
     n = 48
     k_lens = [200 + 83 * i for i in range(n)]
     _run(context, [1] * n, k_lens, 16, 16, d, t, torch.finfo(TYPES[t]).eps ** 2, seed=d, spread=spread)
+
+
+@pytest.mark.parametrize("q_lens, k_lens", [((1,), (300,)), ((3, 40), (300, 250)), ((1,) * 40, (300,) * 40),
+                                            ((200,), (300,)), ((1,), (3000,))])
+@pytest.mark.parametrize("direct", [True, False])
+@pytest.mark.parametrize("low", ["first", "every other 32"])
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_values_as_large_as_their_sums_allow(context, t, low, direct, q_lens, k_lens):
+    """Some states' scores are 0, those of others after them just under 8 in base 2, so that weights reach 2^8 where the
+    maximum is that of the first; times the number of states the largest value is just what F32 holds.
+
+    All values are positive: a relative error. Scores are exact; weights are off by 2^-21, sums of n by n 2^-23, a
+    16-bit weight and the output by half a step each."""
+    d, heads, most = 64, 2, max(k_lens)
+    top = min(3.3e38 / most, 65000.0 if t == "f16" else 3e38)
+    g = torch.Generator().manual_seed(most)
+    step = d if direct else d + 1     # (rows that start at any element go another way)
+    wide = torch.zeros(2, sum(k_lens), heads * step, dtype=TYPES[t])
+    k, v = (wide[i].unflatten(1, (heads, step))[..., :d] for i in range(2))
+    at = 0
+    for n in k_lens:
+        j = torch.arange(n)
+        k[at:at + n, :, 0] = torch.where(j >= 70 if low == "first" else j % 64 >= 32, 7.875, 0.0)[:, None].to(k.dtype)
+        at += n
+    v.copy_(top * (0.25 + 0.75 * torch.rand(sum(k_lens), heads, d, generator=g).double()))
+    wide = wide.cuda()
+    k, v = (wide[i].unflatten(1, (heads, step))[..., :d] for i in range(2))
+    q = torch.zeros(sum(q_lens), heads, d, dtype=TYPES[t], device="cuda")
+    q[..., 0] = 1
+    out = torch.empty_like(q)
+    plan = context.cross_plan(q_lens, k_lens, heads, heads, d, TYPES[t])
+    ws = torch.full((plan.workspace_bytes,), 0xff, dtype=torch.uint8, device="cuda")
+    plan.run(q, k, v, out, scale=0.6931471805599453, workspace=ws, stream=_stream())
+    plan.close()
+    half = torch.finfo(TYPES[t]).eps / 2
+    qat = kat = 0
+    for nq, nk in zip(q_lens, k_lens):
+        p = torch.softmax(k[kat:kat + nk, :, 0].double() * 0.6931471805599453, 0)
+        want = (p[..., None] * v[kat:kat + nk].double()).sum(0)
+        o = out[qat:qat + nq].double()
+        qat, kat = qat + nq, kat + nk
+        tol = want * (2.0 ** -20 + nk * 2.0 ** -23 + half + (0 if t == "f32" else half)) * 1.01
+        assert ((o - want).abs() <= tol).all()

@@ -10,9 +10,10 @@
 // against V's columns for the same keys in that order (16-bit values by LDS
 // reads that transpose, F32 values one by one).
 //
-// The softmax is the running one, in base 2 and F32; its maximum moves only
-// when a score passes it by more than 2^8, so most tiles rescale nothing. The
-// scale is positive here (the launcher turns q around for a negative one).
+// The softmax is the running one, in base 2 and F32, and most tiles rescale
+// nothing: what it takes for a row's maximum moves only when a score is 2^8
+// above the one that it was set by. The scale is positive here (the launcher
+// turns q around for a negative one).
 //
 // One token a sequence is bound by the keys' and values' bytes: 48 by 200 to
 // 4096 states, 16 heads of 64, BF16, take 92 us with the join (4.6 TB/s). Long
@@ -120,7 +121,11 @@ cross_tiles(CrossArgs a) {
     constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR, DT = DP / 32;
     constexpr int E = Chunk<T>::N, NL = KB * CPR / 64 / WAVES;
     static_assert(NL * 64 * WAVES == KB * CPR, "whole loads a wave");
-    constexpr float LAG = 8.0f;
+    // m is LEAD above the maximum (base 2) that it was set by, and is set again
+    // by one that is LAG above that. With a LEAD of LAG weights are 1 at most, so
+    // that values of F32's size add up to finite sums. F16's need no such room,
+    // and its weights have no range to give away: there they reach 2^LAG.
+    constexpr float LAG = 8.0f, LEAD = std::is_same<T, _Float16>::value ? 0.0f : LAG;
     constexpr uint64_t FULL = KB == 64 ? ~0ull : 0xffffffffull;
     typedef typename Chunk<T>::vec vec;
     typedef typename Mma<T>::frag frag;
@@ -309,9 +314,9 @@ cross_tiles(CrossArgs a) {
             }
         }
     };
-    const auto raise = [&](float mx) {   // the maximum so far, where scores pass it by LAG
-        if (__ballot(mx > m + LAG) == 0) return;
-        const float mn = fmaxf(m, mx);
+    const auto raise = [&](float mx) {   // m, for scores of up to mx
+        if (__ballot(mx > m + (LAG - LEAD)) == 0) return;
+        const float mn = fmaxf(m, mx + LEAD);
         // (Equal: both infinite, of one sign.)
         const float f = __builtin_amdgcn_exp2f(m == mn ? 0.0f : m - mn);
 #pragma unroll
