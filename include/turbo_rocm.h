@@ -299,6 +299,14 @@ int32_t turbo_rocm_cross_check(const turbo_rocm_cross_desc *desc, const turbo_ro
  * core/cuda/backend.cpp:2430-2440, 3006-3010). Process-wide. */
 int32_t turbo_rocm_fail_variant(const char *name, turbo_error *err);
 
+/* Which kernel turbo_rocm_linear_i8 runs for [m, k] codes by [n, k] weights,
+ * without a device: 0 for k below 16, 1 to 4 for pieces of so many 16 rows, 64,
+ * 128 or 256 for tiles of that edge (a product of more than 2^22 64 x 64 tiles
+ * goes by halves, each with its own). aligned: both operands' addresses and
+ * strides, and k, are multiples of 16. */
+int32_t turbo_rocm_linear_i8_kernel(uint32_t m, uint32_t n, uint32_t k, uint32_t aligned, uint32_t *kernel,
+                                    turbo_error *err);
+
 /* The last run's packing, read back from the device: each row's first packed
  * token and length ([batch] each), each packed token's r * seq + p ([tokens]),
  * and the packed token count. */

@@ -224,3 +224,17 @@ def test_the_host_side_refuses_what_the_struct_cannot_say():
     host.is_cuda = False
     with pytest.raises(ValueError):
         _norm(x=host)
+
+
+def test_the_int8_products_of_the_tests_reach_every_kernel():
+    from test_gpu_linear_kernels import KERNELS
+    for kernel, aligned, m, n, k in KERNELS:
+        assert O.linear_i8_kernel(m, n, k, aligned) == kernel, (m, n, k)
+        assert not aligned or k % 16 == 0 or kernel == 0
+    # (Tiles of 256 need whole chunks; the others go both ways, tiles with few stages and with many.)
+    assert {(c[0], c[1]) for c in KERNELS} == {(i, a) for i in (0, 1, 2, 3, 4, 64, 128, 256) for a in (True, False)} - {(256, False)}
+    assert {(c[0], c[1]) for c in KERNELS if c[0] >= 64 and c[4] > 3 * 128} == {(64, True), (64, False), (128, True),
+                                                                                (128, False), (256, True)}
+    for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 131072), (1 << 31, 1, 1)):
+        with pytest.raises(T.TurboError):
+            O.linear_i8_kernel(*bad, True)

@@ -361,6 +361,36 @@ template <int MT> static hipError_t launch_rows(hipStream_t s, const LinearArgs 
     return enqueue(linear_i8_rows<WAVES, MT>, grid, dim3(64 * WAVES), 0, s, a, blocks);
 }
 
+int linear_i8_kernel(int m, int n, int k, bool aligned) {
+    // By the estimated time in us, fitted to 52 shapes of 1 to 30000 rows, N of
+    // 100 to 30000 and K of 32 to 8192 (its choice is the fastest measured or
+    // within 10% of it). What a compute unit reads sets the pace: 36
+    // KB/us of 16-row pieces and 0.4 us for each one's sums, or a stage of a tile
+    // in 0.25 to 1.75 us (64 x 64: 16 KB; 128 x 128: 32 KB, slower with every
+    // unit at work; 256 x 256: 64 KB) and its start and end.
+    // us measured, rows kernel / 64 / 128 / 256: 48 x 1024 x 4096 6.6, 11.3,
+    // 23.7, 51; 256 x 1024 x 1024 6.1, 5.2, 10.0, 19; 2048 x 4096 x 1024 -,
+    // 18.8, 16.2, 21.9; 6532 x 7168 x 64 312, 39, 42, 33.
+    const double stages = (k + 127) / 128;
+    const auto blocks = [&](double bm, double bn) { return std::ceil(m / bm) * std::ceil(n / bn); };
+    const auto rounds = [](double n) { return std::ceil(n / 256); };
+    double least = INFINITY;
+    int best = 0;
+    const auto offer = [&](int which, double time) {
+        if (time < least) least = time, best = which;
+    };
+    for (int mt = 1; mt <= 4; ++mt)
+        if (m > 16 * (mt - 1)) {
+            const double n = blocks(16.0 * mt, 16);
+            offer(mt, rounds(n) * k * (1 + mt) * 16 / 36000 + n / 256 * mt * 0.4);
+        }
+    offer(64, std::fmax(1, blocks(64, 64) / 256) * (stages * 0.25 + 0.8));
+    const double n128 = blocks(128, 128);
+    offer(128, rounds(n128) * (stages * (n128 < 256 ? 0.63 : 0.83) + 4));
+    if (aligned) offer(256, rounds(blocks(256, 256)) * (stages * 1.75 + 8));   // (no registers to hold a stage)
+    return best;
+}
+
 hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
     if (a.m <= 0 || a.n <= 0) return hipSuccess;
     if (a.k < 16) {
@@ -387,33 +417,7 @@ hipError_t linear_i8(hipStream_t s, const LinearArgs &a) {
     }
     const auto whole = [](const void *p, uint64_t ld) { return (reinterpret_cast<uintptr_t>(p) | ld) % 16 == 0; };
     const bool direct = whole(a.a, a.lda) && whole(a.w, a.ldw) && a.k % 16 == 0;
-    // The kernel by its estimated time in us, fitted to 52 shapes of 1 to 30000
-    // rows, N of 100 to 30000 and K of 32 to 8192 (its choice is the fastest
-    // measured or within 10% of it). What a compute unit reads sets the pace: 36
-    // KB/us of 16-row pieces and 0.4 us for each one's sums, or a stage of a tile
-    // in 0.25 to 1.75 us (64 x 64: 16 KB; 128 x 128: 32 KB, slower with every
-    // unit at work; 256 x 256: 64 KB) and its start and end.
-    // us measured, rows kernel / 64 / 128 / 256: 48 x 1024 x 4096 6.6, 11.3,
-    // 23.7, 51; 256 x 1024 x 1024 6.1, 5.2, 10.0, 19; 2048 x 4096 x 1024 -,
-    // 18.8, 16.2, 21.9; 6532 x 7168 x 64 312, 39, 42, 33.
-    const double stages = (a.k + 127) / 128;
-    const auto blocks = [&](double bm, double bn) { return std::ceil(a.m / bm) * std::ceil(a.n / bn); };
-    const auto rounds = [](double n) { return std::ceil(n / 256); };
-    double least = INFINITY;
-    int best = 0;
-    const auto offer = [&](int which, double time) {
-        if (time < least) least = time, best = which;
-    };
-    for (int mt = 1; mt <= 4; ++mt)
-        if (a.m > 16 * (mt - 1)) {
-            const double n = blocks(16.0 * mt, 16);
-            offer(mt, rounds(n) * a.k * (1 + mt) * 16 / 36000 + n / 256 * mt * 0.4);
-        }
-    offer(64, std::fmax(1, blocks(64, 64) / 256) * (stages * 0.25 + 0.8));
-    const double n128 = blocks(128, 128);
-    offer(128, rounds(n128) * (stages * (n128 < 256 ? 0.63 : 0.83) + 4));
-    if (direct) offer(256, rounds(blocks(256, 256)) * (stages * 1.75 + 8));   // (no registers to hold a stage)
-    switch (best) {
+    switch (linear_i8_kernel(a.m, a.n, a.k, direct)) {
     case 1: return launch_rows<1>(s, a);
     case 2: return launch_rows<2>(s, a);
     case 3: return launch_rows<3>(s, a);

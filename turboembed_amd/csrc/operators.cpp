@@ -572,6 +572,17 @@ int32_t turbo_rocm_cross_check(const turbo_rocm_cross_desc *desc, const turbo_ro
     });
 }
 
+int32_t turbo_rocm_linear_i8_kernel(uint32_t m, uint32_t n, uint32_t k, uint32_t aligned, uint32_t *kernel,
+                                    turbo_error *err) {
+    return guarded(err, [&] {
+        if (!kernel) refuse(0, "nowhere to leave the kernel");
+        if (m == 0 || n == 0 || m > (uint32_t)INT32_MAX || n > (uint32_t)INT32_MAX || k > I8_INNER_MAX)
+            misshapen(0, "a product of " + std::to_string(m) + " x " + std::to_string(n) + " x " + std::to_string(k));
+        *kernel = k < 16 ? 0 : (uint32_t)linear_i8_kernel((int)m, (int)n, (int)k, aligned != 0);
+        return TURBO_OK;
+    });
+}
+
 int32_t turbo_rocm_rms_norm(void *ctx, const turbo_rocm_rms_norm_call *call, turbo_error *err) {
     return guarded(err, [&] {
         rms_norm(static_cast<Context *>(ctx), call);

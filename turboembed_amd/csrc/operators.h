@@ -40,6 +40,10 @@ struct LinearArgs {
     int m, n, k;
 };
 hipError_t linear_i8(hipStream_t s, const LinearArgs &a);
+// The kernel that linear_i8 takes for an inner width of 16 or more: 1 to 4,
+// pieces of so many 16 rows, or 64, 128 or 256, tiles of that edge. aligned:
+// operands of whole aligned 16-byte chunks.
+int linear_i8_kernel(int m, int n, int k, bool aligned);
 
 // Cross attention's work, as a plan holds it on the device. The rows of a
 // (sequence, key head) are its query tokens' heads that read the key head:

@@ -197,6 +197,14 @@ def check_cross(q_lens, k_lens, heads, kv_heads, width, dtype, q=None, k=None, v
     _call("turbo_rocm_cross_check", C.byref(d), packed)
 
 
+def linear_i8_kernel(m, n, k, aligned):
+    """The kernel of an int8 product (turbo_rocm_linear_i8_kernel); a test hook."""
+    from . import _ok
+    kernel, err = C.c_uint32(), S.new_error()
+    _ok(_lib().turbo_rocm_linear_i8_kernel(m, n, k, 1 if aligned else 0, C.byref(kernel), C.byref(err)), err)
+    return kernel.value
+
+
 class CrossPlan:
     """Cross attention of sequences of these lengths (turbo_rocm_cross_plan_create)."""
 
