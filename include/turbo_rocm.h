@@ -307,6 +307,11 @@ int32_t turbo_rocm_fail_variant(const char *name, turbo_error *err);
 int32_t turbo_rocm_linear_i8_kernel(uint32_t m, uint32_t n, uint32_t k, uint32_t aligned, uint32_t *kernel,
                                     turbo_error *err);
 
+/* How a cross attention plan of this description is cut, without a device: the
+ * most rows (query tokens' heads that read one key head) of a workgroup, 32 or
+ * 128, and the most states; a sequence of more states is joined from parts. */
+int32_t turbo_rocm_cross_cut(const turbo_rocm_cross_desc *desc, uint32_t *rows, uint64_t *states, turbo_error *err);
+
 /* The last run's packing, read back from the device: each row's first packed
  * token and length ([batch] each), each packed token's r * seq + p ([tokens]),
  * and the packed token count. */

@@ -238,3 +238,21 @@ def test_the_int8_products_of_the_tests_reach_every_kernel():
     for bad in ((0, 1, 1), (1, 0, 1), (1, 1, 131072), (1 << 31, 1, 1)):
         with pytest.raises(T.TurboError):
             O.linear_i8_kernel(*bad, True)
+
+
+def test_the_attentions_of_the_tests_reach_every_kernel():
+    from test_gpu_cross_kernels import KERNELS, lengths
+    seen, cuts = set(), set()
+    for half, rows, one_tile, joined, n, nq, most, kv, share, d in KERNELS:
+        k_lens = lengths(n, most)
+        r, states = O.cross_cut([nq] * n, k_lens, kv * share, kv, d, F16 if half else F32)
+        assert (r, max(k_lens) > states, nq * share <= 32) == (rows, joined, one_tile), (half, rows, n, nq, most, d)
+        # (One wave's kernel is the same for one row tile and for several; an F32 one for four waves too.)
+        seen.add((half, rows, one_tile if half and rows == 128 else None, (d + 31) // 32))
+        cuts.add((half, rows, one_tile, joined))
+    want = {(half, 32, None, w) for half in (True, False) for w in (1, 2, 3, 4)}
+    want |= {(True, 128, one, w) for one in (True, False) for w in (1, 2, 3, 4)} | {(False, 128, None, w) for w in (1, 2, 3, 4)}
+    assert seen == want
+    assert cuts == {(h, r, o, j) for h in (True, False) for r in (32, 128) for o in (True, False) for j in (True, False)}
+    with pytest.raises(T.TurboError):
+        O.cross_cut((1,), (1,), 3, 2, 64, F16)

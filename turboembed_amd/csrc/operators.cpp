@@ -583,6 +583,16 @@ int32_t turbo_rocm_linear_i8_kernel(uint32_t m, uint32_t n, uint32_t k, uint32_t
     });
 }
 
+int32_t turbo_rocm_cross_cut(const turbo_rocm_cross_desc *desc, uint32_t *rows, uint64_t *states, turbo_error *err) {
+    return guarded(err, [&] {
+        check_desc(desc);
+        if (!rows || !states) refuse(0, "nowhere to leave the cut");
+        const Cut cut = choose_cut(*desc);
+        *rows = (uint32_t)cut.rows, *states = cut.slice;
+        return TURBO_OK;
+    });
+}
+
 int32_t turbo_rocm_rms_norm(void *ctx, const turbo_rocm_rms_norm_call *call, turbo_error *err) {
     return guarded(err, [&] {
         rms_norm(static_cast<Context *>(ctx), call);

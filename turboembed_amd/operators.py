@@ -197,6 +197,15 @@ def check_cross(q_lens, k_lens, heads, kv_heads, width, dtype, q=None, k=None, v
     _call("turbo_rocm_cross_check", C.byref(d), packed)
 
 
+def cross_cut(q_lens, k_lens, heads, kv_heads, width, dtype):
+    """(rows, states) of a plan's largest workgroup (turbo_rocm_cross_cut); a test hook."""
+    from . import _ok
+    d = _cross_desc(q_lens, k_lens, heads, kv_heads, width, dtype)
+    rows, states, err = C.c_uint32(), C.c_uint64(), S.new_error()
+    _ok(_lib().turbo_rocm_cross_cut(C.byref(d), C.byref(rows), C.byref(states), C.byref(err)), err)
+    return rows.value, states.value
+
+
 def linear_i8_kernel(m, n, k, aligned):
     """The kernel of an int8 product (turbo_rocm_linear_i8_kernel); a test hook."""
     from . import _ok
