@@ -256,3 +256,10 @@ def test_the_attentions_of_the_tests_reach_every_kernel():
     assert cuts == {(h, r, o, j) for h in (True, False) for r in (32, 128) for o in (True, False) for j in (True, False)}
     with pytest.raises(T.TurboError):
         O.cross_cut((1,), (1,), 3, 2, 64, F16)
+
+
+def test_an_array_over_a_closed_buffer_is_refused():
+    class Closed:
+        t, h, nbytes = T.table(), None, 64
+    with pytest.raises(ValueError, match="closed"):
+        T.DeviceArray(Closed, (16,), F32)

@@ -53,6 +53,8 @@ class DeviceArray:
         self.strides = tuple(strides)
         if not 0 <= offset <= buffer.nbytes:
             raise ValueError(f"an array from byte {offset} of a buffer of {buffer.nbytes}")
+        if not buffer.h:
+            raise ValueError("an array of a buffer that is closed")
         h = S.turbo_native_handle()
         h.struct_size = C.sizeof(h)
         from . import _ok
