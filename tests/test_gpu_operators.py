@@ -185,3 +185,53 @@ def test_an_error_of_the_caller_s_own_is_the_caller_s(context, waits):
     torch.cuda.synchronize()
     assert all(torch.equal(g, t) and (g != 0).any() for g, t in zip(got, (y, c, s, o, a)))
     plan.close()
+
+
+def test_a_session_s_states_without_a_copy(context):
+    """A range for each token: the run's output is the tokens' states, read by the operators where it lies."""
+    import numpy as np
+    import small
+    desc = small.bert(seed=5, hidden=96, heads=3, inter=64)
+    model = context.load(desc)
+    s = model.session(3, 24, S.TURBO_PRECISION_EXACT, max_ranges=72)
+    with pytest.raises(T.TurboError) as e:
+        s.output()
+    assert e.value.code == S.TURBO_E_INVALID_STATE
+    ids = np.random.Generator(np.random.PCG64(1)).integers(3, desc.vocab_size - 1, size=(3, 24)).astype(np.int32)
+    lens = [24, 7, 15]
+    mask = (np.arange(24)[None] < np.array(lens)[:, None]).astype(np.int32)
+    s.write_ranges(ids, mask, [(r, i, i + 1) for r in range(3) for i in range(lens[r])], normalize=S.TURBO_NORMALIZE_NONE)
+    s.run()
+    states = s.output()
+    want = torch.from_numpy(s.hidden()).cuda()
+    assert states.shape == (46, 96) == tuple(want.shape)
+    new = lambda *z, t=torch.int8: torch.zeros(*z, dtype=t, device="cuda")  # noqa: E731
+    c, k, cw, kw = new(46, 96), new(46, t=torch.float32), new(46, 96), new(46, t=torch.float32)
+    at = torch.cuda.current_stream().cuda_stream
+    for stream in (None, at):
+        c.zero_()
+        torch.cuda.synchronize()
+        context.quantize_tokens(states, c, k, stream=stream)
+        context.quantize_tokens(want, cw, kw, stream=at)
+        torch.cuda.synchronize()
+        assert torch.equal(c, cw) and torch.equal(k, kw) and (k > 0).all()
+    # Attention of three tokens a row to its states, which are keys and values.
+    k3 = T.DeviceArray(states.buffer, (46, 3, 32), S.TURBO_DTYPE_F32)
+    plan = context.cross_plan([3, 3, 3], lens, 3, 3, 32, torch.float32)
+    q = torch.randn(9, 3, 32, device="cuda")
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+    ws = torch.empty(max(1, plan.workspace_bytes), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    plan.run(q, k3, k3, a, workspace=ws)
+    plan.run(q, want.view(46, 3, 32), want.view(46, 3, 32), b, workspace=ws)
+    assert torch.equal(a, b) and (a != 0).any()
+    plan.close()
+    # Rows that are written and have not run are not the output's.
+    s.write_tokens(ids, mask)
+    assert s.output().shape == (46, 96)
+    s.close()
+    with pytest.raises(ValueError, match="closed"):
+        context.quantize_tokens(states, c, k)
+    with pytest.raises(ValueError, match="closed"):
+        s.output()
+    model.close()

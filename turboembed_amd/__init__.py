@@ -440,7 +440,16 @@ class Session:
         err = S.new_error()
         _ok(self.t.session_run(self.h, C.byref(out), C.byref(err)), err)
         self.run_info = out
+        self._ran = self.n_out, self.od
         return out
+
+    def output(self):
+        """The last run's vectors where the run left them, as an array of the
+        operators on device memory: [n, output_dim] F32, with a range for each
+        token its states. They are there when run returns, until the next run."""
+        if self.run_info is None:
+            raise TurboError(S.TURBO_E_INVALID_STATE, 0, "the session has not run")
+        return DeviceArray(_Output(self), self._ran, S.TURBO_DTYPE_F32)
 
     def read(self):
         """The last run's vectors, [n, output_dim] F32, via buffer_read."""
@@ -562,6 +571,19 @@ class Session:
         if self.h:
             self.t.session_release(self.h)
             self.h = None
+
+
+class _Output:
+    """A session's output buffer, as DeviceArray takes one."""
+
+    def __init__(self, session):
+        self.session, self.t, self.ctx = session, session.t, session.model.ctx
+        n, width = session._ran
+        self.nbytes = n * width * 4
+
+    @property
+    def h(self):
+        return self.session.run_info.output if self.session.h else None
 
 
 _cache = None

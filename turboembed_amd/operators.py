@@ -40,7 +40,7 @@ def dtype_code(dtype):
 
 class DeviceArray:
     """An array in a buffer of the context's (Context.buffer: DEVICE, PINNED
-    or SHARED): shape, and strides in elements (row after row by default),
+    or SHARED; a session's output is one by Session.output): shape, and strides in elements (row after row by default),
     from `offset` bytes into it."""
 
     def __init__(self, buffer, shape, dtype, strides=None, offset=0):
