@@ -263,3 +263,13 @@ def test_an_array_over_a_closed_buffer_is_refused():
         t, h, nbytes = T.table(), None, 64
     with pytest.raises(ValueError, match="closed"):
         T.DeviceArray(Closed, (16,), F32)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(q_lens=((1 << 32) + 2, 0, 3)), dict(k_lens=(4, (1 << 33) + 5, 0)), dict(q_lens=(2, -1, 3)), dict(k_lens=(4, 5, -4)),
+    dict(heads=(1 << 32) + 6), dict(kv_heads=(1 << 32) + 2), dict(width=(1 << 32) + 40)])
+def test_a_plan_s_numbers_are_not_cut_to_32_bits(kw):
+    a = dict(dict(q_lens=(2, 0, 3), k_lens=(4, 5, 0), heads=6, kv_heads=2, width=40), **kw)
+    O.check_cross((2, 0, 3), (4, 5, 0), 6, 2, 40, F16)
+    with pytest.raises(ValueError):
+        O.check_cross(a["q_lens"], a["k_lens"], a["heads"], a["kv_heads"], a["width"], F16)

@@ -170,17 +170,27 @@ def linear_i8(ctx, codes, scales, weight, weight_scales, out, bias=None, stream=
                        *_tensor(weight_scales, on), *_tensor(bias, on), *_tensor(out, on)))
 
 
+def _u32(values, what):
+    # (ctypes would take a number's lowest 32 bits.)
+    for x in values:
+        if not 0 <= x < 1 << 32:
+            raise ValueError(f"{what} of {x}")
+    return values
+
+
 def _lengths(q_lens, k_lens):
     n = len(q_lens)
     if len(k_lens) != n:
         raise ValueError(f"{n} query lengths and {len(k_lens)} key lengths")
-    return n, (C.c_uint32 * max(1, n))(*q_lens), (C.c_uint32 * max(1, n))(*k_lens)
+    return (n, (C.c_uint32 * max(1, n))(*_u32(q_lens, "a query length")),
+            (C.c_uint32 * max(1, n))(*_u32(k_lens, "a key length")))
 
 
 def _cross_desc(q_lens, k_lens, heads, kv_heads, width, dtype):
     d = S.turbo_rocm_cross_desc()
     d.struct_size = C.sizeof(d)
-    d.dtype, d.heads, d.kv_heads, d.width = dtype_code(dtype), heads, kv_heads, width
+    d.dtype = dtype_code(dtype)
+    d.heads, d.kv_heads, d.width = _u32((heads, kv_heads, width), "heads or a width")
     d.batch, d.q_lens, d.k_lens = _lengths(q_lens, k_lens)
     return d
 
