@@ -208,7 +208,8 @@ int32_t turbo_rocm_quantize_tokens(void *ctx, const turbo_rocm_quantize_tokens_c
 /* turbo_rocm_linear_i8: out[m, n] = (sum_k codes[m, k] weight[n, k]) *
  * scales[m] * weight_scales[n] + bias[n], the sum exact in 32-bit integers
  * (inner width at most 131071, where the largest sum still fits), the rest in
- * F32, rounded once to out's type. codes [M, K] and weight [N, K] I8, scales
+ * F32 (the sum, its product with scales[m] and the multiply-add with the bias
+ * round there), rounded once to out's type. codes [M, K] and weight [N, K] I8, scales
  * [M], weight_scales [N] and bias [N] (optional) F32, out [M, N] F32, F16 or
  * BF16. K 0 gives the bias (or zeros, as an empty sum times the scales). out
  * may not overlap an input. */

@@ -16,10 +16,10 @@
 // turns q around for a negative one).
 //
 // One token a sequence is bound by the keys' and values' bytes: 48 by 200 to
-// 4096 states, 16 heads of 64, BF16, take 92 us with the join (4.6 TB/s). Long
+// 4096 states, 16 heads of 64, BF16, take 93 us with the join (4.5 TB/s). Long
 // F16 queries are bound by the softmax's vector instructions beside the
 // products: 8 x 1024-2048 tokens by 2048-8192 states, 16 heads of 64, take 289
-// us (820 TFLOP/s); heads of 128 in BF16 reach 875. F32 is bound by its matrix
+// us (815 TFLOP/s); 4 x 1024 by 4096 with 16 heads of 128 in BF16 137 (1000). F32 is bound by its matrix
 // instructions, 64 cycles each: a tile of 32 keys by 32 rows of 64 is 4096
 // cycles; 24 x 5-77 tokens by 33-500 states, 12 heads, take 33 us.
 // (Tiles of 32 keys where a wave is alone, so that more of them fit; of 64

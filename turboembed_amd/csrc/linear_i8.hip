@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(256) linear_i8_narrow(LinearArgs a) {
 // Bound by w's bytes, each read once, straight into the matrix instruction's
 // registers: a lane 16 bytes of a column's row, four lanes 64 consecutive ones.
 // The waves' sums meet in LDS. One row by 4096 x 4096 takes 5.7 us (2.9 TB/s,
-// a launch's start and end among it), 48 rows by 1024 x 4096 6.6.
+// a launch's start and end among it), 48 rows by 1024 x 4096 7.0.
 template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linear_i8_rows(LinearArgs a, uint64_t blocks) {
     __shared__ __attribute__((aligned(16))) i32x4 part[WAVES][MT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -146,12 +146,12 @@ template <int WAVES, int MT> __global__ void __launch_bounds__(64 * WAVES) linea
 // (Three and four stages were no faster: a compute unit reads some 20 to 27
 // bytes a clock, and the stages wait for that. A 256 x 256 tile asks for 32;
 // on random operands the chip's power holds the clock at 1.9 GHz besides:
-// 32768 x 4096 x 4096 takes 535 us (2.05 POP/s), 433 on zeros.)
+// 32768 x 4096 x 4096 takes 537 us (2.05 POP/s), 436 on zeros.)
 // LDS rows are 128 bytes, chunk c of row r at place c ^ (r / 2 % 8), so that
 // the 16 rows of a read's pass (256 bytes, two rows a bank round) lie in
 // different banks. DIRECT (16-byte aligned operands and strides, K a multiple
 // of 16): memory to LDS without registers; without it 1111 x 1001 x 1537 takes
-// 13.3 us, 7.4 at K = 1536.
+// 13.7 us, 8.1 at K = 1536.
 template <int BM, int BN, int WM, int WN, bool DIRECT>
 __global__ void __launch_bounds__(64 * WM * WN) linear_i8_tiles(LinearArgs a, int grid_n) {
     constexpr int WAVES = WM * WN, ROWS = BM + BN, STAGE = ROWS * 128;

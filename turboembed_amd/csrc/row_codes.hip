@@ -5,10 +5,11 @@
 // residual) are read once, everything else is made from the registers, and
 // the outputs are written once. The weight is read twice, from the caches.
 // Bound by those bytes: 4807 x 1023 F32 rows and their norm take 15.4 us (5.1
-// TB/s, a large copy's rate), 65536 x 1024 F16 rows to codes 42 (4.8), 65536 x
-// 4096 BF16 rows with a residual to codes 442 (4.25, as the norm alone does: a
+// TB/s, a large copy's rate), 65536 x 1024 F16 rows to codes 44.4 (4.5), 65536 x
+// 4096 BF16 rows with a residual to codes 443 (4.25, as the norm alone does: a
 // workgroup reads its row, exchanges sums and writes in turn). 16-bit rows that
-// no vector's alignment divides reach two thirds of that.
+// no vector's alignment divides reach two thirds of that (26214 x 2500 F16, the
+// same: 2.8; x 2504: 3.2).
 //
 // The codes are those of the definition, not of a rounded norm: code_i = the
 // whole number nearest to 127 y_i / max|y| = 127 c_i / max|c|, c = v w, as the
