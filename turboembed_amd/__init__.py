@@ -446,7 +446,8 @@ class Session:
     def output(self):
         """The last run's vectors where the run left them, as an array of the
         operators on device memory: [n, output_dim] F32, with a range for each
-        token its states. They are there when run returns, until the next run."""
+        token its states. They are there when run returns, until the next run
+        (or read_quantized, which leaves codes in their place)."""
         if self.run_info is None:
             raise TurboError(S.TURBO_E_INVALID_STATE, 0, "the session has not run")
         return DeviceArray(_Output(self), self._ran, S.TURBO_DTYPE_F32)

@@ -19,9 +19,10 @@
 // 4096 states, 16 heads of 64, BF16, take 93 us with the join (4.5 TB/s). Long
 // F16 queries are bound by the softmax's vector instructions beside the
 // products: 8 x 1024-2048 tokens by 2048-8192 states, 16 heads of 64, take 289
-// us (815 TFLOP/s); 4 x 1024 by 4096 with 16 heads of 128 in BF16 137 (1000). F32 is bound by its matrix
-// instructions, 64 cycles each: a tile of 32 keys by 32 rows of 64 is 4096
-// cycles; 24 x 5-77 tokens by 33-500 states, 12 heads, take 33 us.
+// us (815 TFLOP/s); 4 x 1024 by 4096, 16 heads of 128 in BF16, 137 (1000). F32
+// is bound by its matrix instructions, 64 cycles each: a tile of 32 keys by 32
+// rows of 64 is 4096 cycles; 24 x 5-77 tokens by 33-500 states, 12 heads, take
+// 33 us.
 // (Tiles of 32 keys where a wave is alone, so that more of them fit; of 64
 // where four share them, which halves the barriers.)
 #include <hip/hip_runtime.h>

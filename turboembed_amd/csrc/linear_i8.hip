@@ -364,10 +364,10 @@ template <int MT> static hipError_t launch_rows(hipStream_t s, const LinearArgs 
 int linear_i8_kernel(int m, int n, int k, bool aligned) {
     // By the estimated time in us, fitted to 52 shapes of 1 to 30000 rows, N of
     // 100 to 30000 and K of 32 to 8192 (its choice is the fastest measured or
-    // within 10% of it). What a compute unit reads sets the pace: 36
-    // KB/us of 16-row pieces and 0.4 us for each one's sums, or a stage of a tile
-    // in 0.25 to 1.75 us (64 x 64: 16 KB; 128 x 128: 32 KB, slower with every
-    // unit at work; 256 x 256: 64 KB) and its start and end.
+    // within 10% of it). What a compute unit reads sets the pace: 36 KB/us of
+    // 16-row pieces and 0.4 us for each one's sums, or a stage of a tile in 0.25
+    // to 1.75 us (64 x 64: 16 KB; 128 x 128: 32 KB, slower with every unit at
+    // work; 256 x 256: 64 KB) and its start and end.
     // us measured, rows kernel / 64 / 128 / 256: 48 x 1024 x 4096 6.6, 11.3,
     // 23.7, 51; 256 x 1024 x 1024 6.1, 5.2, 10.0, 19; 2048 x 4096 x 1024 -,
     // 18.8, 16.2, 21.9; 6532 x 7168 x 64 312, 39, 42, 33.
