@@ -119,8 +119,9 @@ int32_t turbo_rocm_buffer_quantize_static(void *buffer, uint32_t quantization, c
  * What a program needs to run layers of its own over a session's states
  * (taps, hidden states, imported embeddings): an RMS norm with the residual's
  * addition and int8 codes out, those codes of any rows, the int8 product on
- * codes and scales, and the attention of its tokens to an encoder's states of
- * another length. Like buffer_quantize they work on memory that the caller
+ * codes and scales, the attention of its tokens to an encoder's states of
+ * another length, and that of its tokens to those before them, over a prompt or
+ * a cache of states. Like buffer_quantize they work on memory that the caller
  * owns.
  *
  * Each takes a context and a call struct whose first field is struct_size
@@ -287,6 +288,116 @@ int32_t turbo_rocm_cross_attention(void *plan, const turbo_rocm_cross_attention_
  * without a device; call may be NULL. */
 int32_t turbo_rocm_cross_check(const turbo_rocm_cross_desc *desc, const turbo_rocm_cross_attention_call *call,
                                turbo_error *err);
+
+/* ---- A program's own tokens: attention over a prompt, and over a cache of states ----
+ *
+ * A program's layers keep the keys and values of its tokens (states) in a
+ * cache: `slots` rows of kv_heads heads of one width, of which each
+ * page_tokens consecutive ones are a page, of any number of sequences in any
+ * order. One set of arrays on the device says whose they are, for the write,
+ * the attention and the read of a step alike, so that a captured graph of them
+ * serves every step: only what the arrays hold changes.
+ *
+ *   starts [sequences + 1] I32: sequence i's new tokens are the call's rows
+ *     starts[i] .. starts[i + 1] - 1, m_i of them. It must not descend (else
+ *     which rows are whose is undefined, within the call's rows). Rows of no
+ *     sequence are left as they were.
+ *   lengths [sequences] I32: the states that the sequence has with its new
+ *     tokens, which are the last of them: row j of m_i is at position
+ *     lengths[i] - m_i + j. Below 0 is as 0.
+ *   pages [sequences, columns] I32: position p is in slot
+ *     pages[i, p / page_tokens] * page_tokens + p % page_tokens.
+ *
+ * A position below 0, past the last column, or on a page that the cache does
+ * not have (below 0, or slots / page_tokens or more) is no state: a token
+ * there is not written, its row is read back as zeros, and no row attends to
+ * it. These values are read by the kernels alone and may be anything: whatever
+ * they are, nothing outside of the arrays is touched. Sequences may share
+ * pages; where two new tokens of one call have the same slot, what it holds
+ * after a write is undefined. (A row's time is its positions': a length far
+ * past the states that there are costs what so many states would.)
+ *
+ * k and v [slots, kv_heads, width]: F32, F16 or BF16 as the call's rows, or I8
+ * with k_scales and v_scales [slots, kv_heads] F32, where a state's head is its
+ * codes times its scale. page_tokens 1 or more; any strides. At most 2^30
+ * slots, positions (columns * page_tokens) of a sequence, and rows times heads
+ * of a call (TURBO_E_CAPACITY). An error's field counts the arrays of the call
+ * and then these, in their order. reserved must be 0. */
+typedef struct turbo_rocm_cache {
+    turbo_rocm_tensor k, v, k_scales, v_scales, starts, lengths, pages;
+    uint32_t page_tokens;
+    uint32_t reserved;
+} turbo_rocm_cache;
+
+/* turbo_rocm_cache_write: the new tokens' k and v [tokens, kv_heads, width]
+ * (F32, F16 or BF16; widths 1 to 128) into their slots: as they are, bit for
+ * bit, or as the codes and scale (quantize_tokens) of each head's row. Other
+ * slots are left as they were. The cache's k, v and scales may not overlap each
+ * other or an input.
+ *
+ * turbo_rocm_cache_read: the way back, out of the new tokens' slots into k and v
+ * [tokens, kv_heads, width], of the states' type or, of I8 states, any: a copy, or
+ * codes times their scale rounded once. Rows without a slot become zeros. */
+typedef struct turbo_rocm_cache_rows_call {
+    uint32_t struct_size;
+    uint32_t flags;
+    void    *stream;
+    turbo_rocm_tensor k, v;
+    turbo_rocm_cache cache;
+} turbo_rocm_cache_rows_call;
+int32_t turbo_rocm_cache_write(void *ctx, const turbo_rocm_cache_rows_call *call, turbo_error *err);
+int32_t turbo_rocm_cache_read(void *ctx, const turbo_rocm_cache_rows_call *call, turbo_error *err);
+
+/* turbo_rocm_cache_attention: each new token's heads attend to the states of
+ * its sequence up to its own position, the last `window` of them (0: all):
+ *
+ *   out[t, h] = sum_p w_p v[p, h'],  w = softmax over p of scale * q[t, h] . k[p, h']
+ *
+ * h' = h / (heads / kv_heads), as in cross attention. q and out [tokens, heads,
+ * width] F32, F16 or BF16; one token of a sequence or thousands. A row that sees
+ * no state is zeros. What a state that a row does not see holds, its scale with
+ * it, changes nothing of that row, an infinity or a NaN included. Numerics,
+ * infinities and NaN are those of cross attention; int8 states are used
+ * unrounded (a probability times its value's scale is what is rounded).
+ *
+ * workspace: 16-byte aligned memory of the context's device, of the bytes that
+ * turbo_rocm_cache_workspace gives for at least as many tokens and sequences,
+ * for this call alone until it has finished; it holds nothing between calls.
+ * out may not overlap an input or the workspace. */
+typedef struct turbo_rocm_cache_attention_call {
+    uint32_t struct_size;
+    uint32_t flags;
+    void    *stream;
+    void    *workspace;
+    uint64_t workspace_bytes;
+    double   scale;
+    uint32_t window;
+    uint32_t reserved;
+    turbo_rocm_tensor q, out;
+    turbo_rocm_cache cache;
+} turbo_rocm_cache_attention_call;
+int32_t turbo_rocm_cache_attention(void *ctx, const turbo_rocm_cache_attention_call *call, turbo_error *err);
+
+/* The workspace of calls of up to so many tokens and sequences, without a
+ * device. dtype is that of q. */
+int32_t turbo_rocm_cache_workspace(uint64_t tokens, uint64_t sequences, uint32_t heads, uint32_t kv_heads,
+                                   uint32_t width, uint32_t dtype, uint64_t *bytes, turbo_error *err);
+
+/* turbo_rocm_prompt_attention: the same over the call's own rows, where no
+ * state came before them: token t of a sequence attends to the sequence's rows
+ * of k and v [tokens, kv_heads, width] up to its own, the last `window` of them
+ * (0: all). q and out [tokens, heads, width], all of one type; starts as above.
+ * out may not overlap an input. */
+typedef struct turbo_rocm_prompt_attention_call {
+    uint32_t struct_size;
+    uint32_t flags;
+    void    *stream;
+    double   scale;
+    uint32_t window;
+    uint32_t reserved;
+    turbo_rocm_tensor q, k, v, starts, out;
+} turbo_rocm_prompt_attention_call;
+int32_t turbo_rocm_prompt_attention(void *ctx, const turbo_rocm_prompt_attention_call *call, turbo_error *err);
 
 /* ---- Test and measurement hooks (no counterpart in the reference's seam; the
  * reference's CUDA backend keeps similar ones, core/src/cuda.rs:177-499) ---- */

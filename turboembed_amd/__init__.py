@@ -20,7 +20,7 @@ import numpy as np
 from . import operators
 from . import seam as S
 from .model import ModelDesc  # noqa: F401  (re-exported)
-from .operators import DeviceArray  # noqa: F401  (re-exported)
+from .operators import DeviceArray, StateCache  # noqa: F401  (re-exported)
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libturbo_rocm.so")
@@ -78,6 +78,11 @@ def library():
         "turbo_rocm_linear_i8": [P, C.c_char_p, E],
         "turbo_rocm_cross_plan_create": [P, C.POINTER(S.turbo_rocm_cross_desc), C.POINTER(C.c_uint64), C.POINTER(P), E],
         "turbo_rocm_cross_attention": [P, C.c_char_p, E],
+        "turbo_rocm_prompt_attention": [P, C.c_char_p, E],
+        "turbo_rocm_cache_write": [P, C.c_char_p, E],
+        "turbo_rocm_cache_read": [P, C.c_char_p, E],
+        "turbo_rocm_cache_attention": [P, C.c_char_p, E],
+        "turbo_rocm_cache_workspace": [C.c_uint64, C.c_uint64, u32, u32, u32, u32, C.POINTER(C.c_uint64), E],
         "turbo_rocm_linear_i8_kernel": [u32, u32, u32, u32, C.POINTER(u32), E],
         "turbo_rocm_cross_cut": [C.POINTER(S.turbo_rocm_cross_desc), C.POINTER(u32), C.POINTER(C.c_uint64), E],
         "turbo_rocm_cross_check": [C.POINTER(S.turbo_rocm_cross_desc), C.c_char_p, E],
@@ -180,6 +185,21 @@ class Context:
     def cross_plan(self, q_lens, k_lens, heads, kv_heads, width, dtype):
         """A CrossPlan: attention of sequences of q_lens tokens to k_lens states."""
         return operators.CrossPlan(self, q_lens, k_lens, heads, kv_heads, width, dtype)
+
+    def prompt_attention(self, q, k, v, starts, out, window=0, scale=None, stream=None):
+        operators.prompt_attention(self, q, k, v, starts, out, window, scale, stream)
+
+    def cache_write(self, k, v, cache, starts, lengths, pages, stream=None):
+        operators.cache_write(self, k, v, cache, starts, lengths, pages, stream)
+
+    def cache_read(self, cache, starts, lengths, pages, k, v, stream=None):
+        operators.cache_read(self, cache, starts, lengths, pages, k, v, stream)
+
+    def cache_workspace(self, tokens, sequences, heads, kv_heads, width, dtype):
+        return operators.cache_workspace(tokens, sequences, heads, kv_heads, width, dtype)
+
+    def cache_attention(self, q, cache, starts, lengths, pages, out, window=0, scale=None, workspace=None, stream=None):
+        operators.cache_attention(self, q, cache, starts, lengths, pages, out, window, scale, workspace, stream)
 
     def close(self):
         if self.h:

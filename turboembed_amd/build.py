@@ -18,8 +18,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["rowwise.hip", "gemm.hip", "gemm_direct.hip", "gemm_f32.hip", "attention.hip",
            "attention_f32p.hip", "head.hip", "row_codes.hip", "linear_i8.hip",
-           "cross_attention.hip", "session.cpp", "backend.cpp", "checks.cpp", "rerank.cpp",
-           "operators.cpp", "autotune.cpp", "allocs.cpp"]
+           "cross_attention.hip", "cache_rows.hip", "self_attention.hip", "session.cpp", "backend.cpp",
+           "checks.cpp", "rerank.cpp", "operators.cpp", "cache.cpp", "autotune.cpp", "allocs.cpp"]
 
 # The backend's own heap allocations are counted (allocs.cpp): its objects'
 # calls of these go to the __wrap_ functions there first.

@@ -20,65 +20,16 @@
 // (nearest_code).
 #include <hip/hip_runtime.h>
 
-#include "devmath.h"
+#include "codes.h"
 #include "launch.h"
 #include "operators.h"
 
 namespace rocm {
 
-// Eight consecutive values at p, of which the first n exist (the rest read as
-// 0). Rows may start at any element, so the vectors are read at its alignment.
-template <typename H> __device__ __forceinline__ void read8(const H *p, int n, float (&v)[8]) {
-    typedef H loose8 __attribute__((ext_vector_type(8), aligned(sizeof(H))));
-    if (n >= 8) {
-        const loose8 q = *(const loose8 *)p;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = to_f32(q[k]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = k < n ? to_f32(p[k]) : 0.0f;
-    }
-}
-
-template <typename H> __device__ __forceinline__ void write8(H *p, int n, const float (&v)[8]) {
-    typedef H loose8 __attribute__((ext_vector_type(8), aligned(sizeof(H))));
-    if (n >= 8) {
-        loose8 q;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) q[k] = from_f32<H>(v[k]);
-        *(loose8 *)p = q;
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < n) p[k] = from_f32<H>(v[k]);
-    }
-}
-
-// d as an F32 that rounds to 16 bits as d itself does: cut off, and odd where
-// anything was. (Below F32's smallest normal number its own rounding still
-// comes first.) 65536 x 1024 F16 rows and their norm take 54.4 us so, 51.0 with
-// d rounded to F32, one output in some 15,000 to the wrong side.
-__device__ __forceinline__ float odd_f32(double d) {
-    constexpr uint32_t REST = 0x1fffffff;   // what F32 has no room for
-    const uint64_t u = __builtin_bit_cast(uint64_t, d);
-    const uint32_t low = (uint32_t)u, odd = low | ((low & REST) + REST);
-    return (float)__builtin_bit_cast(double, (u >> 32 << 32) | (odd & ~REST));
-}
-
 __device__ __forceinline__ void write8(void *p, Dt t, uint64_t at, int n, const float (&v)[8]) {
     if (t == Dt::F32) write8((float *)p + at, n, v);
     else if (t == Dt::F16) write8((_Float16 *)p + at, n, v);
     else write8((__bf16 *)p + at, n, v);
-}
-
-// The whole number nearest to 127 c / top (ties to even), |c| <= top, without
-// rounding: low, the whole number below it, and a half are compared with it as
-// exact sums of two numbers each.
-__device__ __forceinline__ int nearest_code(double c, double top, double low) {
-#pragma clang fp contract(off)
-    const double half = low + 0.5, a = 127.0 * c, b = half * top;
-    const double d = (a - b) + (fma(127.0, c, -a) - fma(half, top, -b));
-    return (int)(d > 0.0 ? low + 1.0 : d < 0.0 ? low : 2.0 * rint(0.5 * half));
 }
 
 // A row's sum of squares, largest magnitude and sign of what is no number.

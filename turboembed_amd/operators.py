@@ -1,7 +1,7 @@
 """Operators on device memory, for programs that run layers of their own over a session's states.
 
-rms_norm, quantize_tokens, linear_i8 and CrossPlan.run call the entry points
-of the same names in turbo_rocm.h, which say what each computes, what it
+rms_norm, quantize_tokens, linear_i8, CrossPlan.run, prompt_attention and the
+cache's functions call the entry points of the same names in turbo_rocm.h, which say what each computes, what it
 checks and how it runs. Their arrays are tensors on the context's GPU that
 answer data_ptr(), shape, stride(), dtype and get_device() as torch's do (this
 package imports no torch), or a `DeviceArray` over one of that GPU's buffers. Outputs are the caller's:
@@ -119,6 +119,11 @@ _NORM = struct.Struct("=IIQd" + 7 * _T)
 _CODES = struct.Struct("=IIQ" + 3 * _T)
 _LINEAR = struct.Struct("=IIQ" + 6 * _T)
 _CROSS = struct.Struct("=IIQQQd" + 5 * _T)
+
+
+_ROWS = struct.Struct("=IIQ" + 9 * _T + "II")
+_PROMPT = struct.Struct("=IIQdII" + 5 * _T)
+_CACHED = struct.Struct("=IIQQQdII" + 9 * _T + "II")
 
 
 _functions = {}   # the library's, once looked up
@@ -253,6 +258,72 @@ class CrossPlan:
         if self.h:
             _lib().turbo_rocm_cross_plan_release(self.h)
             self.h = None
+
+
+class StateCache:
+    """States in pages of page_tokens slots: k and v [slots, kv_heads, width],
+    I8 ones with their scales [slots, kv_heads] (turbo_rocm_cache)."""
+
+    def __init__(self, k, v, page_tokens, k_scales=None, v_scales=None):
+        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
+        self.page_tokens, = _u32((page_tokens,), "a page")
+
+    def _packed(self, starts, lengths, pages, on):
+        return (*_tensor(self.k, on), *_tensor(self.v, on), *_tensor(self.k_scales, on), *_tensor(self.v_scales, on),
+                *_tensor(starts, on), *_tensor(lengths, on), *_tensor(pages, on), self.page_tokens, 0)
+
+
+def _rows(name, ctx, k, v, cache, starts, lengths, pages, stream):
+    h, on = _handle(ctx)
+    _call(name, h, _ROWS.pack(_ROWS.size, *_on(stream), *_tensor(k, on), *_tensor(v, on),
+                              *cache._packed(starts, lengths, pages, on)))
+
+
+def cache_write(ctx, k, v, cache, starts, lengths, pages, stream=None):
+    """The new tokens' k and v into their slots of the cache."""
+    _rows("turbo_rocm_cache_write", ctx, k, v, cache, starts, lengths, pages, stream)
+
+
+def cache_read(ctx, cache, starts, lengths, pages, k, v, stream=None):
+    """What the new tokens' slots hold into k and v."""
+    _rows("turbo_rocm_cache_read", ctx, k, v, cache, starts, lengths, pages, stream)
+
+
+def cache_workspace(tokens, sequences, heads, kv_heads, width, dtype):
+    """The bytes of workspace that cache_attention needs for up to so many
+    tokens and sequences."""
+    from . import _ok
+    for n in (tokens, sequences):
+        if not 0 <= n < 1 << 64:
+            raise ValueError(f"{n} tokens or sequences")
+    need, err = C.c_uint64(), S.new_error()
+    _ok(_lib().turbo_rocm_cache_workspace(tokens, sequences, *_u32((heads, kv_heads, width), "heads or a width"),
+                                          dtype_code(dtype), C.byref(need), C.byref(err)), err)
+    return need.value
+
+
+def cache_attention(ctx, q, cache, starts, lengths, pages, out, window=0, scale=None, workspace=None, stream=None):
+    """Each new token's attention to its sequence's states up to its own, the
+    last `window` of them (0: all), into out; scale 1 / sqrt(width) by
+    default. workspace: a 1-d tensor (or DeviceArray) of cache_workspace
+    bytes I8 or U8, this call's own until it is done."""
+    h, on = _handle(ctx)
+    w, wn = (0, 0) if workspace is None else _tensor(workspace, on)[:2]
+    _call("turbo_rocm_cache_attention", h,
+          _CACHED.pack(_CACHED.size, *_on(stream), w, wn, max(1, q.shape[-1]) ** -0.5 if scale is None else scale,
+                       *_u32((window,), "a window"), 0, *_tensor(q, on), *_tensor(out, on),
+                       *cache._packed(starts, lengths, pages, on)))
+
+
+def prompt_attention(ctx, q, k, v, starts, out, window=0, scale=None, stream=None):
+    """Each token's attention to its sequence's rows of k and v up to its own,
+    the last `window` of them (0: all), into out; scale 1 / sqrt(width) by
+    default."""
+    h, on = _handle(ctx)
+    _call("turbo_rocm_prompt_attention", h,
+          _PROMPT.pack(_PROMPT.size, *_on(stream), max(1, q.shape[-1]) ** -0.5 if scale is None else scale,
+                       *_u32((window,), "a window"), 0, *_tensor(q, on), *_tensor(k, on), *_tensor(v, on),
+                       *_tensor(starts, on), *_tensor(out, on)))
 
 
 def _lib():
