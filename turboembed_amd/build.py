@@ -18,8 +18,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["rowwise.hip", "gemm.hip", "gemm_direct.hip", "gemm_f32.hip", "attention.hip",
            "attention_f32p.hip", "head.hip", "row_codes.hip", "linear_i8.hip",
-           "cross_attention.hip", "cache_rows.hip", "self_attention.hip", "session.cpp", "backend.cpp",
-           "checks.cpp", "rerank.cpp", "operators.cpp", "cache.cpp", "autotune.cpp", "allocs.cpp"]
+           "cross_attention.hip", "cache_rows.hip", "self_f32.hip", "self_f16.hip", "self_bf16.hip", "session.cpp", "backend.cpp",
+           "checks.cpp", "rerank.cpp", "operators.cpp", "cache.cpp", "self_attention.cpp", "autotune.cpp", "allocs.cpp"]
 
 # The backend's own heap allocations are counted (allocs.cpp): its objects'
 # calls of these go to the __wrap_ functions there first.
@@ -31,8 +31,9 @@ WRAPPED = ["malloc", "calloc", "realloc", "aligned_alloc", "posix_memalign", "_Z
 # accumulation registers; and no NaN operands (its inputs are finite), so a
 # max of scores is one v_max3_f32 without a quieting v_max_f32 per score.
 EXTRA = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"] for f in ("attention.hip", "attention_f32p.hip")}
-# (Cross attention's inputs may be anything: the first of the two alone.)
-EXTRA["cross_attention.hip"] = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+# (The inputs of attention on a caller's memory may be anything: the first of the two alone.)
+EXTRA.update({f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("cross_attention.hip", "self_f32.hip", "self_f16.hip",
+                                                                "self_bf16.hip")})
 
 FLAGS = [
     "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",

@@ -1,6 +1,6 @@
 // A cache of states in pages, and the attention of a call's own tokens
 // (turbo_rocm.h): checks and entry points. The kernels are in cache_rows.hip
-// and self_attention.hip.
+// and self_tiles.h.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -92,6 +92,7 @@ CacheArgs check_cache(const turbo_rocm_cache &c, uint32_t field, uint32_t own, u
     r.page_row = c.pages.stride[0], r.paged = true;
     r.seqs = (int)seqs, r.columns = (int)columns, r.page_tokens = (int)c.page_tokens;
     r.page_count = (int)(slots / c.page_tokens);
+    if (r.page_count == 0) r.columns = 0;   // no page, no position
     r.tokens = (int)tokens, r.kv = (int)kv, r.width = (int)width;
     return r;
 }
@@ -165,7 +166,8 @@ void prompt(Context *c, const turbo_rocm_prompt_attention_call *call) {
     a.c.starts = static_cast<const int32_t *>(address(call->starts));
     a.c.seqs = (int)seqs, a.c.tokens = (int)tokens, a.c.kv = (int)kv, a.c.width = (int)width;
     attend(a, call->q, call->out, call->scale, call->window, heads);
-    run_call(c, call, "prompt_attention", [&](hipStream_t s) { return self_attention(s, a); });
+    const SelfLaunch f = self_plan(a);
+    run_call(c, call, "prompt_attention", [&](hipStream_t s) { return self_attention(s, a, f); });
 }
 
 void cached(Context *c, const turbo_rocm_cache_attention_call *call) {
@@ -188,7 +190,7 @@ void cached(Context *c, const turbo_rocm_cache_attention_call *call) {
     for (const Arg &i : {q, h.k, h.v, h.ks, h.vs, h.starts, h.lengths, h.pages}) check_clear(out, i);
     a.i8 = call->cache.k.dtype == TURBO_DTYPE_I8;
     attend(a, call->q, call->out, call->scale, call->window, heads);
-    const uint64_t need = self_workspace(tokens, (uint64_t)a.c.seqs, (int)heads, (int)kv, (int)width, a.dt);
+    const uint64_t need = self_workspace(tokens, (uint64_t)a.c.seqs, (int)heads, (int)kv, (int)width);
     if (call->workspace_bytes < need || (need && !call->workspace))
         fail(TURBO_E_CAPACITY, "rocm: a workspace of " + std::to_string(call->workspace_bytes) + " bytes, not " +
                                    std::to_string(need));
@@ -200,7 +202,8 @@ void cached(Context *c, const turbo_rocm_cache_attention_call *call) {
             check_clear(i, Arg{&ws, "the workspace", 0});
     }
     a.ws = static_cast<float *>(call->workspace);
-    run_call(c, call, "cache_attention", [&](hipStream_t s) { return self_attention(s, a); });
+    const SelfLaunch f = self_plan(a);
+    run_call(c, call, "cache_attention", [&](hipStream_t s) { return self_attention(s, a, f); });
 }
 
 }  // namespace
@@ -245,7 +248,7 @@ int32_t turbo_rocm_cache_workspace(uint64_t tokens, uint64_t sequences, uint32_t
         Tensor q{};
         q.shape[0] = tokens;
         check_heads(Arg{&q, "q", 0}, heads, kv_heads, width);
-        *bytes = self_workspace(tokens, sequences, (int)heads, (int)kv_heads, (int)width, dt_of(dtype));
+        *bytes = self_workspace(tokens, sequences, (int)heads, (int)kv_heads, (int)width);
         return TURBO_OK;
     });
 }

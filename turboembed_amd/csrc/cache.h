@@ -1,5 +1,5 @@
 // States in the pages of a cache, and the sequences that own them: how the
-// kernels of cache_rows.hip and self_attention.hip find a token's sequence,
+// kernels of cache_rows.hip and self_tiles.h find a token's sequence,
 // its position and a position's slot. What the arrays hold is the caller's
 // and may be anything: whatever they hold, no index leaves its array.
 #pragma once
@@ -78,8 +78,39 @@ struct SelfArgs {
     float scale;             // of a score, times log2(e); positive...
     float turn;              // ...with 1, -1 or 0 times q
 };
-hipError_t self_attention(hipStream_t s, const SelfArgs &a);
+
+// How keys and values reach LDS: in aligned whole chunks, by themselves;
+// through registers, at any alignment; or as codes.
+enum class Held : int { Chunks, Loose, Codes };
+
+// How a call is launched, from what the host knows of it: its rows and
+// sequences, not their lengths.
+struct SelfLaunch {
+    Held held;
+    int waves;           // of a workgroup
+    uint32_t groups;     // workgroups: of a prompt, the most blocks that there can be
+    int part_rows;       // the most rows of a part
+};
+SelfLaunch self_plan(const SelfArgs &a);
 // The bytes of workspace that calls of up to so many tokens and sequences need.
-uint64_t self_workspace(uint64_t tokens, uint64_t seqs, int heads, int kv, int width, Dt dt);
+uint64_t self_workspace(uint64_t tokens, uint64_t seqs, int heads, int kv, int width);
+hipError_t self_attention(hipStream_t s, const SelfArgs &a, const SelfLaunch &f);
+hipError_t self_f32(hipStream_t s, const SelfArgs &a, const SelfLaunch &f);
+hipError_t self_f16(hipStream_t s, const SelfArgs &a, const SelfLaunch &f);
+hipError_t self_bf16(hipStream_t s, const SelfArgs &a, const SelfLaunch &f);
+
+// A block whose tiles are cut over workgroups: each leaves a part, and says so
+// here. front: it starts inside of a block; done: it ends that block.
+struct SelfMark {
+    int front, done;
+    int q0, kv, row0, rows;
+    int pad[2];
+};
+// A part's floats, of up to `rows` rows: their sums, four columns of every row
+// after another, then each row's maximum (base 2) and sum of weights; a row
+// without a finite maximum leaves 1 for that sum if it had a state.
+inline __host__ __device__ uint64_t self_part_floats(int rows, int width) {
+    return ((uint64_t)rows * ((width + 3) / 4 * 4 + 2) + 3) / 4 * 4;
+}
 
 }  // namespace rocm

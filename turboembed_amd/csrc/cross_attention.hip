@@ -30,52 +30,11 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "devmath.h"
-#include "gemm_tile.h"
+#include "attention_tile.h"
 #include "launch.h"
 #include "operators.h"
 
 namespace rocm {
-
-// The sum of a lane's value and the lane 32 away's, and the larger of the two.
-__device__ __forceinline__ float both_sum(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float both_max(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-template <typename T> struct Chunk {   // 16 bytes of a row
-    static constexpr int N = 16 / sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
-    typedef T loose __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-};
-
-// The N elements at p, of which n exist (the rest 0).
-template <typename T> __device__ __forceinline__ typename Chunk<T>::vec read_chunk(const T *p, int n) {
-    typename Chunk<T>::vec v;
-    if (n >= Chunk<T>::N) return *(const typename Chunk<T>::loose *)p;
-#pragma unroll
-    for (int i = 0; i < Chunk<T>::N; ++i) v[i] = i < n ? p[i] : (T)0.0f;
-    return v;
-}
-
-// Of each of two weights (0 or more) a number of T one to two of its steps
-// below, so that what is left of it is at least a step: both terms of a weight
-// are positive, and an infinite value stays what its product gives.
-template <typename T>
-__device__ __forceinline__ auto below(float w0, float w1) {
-    typedef unsigned short bits2 __attribute__((ext_vector_type(2)));
-    typedef T two __attribute__((ext_vector_type(2)));
-    bits2 b;
-    if constexpr (std::is_same<T, _Float16>::value) b = __builtin_bit_cast(bits2, __builtin_amdgcn_cvt_pkrtz(w0, w1));
-    else b = bits2{(unsigned short)(__float_as_uint(w0) >> 16), (unsigned short)(__float_as_uint(w1) >> 16)};
-    return __builtin_bit_cast(two, __builtin_elementwise_sub_sat(b, bits2{1, 1}));
-}
 
 // Where a part of `rows` rows lies in the workspace.
 __device__ __forceinline__ float *part_of(const CrossArgs &a, int part) {

@@ -1,0 +1,62 @@
+// How attention of a call's own tokens is launched (its kernels: self_tiles.h).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "array_checks.h"
+#include "cache.h"
+
+namespace rocm {
+
+namespace {
+
+// Workgroups of a call over a cache: as many as a card holds at once, of blocks
+// of 32 rows (a wave) or 128 (four).
+int most_groups(int waves) { return waves == 1 ? 1280 : 512; }
+
+uint64_t parts_bytes(uint64_t groups, int rows, uint64_t all_rows, int width) {
+    return groups * (sizeof(SelfMark) + 2 * 4 * self_part_floats((int)std::min<uint64_t>(rows, all_rows), width));
+}
+
+}  // namespace
+
+SelfLaunch self_plan(const SelfArgs &a) {
+    SelfLaunch f{};
+    const uint64_t size = dt_bytes(a.dt), tokens = a.c.tokens, rows = tokens * a.share;   // (of a key head)
+    const uint64_t seqs = std::min<uint64_t>(a.c.seqs, tokens);
+    const auto whole = [&](const void *p, const uint64_t (&stride)[2]) {
+        return (reinterpret_cast<uintptr_t>(p) | stride[0] * size | stride[1] * size) % 16 == 0;
+    };
+    // (Keys and values in aligned whole chunks, a tile of them within 31 bits.)
+    const bool chunks = a.c.width * size % 16 == 0 && whole(a.c.k, a.c.ks) && whole(a.c.v, a.c.vs) &&
+                        std::max(a.c.ks[0], a.c.vs[0]) < (1u << 31) / 64 / 4;
+    f.held = a.i8 ? Held::Codes : chunks ? Held::Chunks : Held::Loose;
+    // Blocks of 128 rows, where sequences have more than a wave's on average and
+    // there are enough of them for every compute unit.
+    f.waves = 1;
+    if (f.held != Held::Loose && rows > 32 * seqs && (a.c.paged || a.c.kv * (rows / 128 + seqs) >= 512)) f.waves = 4;
+    const uint64_t blocks = a.c.kv * (rows / (32 * f.waves) + seqs);   // at most
+    if (!a.c.paged) {
+        if (blocks * 64 * f.waves > 1ull << 31)
+            fail(TURBO_E_CAPACITY, "rocm: a prompt of " + std::to_string(blocks) + " workgroups");
+        f.groups = (uint32_t)blocks;
+        return f;
+    }
+    const uint64_t tiles = ((uint64_t)room(a.c) + 31) / 32;
+    f.groups = (uint32_t)std::min<uint64_t>(most_groups(f.waves), std::max<uint64_t>(1, blocks * std::max<uint64_t>(1, tiles)));
+    f.part_rows = (int)std::min<uint64_t>(32 * f.waves, rows);
+    return f;
+}
+
+uint64_t self_workspace(uint64_t tokens, uint64_t seqs, int heads, int kv, int width) {
+    if (tokens == 0 || seqs == 0) return 0;
+    const uint64_t rows = tokens * (heads / kv);
+    return std::max(parts_bytes(most_groups(1), 32, rows, width), parts_bytes(most_groups(4), 128, rows, width));
+}
+
+hipError_t self_attention(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
+    if (a.c.tokens == 0 || a.c.seqs == 0) return hipSuccess;
+    return a.dt == Dt::F32 ? self_f32(s, a, f) : a.dt == Dt::F16 ? self_f16(s, a, f) : self_bf16(s, a, f);
+}
+
+}  // namespace rocm

@@ -1,0 +1,1046 @@
+// The kernel of attention of a call's own tokens: each to the states of its
+// sequence up to its own, over the rows of the call (a whole prompt) or over
+// the pages of a cache.
+//
+// The rows of a (sequence, key head) are its tokens' heads that read it, row r
+// token r / share, head kv * share + r % share: its keys and values are read
+// once for all of them. 32 of them are a wave's; a block is one wave's or four
+// waves'. A block's keys pass through LDS in tiles of KB. Scores are computed
+// transposed, S^T = K Q^T, so that a lane holds one row (lane % 32) and 16 of 32
+// keys, the other 16 in the lane 32 away; O^T += V^T P^T then takes P as the score
+// registers hold it, against V's columns for the same keys in that order (16-bit
+// values by LDS reads that transpose, F32 values one by one). The softmax is the
+// running one, in base 2 and F32: what it takes for a row's maximum moves only
+// when a score is 2^8 above the one that it was set by.
+//
+// Int8 states come through registers, a tile ahead: their codes are numbers of
+// every type, so LDS holds them as such, unscaled. A key's scale is a factor of
+// its scores, a value's one of its weights.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_tile.h"
+#include "cache_find.h"
+#include "launch.h"
+
+namespace rocm {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T, Held HELD, int DP, int WAVES> struct SelfTile {
+    static constexpr bool F32 = std::is_same<T, float>::value;
+    static constexpr bool CODES = HELD == Held::Codes;
+    static constexpr int ROWS = 32 * WAVES;
+    static constexpr int KB = WAVES == 1 || F32 ? 32 : 64;
+    static constexpr int PITCH = DP * (int)sizeof(T), CPR = PITCH / 16;   // a row's bytes and chunks in LDS
+    static constexpr int BUF = KB * PITCH;
+    // (A wave alone writes a tile of codes once it has read the one before.)
+    static constexpr int BUFS = CODES && WAVES == 1 ? 1 : 2;
+    static constexpr int TILES = BUFS * 2 * BUF;
+    // Behind the tiles: of codes, each buffer's scales of K and V, the exponent
+    // of the unit of V's, and the keys to be added alone; of others, the keys
+    // whose values are none, as each wave finds them.
+    static constexpr int SIDE = (2 * KB + 4) * 4;
+    static constexpr int LDS = TILES + (CODES ? BUFS * SIDE : WAVES > 1 ? BUFS * 8 * WAVES : 0);
+    static constexpr int OCC = F32 ? (DP <= (HELD == Held::Chunks ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;
+    // LDS serves 256 bytes a cycle: 16 keys of one chunk of K (a 16-byte
+    // read's pass), 4 keys of 4 chunks of V (a transposing read's).
+    static constexpr int PERIOD = CPR % 16 == 0 ? 1 : CPR % 8 == 0 ? 2 : 4;   // keys until the banks repeat
+    static __device__ __forceinline__ int swap_k(int key) { return key / PERIOD % (16 / PERIOD); }
+    static __device__ __forceinline__ int swap_v(int key) {
+        if (F32) return CPR % 16 == 0 ? (key >> 2 & 1) * 8 : 0;
+        return PERIOD == 1 ? (key & 3) * 4 : PERIOD == 2 ? (key >> 1 & 1) * 4 : 0;
+    }
+    // Codes that a lane moves at once: the most of which a tile is whole loads.
+    static constexpr int unit() {
+        for (int u = 16; u > 4; u /= 2)
+            if (KB * (DP / u) % (64 * WAVES) == 0 && DP % u == 0) return u;
+        return 4;
+    }
+};
+
+// ---- which rows and keys a workgroup takes ---------------------------------------
+
+// A block: rows row0 .. of a (sequence, key head), their keys in tiles first ..
+// first + tiles - 1.
+struct Block {
+    int q0;             // the sequence's first token
+    int kv, row0, rows;
+    int at0, last;      // the first and the last row's tokens' positions
+    int hi;             // keys from hi on are past every row, or the pages
+    int first, tiles;
+};
+
+// A sequence's blocks of ROWS rows, and what they cost: a block's keys and a
+// fixed OVERHEAD, times share (so that row r of them is at r), in closed form.
+struct Blocks {
+    uint64_t a, most, slope;
+    int n, linear;      // blocks; those below `most`
+};
+constexpr int OVERHEAD = 96;   // keys that a block's start and end are worth
+
+__device__ __forceinline__ int blocks_of(const Seq &s, int share, int rows) {
+    return (int)(((uint32_t)s.rows * (uint32_t)share + rows - 1) / (uint32_t)rows);
+}
+
+// a / b where it is below 2^52, by F64.
+__device__ __forceinline__ uint64_t quotient(uint64_t a, uint64_t b) {
+    uint64_t q = (uint64_t)((double)a / (double)b);
+    if (q * b > a) --q;
+    if ((q + 1) * b <= a) ++q;
+    return q;
+}
+
+__device__ __forceinline__ Blocks cost_of(const SelfArgs &a, const Seq &s, int rows) {
+    Blocks b;
+    b.n = blocks_of(s, a.share, rows);
+    const int past = within(s.first(), 0, room(a.c));
+    b.a = (uint64_t)a.share * (uint64_t)(past + OVERHEAD);
+    b.slope = (uint64_t)rows;
+    b.linear = b.n;
+    b.most = 0;
+    if (a.window < room(a.c)) {
+        b.most = (uint64_t)a.share * (uint64_t)(a.window + OVERHEAD) + rows;
+        b.linear = b.most < b.a ? 0 : (int)min((uint64_t)b.n, quotient(b.most - b.a, b.slope));
+    }
+    return b;
+}
+// The cost of the first n blocks.
+__device__ __forceinline__ uint64_t cost_to(const Blocks &b, int n) {
+    const uint64_t l = (uint64_t)min(n, b.linear);
+    return l * b.a + b.slope * (l * (l + 1) / 2) + (uint64_t)(n - (int)l) * b.most;
+}
+
+template <int ROWS, int KB> __device__ __forceinline__ Block block_of(const SelfArgs &a, const Seq &s, int kv, int b) {
+    Block k;
+    const int all = s.rows * a.share;
+    k.q0 = s.row0, k.kv = kv, k.row0 = b * ROWS;
+    k.rows = min(ROWS, all - k.row0);
+    k.at0 = s.first() + k.row0 / a.share;
+    k.last = s.first() + (k.row0 + k.rows - 1) / a.share;
+    k.hi = a.c.paged ? (k.last < room(a.c) ? k.last + 1 : room(a.c)) : k.last + 1;
+    const int lo = a.window > k.at0 ? 0 : k.at0 - a.window + 1;
+    k.first = lo / KB;
+    k.tiles = max(0, (k.hi + KB - 1) / KB - k.first);
+    return k;
+}
+
+// The sum of a wave's values up to and with each lane's.
+__device__ __forceinline__ uint64_t prefix_sum(uint64_t v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)v, o, 64), hi = (uint32_t)__shfl_up((int)(v >> 32), o, 64);
+        if (lane >= o) v += (uint64_t)hi << 32 | lo;
+    }
+    return v;
+}
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+
+// A place in the order of all blocks' tiles: sequence, key head, block, tile.
+struct Place {
+    int seq, kv, block, tile;
+    __device__ bool operator==(const Place &o) const {
+        return seq == o.seq && kv == o.kv && block == o.block && tile == o.tile;
+    }
+};
+
+// A call over a cache is cut into equal costs, one a workgroup, wherever the
+// cuts fall: its lengths are on the device, and one token's sequences may be as
+// different as they like. from .. to are workgroup g's places.
+template <int ROWS, int KB> struct Cuts {
+    Place from, to;
+    bool any;
+    __device__ __forceinline__ Cuts(const SelfArgs &a, int g, int groups, uint64_t least) {
+        const int lane = threadIdx.x & 63, n = a.c.seqs;
+        uint64_t total = 0, cost = 0;
+        Blocks mine{};
+        Seq seq{};
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            cost = 0;
+            if (i0 + lane < n) {
+                seq = seq_of(a.c, i0 + lane);
+                mine = cost_of(a, seq, ROWS);
+                cost = a.c.kv * cost_to(mine, mine.n);
+            }
+            cost = prefix_sum(cost);
+            total += lane_of(cost, 63);
+        }
+        // (No more workgroups than their least work makes worth while.)
+        const uint64_t worth = quotient(total + least - 1, least);
+        if (worth < (uint64_t)groups) groups = max(1, (int)worth);
+        any = total > 0 && g < groups;
+        if (!any) return;
+        // Lane 0 finds workgroup g's first place, lane 1 the next one's.
+        const uint64_t each = quotient(total, (uint64_t)groups), rest = total - each * (uint64_t)groups;
+        const auto cut = [&](uint64_t i) { return each * i + min(i, rest); };
+        const uint64_t f = cut((uint64_t)g + (lane & 1));
+        const uint64_t f0 = lane_of(f, 0), f1 = lane_of(f, 1);
+        // The sequences of both, and their costs' start.
+        int at = n;
+        uint64_t before = total, seen = 0;
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            if (n > 64) {
+                cost = 0;
+                if (i0 + lane < n) {
+                    const Seq s = seq_of(a.c, i0 + lane);
+                    const Blocks m = cost_of(a, s, ROWS);
+                    cost = a.c.kv * cost_to(m, m.n);
+                }
+                cost = prefix_sum(cost);
+            }
+            const uint64_t past0 = __ballot(seen + cost > f0), past1 = __ballot(seen + cost > f1);
+            const uint64_t past = lane & 1 ? past1 : past0;
+            const int first = past ? __ffsll((unsigned long long)past) - 1 : 64;
+            uint32_t lo = (uint32_t)__shfl((int)(uint32_t)cost, (first + 63) & 63, 64);
+            uint32_t hi = (uint32_t)__shfl((int)(cost >> 32), (first + 63) & 63, 64);
+            if (at == n && past) at = i0 + first, before = seen + (first ? (uint64_t)hi << 32 | lo : 0);
+            seen += lane_of(cost, 63);
+        }
+        Place p{at, 0, 0, 0};
+        if (at < n) {
+            const Seq s = seq_of(a.c, at);
+            const Blocks m = cost_of(a, s, ROWS);
+            const uint64_t head = cost_to(m, m.n), o = f - before;
+            p.kv = (int)quotient(o, head);
+            const uint64_t rest = o - p.kv * head;
+            int lo = 0, hi = m.n;      // cost_to(lo) <= rest < cost_to(hi)
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (cost_to(m, mid) <= rest) lo = mid;
+                else hi = mid;
+            }
+            p.block = lo;
+            const uint64_t c0 = cost_to(m, lo), c = cost_to(m, lo + 1) - c0;
+            const Block b = block_of<ROWS, KB>(a, s, p.kv, lo);
+            p.tile = min(b.tiles, (int)((double)(rest - c0) / (double)c * (double)b.tiles));
+            // (A cut next to a block's end goes there: a part costs its way to memory.)
+            const int near = (int)min((uint64_t)b.tiles, quotient(each, (uint64_t)a.share * KB * 8));
+            if (p.tile <= near && p.tile * 2 < b.tiles) p.tile = 0;
+            else if (b.tiles - p.tile <= near) p.tile = b.tiles;
+            if (p.tile == b.tiles) {
+                p.tile = 0;
+                if (b.tiles > 0 && ++p.block == m.n) {
+                    p.block = 0;
+                    if (++p.kv == a.c.kv) p.kv = 0, ++p.seq;
+                }
+            }
+        }
+        const auto one = [&](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
+        from = Place{one(p.seq, 0), one(p.kv, 0), one(p.block, 0), one(p.tile, 0)};
+        to = Place{one(p.seq, 1), one(p.kv, 1), one(p.block, 1), one(p.tile, 1)};
+        // (A sequence without rows has no place.)
+        const auto settle = [&](Place &q) {
+            while (q.seq < n && seq_of(a.c, q.seq).rows == 0) ++q.seq;
+        };
+        settle(from), settle(to);
+    }
+};
+
+// Workgroup x's (sequence, key head, block) of a prompt: the blocks with the
+// most keys first, over all sequences, so that the last to run are short; of one
+// number, the key heads next to each other (8 of them go to as many XCDs). Of
+// more than HELD sequences, whose numbers LDS does not hold: one after another.
+template <int ROWS, int HELD> struct Turn {
+    int seq, kv, block;
+    bool any;
+    __device__ __forceinline__ Turn(const SelfArgs &a, uint32_t x, char *lds, int threads) {
+        const int lane = threadIdx.x & 63, n = a.c.seqs, kv_heads = a.c.kv;
+        int *count = (int *)lds;
+        const auto blocks = [&](int i) { return i < n ? blocks_of(seq_of(a.c, i), a.share, ROWS) : 0; };
+        any = false;
+        const int item = (int)(x / (uint32_t)kv_heads);
+        kv = (int)(x - (uint32_t)item * (uint32_t)kv_heads);
+        if (n > HELD) {
+            int seen = 0;
+            for (int i0 = 0; i0 < n; i0 += 64) {
+                const int b = blocks(i0 + lane), sum = (int)prefix_sum((uint64_t)b);
+                const uint64_t past = __ballot(seen + sum > item);
+                if (past) {
+                    const int l = __ffsll((unsigned long long)past) - 1;
+                    seq = i0 + l;
+                    block = item - seen - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(b, l));
+                    any = true;
+                    return;
+                }
+                seen += __builtin_amdgcn_readlane(sum, 63);
+            }
+            return;
+        }
+        int own = 0;    // the first 64 sequences' in registers
+        if (n <= 64) {
+            own = blocks(lane);
+        } else {
+            for (int i = threadIdx.x; i < n; i += threads) count[i] = blocks(i);
+            __syncthreads();
+        }
+        const auto at = [&](int i0) { return n <= 64 ? own : i0 + lane < n ? count[i0 + lane] : 0; };
+        // The blocks numbered b or more of all sequences.
+        const auto from = [&](int b) {
+            int sum = 0;
+            for (int i0 = 0; i0 < n; i0 += 64) {
+                const uint32_t v = (uint32_t)max(0, at(i0) - b);
+                for (int k = 0; __ballot(v >> k) != 0; ++k) sum += __popcll(__ballot(v >> k & 1)) << k;
+            }
+            return sum;
+        };
+        if (item >= from(0)) return;
+        int lo = 0, hi = a.c.tokens;   // from(hi) <= item < from(lo)
+        hi = (int)(((uint64_t)hi * a.share + ROWS - 1) / ROWS);
+        while (hi - lo > 1) {
+            const int mid = lo + (hi - lo) / 2;
+            if (from(mid) > item) lo = mid;
+            else hi = mid;
+        }
+        block = lo;
+        int left = item - from(lo + 1);      // of the sequences with more than lo blocks, in order
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            uint64_t has = __ballot(at(i0) > lo);
+            if (left >= __popcll(has)) {
+                left -= __popcll(has);
+                continue;
+            }
+            for (; left > 0; --left) has &= has - 1;
+            seq = i0 + __ffsll((unsigned long long)has) - 1;
+            any = true;
+            break;
+        }
+        if (n > 64) __syncthreads();   // (count lies where tiles will)
+    }
+};
+
+// ---- parts ---------------------------------------------------------------------------
+
+// Workgroup g's marks, then its parts: 2 g of the block that it starts inside
+// of, 2 g + 1 of the one that it leaves unfinished.
+struct SelfParts {
+    SelfMark *marks;
+    float *parts;
+    uint64_t pitch;
+    int groups;
+    uint64_t least;      // cost
+    __device__ __forceinline__ float *part(int i) const { return parts + (uint64_t)i * pitch; }
+};
+
+// ---- the kernel ------------------------------------------------------------------------
+
+template <typename T>
+__device__ __forceinline__ void two_of(float w0, float w1, T (&hi)[2], T (&lo)[2], bool positive) {
+    if (positive) {
+        const auto b = below<T>(w0, w1);
+        hi[0] = b[0], hi[1] = b[1];
+        lo[0] = from_f32<T>(w0 - to_f32(hi[0])), lo[1] = from_f32<T>(w1 - to_f32(hi[1]));
+    } else {
+        hi[0] = from_f32<T>(w0), hi[1] = from_f32<T>(w1);
+        lo[0] = from_f32<T>(w0 - to_f32(hi[0])), lo[1] = from_f32<T>(w1 - to_f32(hi[1]));
+    }
+}
+
+template <typename T, Held HELD, bool PAGED, int DP, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SelfTile<T, HELD, DP, WAVES>::OCC)))
+self_tiles(SelfArgs a, SelfParts parts) {
+    using C = SelfTile<T, HELD, DP, WAVES>;
+    constexpr bool F32 = C::F32, CODES = C::CODES, F16 = std::is_same<T, _Float16>::value, TWO = WAVES == 1 && !F32;
+    constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR, DT = DP / 32;
+    constexpr int E = Chunk<T>::N, ROWS = C::ROWS;
+    // m is LEAD above the maximum (base 2) that it was set by, and is set again
+    // by one that is LAG above that. With a LEAD of LAG weights are 1 at most, so
+    // that values of F32's size add up to finite sums. F16's need no such room,
+    // and its weights have no range to give away: there they reach 2^LAG.
+    constexpr float LAG = 8.0f, LEAD = F16 ? 0.0f : LAG;
+    constexpr uint64_t FULL = KB == 64 ? ~0ull : 0xffffffffull;
+    constexpr int LEAST_UNIT = -40;   // (127 times half of that is nothing in F16)
+    typedef typename Chunk<T>::vec vec;
+    typedef typename Mma<T>::frag frag;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5, d = a.c.width;
+    const CacheArgs &c = a.c;
+
+    // ---- a tile's way to LDS
+    // Of chunks, load j of a wave fills 64 in order; of codes, 64 units.
+    constexpr int UN = CODES ? C::unit() : E, UPR = DP / UN;
+    constexpr int NL = KB * UPR / 64 / WAVES;
+    static_assert(NL * 64 * WAVES == KB * UPR, "whole loads a wave");
+    constexpr int GROUP = 16;                 // keys that lie in one page, where pages are whole groups
+    constexpr int PER = CPR / 4;              // ...and their loads of chunks
+    const auto unit_of = [&](int j) { return (wave * NL + j) * 64 + lane; };
+    const auto key_of = [&](int j) { return unit_of(j) / UPR; };
+    const auto col_k = [&](int j) { return CODES ? unit_of(j) % UPR * UN : (unit_of(j) % CPR ^ C::swap_k(key_of(j))) * E; };
+    const auto col_v = [&](int j) { return CODES ? unit_of(j) % UPR * UN : (unit_of(j) % CPR ^ C::swap_v(key_of(j))) * E; };
+    typedef typename std::conditional<CODES, int8_t, T>::type H;
+    // (Chunks: bytes from a tile's or a group's first key, which 31 bits hold.)
+    uint32_t ko[NL], vo[NL];
+    if constexpr (HELD == Held::Chunks)
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+            const uint32_t key = PAGED ? key_of(j) % GROUP : key_of(j);
+            ko[j] = (key * (uint32_t)c.ks[0] + col_k(j)) * (uint32_t)sizeof(T);
+            vo[j] = (key * (uint32_t)c.vs[0] + col_v(j)) * (uint32_t)sizeof(T);
+        }
+    const bool groups_whole = PAGED && c.page_tokens % GROUP == 0;   // uniform
+
+    if (HELD == Held::Chunks && d < DP) {   // uniform
+        // (Columns past the width keep these zeros.)
+        for (int i = tid; i < C::TILES / 16; i += 64 * WAVES) *(vec *)(smem + i * 16) = vec{};
+    }
+
+    Place at{}, end{};
+    bool front = false, done = false;    // this workgroup starts inside of a block; it has ended it
+    Block front_block{};
+    if constexpr (PAGED) {
+        const Cuts<ROWS, KB> cuts(a, (int)blockIdx.x, parts.groups, parts.least);
+        if (cuts.any) at = cuts.from, end = cuts.to, front = at.tile > 0;
+        else at = end = Place{c.seqs, 0, 0, 0};
+    } else {
+        const Turn<ROWS, C::TILES / 4> turn(a, blockIdx.x, smem, 64 * WAVES);
+        if (!turn.any) return;
+        at = Place{turn.seq, turn.kv, turn.block, 0};
+        if (HELD == Held::Chunks && d < DP && c.seqs > 64) {
+            __syncthreads();
+            for (int i = tid; i < C::TILES / 16; i += 64 * WAVES) *(vec *)(smem + i * 16) = vec{};
+        }
+    }
+    // (A workgroup that begins where it ends, inside of a block, leaves a part
+    // without keys.)
+    bool more = !PAGED || !(at == end) || front;
+    while (more) {
+        const Seq seq = seq_of(c, at.seq);
+        const Block b = block_of<ROWS, KB>(a, seq, at.kv, at.block);
+        const bool last_here = PAGED && at.seq == end.seq && at.kv == end.kv && at.block == end.block;
+        const bool begun = at.tile > 0, ends = !last_here || end.tile == b.tiles;
+        const int t0 = b.first + at.tile, t1 = b.first + (last_here ? end.tile : b.tiles);
+        __syncthreads();    // every wave has read the block before
+
+        const bool work = 32 * wave < b.rows;   // this wave has rows
+        const int row = b.row0 + min(32 * wave + r, b.rows - 1);
+        const int of_token = a.share == 1 ? row : row / a.share;
+        const uint64_t token = (uint64_t)b.q0 + of_token, head = (uint64_t)b.kv * a.share + (row - of_token * a.share);
+        // The keys that this lane's row sees, and those that every row of the
+        // block does.
+        const int pos = seq.first() + of_token;
+        const int low = a.window > pos ? 0 : pos - a.window + 1;
+        const int all_hi = b.at0, all_lo = a.window > b.last ? 0 : b.last - a.window + 1;
+        const H *K0 = (const H *)c.k + b.kv * c.ks[1], *V0 = (const H *)c.v + b.kv * c.vs[1];
+
+        // The slot of key `lane` of a tile, or -1: no state.
+        const auto slot_at = [&](int t) {
+            const int p = t * KB + lane;
+            if (!PAGED) return lane < KB && p < b.hi ? b.q0 + p : -1;
+            return t < t1 && lane < KB && p < b.hi ? slot_of(c, at.seq, p) : -1;
+        };
+        int slot = -1, next_slot = -1;
+        bool alive = false;             // of the tile on its way: key `lane` is a state
+        // Codes on their way, and their scales (a lane a key).
+        typedef uint32_t codes_t __attribute__((ext_vector_type(UN >= 16 ? 4 : UN >= 8 ? 2 : 1), aligned(1)));
+        codes_t kq[CODES ? NL : 1], vq[CODES ? NL : 1];
+        float sk = 0.0f, sv = 0.0f;
+        int unit = LEAST_UNIT;          // the exponent of the weights' unit (F16 codes)
+
+        const auto read_codes = [&](const int8_t *p, int n) {
+            codes_t q{};
+            if (n >= UN) return *(const codes_t *)p;
+            if (n > 0) {
+#pragma unroll
+                for (int i = 0; i < UN; ++i)
+                    if (i < n) q[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+            }
+            return q;
+        };
+        // Starts the tile of `slot` on its way; without pages, tile t.
+        const auto load = [&](int t, int buf) {
+            char *K = smem + buf * 2 * BUF, *V = K + BUF;
+            alive = slot >= 0;
+            if constexpr (HELD == Held::Chunks) {
+                // (As buffer loads where a base is common to the lanes: those
+                // take 32-bit offsets.)
+                typedef __attribute__((address_space(3))) void *to;
+                typedef __attribute__((address_space(1))) const void *from;
+                if (!PAGED || groups_whole) {   // uniform
+                    const int last = b.hi - 1 - t * KB;
+                    const auto rsrc = [](const T *p) {
+                        return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, -1, 0x00020000);
+                    };
+                    const auto send = [&](__amdgpu_buffer_rsrc_t tile, uint32_t at, char *dst) {
+                        __builtin_amdgcn_raw_ptr_buffer_load_lds(tile, (to)dst, 16, (int)at, 0, 0, 0);
+                    };
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) {
+                        uint64_t s;
+                        uint32_t back = 0;
+                        if constexpr (PAGED) {
+                            // (Without a page: slot 0, whose keys are not looked at.)
+                            s = (uint64_t)max(0, __builtin_amdgcn_readlane(slot, (wave * NL + j) / PER * GROUP));
+                        } else {
+                            s = (uint64_t)b.q0 + (uint64_t)t * KB;
+                            if (last < KB - 1) back = (uint32_t)max(0, key_of(j) - last) * (uint32_t)sizeof(T);
+                        }
+                        if (d == DP || col_k(j) < d)
+                            send(rsrc(K0 + s * c.ks[0]), ko[j] - back * (uint32_t)c.ks[0], K + (wave * NL + j) * 1024);
+                        if (d == DP || col_v(j) < d)
+                            send(rsrc(V0 + s * c.vs[0]), vo[j] - back * (uint32_t)c.vs[0], V + (wave * NL + j) * 1024);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) {
+                        const uint64_t s = (uint64_t)max(0, __shfl(slot, key_of(j), 64));
+                        if (d == DP || col_k(j) < d)
+                            __builtin_amdgcn_global_load_lds((from)(K0 + s * c.ks[0] + col_k(j)),
+                                                             (to)(K + (wave * NL + j) * 1024), 16, 0, 0);
+                        if (d == DP || col_v(j) < d)
+                            __builtin_amdgcn_global_load_lds((from)(V0 + s * c.vs[0] + col_v(j)),
+                                                             (to)(V + (wave * NL + j) * 1024), 16, 0, 0);
+                    }
+                }
+            } else if constexpr (HELD == Held::Loose) {
+#pragma unroll
+                for (int j = 0; j < NL; ++j) {
+                    const int s = __shfl(slot, key_of(j), 64), at = unit_of(j) * 16, nk = d - col_k(j), nv = d - col_v(j);
+                    *(vec *)(K + at) = s >= 0 && nk > 0 ? read_chunk(K0 + (uint64_t)s * c.ks[0] + col_k(j), nk) : vec{};
+                    *(vec *)(V + at) = s >= 0 && nv > 0 ? read_chunk(V0 + (uint64_t)s * c.vs[0] + col_v(j), nv) : vec{};
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NL; ++j) {
+                    const int s = __shfl(slot, key_of(j), 64), n = s >= 0 ? d - col_k(j) : 0;
+                    const uint64_t at = (uint64_t)max(0, s);
+                    kq[j] = read_codes(K0 + at * c.ks[0] + col_k(j), n);
+                    vq[j] = read_codes(V0 + at * c.vs[0] + col_v(j), n);
+                }
+                if (wave == 0) {
+                    sk = alive ? c.k_scales[(uint64_t)slot * c.kss + b.kv] : 0.0f;
+                    sv = alive ? c.v_scales[(uint64_t)slot * c.vss + b.kv] : 0.0f;
+                }
+            }
+        };
+        // Codes that have come, as numbers of T, into LDS, and their scales.
+        const auto put = [&](int t, int buf) {
+            if constexpr (CODES) {
+                char *K = smem + buf * 2 * BUF, *V = K + BUF;
+                float *side = (float *)(smem + C::TILES + buf * C::SIDE);
+                const auto spread = [&](const codes_t &q, char *row, int col, int swap) {
+#pragma unroll
+                    for (int e0 = 0; e0 < UN; e0 += E) {
+                        vec x;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            const int i = e0 + e;
+                            x[e] = (T)(float)(int8_t)(q[i / 4] >> (8 * (i & 3)));
+                        }
+                        *(vec *)(row + (((col + e0) / E) ^ swap) * 16) = x;
+                    }
+                };
+#pragma unroll
+                for (int j = 0; j < NL; ++j) {
+                    const int key = key_of(j);
+                    spread(kq[j], K + key * PITCH, col_k(j), C::swap_k(key));
+                    spread(vq[j], V + key * PITCH, col_v(j), C::swap_v(key));
+                }
+                if (wave == 0) {
+                    bool alone = !(fabsf(sv) < INFINITY);
+                    if constexpr (F16) {
+                        // F16 weights have no range for a scale's: they are of its
+                        // size against a power of 2 that is twice to four times the
+                        // largest so far. One that not every row sees has no say in
+                        // that; a larger one is added alone, in F32.
+                        const bool common = t * KB + lane <= all_hi && t * KB + lane >= all_lo;
+                        float top = lane < KB && common && !alone ? fabsf(sv) : 0.0f;
+#pragma unroll
+                        for (int o = KB / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+                        const int e = min(126, (int)(__float_as_uint(top) >> 23) - 127 + 2);
+                        unit = __builtin_amdgcn_readfirstlane(max(unit, e));
+                        alone |= !common && fabsf(sv) > __uint_as_float((uint32_t)(127 + unit) << 23);
+                    }
+                    if (lane < KB) {
+                        side[lane] = sk;
+                        side[KB + lane] = F16 ? sv * __uint_as_float((uint32_t)(127 - unit) << 23) : sv;
+                    }
+                    const uint64_t none = __ballot(lane < KB && alone);
+                    if (lane == 0) {
+                        ((int *)side)[2 * KB] = unit;
+                        ((uint32_t *)side)[2 * KB + 2] = (uint32_t)none, ((uint32_t *)side)[2 * KB + 3] = (uint32_t)(none >> 32);
+                    }
+                }
+            }
+        };
+
+        // ---- the tiles
+        if (t0 < t1) {
+            slot = slot_at(t0);
+            load(t0, 0);
+            next_slot = slot_at(t0 + 1);
+        }
+        // This row's q: of each 2 E columns the lane's half's E.
+        vec q[CPR / 2];
+        {
+            const T *p = (const T *)a.q + token * a.qs[0] + head * a.qs[1];
+#pragma unroll
+            for (int s = 0; s < CPR / 2; ++s) {
+                const int col = (2 * s + h) * E;
+                q[s] = read_chunk(p + col, d - col);
+            }
+            if (a.turn != 1.0f)   // uniform
+#pragma unroll
+                for (int s = 0; s < CPR / 2; ++s)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) q[s][e] = from_f32<T>(to_f32(q[s][e]) * a.turn);
+        }
+
+        floatx16 o[DT];
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] = floatx16{};
+        float m = -INFINITY, l = 0.0f;
+        bool any = false, far = false;   // this row has seen a state; a maximum past 2^24
+        int my_unit = LEAST_UNIT;        // of o's sums
+
+        // S^T of 32 keys. Register i is key 8 (i / 4) + 4 h + i % 4.
+        const int kr = r * PITCH, ks = C::swap_k(r);   // (32 keys on, the swap is the same)
+        const auto scores = [&](const char *K, floatx16 (&s)[SUB]) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) s[u] = floatx16{};
+            const auto chunk = [&](int x, int u) {
+                return *(const vec *)(K + 32 * u * PITCH + kr + ((2 * x + h) ^ ks) * 16);
+            };
+            if constexpr (F32) {
+                // (A chunk read two ahead of its products, which are slow enough to hide it.)
+                vec k[3] = {chunk(0, 0), chunk(1, 0)};
+#pragma unroll
+                for (int x = 0; x < CPR / 2; ++x) {
+                    if (x + 2 < CPR / 2) k[(x + 2) % 3] = chunk(x + 2, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) s[0] = Mma<T>::run(k[x % 3][e], q[x][e], s[0]);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < CPR / 2; ++x)
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) s[u] = Mma<T>::run(chunk(x, u), q[x], s[u]);
+            }
+        };
+        // O^T += V^T P^T over 32 keys; weight(i) is register i's, in order.
+        const auto add_values = [&](const char *V, auto weight) {
+            if constexpr (F32) {
+                // (Values and weights two keys ahead of their products.)
+                float v[3][DT], p[3];
+                const auto ahead = [&](int i) {
+                    const int key = 8 * (i >> 2) + 4 * h + (i & 3);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+                        v[i % 3][t] =
+                            *(const float *)(V + key * PITCH + (((r >> 2) + 8 * t) ^ C::swap_v(key)) * 16 + (r & 3) * 4);
+                    p[i % 3] = weight(i);
+                };
+                ahead(0), ahead(1);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (i + 2 < 16) ahead(i + 2);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) o[t] = Mma<T>::run(v[i % 3][t], p[i % 3], o[t]);
+                }
+            } else {
+                // 16 keys a product: registers 8 j .. 8 j + 7. A group of 16 lanes
+                // reads 4 keys by 16 columns, and a lane gets its column's 4.
+                typedef short s4 __attribute__((ext_vector_type(4)));
+                const int g = lane >> 4, n = lane & 15, key = 4 * (g >> 1) + (n >> 2);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    frag f, rest, vt[DT];
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const float w0 = weight(8 * j + e), w1 = weight(8 * j + e + 1);
+                        if constexpr (TWO) {
+                            T hi[2], lo[2];
+                            two_of<T>(w0, w1, hi, lo, !CODES);
+                            f[e] = hi[0], f[e + 1] = hi[1], rest[e] = lo[0], rest[e + 1] = lo[1];
+                        } else {
+                            f[e] = from_f32<T>(w0), f[e + 1] = from_f32<T>(w1);
+                        }
+                    }
+#pragma unroll
+                    for (int t = 0; t < DT; ++t) {
+                        const int x = 4 * t + 2 * (g & 1) + ((n >> 1) & 1);
+                        const auto place = [&](int k) {
+                            return (__attribute__((address_space(3))) s4 *)(V + k * PITCH + (x ^ C::swap_v(k)) * 16 +
+                                                                             (n & 1) * 8);
+                        };
+                        struct {
+                            s4 lo, hi;
+                        } v;
+                        v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(16 * j + key));
+                        v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(16 * j + 8 + key));
+                        vt[t] = __builtin_bit_cast(frag, v);
+                        o[t] = Mma<T>::run(vt[t], f, o[t]);
+                    }
+                    if constexpr (TWO)
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) o[t] = Mma<T>::run(vt[t], rest, o[t]);
+                }
+            }
+        };
+        const auto raise = [&](float mx) {   // m, for scores of up to mx
+            if (__ballot(mx > m + (LAG - LEAD)) == 0) return;
+            const float mn = fmaxf(m, mx + LEAD);
+            // (Equal: both infinite, of one sign.)
+            const float f = __builtin_amdgcn_exp2f(m == mn ? 0.0f : m - mn);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] *= f;
+            l *= f;
+            m = mn;
+            far = __ballot(fabsf(m) > 16777216.0f && m != -INFINITY) != 0;
+        };
+        // Values that are no numbers weigh nothing for the rows that do not see
+        // them, and 0 times them is no number either: where some row does not,
+        // their keys are added one by one, and are 0 for the products.
+        const auto add_alone = [&](const char *V, const float *side, const floatx16 (&s)[SUB], uint64_t seen, uint64_t bad,
+                                   float scale, float base) {
+            for (; bad; bad &= bad - 1) {
+                const int key = __ffsll((unsigned long long)bad) - 1;
+                const int u = key >> 5, i = (key >> 3 & 3) * 4 + (key & 3), from = key >> 2 & 1;
+                float x = 0.0f;
+#pragma unroll
+                for (int v = 0; v < SUB; ++v)
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) x = u == v && i == n ? s[v][n] : x;
+                x = __shfl(x, r + 32 * from, 64);
+                float w = __builtin_amdgcn_exp2f(fmaf(x, scale, -base));
+                if constexpr (CODES) w *= side[KB + key];
+                const bool see = seen >> key & 1;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) {
+                        const int col = 32 * t + 8 * (n >> 2) + 4 * h + (n & 3);
+                        const T v = *(const T *)(V + key * PITCH + (col / E ^ C::swap_v(key)) * 16 + col % E * (int)sizeof(T));
+                        o[t][n] = see ? fmaf(w, to_f32(v), o[t][n]) : o[t][n];
+                    }
+            }
+        };
+        const auto tile = [&](const char *K, float *side, uint64_t live, int t, uint64_t bad) {
+            floatx16 s[SUB];
+            scores(K, s);
+            if constexpr (CODES) {
+#pragma unroll
+                for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 f = *(const f32x4 *)(side + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[u][4 * g + e] *= f[e];
+                    }
+                if constexpr (F16) {
+                    const int now = uniform(((const int *)side)[2 * KB]);
+                    if (now != my_unit) {   // uniform
+                        const float f = my_unit - now < -126 ? 0.0f : __uint_as_float((uint32_t)(127 + my_unit - now) << 23);
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) o[t] *= f;
+                        my_unit = now;
+                    }
+                }
+            }
+            uint64_t seen = live;
+            if (t * KB + KB - 1 > all_hi || t * KB < all_lo) {   // uniform
+                const int lo = max(0, low - t * KB), hi = min(KB - 1, pos - t * KB);
+                seen = lo > hi ? 0 : seen & (~0ull << lo) & (~0ull >> (63 - hi));
+            }
+            any |= seen != 0;
+            if (__ballot(seen != FULL) != 0) {
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    const uint32_t word = (uint32_t)(seen >> (32 * u)) >> (4 * h);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[u][i] = (word >> (8 * (i >> 2) + (i & 3))) & 1u ? s[u][i] : -INFINITY;
+                }
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+            raise(both_max(mx) * a.scale);
+            const float base = m == -INFINITY ? 0.0f : m;
+            // A score's distance from the maximum in one rounding; where the
+            // maximum is so large that its own rounding shows, from the rounded
+            // score, which is no larger.
+            float scale = a.scale;
+            if (far) {   // uniform
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) s[u] *= scale;
+                scale = 1.0f;
+            }
+            if (bad) add_alone(K + BUF, side, s, seen, bad, scale, base);
+            return [=, &l, &add_values](const char *V) {
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    float sum = 0.0f;
+                    f32x4 sv[4];
+                    if constexpr (CODES)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) sv[g] = *(const f32x4 *)(side + KB + 32 * u + 8 * g + 4 * h);
+                    add_values(V + 32 * u * PITCH, [&](int i) {
+                        const float w = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
+                        sum += w;
+                        if constexpr (CODES) return w * sv[i >> 2][i & 3];
+                        return w;
+                    });
+                    l += sum;
+                }
+            };
+        };
+
+        for (int t = t0, buf = 0; t < t1; ++t, buf ^= C::BUFS - 1) {
+            char *K = smem + buf * 2 * BUF, *V = K + BUF;
+            float *side = (float *)(smem + C::TILES + buf * C::SIDE);
+            if constexpr (CODES) put(t, buf);
+            else __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
+            const uint64_t live = __ballot(alive);
+            const bool partial = t * KB + KB - 1 > all_hi || t * KB < all_lo;   // uniform: not every row sees all of it
+            if (!CODES && live != FULL) {   // uniform
+                // A value that is no state's weighs 0, but not if it is no number.
+#pragma unroll
+                for (int j = 0; j < NL; ++j)
+                    if (!((live >> key_of(j)) & 1)) *(vec *)(V + unit_of(j) * 16) = vec{};
+            }
+            uint64_t bad = 0;
+            if (!CODES && partial) {
+                // Keys of this wave's chunks with an infinity or a NaN among their values.
+#pragma unroll
+                for (int j = 0; j < NL; ++j) {
+                    const vec x = *(const vec *)(V + unit_of(j) * 16);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) sum = fmaf(to_f32(x[e]), 0.0f, sum);
+                    uint64_t lanes = __ballot(sum != 0.0f);   // (0 times a number is 0)
+                    for (; lanes; lanes &= lanes - 1)
+                        bad |= 1ull << (((wave * NL + j) * 64 + __ffsll((unsigned long long)lanes) - 1) / CPR);
+                }
+                if (WAVES > 1 && lane == 0) ((uint64_t *)(smem + C::TILES))[buf * WAVES + wave] = bad;
+            }
+            __syncthreads();   // the tile is there, and the other one read
+            if (CODES && partial)
+                bad = (uint64_t)(uint32_t)uniform(((const int *)side)[2 * KB + 2]) |
+                      (uint64_t)(uint32_t)uniform(((const int *)side)[2 * KB + 3]) << 32;
+            if (!CODES && WAVES > 1 && partial) {
+                bad = 0;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) bad |= ((const uint64_t *)(smem + C::TILES))[buf * WAVES + w];
+                bad = (uint64_t)(uint32_t)uniform((int)bad) | (uint64_t)(uint32_t)uniform((int)(bad >> 32)) << 32;
+            }
+            if (t + 1 < t1) {
+                slot = next_slot;
+                load(t + 1, buf ^ 1);
+                next_slot = slot_at(t + 2);
+            }
+            const auto zero = [&] {   // (called by all waves: bad is the same for all)
+                __syncthreads();
+                if constexpr (CODES) {
+                    if (tid < KB && (bad >> tid & 1)) side[KB + tid] = 0.0f;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NL; ++j)
+                        if ((bad >> key_of(j)) & 1) *(vec *)(V + unit_of(j) * 16) = vec{};
+                }
+                __syncthreads();
+            };
+            if (work && live != 0) {
+                const auto add = tile(K, side, live, t, bad);
+                if (bad) zero();
+                add(V);
+            } else if (bad) {
+                zero();
+            }
+        }
+
+        if (work) {
+            l = both_sum(l);
+            if constexpr (CODES && F16) {
+                const float f = __uint_as_float((uint32_t)(127 + my_unit) << 23);
+#pragma unroll
+                for (int t = 0; t < DT; ++t) o[t] *= f;
+            }
+            if (32 * wave + r < b.rows) {
+                if (!PAGED || (!begun && ends)) {
+                    const float inv = any ? 1.0f / l : 0.0f;   // (all scores minus infinity: 0 times infinity)
+                    T *out = (T *)a.out + token * a.os[0] + head * a.os[1];
+                    typedef T loose4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const int col = 32 * t + 8 * g + 4 * h;
+                            const loose4 y{from_f32<T>(o[t][4 * g] * inv), from_f32<T>(o[t][4 * g + 1] * inv),
+                                           from_f32<T>(o[t][4 * g + 2] * inv), from_f32<T>(o[t][4 * g + 3] * inv)};
+                            if (col + 4 <= d) {
+                                *(loose4 *)(out + col) = y;
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 3; ++e)
+                                    if (col + e < d) out[col + e] = y[e];
+                            }
+                        }
+                } else {
+                    // Four columns of every row, then the next four; then the maxima and sums.
+                    f32x4 *p = (f32x4 *)parts.part(2 * blockIdx.x + (begun ? 0 : 1));
+                    const int at = 32 * wave + r, groups = (d + 3) / 4;
+#pragma unroll
+                    for (int t = 0; t < DT; ++t)
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            const int x = 8 * t + 2 * g + h;
+                            if (x < groups)
+                                p[x * b.rows + at] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
+                        }
+                    if (h == 0) {
+                        float2 *ml = (float2 *)(p + groups * b.rows);
+                        ml[at] = float2{m, any && m == -INFINITY && l == 0.0f ? 1.0f : l};
+                    }
+                }
+            }
+        }
+        if constexpr (!PAGED) {
+            more = false;
+        } else {
+            if (begun) front_block = b, done = ends;
+            // On to the next block.
+            if (last_here) {
+                more = false;
+            } else {
+                at.tile = 0;
+                if (++at.block == blocks_of(seq, a.share, ROWS)) {
+                    at.block = 0;
+                    if (++at.kv == c.kv) {
+                        at.kv = 0;
+                        do ++at.seq;
+                        while (at.seq < c.seqs && seq_of(c, at.seq).rows == 0);
+                    }
+                }
+                more = at.seq < c.seqs && !(at == end);
+            }
+        }
+    }
+    if (PAGED && tid == 0)
+        parts.marks[blockIdx.x] =
+            SelfMark{front, done, front_block.q0, front_block.kv, front_block.row0, front_block.rows, {0, 0}};
+}
+
+// The parts of blocks that were cut: a wave a row, a quarter or less of its
+// lanes a part.
+template <typename T, int DP> __global__ void __launch_bounds__(256) self_join(SelfArgs a, SelfParts parts) {
+    const int x = (int)blockIdx.x, lane = threadIdx.x & 63, d = a.c.width;
+    const SelfMark mark = parts.marks[x];
+    if (!(mark.front && mark.done)) return;
+    // The workgroups before it that lie inside of the block, and the one that began it.
+    int inside = 0;
+    for (int g = x - 1;; g -= 64) {
+        const bool in = g - lane >= 0 && parts.marks[g - lane].front && !parts.marks[g - lane].done;
+        const uint64_t not_in = ~__ballot(in);
+        if (not_in) {
+            inside += __ffsll((unsigned long long)not_in) - 1;
+            break;
+        }
+        inside += 64;
+    }
+    const int n = inside + 2, first = x - inside - 1;
+    const auto part = [&](int p) { return parts.part(p == 0 ? 2 * first + 1 : 2 * (first + p)); };
+    constexpr int COLS = DP / 4, AT_ONCE = 64 / COLS;    // lanes of a part (groups of four columns; 96: 24)
+    const int sub = lane / COLS, col = lane % COLS, groups = (d + 3) / 4, rows = mark.rows;
+    for (int i = blockIdx.y * 4 + (threadIdx.x >> 6); i < rows; i += gridDim.y * 4) {
+        // A lane a part: its maximum and sum.
+        const auto ml = [&](int p) { return ((const float2 *)((const f32x4 *)part(p) + groups * rows))[i]; };
+        float m = -INFINITY;
+        for (int p = lane; p < n; p += 64) m = fmaxf(m, ml(p).x);
+#pragma unroll
+        for (int w = 32; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
+        float l = 0.0f;
+        f32x4 o{};
+        for (int p0 = 0; p0 < n; p0 += 64) {
+            const int k = min(64, n - p0);
+            float w = 0.0f;
+            if (lane < k) {
+                const float2 q = ml(p0 + lane);
+                w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(q.x - m);
+                l = fmaf(w, q.y, l);
+            }
+#pragma unroll 4
+            for (int p1 = 0; p1 < k; p1 += AT_ONCE) {   // (every lane, for the shuffle)
+                const int p = p1 + sub;
+                const float wp = __shfl(w, min(p, 63), 64);
+                if (p < k && sub < AT_ONCE && col < groups) {
+                    const f32x4 v = ((const f32x4 *)part(p0 + p))[col * rows + i];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = fmaf(wp, v[e], o[e]);
+                }
+            }
+        }
+        l = wave_sum(l);
+        // The lanes of the same columns. (96: 24 lanes, 2 of them.)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float total = o[e];
+#pragma unroll
+            for (int s = 1; s < AT_ONCE; ++s) total += __shfl(o[e], col + s * COLS, 64);
+            o[e] = total;
+        }
+        if (lane >= COLS) continue;
+        // No maximum: no state (0), or scores of minus infinity alone.
+        const float inv = m == -INFINITY ? (l == 0.0f ? 0.0f : __builtin_nanf("")) : 1.0f / l;
+        const int row = mark.row0 + i;
+        T *out = (T *)a.out + ((uint64_t)mark.q0 + row / a.share) * a.os[0] +
+                 ((uint64_t)mark.kv * a.share + row % a.share) * a.os[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (4 * col + e < d) out[4 * col + e] = from_f32<T>(o[e] * inv);
+    }
+}
+
+// ---- launches --------------------------------------------------------------------------
+
+template <typename T, Held HELD, bool PAGED, int DP, int WAVES>
+static hipError_t launch_tiles(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
+    using C = SelfTile<T, HELD, DP, WAVES>;
+    SelfParts parts{};
+    if (PAGED) {
+        parts.marks = (SelfMark *)a.ws;
+        parts.parts = (float *)(parts.marks + f.groups);
+        parts.pitch = self_part_floats(f.part_rows, a.c.width);
+        parts.groups = (int)f.groups;
+        parts.least = (uint64_t)a.share * 4 * C::KB;
+    }
+    const hipError_t e = enqueue(self_tiles<T, HELD, PAGED, DP, WAVES>, dim3(f.groups), dim3(64 * WAVES), C::LDS, s, a, parts);
+    // (Blocks of one tile are not cut.)
+    if (e != hipSuccess || !PAGED || room(a.c) <= C::KB) return e;
+    return enqueue(self_join<T, DP>, dim3(f.groups, (f.part_rows + 15) / 16), dim3(256), 0, s, a, parts);
+}
+
+template <typename T, bool PAGED, int DP> static hipError_t launch_held(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
+    if constexpr (PAGED)
+        if (f.held == Held::Codes)
+            return f.waves == 1 ? launch_tiles<T, Held::Codes, true, DP, 1>(s, a, f)
+                                : launch_tiles<T, Held::Codes, true, DP, 4>(s, a, f);
+    if (f.held == Held::Loose) return launch_tiles<T, Held::Loose, PAGED, DP, 1>(s, a, f);
+    return f.waves == 1 ? launch_tiles<T, Held::Chunks, PAGED, DP, 1>(s, a, f)
+                        : launch_tiles<T, Held::Chunks, PAGED, DP, 4>(s, a, f);
+}
+
+template <typename T> static hipError_t launch_self(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
+    const auto go = [&](auto paged) {
+        constexpr bool PAGED = decltype(paged)::value;
+        if (a.c.width <= 32) return launch_held<T, PAGED, 32>(s, a, f);
+        if (a.c.width <= 64) return launch_held<T, PAGED, 64>(s, a, f);
+        if (a.c.width <= 96) return launch_held<T, PAGED, 96>(s, a, f);
+        return launch_held<T, PAGED, 128>(s, a, f);
+    };
+    return a.c.paged ? go(std::true_type()) : go(std::false_type());
+}
+
+}  // namespace rocm
