@@ -49,4 +49,29 @@ __device__ __forceinline__ auto below(float w0, float w1) {
     return __builtin_bit_cast(two, __builtin_elementwise_sub_sat(b, bits2{1, 1}));
 }
 
+// Codes as numbers of T, a word's four at a time.
+__device__ __forceinline__ void numbers_of(uint32_t w, float *v) {
+    // (Of the word and of its upper three bytes, as the conversions that pick a
+    // byte take them: bytes 0 and 2 of each.)
+    uint32_t u = w >> 8;
+    asm volatile("" : "+v"(u));
+    v[0] = (float)(int8_t)w, v[1] = (float)(int8_t)u, v[2] = (float)(int8_t)(w >> 16), v[3] = (float)(int8_t)(u >> 16);
+}
+template <typename T> __device__ __forceinline__ void numbers_of(uint32_t w, T *v) {
+    if constexpr (std::is_same<T, _Float16>::value) {
+        // 1024 and a number of 10 bits is 0x6400 and its bits: each code plus
+        // 128, less 1152, exactly.
+        typedef _Float16 two __attribute__((ext_vector_type(2)));
+        const uint32_t u = w ^ 0x80808080u;
+        const two a = __builtin_bit_cast(two, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - two{1152, 1152};
+        const two b = __builtin_bit_cast(two, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - two{1152, 1152};
+        v[0] = a[0], v[1] = a[1], v[2] = b[0], v[3] = b[1];
+    } else {
+        float f[4];
+        numbers_of(w, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(f[e]);
+    }
+}
+
 }  // namespace rocm

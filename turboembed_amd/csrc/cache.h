@@ -80,8 +80,9 @@ struct SelfArgs {
 };
 
 // How keys and values reach LDS: in aligned whole chunks, by themselves;
-// through registers, at any alignment; or as codes.
-enum class Held : int { Chunks, Loose, Codes };
+// through registers, at any alignment; int8 states as numbers, through
+// registers; or as they are, in aligned whole chunks, by themselves.
+enum class Held : int { Chunks, Loose, Codes, Bytes };
 
 // How a call is launched, from what the host knows of it: its rows and
 // sequences, not their lengths.

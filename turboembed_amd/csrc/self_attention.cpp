@@ -22,8 +22,8 @@ uint64_t parts_bytes(uint64_t groups, int rows, uint64_t all_rows, int width) {
 
 SelfLaunch self_plan(const SelfArgs &a) {
     SelfLaunch f{};
-    const uint64_t size = dt_bytes(a.dt), tokens = a.c.tokens, rows = tokens * a.share;   // (of a key head)
-    const uint64_t seqs = std::min<uint64_t>(a.c.seqs, tokens);
+    const uint64_t tokens = a.c.tokens, rows = tokens * a.share;   // (of a key head)
+    const uint64_t seqs = std::min<uint64_t>(a.c.seqs, tokens), size = a.i8 ? 1 : dt_bytes(a.dt);
     const auto whole = [&](const void *p, const uint64_t (&stride)[2]) {
         return (reinterpret_cast<uintptr_t>(p) | stride[0] * size | stride[1] * size) % 16 == 0;
     };
@@ -35,6 +35,9 @@ SelfLaunch self_plan(const SelfArgs &a) {
     // there are enough of them for every compute unit.
     f.waves = 1;
     if (f.held != Held::Loose && rows > 32 * seqs && (a.c.paged || a.c.kv * (rows / 128 + seqs) >= 512)) f.waves = 4;
+    // A wave alone makes numbers of codes as it reads them, four of them once.
+    // (F32's slow products leave it no need to.)
+    if (a.i8 && f.waves == 1 && chunks && a.dt != Dt::F32) f.held = Held::Bytes;
     const uint64_t blocks = a.c.kv * (rows / (32 * f.waves) + seqs);   // at most
     if (!a.c.paged) {
         if (blocks * 64 * f.waves > 1ull << 31)

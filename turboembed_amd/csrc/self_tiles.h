@@ -13,9 +13,10 @@
 // running one, in base 2 and F32: what it takes for a row's maximum moves only
 // when a score is 2^8 above the one that it was set by.
 //
-// Int8 states come through registers, a tile ahead: their codes are numbers of
-// every type, so LDS holds them as such, unscaled. A key's scale is a factor of
-// its scores, a value's one of its weights.
+// Int8 states' codes are numbers of every type, so they go into the products
+// unscaled: a key's scale is a factor of its scores, a value's one of its
+// weights. Four waves get them through registers, a tile ahead, and as numbers
+// into LDS; a wave alone has the codes themselves in LDS.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -33,13 +34,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T, Held HELD, int DP, int WAVES> struct SelfTile {
     static constexpr bool F32 = std::is_same<T, float>::value;
-    static constexpr bool CODES = HELD == Held::Codes;
+    static constexpr bool BYTES = HELD == Held::Bytes, CODES = HELD == Held::Codes || BYTES;
     static constexpr int ROWS = 32 * WAVES;
     static constexpr int KB = WAVES == 1 || F32 ? 32 : 64;
-    static constexpr int PITCH = DP * (int)sizeof(T), CPR = PITCH / 16;   // a row's bytes and chunks in LDS
+    static constexpr int PITCH = DP * (BYTES ? 1 : (int)sizeof(T)), CPR = PITCH / 16;   // a row's bytes and chunks in LDS
     static constexpr int BUF = KB * PITCH;
-    // (A wave alone writes a tile of codes once it has read the one before.)
-    static constexpr int BUFS = CODES && WAVES == 1 ? 1 : 2;
+    // (A wave alone writes a tile of codes' numbers once it has read the one before.)
+    static constexpr int BUFS = HELD == Held::Codes && WAVES == 1 ? 1 : 2;
     static constexpr int TILES = BUFS * 2 * BUF;
     // Behind the tiles: of codes, each buffer's scales of K and V, the exponent
     // of the unit of V's, and the keys to be added alone; of others, the keys
@@ -49,9 +50,11 @@ template <typename T, Held HELD, int DP, int WAVES> struct SelfTile {
     static constexpr int OCC = F32 ? (DP <= (HELD == Held::Chunks ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;
     // LDS serves 256 bytes a cycle: 16 keys of one chunk of K (a 16-byte
     // read's pass), 4 keys of 4 chunks of V (a transposing read's).
-    static constexpr int PERIOD = CPR % 16 == 0 ? 1 : CPR % 8 == 0 ? 2 : 4;   // keys until the banks repeat
-    static __device__ __forceinline__ int swap_k(int key) { return key / PERIOD % (16 / PERIOD); }
+    static constexpr int PERIOD = CPR % 16 == 0 ? 1 : CPR % 8 == 0 ? 2 : CPR % 4 == 0 ? 4 : 8;   // keys until the banks repeat
+    static __device__ __forceinline__ int swap_k(int key) { return CPR == 6 ? 0 : key / PERIOD % (16 / PERIOD); }
     static __device__ __forceinline__ int swap_v(int key) {
+        // (Of codes: 8 keys of 2 chunks, 0 to 3 and 8 to 11 or those 4 on.)
+        if (BYTES) return CPR % 8 == 0 ? 2 * ((key >> 1 & 1) | (key >> 3 & 1) << 1) : CPR % 4 == 0 ? 2 * (key >> 3 & 1) : 0;
         if (F32) return CPR % 16 == 0 ? (key >> 2 & 1) * 8 : 0;
         return PERIOD == 1 ? (key & 3) * 4 : PERIOD == 2 ? (key >> 1 & 1) * 4 : 0;
     }
@@ -331,6 +334,13 @@ struct SelfParts {
 
 // ---- the kernel ------------------------------------------------------------------------
 
+// v, as one that the compiler knows nothing of: what is made of it in a path
+// that is rarely taken is made there, and no register holds it meanwhile.
+__device__ __forceinline__ int fresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 template <typename T>
 __device__ __forceinline__ void two_of(float w0, float w1, T (&hi)[2], T (&lo)[2], bool positive) {
     if (positive) {
@@ -366,27 +376,34 @@ self_tiles(SelfArgs a, SelfParts parts) {
     const CacheArgs &c = a.c;
 
     // ---- a tile's way to LDS
-    // Of chunks, load j of a wave fills 64 in order; of codes, 64 units.
-    constexpr int UN = CODES ? C::unit() : E, UPR = DP / UN;
+    // Of chunks, load j of a wave fills 64 in order; of codes that come through
+    // registers, 64 units.
+    constexpr bool STAGED = HELD == Held::Codes, BYTES = C::BYTES, DIRECT = HELD == Held::Chunks || BYTES;
+    typedef typename std::conditional<CODES, int8_t, T>::type H;
+    constexpr int UN = STAGED ? C::unit() : 16 / (int)sizeof(H), UPR = DP / UN;
     constexpr int NL = KB * UPR / 64 / WAVES;
     static_assert(NL * 64 * WAVES == KB * UPR, "whole loads a wave");
     constexpr int GROUP = 16;                 // keys that lie in one page, where pages are whole groups
-    constexpr int PER = CPR / 4;              // ...and their loads of chunks
-    const auto unit_of = [&](int j) { return (wave * NL + j) * 64 + lane; };
-    const auto key_of = [&](int j) { return unit_of(j) / UPR; };
-    const auto col_k = [&](int j) { return CODES ? unit_of(j) % UPR * UN : (unit_of(j) % CPR ^ C::swap_k(key_of(j))) * E; };
-    const auto col_v = [&](int j) { return CODES ? unit_of(j) % UPR * UN : (unit_of(j) % CPR ^ C::swap_v(key_of(j))) * E; };
-    typedef typename std::conditional<CODES, int8_t, T>::type H;
+    const auto group_at = [&](int j) { return (wave * NL + j) * 64 / CPR / GROUP * GROUP; };
+    const auto unit_at = [&](int j, int l) { return (wave * NL + j) * 64 + l; };
+    const auto key_at = [&](int j, int l) { return unit_at(j, l) / UPR; };
+    const auto col_k_at = [&](int j, int l) {
+        return (STAGED ? unit_at(j, l) % UPR : unit_at(j, l) % CPR ^ C::swap_k(key_at(j, l))) * UN;
+    };
+    const auto col_v_at = [&](int j, int l) {
+        return (STAGED ? unit_at(j, l) % UPR : unit_at(j, l) % CPR ^ C::swap_v(key_at(j, l))) * UN;
+    };
     // (Chunks: bytes from a tile's or a group's first key, which 31 bits hold.)
     uint32_t ko[NL], vo[NL];
-    if constexpr (HELD == Held::Chunks)
+    if constexpr (DIRECT)
 #pragma unroll
         for (int j = 0; j < NL; ++j) {
-            const uint32_t key = PAGED ? key_of(j) % GROUP : key_of(j);
-            ko[j] = (key * (uint32_t)c.ks[0] + col_k(j)) * (uint32_t)sizeof(T);
-            vo[j] = (key * (uint32_t)c.vs[0] + col_v(j)) * (uint32_t)sizeof(T);
+            const uint32_t key = PAGED ? key_at(j, lane) % GROUP : key_at(j, lane);
+            ko[j] = (key * (uint32_t)c.ks[0] + col_k_at(j, lane)) * (uint32_t)sizeof(H);
+            vo[j] = (key * (uint32_t)c.vs[0] + col_v_at(j, lane)) * (uint32_t)sizeof(H);
         }
-    const bool groups_whole = PAGED && c.page_tokens % GROUP == 0;   // uniform
+    // (uniform; where a load has keys of two groups, a lane takes its own)
+    const bool groups_whole = PAGED && GROUP * CPR % 64 == 0 && c.page_tokens % GROUP == 0;
 
     if (HELD == Held::Chunks && d < DP) {   // uniform
         // (Columns past the width keep these zeros.)
@@ -394,12 +411,12 @@ self_tiles(SelfArgs a, SelfParts parts) {
     }
 
     Place at{}, end{};
-    bool front = false, done = false;    // this workgroup starts inside of a block; it has ended it
-    Block front_block{};
+    bool front = false;    // this workgroup starts inside of a block
     if constexpr (PAGED) {
         const Cuts<ROWS, KB> cuts(a, (int)blockIdx.x, parts.groups, parts.least);
         if (cuts.any) at = cuts.from, end = cuts.to, front = at.tile > 0;
         else at = end = Place{c.seqs, 0, 0, 0};
+        if (!front && tid == 0) parts.marks[blockIdx.x] = SelfMark{};
     } else {
         const Turn<ROWS, C::TILES / 4> turn(a, blockIdx.x, smem, 64 * WAVES);
         if (!turn.any) return;
@@ -441,17 +458,26 @@ self_tiles(SelfArgs a, SelfParts parts) {
         bool alive = false;             // of the tile on its way: key `lane` is a state
         // Codes on their way, and their scales (a lane a key).
         typedef uint32_t codes_t __attribute__((ext_vector_type(UN >= 16 ? 4 : UN >= 8 ? 2 : 1), aligned(1)));
-        codes_t kq[CODES ? NL : 1], vq[CODES ? NL : 1];
+        codes_t kq[STAGED ? NL : 1], vq[STAGED ? NL : 1];
         float sk = 0.0f, sv = 0.0f;
         int unit = LEAST_UNIT;          // the exponent of the weights' unit (F16 codes)
 
-        const auto read_codes = [&](const int8_t *p, int n) {
+        // n of a unit's codes, a word at a time.
+        const auto some_codes = [&](const int8_t *p, int n) {
+            typedef uint32_t loose __attribute__((aligned(1)));
             codes_t q{};
-            if (n >= UN) return *(const codes_t *)p;
-            if (n > 0) {
 #pragma unroll
-                for (int i = 0; i < UN; ++i)
-                    if (i < n) q[i / 4] |= (uint32_t)(uint8_t)p[i] << (8 * (i & 3));
+            for (int w = 0; w < UN / 4; ++w) {
+                uint32_t x = 0;
+                if (n >= 4 * w + 4) {
+                    x = *(const loose *)(p + 4 * w);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        if (4 * w + i < n) x |= (uint32_t)(uint8_t)p[4 * w + i] << (8 * i);
+                }
+                q[w] = x;
+                __builtin_amdgcn_sched_barrier(0);
             }
             return q;
         };
@@ -459,69 +485,96 @@ self_tiles(SelfArgs a, SelfParts parts) {
         const auto load = [&](int t, int buf) {
             char *K = smem + buf * 2 * BUF, *V = K + BUF;
             alive = slot >= 0;
-            if constexpr (HELD == Held::Chunks) {
-                // (As buffer loads where a base is common to the lanes: those
-                // take 32-bit offsets.)
-                typedef __attribute__((address_space(3))) void *to;
-                typedef __attribute__((address_space(1))) const void *from;
-                if (!PAGED || groups_whole) {   // uniform
-                    const int last = b.hi - 1 - t * KB;
-                    const auto rsrc = [](const T *p) {
-                        return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, -1, 0x00020000);
-                    };
-                    const auto send = [&](__amdgpu_buffer_rsrc_t tile, uint32_t at, char *dst) {
-                        __builtin_amdgcn_raw_ptr_buffer_load_lds(tile, (to)dst, 16, (int)at, 0, 0, 0);
-                    };
-#pragma unroll
-                    for (int j = 0; j < NL; ++j) {
-                        uint64_t s;
-                        uint32_t back = 0;
-                        if constexpr (PAGED) {
-                            // (Without a page: slot 0, whose keys are not looked at.)
-                            s = (uint64_t)max(0, __builtin_amdgcn_readlane(slot, (wave * NL + j) / PER * GROUP));
-                        } else {
-                            s = (uint64_t)b.q0 + (uint64_t)t * KB;
-                            if (last < KB - 1) back = (uint32_t)max(0, key_of(j) - last) * (uint32_t)sizeof(T);
-                        }
-                        if (d == DP || col_k(j) < d)
-                            send(rsrc(K0 + s * c.ks[0]), ko[j] - back * (uint32_t)c.ks[0], K + (wave * NL + j) * 1024);
-                        if (d == DP || col_v(j) < d)
-                            send(rsrc(V0 + s * c.vs[0]), vo[j] - back * (uint32_t)c.vs[0], V + (wave * NL + j) * 1024);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < NL; ++j) {
-                        const uint64_t s = (uint64_t)max(0, __shfl(slot, key_of(j), 64));
-                        if (d == DP || col_k(j) < d)
-                            __builtin_amdgcn_global_load_lds((from)(K0 + s * c.ks[0] + col_k(j)),
-                                                             (to)(K + (wave * NL + j) * 1024), 16, 0, 0);
-                        if (d == DP || col_v(j) < d)
-                            __builtin_amdgcn_global_load_lds((from)(V0 + s * c.vs[0] + col_v(j)),
-                                                             (to)(V + (wave * NL + j) * 1024), 16, 0, 0);
-                    }
-                }
-            } else if constexpr (HELD == Held::Loose) {
-#pragma unroll
-                for (int j = 0; j < NL; ++j) {
-                    const int s = __shfl(slot, key_of(j), 64), at = unit_of(j) * 16, nk = d - col_k(j), nv = d - col_v(j);
-                    *(vec *)(K + at) = s >= 0 && nk > 0 ? read_chunk(K0 + (uint64_t)s * c.ks[0] + col_k(j), nk) : vec{};
-                    *(vec *)(V + at) = s >= 0 && nv > 0 ? read_chunk(V0 + (uint64_t)s * c.vs[0] + col_v(j), nv) : vec{};
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < NL; ++j) {
-                    const int s = __shfl(slot, key_of(j), 64), n = s >= 0 ? d - col_k(j) : 0;
-                    const uint64_t at = (uint64_t)max(0, s);
-                    kq[j] = read_codes(K0 + at * c.ks[0] + col_k(j), n);
-                    vq[j] = read_codes(V0 + at * c.vs[0] + col_v(j), n);
-                }
+            if constexpr (CODES)
                 if (wave == 0) {
                     sk = alive ? c.k_scales[(uint64_t)slot * c.kss + b.kv] : 0.0f;
                     sv = alive ? c.v_scales[(uint64_t)slot * c.vss + b.kv] : 0.0f;
                 }
+            if constexpr (DIRECT) {
+                // (As buffer loads where a base is common to the lanes: those
+                // take 32-bit offsets.)
+                typedef __attribute__((address_space(3))) void *to;
+                typedef __attribute__((address_space(1))) const void *from;
+                const auto rsrc = [](const H *p) {
+                    return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, -1, 0x00020000);
+                };
+                const auto send = [&](__amdgpu_buffer_rsrc_t tile, uint32_t at, char *dst) {
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(tile, (to)dst, 16, (int)at, 0, 0, 0);
+                };
+                const auto base = [&](int j) {
+                    // (Without a page: slot 0, whose keys are not looked at.)
+                    if constexpr (PAGED)
+                        return (uint64_t)max(0, __builtin_amdgcn_readlane(slot, group_at(j)));
+                    return (uint64_t)b.q0 + (uint64_t)t * KB;
+                };
+                const int last = b.hi - 1 - t * KB;
+                if ((PAGED ? groups_whole : last >= KB - 1) && d == DP) {   // uniform
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) {
+                        const uint64_t s = base(j);
+                        send(rsrc(K0 + s * c.ks[0]), ko[j], K + (wave * NL + j) * 1024);
+                        send(rsrc(V0 + s * c.vs[0]), vo[j], V + (wave * NL + j) * 1024);
+                    }
+                } else if (!PAGED || groups_whole) {   // uniform
+                    const int lane = fresh(tid & 63);
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) {
+                        const uint64_t s = base(j);
+                        const uint32_t back = PAGED ? 0 : (uint32_t)max(0, key_at(j, lane) - last) * (uint32_t)sizeof(H);
+                        if (col_k_at(j, lane) < d)
+                            send(rsrc(K0 + s * c.ks[0]), ko[j] - back * (uint32_t)c.ks[0], K + (wave * NL + j) * 1024);
+                        if (col_v_at(j, lane) < d)
+                            send(rsrc(V0 + s * c.vs[0]), vo[j] - back * (uint32_t)c.vs[0], V + (wave * NL + j) * 1024);
+                    }
+                } else {
+                    const int lane = fresh(tid & 63);
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) {
+                        const uint64_t s = (uint64_t)max(0, __shfl(slot, key_at(j, lane), 64));
+                        const int ck = col_k_at(j, lane), cv = col_v_at(j, lane);
+                        if (ck < d)
+                            __builtin_amdgcn_global_load_lds((from)(K0 + s * c.ks[0] + ck), (to)(K + (wave * NL + j) * 1024),
+                                                             16, 0, 0);
+                        if (cv < d)
+                            __builtin_amdgcn_global_load_lds((from)(V0 + s * c.vs[0] + cv), (to)(V + (wave * NL + j) * 1024),
+                                                             16, 0, 0);
+                    }
+                }
+            } else if constexpr (HELD == Held::Loose) {
+                const int lane = fresh(tid & 63);
+#pragma unroll
+                for (int j = 0; j < NL; ++j) {
+                    const int s = __shfl(slot, key_at(j, lane), 64), at = unit_at(j, lane) * 16;
+                    const int ck = col_k_at(j, lane), cv = col_v_at(j, lane), nk = d - ck, nv = d - cv;
+                    *(vec *)(K + at) = s >= 0 && nk > 0 ? read_chunk(K0 + (uint64_t)s * c.ks[0] + ck, nk) : vec{};
+                    *(vec *)(V + at) = s >= 0 && nv > 0 ? read_chunk(V0 + (uint64_t)s * c.vs[0] + cv, nv) : vec{};
+                }
+            } else {
+                if (d % UN == 0) {   // uniform
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) {
+                        // (Without a state: slot 0's; past the width: the first
+                        // ones again. Neither counts: their weights are 0, the
+                        // sums of those columns nobody's, and codes are numbers.)
+                        const uint64_t s = (uint64_t)max(0, __shfl(slot, key_at(j, lane), 64));
+                        const int col = d == DP || col_k_at(j, lane) < d ? col_k_at(j, lane) : 0;
+                        kq[j] = *(const codes_t *)(K0 + s * c.ks[0] + col);
+                        vq[j] = *(const codes_t *)(V0 + s * c.vs[0] + col);
+                    }
+                } else {
+                    const int lane = fresh(tid & 63);
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) {
+                        const uint64_t s = (uint64_t)max(0, __shfl(slot, key_at(j, lane), 64));
+                        const int col = col_k_at(j, lane);
+                        kq[j] = some_codes(K0 + s * c.ks[0] + col, d - col);
+                        vq[j] = some_codes(V0 + s * c.vs[0] + col, d - col);
+                    }
+                }
             }
         };
-        // Codes that have come, as numbers of T, into LDS, and their scales.
+        // Codes that have come through registers, as numbers of T, into LDS, and the
+        // scales of all codes.
         const auto put = [&](int t, int buf) {
             if constexpr (CODES) {
                 char *K = smem + buf * 2 * BUF, *V = K + BUF;
@@ -529,20 +582,23 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 const auto spread = [&](const codes_t &q, char *row, int col, int swap) {
 #pragma unroll
                     for (int e0 = 0; e0 < UN; e0 += E) {
-                        vec x;
+                        T x[E];
 #pragma unroll
-                        for (int e = 0; e < E; ++e) {
-                            const int i = e0 + e;
-                            x[e] = (T)(float)(int8_t)(q[i / 4] >> (8 * (i & 3)));
-                        }
-                        *(vec *)(row + (((col + e0) / E) ^ swap) * 16) = x;
+                        for (int e = 0; e < E; e += 4) numbers_of(q[(e0 + e) / 4], x + e);
+                        vec y;
+#pragma unroll
+                        for (int e = 0; e < E; ++e) y[e] = x[e];
+                        *(vec *)(row + (((col + e0) / E) ^ swap) * 16) = y;
                     }
                 };
+                if constexpr (STAGED)
 #pragma unroll
                 for (int j = 0; j < NL; ++j) {
-                    const int key = key_of(j);
-                    spread(kq[j], K + key * PITCH, col_k(j), C::swap_k(key));
-                    spread(vq[j], V + key * PITCH, col_v(j), C::swap_v(key));
+                    const int key = key_at(j, lane), col = col_k_at(j, lane);
+                    spread(kq[j], K + key * PITCH, col, C::swap_k(key));
+                    __builtin_amdgcn_sched_barrier(0);   // (one unit's numbers in registers at a time)
+                    spread(vq[j], V + key * PITCH, col, C::swap_v(key));
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 if (wave == 0) {
                     bool alone = !(fabsf(sv) < INFINITY);
@@ -578,18 +634,21 @@ self_tiles(SelfArgs a, SelfParts parts) {
             load(t0, 0);
             next_slot = slot_at(t0 + 1);
         }
-        // This row's q: of each 2 E columns the lane's half's E.
-        vec q[CPR / 2];
+        // This row's q: of each 2 E columns the lane's half's E (of codes as they
+        // are, whose chunks are 2 E: of each 4 E the half's 2 E).
+        constexpr int NQ = DP / (2 * E);
+        vec q[NQ];
         {
+            const int h = fresh(lane) >> 5;   // (else its comparisons are kept from block to block)
             const T *p = (const T *)a.q + token * a.qs[0] + head * a.qs[1];
 #pragma unroll
-            for (int s = 0; s < CPR / 2; ++s) {
-                const int col = (2 * s + h) * E;
+            for (int s = 0; s < NQ; ++s) {
+                const int col = BYTES ? (2 * (s >> 1) + h) * 2 * E + (s & 1) * E : (2 * s + h) * E;
                 q[s] = read_chunk(p + col, d - col);
             }
             if (a.turn != 1.0f)   // uniform
 #pragma unroll
-                for (int s = 0; s < CPR / 2; ++s)
+                for (int s = 0; s < NQ; ++s)
 #pragma unroll
                     for (int e = 0; e < E; ++e) q[s][e] = from_f32<T>(to_f32(q[s][e]) * a.turn);
         }
@@ -609,7 +668,22 @@ self_tiles(SelfArgs a, SelfParts parts) {
             const auto chunk = [&](int x, int u) {
                 return *(const vec *)(K + 32 * u * PITCH + kr + ((2 * x + h) ^ ks) * 16);
             };
-            if constexpr (F32) {
+            if constexpr (BYTES) {
+#pragma unroll
+                for (int x = 0; x < CPR / 2; ++x) {
+                    typedef uint32_t words __attribute__((ext_vector_type(4)));
+                    const words w = *(const words *)(K + kr + ((2 * x + h) ^ ks) * 16);
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        T n[8];
+                        numbers_of(w[2 * z], n), numbers_of(w[2 * z + 1], n + 4);
+                        frag f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = n[e];
+                        s[0] = Mma<T>::run(f, q[2 * x + z], s[0]);
+                    }
+                }
+            } else if constexpr (F32) {
                 // (A chunk read two ahead of its products, which are slow enough to hide it.)
                 vec k[3] = {chunk(0, 0), chunk(1, 0)};
 #pragma unroll
@@ -668,17 +742,30 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     }
 #pragma unroll
                     for (int t = 0; t < DT; ++t) {
-                        const int x = 4 * t + 2 * (g & 1) + ((n >> 1) & 1);
-                        const auto place = [&](int k) {
-                            return (__attribute__((address_space(3))) s4 *)(V + k * PITCH + (x ^ C::swap_v(k)) * 16 +
-                                                                             (n & 1) * 8);
-                        };
-                        struct {
-                            s4 lo, hi;
-                        } v;
-                        v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(16 * j + key));
-                        v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(16 * j + 8 + key));
-                        vt[t] = __builtin_bit_cast(frag, v);
+                        if constexpr (BYTES) {
+                            // (Codes: 8 keys by 16 columns, and a lane gets its column's 8.)
+                            typedef int w2 __attribute__((ext_vector_type(2)));
+                            const int k = 16 * j + 8 * (n >> 3) + 4 * h + ((n >> 1) & 3);
+                            const w2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                (__attribute__((address_space(3))) w2 *)(V + k * PITCH +
+                                                                         ((2 * t + (g & 1)) ^ C::swap_v(k)) * 16 + (n & 1) * 8));
+                            T y[8];
+                            numbers_of((uint32_t)w[0], y), numbers_of((uint32_t)w[1], y + 4);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) vt[t][e] = y[e];
+                        } else {
+                            const int x = 4 * t + 2 * (g & 1) + ((n >> 1) & 1);
+                            const auto place = [&](int k) {
+                                return (__attribute__((address_space(3))) s4 *)(V + k * PITCH + (x ^ C::swap_v(k)) * 16 +
+                                                                                 (n & 1) * 8);
+                            };
+                            struct {
+                                s4 lo, hi;
+                            } v;
+                            v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(16 * j + key));
+                            v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(16 * j + 8 + key));
+                            vt[t] = __builtin_bit_cast(frag, v);
+                        }
                         o[t] = Mma<T>::run(vt[t], f, o[t]);
                     }
                     if constexpr (TWO)
@@ -703,6 +790,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
         // their keys are added one by one, and are 0 for the products.
         const auto add_alone = [&](const char *V, const float *side, const floatx16 (&s)[SUB], uint64_t seen, uint64_t bad,
                                    float scale, float base) {
+            const int h = fresh(lane) >> 5;
             for (; bad; bad &= bad - 1) {
                 const int key = __ffsll((unsigned long long)bad) - 1;
                 const int u = key >> 5, i = (key >> 3 & 3) * 4 + (key & 3), from = key >> 2 & 1;
@@ -715,13 +803,27 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 float w = __builtin_amdgcn_exp2f(fmaf(x, scale, -base));
                 if constexpr (CODES) w *= side[KB + key];
                 const bool see = seen >> key & 1;
+                // (Four at a time: this path is to cost no registers.)
+                typedef T four __attribute__((ext_vector_type(4)));
+                const char *row = V + key * PITCH + (BYTES ? 4 * h : F32 ? 0 : 8 * h);
+                const int swap = C::swap_v(key);
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
 #pragma unroll
-                    for (int n = 0; n < 16; ++n) {
-                        const int col = 32 * t + 8 * (n >> 2) + 4 * h + (n & 3);
-                        const T v = *(const T *)(V + key * PITCH + (col / E ^ C::swap_v(key)) * 16 + col % E * (int)sizeof(T));
-                        o[t][n] = see ? fmaf(w, to_f32(v), o[t][n]) : o[t][n];
+                    for (int g = 0; g < 4; ++g) {
+                        four v;
+                        if constexpr (BYTES) {
+                            T n[4];
+                            numbers_of(*(const uint32_t *)(row + ((2 * t + (g >> 1)) ^ swap) * 16 + (g & 1) * 8), n);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] = n[e];
+                        } else {
+                            v = *(const four *)(row + ((F32 ? 8 * t + 2 * g + h : 4 * t + g) ^ swap) * 16);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[t][4 * g + e] = see ? fmaf(w, to_f32(v[e]), o[t][4 * g + e]) : o[t][4 * g + e];
+                        __builtin_amdgcn_sched_barrier(0);
                     }
             }
         };
@@ -801,22 +903,24 @@ self_tiles(SelfArgs a, SelfParts parts) {
         for (int t = t0, buf = 0; t < t1; ++t, buf ^= C::BUFS - 1) {
             char *K = smem + buf * 2 * BUF, *V = K + BUF;
             float *side = (float *)(smem + C::TILES + buf * C::SIDE);
+            if constexpr (!STAGED) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
             if constexpr (CODES) put(t, buf);
-            else __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
             const uint64_t live = __ballot(alive);
             const bool partial = t * KB + KB - 1 > all_hi || t * KB < all_lo;   // uniform: not every row sees all of it
             if (!CODES && live != FULL) {   // uniform
                 // A value that is no state's weighs 0, but not if it is no number.
+                const int lane = fresh(tid & 63);
 #pragma unroll
                 for (int j = 0; j < NL; ++j)
-                    if (!((live >> key_of(j)) & 1)) *(vec *)(V + unit_of(j) * 16) = vec{};
+                    if (!((live >> key_at(j, lane)) & 1)) *(vec *)(V + unit_at(j, lane) * 16) = vec{};
             }
             uint64_t bad = 0;
             if (!CODES && partial) {
                 // Keys of this wave's chunks with an infinity or a NaN among their values.
+                const int lane = fresh(tid & 63);
 #pragma unroll
                 for (int j = 0; j < NL; ++j) {
-                    const vec x = *(const vec *)(V + unit_of(j) * 16);
+                    const vec x = *(const vec *)(V + unit_at(j, lane) * 16);
                     float sum = 0.0f;
 #pragma unroll
                     for (int e = 0; e < E; ++e) sum = fmaf(to_f32(x[e]), 0.0f, sum);
@@ -846,9 +950,10 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 if constexpr (CODES) {
                     if (tid < KB && (bad >> tid & 1)) side[KB + tid] = 0.0f;
                 } else {
+                    const int lane = fresh(tid & 63);
 #pragma unroll
                     for (int j = 0; j < NL; ++j)
-                        if ((bad >> key_of(j)) & 1) *(vec *)(V + unit_of(j) * 16) = vec{};
+                        if ((bad >> key_at(j, lane)) & 1) *(vec *)(V + unit_at(j, lane) * 16) = vec{};
                 }
                 __syncthreads();
             };
@@ -862,6 +967,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
         }
 
         if (work) {
+            const int h = fresh(lane) >> 5;
             l = both_sum(l);
             if constexpr (CODES && F16) {
                 const float f = __uint_as_float((uint32_t)(127 + my_unit) << 23);
@@ -910,7 +1016,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
         if constexpr (!PAGED) {
             more = false;
         } else {
-            if (begun) front_block = b, done = ends;
+            if (begun && tid == 0) parts.marks[blockIdx.x] = SelfMark{1, ends, b.q0, b.kv, b.row0, b.rows, {0, 0}};
             // On to the next block.
             if (last_here) {
                 more = false;
@@ -928,9 +1034,6 @@ self_tiles(SelfArgs a, SelfParts parts) {
             }
         }
     }
-    if (PAGED && tid == 0)
-        parts.marks[blockIdx.x] =
-            SelfMark{front, done, front_block.q0, front_block.kv, front_block.row0, front_block.rows, {0, 0}};
 }
 
 // The parts of blocks that were cut: a wave a row, a quarter or less of its
@@ -1027,6 +1130,8 @@ template <typename T, bool PAGED, int DP> static hipError_t launch_held(hipStrea
         if (f.held == Held::Codes)
             return f.waves == 1 ? launch_tiles<T, Held::Codes, true, DP, 1>(s, a, f)
                                 : launch_tiles<T, Held::Codes, true, DP, 4>(s, a, f);
+    if constexpr (PAGED && !std::is_same<T, float>::value)
+        if (f.held == Held::Bytes) return launch_tiles<T, Held::Bytes, true, DP, 1>(s, a, f);
     if (f.held == Held::Loose) return launch_tiles<T, Held::Loose, PAGED, DP, 1>(s, a, f);
     return f.waves == 1 ? launch_tiles<T, Held::Chunks, PAGED, DP, 1>(s, a, f)
                         : launch_tiles<T, Held::Chunks, PAGED, DP, 4>(s, a, f);
