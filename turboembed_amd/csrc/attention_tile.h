@@ -21,6 +21,16 @@ __device__ __forceinline__ float both_max(float v) {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// ...of the four lanes 16 apart.
+__device__ __forceinline__ float four_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return both_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float four_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return both_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
 template <typename T> struct Chunk {   // 16 bytes of a row
     static constexpr int N = 16 / sizeof(T);
     typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
@@ -48,6 +58,25 @@ __device__ __forceinline__ auto below(float w0, float w1) {
     else b = bits2{(unsigned short)(__float_as_uint(w0) >> 16), (unsigned short)(__float_as_uint(w1) >> 16)};
     return __builtin_bit_cast(two, __builtin_elementwise_sub_sat(b, bits2{1, 1}));
 }
+
+// The product whose result has M rows and columns: lane l has column l % M of
+// it, and rows 4 (64 / M) (i / 4) + 4 (l / M) + i % 4 in register i. 16-bit
+// operands: row or column l % M, 8 steps of the inner width from 8 (l / M) on.
+template <typename T, int M> struct Product : Mma<T> {};
+template <> struct Product<_Float16, 16> {
+    typedef half8 frag;
+    typedef floatx4 acc;
+    static __device__ __forceinline__ acc run(frag a, frag b, acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Product<__bf16, 16> {
+    typedef bf16x8 frag;
+    typedef floatx4 acc;
+    static __device__ __forceinline__ acc run(frag a, frag b, acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
 
 // Codes as numbers of T, a word's four at a time.
 __device__ __forceinline__ void numbers_of(uint32_t w, float *v) {

@@ -88,7 +88,7 @@ enum class Held : int { Chunks, Loose, Codes, Bytes };
 // sequences, not their lengths.
 struct SelfLaunch {
     Held held;
-    int waves;           // of a workgroup
+    int rows;            // of a block: 16 or 32 (a wave's), or 128 (four waves')
     uint32_t groups;     // workgroups: of a prompt, the most blocks that there can be
     int part_rows;       // the most rows of a part
 };

@@ -10,9 +10,11 @@ namespace rocm {
 
 namespace {
 
-// Workgroups of a call over a cache: as many as a card holds at once, of blocks
-// of 32 rows (a wave) or 128 (four).
-int most_groups(int waves) { return waves == 1 ? 1280 : 512; }
+// Workgroups of a call over a cache, by its blocks' rows.
+int most_groups(int rows) {
+    if (getenv("TG")) return atoi(getenv("TG"));
+    return rows == 128 ? 512 : 3072;
+}
 
 uint64_t parts_bytes(uint64_t groups, int rows, uint64_t all_rows, int width) {
     return groups * (sizeof(SelfMark) + 2 * 4 * self_part_floats((int)std::min<uint64_t>(rows, all_rows), width));
@@ -32,29 +34,31 @@ SelfLaunch self_plan(const SelfArgs &a) {
                         std::max(a.c.ks[0], a.c.vs[0]) < (1u << 31) / 64 / 4;
     f.held = a.i8 ? Held::Codes : chunks ? Held::Chunks : Held::Loose;
     // Blocks of 128 rows, where sequences have more than a wave's on average and
-    // there are enough of them for every compute unit.
-    f.waves = 1;
-    if (f.held != Held::Loose && rows > 32 * seqs && (a.c.paged || a.c.kv * (rows / 128 + seqs) >= 512)) f.waves = 4;
+    // there are enough of them for every compute unit; of 16, where they have no
+    // more.
+    f.rows = 32;
+    if (f.held != Held::Loose && rows > 32 * seqs && (a.c.paged || a.c.kv * (rows / 128 + seqs) >= 512)) f.rows = 128;
     // A wave alone makes numbers of codes as it reads them, four of them once.
     // (F32's slow products leave it no need to.)
-    if (a.i8 && f.waves == 1 && chunks && a.dt != Dt::F32) f.held = Held::Bytes;
-    const uint64_t blocks = a.c.kv * (rows / (32 * f.waves) + seqs);   // at most
+    if (a.i8 && f.rows == 32 && chunks && a.dt != Dt::F32) f.held = Held::Bytes;
+    if (a.c.paged && a.dt != Dt::F32 && rows <= 16 * seqs && (f.held == Held::Bytes || f.held == Held::Chunks)) f.rows = 16;
+    const uint64_t blocks = a.c.kv * (rows / f.rows + seqs);   // at most
     if (!a.c.paged) {
-        if (blocks * 64 * f.waves > 1ull << 31)
+        if (blocks * (f.rows == 128 ? 256 : 64) > 1ull << 31)
             fail(TURBO_E_CAPACITY, "rocm: a prompt of " + std::to_string(blocks) + " workgroups");
         f.groups = (uint32_t)blocks;
         return f;
     }
     const uint64_t tiles = ((uint64_t)room(a.c) + 31) / 32;
-    f.groups = (uint32_t)std::min<uint64_t>(most_groups(f.waves), std::max<uint64_t>(1, blocks * std::max<uint64_t>(1, tiles)));
-    f.part_rows = (int)std::min<uint64_t>(32 * f.waves, rows);
+    f.groups = (uint32_t)std::min<uint64_t>(most_groups(f.rows), std::max<uint64_t>(1, blocks * std::max<uint64_t>(1, tiles)));
+    f.part_rows = (int)std::min<uint64_t>(f.rows, rows);
     return f;
 }
 
 uint64_t self_workspace(uint64_t tokens, uint64_t seqs, int heads, int kv, int width) {
     if (tokens == 0 || seqs == 0) return 0;
     const uint64_t rows = tokens * (heads / kv);
-    return std::max(parts_bytes(most_groups(1), 32, rows, width), parts_bytes(most_groups(4), 128, rows, width));
+    return std::max(parts_bytes(most_groups(32), 32, rows, width), parts_bytes(most_groups(128), 128, rows, width));
 }
 
 hipError_t self_attention(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {

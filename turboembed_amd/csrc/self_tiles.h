@@ -4,12 +4,12 @@
 //
 // The rows of a (sequence, key head) are its tokens' heads that read it, row r
 // token r / share, head kv * share + r % share: its keys and values are read
-// once for all of them. 32 of them are a wave's; a block is one wave's or four
-// waves'. A block's keys pass through LDS in tiles of KB. Scores are computed
-// transposed, S^T = K Q^T, so that a lane holds one row (lane % 32) and 16 of 32
-// keys, the other 16 in the lane 32 away; O^T += V^T P^T then takes P as the score
-// registers hold it, against V's columns for the same keys in that order (16-bit
-// values by LDS reads that transpose, F32 values one by one). The softmax is the
+// once for all of them. M of them, 32 or 16, are a wave's; a block is one wave's
+// or four waves'. A block's keys pass through LDS in tiles of KB. Scores are
+// computed transposed, S^T = K Q^T, so that a lane holds one row (lane % M) and
+// M / 2 of 32 keys, the others in the lanes M apart; O^T += V^T P^T then takes P as
+// the score registers hold it, against V's columns for the same keys in that
+// order (16-bit values by LDS reads that transpose, F32 values one by one). The softmax is the
 // running one, in base 2 and F32: what it takes for a row's maximum moves only
 // when a score is 2^8 above the one that it was set by.
 //
@@ -32,10 +32,10 @@ namespace rocm {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-template <typename T, Held HELD, int DP, int WAVES> struct SelfTile {
+template <typename T, Held HELD, int DP, int WAVES, int M> struct SelfTile {
     static constexpr bool F32 = std::is_same<T, float>::value;
     static constexpr bool BYTES = HELD == Held::Bytes, CODES = HELD == Held::Codes || BYTES;
-    static constexpr int ROWS = 32 * WAVES;
+    static constexpr int ROWS = M * WAVES;
     static constexpr int KB = WAVES == 1 || F32 ? 32 : 64;
     static constexpr int PITCH = DP * (BYTES ? 1 : (int)sizeof(T)), CPR = PITCH / 16;   // a row's bytes and chunks in LDS
     static constexpr int BUF = KB * PITCH;
@@ -48,15 +48,18 @@ template <typename T, Held HELD, int DP, int WAVES> struct SelfTile {
     static constexpr int SIDE = (2 * KB + 4) * 4;
     static constexpr int LDS = TILES + (CODES ? BUFS * SIDE : WAVES > 1 ? BUFS * 8 * WAVES : 0);
     static constexpr int OCC = F32 ? (DP <= (HELD == Held::Chunks ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;
-    // LDS serves 256 bytes a cycle: 16 keys of one chunk of K (a 16-byte
-    // read's pass), 4 keys of 4 chunks of V (a transposing read's).
+    // LDS serves 256 bytes a cycle, and rows' chunks are swapped so that what it
+    // serves at once lies in different banks: 16 keys of one chunk of K; of V what
+    // 32 lanes read, 8 bytes each, to transpose.
     static constexpr int PERIOD = CPR % 16 == 0 ? 1 : CPR % 8 == 0 ? 2 : CPR % 4 == 0 ? 4 : 8;   // keys until the banks repeat
     static __device__ __forceinline__ int swap_k(int key) { return CPR == 6 ? 0 : key / PERIOD % (16 / PERIOD); }
     static __device__ __forceinline__ int swap_v(int key) {
-        // (Of codes: 8 keys of 2 chunks, 0 to 3 and 8 to 11 or those 4 on.)
-        if (BYTES) return CPR % 8 == 0 ? 2 * ((key >> 1 & 1) | (key >> 3 & 1) << 1) : CPR % 4 == 0 ? 2 * (key >> 3 & 1) : 0;
-        if (F32) return CPR % 16 == 0 ? (key >> 2 & 1) * 8 : 0;
-        return PERIOD == 1 ? (key & 3) * 4 : PERIOD == 2 ? (key >> 1 & 1) * 4 : 0;
+        const int k1 = key >> 1 & 1, k2 = key >> 2 & 1, k3 = key >> 3 & 1, k4 = key >> 4 & 1;
+        if (BYTES && M == 32) return CPR == 8 ? 2 * (k1 | k3 << 1) : CPR == 4 ? 2 * k3 : 0;      // 0-3, 8-11 by two chunks
+        if (BYTES) return CPR == 8 ? k1 | k2 << 1 | k4 << 2 : CPR == 4 ? k2 | k4 << 1 : k4;       // 0-7, 16-23 by one
+        if (F32) return CPR % 16 == 0 ? k2 * 8 : 0;
+        if (M == 16) return 2 * (key / PERIOD % (8 / PERIOD));                                    // 0-7 by two
+        return PERIOD == 1 ? (key & 3) * 4 : PERIOD == 2 ? k1 * 4 : 0;                            // 0-3 by four
     }
     // Codes that a lane moves at once: the most of which a tile is whole loads.
     static constexpr int unit() {
@@ -353,13 +356,18 @@ __device__ __forceinline__ void two_of(float w0, float w1, T (&hi)[2], T (&lo)[2
     }
 }
 
-template <typename T, Held HELD, bool PAGED, int DP, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SelfTile<T, HELD, DP, WAVES>::OCC)))
+template <typename T, Held HELD, bool PAGED, int DP, int WAVES, int M>
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SelfTile<T, HELD, DP, WAVES, M>::OCC)))
 self_tiles(SelfArgs a, SelfParts parts) {
-    using C = SelfTile<T, HELD, DP, WAVES>;
+    using C = SelfTile<T, HELD, DP, WAVES, M>;
+    using Mul = Product<T, M>;
     constexpr bool F32 = C::F32, CODES = C::CODES, F16 = std::is_same<T, _Float16>::value, TWO = WAVES == 1 && !F32;
-    constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR, DT = DP / 32;
+    constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR;
     constexpr int E = Chunk<T>::N, ROWS = C::ROWS;
+    // Lanes of a row; a lane's scores of 32 keys; the results of the product with
+    // V, and a lane's registers of one. Register i: key or column 4 H (i / 4) + 4 h
+    // + i % 4 (h: which of the row's lanes).
+    constexpr int H = 64 / M, NS = M / 2, DT = DP / M, NR = M * M / 64;
     // m is LEAD above the maximum (base 2) that it was set by, and is set again
     // by one that is LAG above that. With a LEAD of LAG weights are 1 at most, so
     // that values of F32's size add up to finite sums. F16's need no such room,
@@ -368,19 +376,21 @@ self_tiles(SelfArgs a, SelfParts parts) {
     constexpr uint64_t FULL = KB == 64 ? ~0ull : 0xffffffffull;
     constexpr int LEAST_UNIT = -40;   // (127 times half of that is nothing in F16)
     typedef typename Chunk<T>::vec vec;
-    typedef typename Mma<T>::frag frag;
+    typedef typename Mul::frag frag;
+    typedef typename Mul::acc acc;
+    typedef float scores_t __attribute__((ext_vector_type(M / 2)));
     extern __shared__ __attribute__((aligned(1024))) char smem[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 31, h = lane >> 5, d = a.c.width;
+    const int r = lane % M, h = lane / M, d = a.c.width;
     const CacheArgs &c = a.c;
 
     // ---- a tile's way to LDS
     // Of chunks, load j of a wave fills 64 in order; of codes that come through
     // registers, 64 units.
     constexpr bool STAGED = HELD == Held::Codes, BYTES = C::BYTES, DIRECT = HELD == Held::Chunks || BYTES;
-    typedef typename std::conditional<CODES, int8_t, T>::type H;
-    constexpr int UN = STAGED ? C::unit() : 16 / (int)sizeof(H), UPR = DP / UN;
+    typedef typename std::conditional<CODES, int8_t, T>::type Kept;
+    constexpr int UN = STAGED ? C::unit() : 16 / (int)sizeof(Kept), UPR = DP / UN;
     constexpr int NL = KB * UPR / 64 / WAVES;
     static_assert(NL * 64 * WAVES == KB * UPR, "whole loads a wave");
     constexpr int GROUP = 16;                 // keys that lie in one page, where pages are whole groups
@@ -399,8 +409,8 @@ self_tiles(SelfArgs a, SelfParts parts) {
 #pragma unroll
         for (int j = 0; j < NL; ++j) {
             const uint32_t key = PAGED ? key_at(j, lane) % GROUP : key_at(j, lane);
-            ko[j] = (key * (uint32_t)c.ks[0] + col_k_at(j, lane)) * (uint32_t)sizeof(H);
-            vo[j] = (key * (uint32_t)c.vs[0] + col_v_at(j, lane)) * (uint32_t)sizeof(H);
+            ko[j] = (key * (uint32_t)c.ks[0] + col_k_at(j, lane)) * (uint32_t)sizeof(Kept);
+            vo[j] = (key * (uint32_t)c.vs[0] + col_v_at(j, lane)) * (uint32_t)sizeof(Kept);
         }
     // (uniform; where a load has keys of two groups, a lane takes its own)
     const bool groups_whole = PAGED && GROUP * CPR % 64 == 0 && c.page_tokens % GROUP == 0;
@@ -437,8 +447,8 @@ self_tiles(SelfArgs a, SelfParts parts) {
         const int t0 = b.first + at.tile, t1 = b.first + (last_here ? end.tile : b.tiles);
         __syncthreads();    // every wave has read the block before
 
-        const bool work = 32 * wave < b.rows;   // this wave has rows
-        const int row = b.row0 + min(32 * wave + r, b.rows - 1);
+        const bool work = M * wave < b.rows;   // this wave has rows
+        const int row = b.row0 + min(M * wave + r, b.rows - 1);
         const int of_token = a.share == 1 ? row : row / a.share;
         const uint64_t token = (uint64_t)b.q0 + of_token, head = (uint64_t)b.kv * a.share + (row - of_token * a.share);
         // The keys that this lane's row sees, and those that every row of the
@@ -446,7 +456,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
         const int pos = seq.first() + of_token;
         const int low = a.window > pos ? 0 : pos - a.window + 1;
         const int all_hi = b.at0, all_lo = a.window > b.last ? 0 : b.last - a.window + 1;
-        const H *K0 = (const H *)c.k + b.kv * c.ks[1], *V0 = (const H *)c.v + b.kv * c.vs[1];
+        const Kept *K0 = (const Kept *)c.k + b.kv * c.ks[1], *V0 = (const Kept *)c.v + b.kv * c.vs[1];
 
         // The slot of key `lane` of a tile, or -1: no state.
         const auto slot_at = [&](int t) {
@@ -495,7 +505,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 // take 32-bit offsets.)
                 typedef __attribute__((address_space(3))) void *to;
                 typedef __attribute__((address_space(1))) const void *from;
-                const auto rsrc = [](const H *p) {
+                const auto rsrc = [](const Kept *p) {
                     return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, -1, 0x00020000);
                 };
                 const auto send = [&](__amdgpu_buffer_rsrc_t tile, uint32_t at, char *dst) {
@@ -520,7 +530,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
 #pragma unroll
                     for (int j = 0; j < NL; ++j) {
                         const uint64_t s = base(j);
-                        const uint32_t back = PAGED ? 0 : (uint32_t)max(0, key_at(j, lane) - last) * (uint32_t)sizeof(H);
+                        const uint32_t back = PAGED ? 0 : (uint32_t)max(0, key_at(j, lane) - last) * (uint32_t)sizeof(Kept);
                         if (col_k_at(j, lane) < d)
                             send(rsrc(K0 + s * c.ks[0]), ko[j] - back * (uint32_t)c.ks[0], K + (wave * NL + j) * 1024);
                         if (col_v_at(j, lane) < d)
@@ -608,12 +618,14 @@ self_tiles(SelfArgs a, SelfParts parts) {
                         // largest so far. One that not every row sees has no say in
                         // that; a larger one is added alone, in F32.
                         const bool common = t * KB + lane <= all_hi && t * KB + lane >= all_lo;
-                        float top = lane < KB && common && !alone ? fabsf(sv) : 0.0f;
+                        const auto past = [&] { return fabsf(sv) > __uint_as_float((uint32_t)(127 + unit) << 23); };
+                        if (__ballot(lane < KB && common && !alone && past()) != 0) {
+                            float top = lane < KB && common && !alone ? fabsf(sv) : 0.0f;
 #pragma unroll
-                        for (int o = KB / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-                        const int e = min(126, (int)(__float_as_uint(top) >> 23) - 127 + 2);
-                        unit = __builtin_amdgcn_readfirstlane(max(unit, e));
-                        alone |= !common && fabsf(sv) > __uint_as_float((uint32_t)(127 + unit) << 23);
+                            for (int o = KB / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+                            unit = uniform(min(126, (int)(__float_as_uint(top) >> 23) - 127 + 2));
+                        }
+                        alone |= !common && past();
                     }
                     if (lane < KB) {
                         side[lane] = sk;
@@ -634,16 +646,17 @@ self_tiles(SelfArgs a, SelfParts parts) {
             load(t0, 0);
             next_slot = slot_at(t0 + 1);
         }
-        // This row's q: of each 2 E columns the lane's half's E (of codes as they
-        // are, whose chunks are 2 E: of each 4 E the half's 2 E).
-        constexpr int NQ = DP / (2 * E);
+        // This row's q: of each H E columns the lane's E. Of codes as they are, whose
+        // chunks are 2 E columns, of each 2 H E the lane's chunk, if they are so many.
+        constexpr int NQ = DP / (H * E);
+        constexpr bool PAIRS = BYTES && NQ % 2 == 0;
         vec q[NQ];
         {
-            const int h = fresh(lane) >> 5;   // (else its comparisons are kept from block to block)
+            const int h = fresh(lane) / M;   // (else its comparisons are kept from block to block)
             const T *p = (const T *)a.q + token * a.qs[0] + head * a.qs[1];
 #pragma unroll
             for (int s = 0; s < NQ; ++s) {
-                const int col = BYTES ? (2 * (s >> 1) + h) * 2 * E + (s & 1) * E : (2 * s + h) * E;
+                const int col = PAIRS ? (H * (s >> 1) + h) * 2 * E + (s & 1) * E : (H * s + h) * E;
                 q[s] = read_chunk(p + col, d - col);
             }
             if (a.turn != 1.0f)   // uniform
@@ -653,52 +666,68 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     for (int e = 0; e < E; ++e) q[s][e] = from_f32<T>(to_f32(q[s][e]) * a.turn);
         }
 
-        floatx16 o[DT];
+        acc o[DT];
 #pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] = floatx16{};
+        for (int t = 0; t < DT; ++t) o[t] = acc{};
         float m = -INFINITY, l = 0.0f;
         bool any = false, far = false;   // this row has seen a state; a maximum past 2^24
         int my_unit = LEAST_UNIT;        // of o's sums
 
-        // S^T of 32 keys. Register i is key 8 (i / 4) + 4 h + i % 4.
-        const int kr = r * PITCH, ks = C::swap_k(r);   // (32 keys on, the swap is the same)
-        const auto scores = [&](const char *K, floatx16 (&s)[SUB]) {
+        // S^T of the tile's keys, 32 of them a scores_t.
+        const int kr = r * PITCH, ks = C::swap_k(r);
+        const auto scores = [&](const char *K, scores_t (&s)[SUB]) {
+            // M keys at a time, from m0 of tile part u: their results go next to each other.
+            constexpr int BLOCKS = 32 / M;
+            acc part[SUB][BLOCKS];
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) s[u] = floatx16{};
-            const auto chunk = [&](int x, int u) {
-                return *(const vec *)(K + 32 * u * PITCH + kr + ((2 * x + h) ^ ks) * 16);
-            };
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int v = 0; v < BLOCKS; ++v) part[u][v] = acc{};
+            // (32 keys on, the swap is the same; 16 on it may not be.)
+            const auto row = [&](int u, int v) { return K + (32 * u + M * v) * PITCH + kr; };
+            const auto swap = [&](int v) { return M == 32 ? ks : C::swap_k(r + M * v); };
             if constexpr (BYTES) {
+                typedef uint32_t words __attribute__((ext_vector_type(PAIRS ? 4 : 2)));
 #pragma unroll
-                for (int x = 0; x < CPR / 2; ++x) {
-                    typedef uint32_t words __attribute__((ext_vector_type(4)));
-                    const words w = *(const words *)(K + kr + ((2 * x + h) ^ ks) * 16);
+                for (int x = 0; x < (PAIRS ? NQ / 2 : NQ); ++x)
 #pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        T n[8];
-                        numbers_of(w[2 * z], n), numbers_of(w[2 * z + 1], n + 4);
-                        frag f;
+                    for (int v = 0; v < BLOCKS; ++v) {
+                        const words w = PAIRS ? *(const words *)(row(0, v) + ((H * x + h) ^ swap(v)) * 16)
+                                              : *(const words *)(row(0, v) + ((H / 2 * x + h / 2) ^ swap(v)) * 16 + h % 2 * 8);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = n[e];
-                        s[0] = Mma<T>::run(f, q[2 * x + z], s[0]);
+                        for (int z = 0; z < (PAIRS ? 2 : 1); ++z) {
+                            T n[8];
+                            numbers_of(w[2 * z], n), numbers_of(w[2 * z + 1], n + 4);
+                            frag f;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) f[e] = n[e];
+                            part[0][v] = Mul::run(f, q[PAIRS ? 2 * x + z : x], part[0][v]);
+                        }
                     }
-                }
             } else if constexpr (F32) {
                 // (A chunk read two ahead of its products, which are slow enough to hide it.)
-                vec k[3] = {chunk(0, 0), chunk(1, 0)};
+                const auto chunk = [&](int x) { return *(const vec *)(row(0, 0) + ((2 * x + h) ^ ks) * 16); };
+                vec k[3] = {chunk(0), chunk(1)};
 #pragma unroll
-                for (int x = 0; x < CPR / 2; ++x) {
-                    if (x + 2 < CPR / 2) k[(x + 2) % 3] = chunk(x + 2, 0);
+                for (int x = 0; x < NQ; ++x) {
+                    if (x + 2 < NQ) k[(x + 2) % 3] = chunk(x + 2);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int e = 0; e < E; ++e) s[0] = Mma<T>::run(k[x % 3][e], q[x][e], s[0]);
+                    for (int e = 0; e < E; ++e) part[0][0] = Mul::run(k[x % 3][e], q[x][e], part[0][0]);
                 }
             } else {
 #pragma unroll
-                for (int x = 0; x < CPR / 2; ++x)
+                for (int x = 0; x < NQ; ++x)
 #pragma unroll
-                    for (int u = 0; u < SUB; ++u) s[u] = Mma<T>::run(chunk(x, u), q[x], s[u]);
+                    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                        for (int v = 0; v < BLOCKS; ++v)
+                            part[u][v] = Mul::run(*(const vec *)(row(u, v) + ((H * x + h) ^ swap(v)) * 16), q[x], part[u][v]);
             }
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < NS; ++i) s[u][i] = part[u][i / NR][i % NR];
         };
         // O^T += V^T P^T over 32 keys; weight(i) is register i's, in order.
         const auto add_values = [&](const char *V, auto weight) {
@@ -719,16 +748,18 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     if (i + 2 < 16) ahead(i + 2);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int t = 0; t < DT; ++t) o[t] = Mma<T>::run(v[i % 3][t], p[i % 3], o[t]);
+                    for (int t = 0; t < DT; ++t) o[t] = Mul::run(v[i % 3][t], p[i % 3], o[t]);
                 }
             } else {
-                // 16 keys a product: registers 8 j .. 8 j + 7. A group of 16 lanes
-                // reads 4 keys by 16 columns, and a lane gets its column's 4.
+                // 8 H keys a product: registers 8 j .. 8 j + 7. A group of 16 lanes
+                // reads 4 keys by 16 columns, and a lane gets its column's 4; of
+                // codes 8 keys.
                 typedef short s4 __attribute__((ext_vector_type(4)));
-                const int g = lane >> 4, n = lane & 15, key = 4 * (g >> 1) + (n >> 2);
+                typedef int w2 __attribute__((ext_vector_type(2)));
+                const int n = lane & 15, half = r >> 4;    // which 16 of the product's columns
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    frag f, rest, vt[DT];
+                for (int j = 0; j < NS / 8; ++j) {
+                    frag f, rest;
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
                         const float w0 = weight(8 * j + e), w1 = weight(8 * j + e + 1);
@@ -740,21 +771,20 @@ self_tiles(SelfArgs a, SelfParts parts) {
                             f[e] = from_f32<T>(w0), f[e + 1] = from_f32<T>(w1);
                         }
                     }
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) {
+                    const auto column = [&](int t) {
                         if constexpr (BYTES) {
-                            // (Codes: 8 keys by 16 columns, and a lane gets its column's 8.)
-                            typedef int w2 __attribute__((ext_vector_type(2)));
-                            const int k = 16 * j + 8 * (n >> 3) + 4 * h + ((n >> 1) & 3);
+                            const int k = 8 * H * j + 4 * H * (n >> 3) + 4 * h + ((n >> 1) & 3);
                             const w2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                                 (__attribute__((address_space(3))) w2 *)(V + k * PITCH +
-                                                                         ((2 * t + (g & 1)) ^ C::swap_v(k)) * 16 + (n & 1) * 8));
+                                                                         ((M / 16 * t + half) ^ C::swap_v(k)) * 16 + (n & 1) * 8));
                             T y[8];
                             numbers_of((uint32_t)w[0], y), numbers_of((uint32_t)w[1], y + 4);
+                            frag v;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) vt[t][e] = y[e];
+                            for (int e = 0; e < 8; ++e) v[e] = y[e];
+                            return v;
                         } else {
-                            const int x = 4 * t + 2 * (g & 1) + ((n >> 1) & 1);
+                            const int x = M / 8 * t + 2 * half + ((n >> 1) & 1), key = 8 * H * j + 4 * h + (n >> 2);
                             const auto place = [&](int k) {
                                 return (__attribute__((address_space(3))) s4 *)(V + k * PITCH + (x ^ C::swap_v(k)) * 16 +
                                                                                  (n & 1) * 8);
@@ -762,15 +792,25 @@ self_tiles(SelfArgs a, SelfParts parts) {
                             struct {
                                 s4 lo, hi;
                             } v;
-                            v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(16 * j + key));
-                            v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(16 * j + 8 + key));
-                            vt[t] = __builtin_bit_cast(frag, v);
+                            v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(key));
+                            v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(key + 4 * H));
+                            return __builtin_bit_cast(frag, v);
                         }
-                        o[t] = Mma<T>::run(vt[t], f, o[t]);
-                    }
-                    if constexpr (TWO)
+                    };
+                    // (Four results at a time: the second numbers' products after the first's.)
+                    constexpr int AT = DT < 4 ? DT : DT % 4 == 0 ? 4 : 3;
 #pragma unroll
-                        for (int t = 0; t < DT; ++t) o[t] = Mma<T>::run(vt[t], rest, o[t]);
+                    for (int t0 = 0; t0 < DT; t0 += AT) {
+                        frag v[AT];
+#pragma unroll
+                        for (int t = 0; t < AT; ++t) {
+                            v[t] = column(t0 + t);
+                            o[t0 + t] = Mul::run(v[t], f, o[t0 + t]);
+                        }
+                        if constexpr (TWO)
+#pragma unroll
+                            for (int t = 0; t < AT; ++t) o[t0 + t] = Mul::run(v[t], rest, o[t0 + t]);
+                    }
                 }
             }
         };
@@ -788,37 +828,39 @@ self_tiles(SelfArgs a, SelfParts parts) {
         // Values that are no numbers weigh nothing for the rows that do not see
         // them, and 0 times them is no number either: where some row does not,
         // their keys are added one by one, and are 0 for the products.
-        const auto add_alone = [&](const char *V, const float *side, const floatx16 (&s)[SUB], uint64_t seen, uint64_t bad,
+        const auto add_alone = [&](const char *V, const float *side, const scores_t (&s)[SUB], uint64_t seen, uint64_t bad,
                                    float scale, float base) {
-            const int h = fresh(lane) >> 5;
+            const int h = fresh(lane) / M;
             for (; bad; bad &= bad - 1) {
                 const int key = __ffsll((unsigned long long)bad) - 1;
-                const int u = key >> 5, i = (key >> 3 & 3) * 4 + (key & 3), from = key >> 2 & 1;
+                const int u = key >> 5, i = (key & 31) / (4 * H) * 4 + (key & 3), from = (key >> 2) % H;
                 float x = 0.0f;
 #pragma unroll
                 for (int v = 0; v < SUB; ++v)
 #pragma unroll
-                    for (int n = 0; n < 16; ++n) x = u == v && i == n ? s[v][n] : x;
-                x = __shfl(x, r + 32 * from, 64);
+                    for (int n = 0; n < NS; ++n) x = u == v && i == n ? s[v][n] : x;
+                x = __shfl(x, r + M * from, 64);
                 float w = __builtin_amdgcn_exp2f(fmaf(x, scale, -base));
                 if constexpr (CODES) w *= side[KB + key];
                 const bool see = seen >> key & 1;
                 // (Four at a time: this path is to cost no registers.)
                 typedef T four __attribute__((ext_vector_type(4)));
-                const char *row = V + key * PITCH + (BYTES ? 4 * h : F32 ? 0 : 8 * h);
+                const char *row = V + key * PITCH;
                 const int swap = C::swap_v(key);
 #pragma unroll
                 for (int t = 0; t < DT; ++t)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
+                    for (int g = 0; g < NR / 4; ++g) {
+                        const int at = (M * t + 4 * H * g + 4 * h) * (BYTES ? 1 : (int)sizeof(T));
+                        const char *p = row + ((at >> 4) ^ swap) * 16 + (at & 15);
                         four v;
                         if constexpr (BYTES) {
                             T n[4];
-                            numbers_of(*(const uint32_t *)(row + ((2 * t + (g >> 1)) ^ swap) * 16 + (g & 1) * 8), n);
+                            numbers_of(*(const uint32_t *)p, n);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) v[e] = n[e];
                         } else {
-                            v = *(const four *)(row + ((F32 ? 8 * t + 2 * g + h : 4 * t + g) ^ swap) * 16);
+                            v = *(const four *)p;
                         }
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
@@ -828,14 +870,14 @@ self_tiles(SelfArgs a, SelfParts parts) {
             }
         };
         const auto tile = [&](const char *K, float *side, uint64_t live, int t, uint64_t bad) {
-            floatx16 s[SUB];
+            scores_t s[SUB];
             scores(K, s);
             if constexpr (CODES) {
 #pragma unroll
                 for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f32x4 f = *(const f32x4 *)(side + 32 * u + 8 * g + 4 * h);
+                    for (int g = 0; g < NS / 4; ++g) {
+                        const f32x4 f = *(const f32x4 *)(side + 32 * u + 4 * H * g + 4 * h);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[u][4 * g + e] *= f[e];
                     }
@@ -860,16 +902,16 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 for (int u = 0; u < SUB; ++u) {
                     const uint32_t word = (uint32_t)(seen >> (32 * u)) >> (4 * h);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[u][i] = (word >> (8 * (i >> 2) + (i & 3))) & 1u ? s[u][i] : -INFINITY;
+                    for (int i = 0; i < NS; ++i)
+                        s[u][i] = (word >> (4 * H * (i >> 2) + (i & 3))) & 1u ? s[u][i] : -INFINITY;
                 }
             }
             float mx = s[0][0];
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-            raise(both_max(mx) * a.scale);
+                for (int i = 0; i < NS; ++i) mx = fmaxf(mx, s[u][i]);
+            raise((M == 32 ? both_max(mx) : four_max(mx)) * a.scale);
             const float base = m == -INFINITY ? 0.0f : m;
             // A score's distance from the maximum in one rounding; where the
             // maximum is so large that its own rounding shows, from the rounded
@@ -885,10 +927,10 @@ self_tiles(SelfArgs a, SelfParts parts) {
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) {
                     float sum = 0.0f;
-                    f32x4 sv[4];
+                    f32x4 sv[NS / 4];
                     if constexpr (CODES)
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) sv[g] = *(const f32x4 *)(side + KB + 32 * u + 8 * g + 4 * h);
+                        for (int g = 0; g < NS / 4; ++g) sv[g] = *(const f32x4 *)(side + KB + 32 * u + 4 * H * g + 4 * h);
                     add_values(V + 32 * u * PITCH, [&](int i) {
                         const float w = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
                         sum += w;
@@ -967,14 +1009,14 @@ self_tiles(SelfArgs a, SelfParts parts) {
         }
 
         if (work) {
-            const int h = fresh(lane) >> 5;
-            l = both_sum(l);
+            const int h = fresh(lane) / M;
+            l = M == 32 ? both_sum(l) : four_sum(l);
             if constexpr (CODES && F16) {
                 const float f = __uint_as_float((uint32_t)(127 + my_unit) << 23);
 #pragma unroll
                 for (int t = 0; t < DT; ++t) o[t] *= f;
             }
-            if (32 * wave + r < b.rows) {
+            if (M * wave + r < b.rows) {
                 if (!PAGED || (!begun && ends)) {
                     const float inv = any ? 1.0f / l : 0.0f;   // (all scores minus infinity: 0 times infinity)
                     T *out = (T *)a.out + token * a.os[0] + head * a.os[1];
@@ -982,8 +1024,8 @@ self_tiles(SelfArgs a, SelfParts parts) {
 #pragma unroll
                     for (int t = 0; t < DT; ++t)
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const int col = 32 * t + 8 * g + 4 * h;
+                        for (int g = 0; g < NR / 4; ++g) {
+                            const int col = M * t + 4 * H * g + 4 * h;
                             const loose4 y{from_f32<T>(o[t][4 * g] * inv), from_f32<T>(o[t][4 * g + 1] * inv),
                                            from_f32<T>(o[t][4 * g + 2] * inv), from_f32<T>(o[t][4 * g + 3] * inv)};
                             if (col + 4 <= d) {
@@ -997,12 +1039,12 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 } else {
                     // Four columns of every row, then the next four; then the maxima and sums.
                     f32x4 *p = (f32x4 *)parts.part(2 * blockIdx.x + (begun ? 0 : 1));
-                    const int at = 32 * wave + r, groups = (d + 3) / 4;
+                    const int at = M * wave + r, groups = (d + 3) / 4;
 #pragma unroll
                     for (int t = 0; t < DT; ++t)
 #pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const int x = 8 * t + 2 * g + h;
+                        for (int g = 0; g < NR / 4; ++g) {
+                            const int x = M / 4 * t + H * g + h;
                             if (x < groups)
                                 p[x * b.rows + at] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
                         }
@@ -1108,9 +1150,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) self_join(S
 
 // ---- launches --------------------------------------------------------------------------
 
-template <typename T, Held HELD, bool PAGED, int DP, int WAVES>
+template <typename T, Held HELD, bool PAGED, int DP, int WAVES, int M = 32>
 static hipError_t launch_tiles(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
-    using C = SelfTile<T, HELD, DP, WAVES>;
+    using C = SelfTile<T, HELD, DP, WAVES, M>;
     SelfParts parts{};
     if (PAGED) {
         parts.marks = (SelfMark *)a.ws;
@@ -1119,21 +1161,28 @@ static hipError_t launch_tiles(hipStream_t s, const SelfArgs &a, const SelfLaunc
         parts.groups = (int)f.groups;
         parts.least = (uint64_t)a.share * 4 * C::KB;
     }
-    const hipError_t e = enqueue(self_tiles<T, HELD, PAGED, DP, WAVES>, dim3(f.groups), dim3(64 * WAVES), C::LDS, s, a, parts);
+    const hipError_t e = enqueue(self_tiles<T, HELD, PAGED, DP, WAVES, M>, dim3(f.groups), dim3(64 * WAVES), C::LDS, s, a, parts);
     // (Blocks of one tile are not cut.)
     if (e != hipSuccess || !PAGED || room(a.c) <= C::KB) return e;
     return enqueue(self_join<T, DP>, dim3(f.groups, (f.part_rows + 15) / 16), dim3(256), 0, s, a, parts);
 }
 
 template <typename T, bool PAGED, int DP> static hipError_t launch_held(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
+    constexpr bool F32 = std::is_same<T, float>::value;
+    // (Blocks of 16 rows: 16-bit tokens over a cache.)
+    if constexpr (PAGED && !F32) {
+        if (f.rows == 16)
+            return f.held == Held::Bytes    ? launch_tiles<T, Held::Bytes, true, DP, 1, 16>(s, a, f)
+                   : f.held == Held::Chunks ? launch_tiles<T, Held::Chunks, true, DP, 1, 16>(s, a, f)
+                                            : hipErrorInvalidValue;
+        if (f.held == Held::Bytes) return launch_tiles<T, Held::Bytes, true, DP, 1>(s, a, f);
+    }
     if constexpr (PAGED)
         if (f.held == Held::Codes)
-            return f.waves == 1 ? launch_tiles<T, Held::Codes, true, DP, 1>(s, a, f)
+            return f.rows == 32 ? launch_tiles<T, Held::Codes, true, DP, 1>(s, a, f)
                                 : launch_tiles<T, Held::Codes, true, DP, 4>(s, a, f);
-    if constexpr (PAGED && !std::is_same<T, float>::value)
-        if (f.held == Held::Bytes) return launch_tiles<T, Held::Bytes, true, DP, 1>(s, a, f);
     if (f.held == Held::Loose) return launch_tiles<T, Held::Loose, PAGED, DP, 1>(s, a, f);
-    return f.waves == 1 ? launch_tiles<T, Held::Chunks, PAGED, DP, 1>(s, a, f)
+    return f.rows == 32 ? launch_tiles<T, Held::Chunks, PAGED, DP, 1>(s, a, f)
                         : launch_tiles<T, Held::Chunks, PAGED, DP, 4>(s, a, f);
 }
 
