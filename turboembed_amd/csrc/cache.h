@@ -90,6 +90,7 @@ struct SelfLaunch {
     Held held;
     int rows;            // of a block: 16 or 32 (a wave's), or 128 (four waves')
     uint32_t groups;     // workgroups: of a prompt, the most blocks that there can be
+    int pieces;          // of a call over a cache, each a workgroup of every key head
     int part_rows;       // the most rows of a part
 };
 SelfLaunch self_plan(const SelfArgs &a);

@@ -10,14 +10,16 @@ namespace rocm {
 
 namespace {
 
-// Workgroups of a call over a cache, by its blocks' rows.
-int most_groups(int rows) {
-    if (getenv("TG")) return atoi(getenv("TG"));
-    return rows == 128 ? 512 : 3072;
+// Pieces of a call over a cache, by its blocks' rows: workgroups enough for a
+// card, and no more.
+uint64_t most_pieces(int rows, int kv) {
+    uint64_t groups = rows == 128 ? 512 : 3072;
+    return std::max<uint64_t>(1, groups / kv);
 }
 
-uint64_t parts_bytes(uint64_t groups, int rows, uint64_t all_rows, int width) {
-    return groups * (sizeof(SelfMark) + 2 * 4 * self_part_floats((int)std::min<uint64_t>(rows, all_rows), width));
+uint64_t parts_bytes(int rows, uint64_t all_rows, int kv, int width) {
+    return most_pieces(rows, kv) * kv *
+           (sizeof(SelfMark) + 2 * 4 * self_part_floats((int)std::min<uint64_t>(rows, all_rows), width));
 }
 
 }  // namespace
@@ -49,8 +51,10 @@ SelfLaunch self_plan(const SelfArgs &a) {
         f.groups = (uint32_t)blocks;
         return f;
     }
-    const uint64_t tiles = ((uint64_t)room(a.c) + 31) / 32;
-    f.groups = (uint32_t)std::min<uint64_t>(most_groups(f.rows), std::max<uint64_t>(1, blocks * std::max<uint64_t>(1, tiles)));
+    // (No more than there can be tiles.)
+    const uint64_t tiles = blocks / a.c.kv * std::max<uint64_t>(1, ((uint64_t)room(a.c) + 31) / 32);
+    f.pieces = (int)std::min<uint64_t>(most_pieces(f.rows, a.c.kv), std::max<uint64_t>(1, tiles));
+    f.groups = (uint32_t)(f.pieces + 7) / 8 * 8 * a.c.kv;
     f.part_rows = (int)std::min<uint64_t>(f.rows, rows);
     return f;
 }
@@ -58,7 +62,7 @@ SelfLaunch self_plan(const SelfArgs &a) {
 uint64_t self_workspace(uint64_t tokens, uint64_t seqs, int heads, int kv, int width) {
     if (tokens == 0 || seqs == 0) return 0;
     const uint64_t rows = tokens * (heads / kv);
-    return std::max(parts_bytes(most_groups(32), 32, rows, width), parts_bytes(most_groups(128), 128, rows, width));
+    return std::max(parts_bytes(32, rows, kv, width), parts_bytes(128, rows, kv, width));
 }
 
 hipError_t self_attention(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {

@@ -150,21 +150,22 @@ __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
 }
 
-// A place in the order of all blocks' tiles: sequence, key head, block, tile.
+// A place in the order of a key head's tiles: sequence, block, tile.
 struct Place {
-    int seq, kv, block, tile;
-    __device__ bool operator==(const Place &o) const {
-        return seq == o.seq && kv == o.kv && block == o.block && tile == o.tile;
-    }
+    int seq, block, tile;
+    __device__ bool operator==(const Place &o) const { return seq == o.seq && block == o.block && tile == o.tile; }
 };
 
-// A call over a cache is cut into equal costs, one a workgroup, wherever the
-// cuts fall: its lengths are on the device, and one token's sequences may be as
-// different as they like. from .. to are workgroup g's places.
+// A call over a cache is cut into pieces of equal cost, wherever the cuts fall:
+// its lengths are on the device, and one token's sequences may be as different
+// as they like. A piece is a workgroup of each key head: those go to one XCD, at
+// about one time, as a slot's heads lie next to each other in the cache's lines
+// (96 tokens over 100-6000 int8 states, 12 heads of 64: 160 us; cut across the
+// heads 200). from .. to are the places of piece g.
 template <int ROWS, int KB> struct Cuts {
     Place from, to;
     bool any;
-    __device__ __forceinline__ Cuts(const SelfArgs &a, int g, int groups, uint64_t least) {
+    __device__ __forceinline__ Cuts(const SelfArgs &a, int g, int pieces, uint64_t least) {
         const int lane = threadIdx.x & 63, n = a.c.seqs;
         uint64_t total = 0, cost = 0;
         Blocks mine{};
@@ -174,18 +175,18 @@ template <int ROWS, int KB> struct Cuts {
             if (i0 + lane < n) {
                 seq = seq_of(a.c, i0 + lane);
                 mine = cost_of(a, seq, ROWS);
-                cost = a.c.kv * cost_to(mine, mine.n);
+                cost = cost_to(mine, mine.n);
             }
             cost = prefix_sum(cost);
             total += lane_of(cost, 63);
         }
-        // (No more workgroups than their least work makes worth while.)
+        // (No more pieces than their least work makes worth while.)
         const uint64_t worth = quotient(total + least - 1, least);
-        if (worth < (uint64_t)groups) groups = max(1, (int)worth);
-        any = total > 0 && g < groups;
+        if (worth < (uint64_t)pieces) pieces = max(1, (int)worth);
+        any = total > 0 && g < pieces;
         if (!any) return;
-        // Lane 0 finds workgroup g's first place, lane 1 the next one's.
-        const uint64_t each = quotient(total, (uint64_t)groups), rest = total - each * (uint64_t)groups;
+        // Lane 0 finds the piece's first place, lane 1 the next one's.
+        const uint64_t each = quotient(total, (uint64_t)pieces), rest = total - each * (uint64_t)pieces;
         const auto cut = [&](uint64_t i) { return each * i + min(i, rest); };
         const uint64_t f = cut((uint64_t)g + (lane & 1));
         const uint64_t f0 = lane_of(f, 0), f1 = lane_of(f, 1);
@@ -198,7 +199,7 @@ template <int ROWS, int KB> struct Cuts {
                 if (i0 + lane < n) {
                     const Seq s = seq_of(a.c, i0 + lane);
                     const Blocks m = cost_of(a, s, ROWS);
-                    cost = a.c.kv * cost_to(m, m.n);
+                    cost = cost_to(m, m.n);
                 }
                 cost = prefix_sum(cost);
             }
@@ -210,13 +211,11 @@ template <int ROWS, int KB> struct Cuts {
             if (at == n && past) at = i0 + first, before = seen + (first ? (uint64_t)hi << 32 | lo : 0);
             seen += lane_of(cost, 63);
         }
-        Place p{at, 0, 0, 0};
+        Place p{at, 0, 0};
         if (at < n) {
             const Seq s = seq_of(a.c, at);
             const Blocks m = cost_of(a, s, ROWS);
-            const uint64_t head = cost_to(m, m.n), o = f - before;
-            p.kv = (int)quotient(o, head);
-            const uint64_t rest = o - p.kv * head;
+            const uint64_t rest = f - before;
             int lo = 0, hi = m.n;      // cost_to(lo) <= rest < cost_to(hi)
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
@@ -225,7 +224,7 @@ template <int ROWS, int KB> struct Cuts {
             }
             p.block = lo;
             const uint64_t c0 = cost_to(m, lo), c = cost_to(m, lo + 1) - c0;
-            const Block b = block_of<ROWS, KB>(a, s, p.kv, lo);
+            const Block b = block_of<ROWS, KB>(a, s, 0, lo);
             p.tile = min(b.tiles, (int)((double)(rest - c0) / (double)c * (double)b.tiles));
             // (A cut next to a block's end goes there: a part costs its way to memory.)
             const int near = (int)min((uint64_t)b.tiles, quotient(each, (uint64_t)a.share * KB * 8));
@@ -233,15 +232,12 @@ template <int ROWS, int KB> struct Cuts {
             else if (b.tiles - p.tile <= near) p.tile = b.tiles;
             if (p.tile == b.tiles) {
                 p.tile = 0;
-                if (b.tiles > 0 && ++p.block == m.n) {
-                    p.block = 0;
-                    if (++p.kv == a.c.kv) p.kv = 0, ++p.seq;
-                }
+                if (b.tiles > 0 && ++p.block == m.n) p.block = 0, ++p.seq;
             }
         }
         const auto one = [&](int v, int l) { return __builtin_amdgcn_readlane(v, l); };
-        from = Place{one(p.seq, 0), one(p.kv, 0), one(p.block, 0), one(p.tile, 0)};
-        to = Place{one(p.seq, 1), one(p.kv, 1), one(p.block, 1), one(p.tile, 1)};
+        from = Place{one(p.seq, 0), one(p.block, 0), one(p.tile, 0)};
+        to = Place{one(p.seq, 1), one(p.block, 1), one(p.tile, 1)};
         // (A sequence without rows has no place.)
         const auto settle = [&](Place &q) {
             while (q.seq < n && seq_of(a.c, q.seq).rows == 0) ++q.seq;
@@ -324,14 +320,20 @@ template <int ROWS, int HELD> struct Turn {
 
 // ---- parts ---------------------------------------------------------------------------
 
-// Workgroup g's marks, then its parts: 2 g of the block that it starts inside
-// of, 2 g + 1 of the one that it leaves unfinished.
+// The marks of piece p and key head h, u = p kv + h, then their parts: 2 u of the
+// block that they start inside of, 2 u + 1 of the one that they leave unfinished.
 struct SelfParts {
     SelfMark *marks;
     float *parts;
     uint64_t pitch;
-    int groups;
+    int pieces;
     uint64_t least;      // cost
+    // Workgroup x: eight pieces of a head, then of the next, so that a piece's
+    // heads go to one XCD.
+    __device__ __forceinline__ void whose(uint32_t x, int kv, int &piece, int &head) const {
+        const uint32_t eight = 8u * (uint32_t)kv, q = x / eight, rest = x - q * eight;
+        head = (int)(rest / 8), piece = (int)(q * 8 + rest % 8);
+    }
     __device__ __forceinline__ float *part(int i) const { return parts + (uint64_t)i * pitch; }
 };
 
@@ -422,15 +424,20 @@ self_tiles(SelfArgs a, SelfParts parts) {
 
     Place at{}, end{};
     bool front = false;    // this workgroup starts inside of a block
+    int kv, unit_id = 0;   // its key head; of its parts
     if constexpr (PAGED) {
-        const Cuts<ROWS, KB> cuts(a, (int)blockIdx.x, parts.groups, parts.least);
+        int piece;
+        parts.whose(blockIdx.x, c.kv, piece, kv);
+        if (piece >= parts.pieces) return;
+        unit_id = piece * c.kv + kv;
+        const Cuts<ROWS, KB> cuts(a, piece, parts.pieces, parts.least);
         if (cuts.any) at = cuts.from, end = cuts.to, front = at.tile > 0;
-        else at = end = Place{c.seqs, 0, 0, 0};
-        if (!front && tid == 0) parts.marks[blockIdx.x] = SelfMark{};
+        else at = end = Place{c.seqs, 0, 0};
+        if (!front && tid == 0) parts.marks[unit_id] = SelfMark{};
     } else {
         const Turn<ROWS, C::TILES / 4> turn(a, blockIdx.x, smem, 64 * WAVES);
         if (!turn.any) return;
-        at = Place{turn.seq, turn.kv, turn.block, 0};
+        at = Place{turn.seq, turn.block, 0}, kv = turn.kv;
         if (HELD == Held::Chunks && d < DP && c.seqs > 64) {
             __syncthreads();
             for (int i = tid; i < C::TILES / 16; i += 64 * WAVES) *(vec *)(smem + i * 16) = vec{};
@@ -441,8 +448,8 @@ self_tiles(SelfArgs a, SelfParts parts) {
     bool more = !PAGED || !(at == end) || front;
     while (more) {
         const Seq seq = seq_of(c, at.seq);
-        const Block b = block_of<ROWS, KB>(a, seq, at.kv, at.block);
-        const bool last_here = PAGED && at.seq == end.seq && at.kv == end.kv && at.block == end.block;
+        const Block b = block_of<ROWS, KB>(a, seq, kv, at.block);
+        const bool last_here = PAGED && at.seq == end.seq && at.block == end.block;
         const bool begun = at.tile > 0, ends = !last_here || end.tile == b.tiles;
         const int t0 = b.first + at.tile, t1 = b.first + (last_here ? end.tile : b.tiles);
         __syncthreads();    // every wave has read the block before
@@ -1038,7 +1045,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
                         }
                 } else {
                     // Four columns of every row, then the next four; then the maxima and sums.
-                    f32x4 *p = (f32x4 *)parts.part(2 * blockIdx.x + (begun ? 0 : 1));
+                    f32x4 *p = (f32x4 *)parts.part(2 * unit_id + (begun ? 0 : 1));
                     const int at = M * wave + r, groups = (d + 3) / 4;
 #pragma unroll
                     for (int t = 0; t < DT; ++t)
@@ -1058,7 +1065,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
         if constexpr (!PAGED) {
             more = false;
         } else {
-            if (begun && tid == 0) parts.marks[blockIdx.x] = SelfMark{1, ends, b.q0, b.kv, b.row0, b.rows, {0, 0}};
+            if (begun && tid == 0) parts.marks[unit_id] = SelfMark{1, ends, b.q0, b.kv, b.row0, b.rows, {0, 0}};
             // On to the next block.
             if (last_here) {
                 more = false;
@@ -1066,11 +1073,8 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 at.tile = 0;
                 if (++at.block == blocks_of(seq, a.share, ROWS)) {
                     at.block = 0;
-                    if (++at.kv == c.kv) {
-                        at.kv = 0;
-                        do ++at.seq;
-                        while (at.seq < c.seqs && seq_of(c, at.seq).rows == 0);
-                    }
+                    do ++at.seq;
+                    while (at.seq < c.seqs && seq_of(c, at.seq).rows == 0);
                 }
                 more = at.seq < c.seqs && !(at == end);
             }
@@ -1081,13 +1085,17 @@ self_tiles(SelfArgs a, SelfParts parts) {
 // The parts of blocks that were cut: a wave a row, a quarter or less of its
 // lanes a part.
 template <typename T, int DP> __global__ void __launch_bounds__(256) self_join(SelfArgs a, SelfParts parts) {
-    const int x = (int)blockIdx.x, lane = threadIdx.x & 63, d = a.c.width;
-    const SelfMark mark = parts.marks[x];
+    const int lane = threadIdx.x & 63, d = a.c.width, kv = a.c.kv;
+    int x, head;
+    parts.whose(blockIdx.x, kv, x, head);
+    if (x >= parts.pieces) return;
+    const SelfMark mark = parts.marks[x * kv + head];
     if (!(mark.front && mark.done)) return;
-    // The workgroups before it that lie inside of the block, and the one that began it.
+    // The pieces before it that lie inside of the block, and the one that began it.
     int inside = 0;
     for (int g = x - 1;; g -= 64) {
-        const bool in = g - lane >= 0 && parts.marks[g - lane].front && !parts.marks[g - lane].done;
+        const SelfMark *before = parts.marks + (g - lane) * kv + head;
+        const bool in = g - lane >= 0 && before->front && !before->done;
         const uint64_t not_in = ~__ballot(in);
         if (not_in) {
             inside += __ffsll((unsigned long long)not_in) - 1;
@@ -1096,7 +1104,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) self_join(S
         inside += 64;
     }
     const int n = inside + 2, first = x - inside - 1;
-    const auto part = [&](int p) { return parts.part(p == 0 ? 2 * first + 1 : 2 * (first + p)); };
+    const auto part = [&](int p) { return parts.part(2 * ((first + p) * kv + head) + (p == 0)); };
     constexpr int COLS = DP / 4, AT_ONCE = 64 / COLS;    // lanes of a part (groups of four columns; 96: 24)
     const int sub = lane / COLS, col = lane % COLS, groups = (d + 3) / 4, rows = mark.rows;
     for (int i = blockIdx.y * 4 + (threadIdx.x >> 6); i < rows; i += gridDim.y * 4) {
@@ -1156,9 +1164,9 @@ static hipError_t launch_tiles(hipStream_t s, const SelfArgs &a, const SelfLaunc
     SelfParts parts{};
     if (PAGED) {
         parts.marks = (SelfMark *)a.ws;
-        parts.parts = (float *)(parts.marks + f.groups);
+        parts.parts = (float *)(parts.marks + (uint64_t)f.pieces * a.c.kv);
         parts.pitch = self_part_floats(f.part_rows, a.c.width);
-        parts.groups = (int)f.groups;
+        parts.pieces = f.pieces;
         parts.least = (uint64_t)a.share * 4 * C::KB;
     }
     const hipError_t e = enqueue(self_tiles<T, HELD, PAGED, DP, WAVES, M>, dim3(f.groups), dim3(64 * WAVES), C::LDS, s, a, parts);
