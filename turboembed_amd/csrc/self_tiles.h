@@ -42,11 +42,11 @@ template <typename T, Held HELD, int DP, int WAVES, int M> struct SelfTile {
     // (A wave alone writes a tile of codes' numbers once it has read the one before.)
     static constexpr int BUFS = HELD == Held::Codes && WAVES == 1 ? 1 : 2;
     static constexpr int TILES = BUFS * 2 * BUF;
-    // Behind the tiles: of codes, each buffer's scales of K and V, the exponent
-    // of the unit of V's, and the keys to be added alone; of others, the keys
-    // whose values are none, as each wave finds them.
-    static constexpr int SIDE = (2 * KB + 4) * 4;
-    static constexpr int LDS = TILES + (CODES ? BUFS * SIDE : WAVES > 1 ? BUFS * 8 * WAVES : 0);
+    // Behind the tiles: of codes, each buffer's scales of K and V, those of V that
+    // are added apart, and the exponent of their unit; then a word a wave.
+    static constexpr int SIDE = (3 * KB + 4) * 4;
+    static constexpr int FLAGS = TILES + (CODES ? BUFS * SIDE : 0);
+    static constexpr int LDS = FLAGS + (WAVES > 1 ? 4 * WAVES : 0);
     static constexpr int OCC = F32 ? (DP <= (HELD == Held::Chunks ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;
     // LDS serves 256 bytes a cycle, and rows' chunks are swapped so that what it
     // serves at once lies in different banks: 16 keys of one chunk of K; of V what
@@ -478,6 +478,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
         codes_t kq[STAGED ? NL : 1], vq[STAGED ? NL : 1];
         float sk = 0.0f, sv = 0.0f;
         int unit = LEAST_UNIT;          // the exponent of the weights' unit (F16 codes)
+        bool apart = false;             // some values are to be added apart
 
         // n of a unit's codes, a word at a time.
         const auto some_codes = [&](const int8_t *p, int n) {
@@ -618,31 +619,33 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (wave == 0) {
-                    bool alone = !(fabsf(sv) < INFINITY);
+                    // Values that some rows do not see, and that those cannot have
+                    // next to theirs, are added apart.
+                    const bool common = t * KB + lane <= all_hi && t * KB + lane >= all_lo;
+                    bool alone = lane < KB && !common && !(fabsf(sv) < INFINITY);
                     if constexpr (F16) {
                         // F16 weights have no range for a scale's: they are of its
                         // size against a power of 2 that is twice to four times the
                         // largest so far. One that not every row sees has no say in
-                        // that; a larger one is added alone, in F32.
-                        const bool common = t * KB + lane <= all_hi && t * KB + lane >= all_lo;
+                        // that; a larger one is apart.
                         const auto past = [&] { return fabsf(sv) > __uint_as_float((uint32_t)(127 + unit) << 23); };
-                        if (__ballot(lane < KB && common && !alone && past()) != 0) {
-                            float top = lane < KB && common && !alone ? fabsf(sv) : 0.0f;
+                        const bool counts = lane < KB && common && fabsf(sv) < INFINITY;
+                        if (__ballot(counts && past()) != 0) {
+                            float top = counts ? fabsf(sv) : 0.0f;
 #pragma unroll
                             for (int o = KB / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
                             unit = uniform(min(126, (int)(__float_as_uint(top) >> 23) - 127 + 2));
                         }
-                        alone |= !common && past();
+                        alone |= lane < KB && !common && past();
                     }
+                    apart |= alone;
                     if (lane < KB) {
+                        const float v = F16 ? sv * __uint_as_float((uint32_t)(127 - unit) << 23) : sv;
                         side[lane] = sk;
-                        side[KB + lane] = F16 ? sv * __uint_as_float((uint32_t)(127 - unit) << 23) : sv;
+                        side[KB + lane] = alone ? 0.0f : v;
+                        side[2 * KB + lane] = alone ? v : 0.0f;
                     }
-                    const uint64_t none = __ballot(lane < KB && alone);
-                    if (lane == 0) {
-                        ((int *)side)[2 * KB] = unit;
-                        ((uint32_t *)side)[2 * KB + 2] = (uint32_t)none, ((uint32_t *)side)[2 * KB + 3] = (uint32_t)(none >> 32);
-                    }
+                    if (lane == 0) ((int *)side)[3 * KB] = unit;
                 }
             }
         };
@@ -832,54 +835,15 @@ self_tiles(SelfArgs a, SelfParts parts) {
             m = mn;
             far = __ballot(fabsf(m) > 16777216.0f && m != -INFINITY) != 0;
         };
-        // Values that are no numbers weigh nothing for the rows that do not see
-        // them, and 0 times them is no number either: where some row does not,
-        // their keys are added one by one, and are 0 for the products.
-        const auto add_alone = [&](const char *V, const float *side, const scores_t (&s)[SUB], uint64_t seen, uint64_t bad,
-                                   float scale, float base) {
-            const int h = fresh(lane) / M;
-            for (; bad; bad &= bad - 1) {
-                const int key = __ffsll((unsigned long long)bad) - 1;
-                const int u = key >> 5, i = (key & 31) / (4 * H) * 4 + (key & 3), from = (key >> 2) % H;
-                float x = 0.0f;
-#pragma unroll
-                for (int v = 0; v < SUB; ++v)
-#pragma unroll
-                    for (int n = 0; n < NS; ++n) x = u == v && i == n ? s[v][n] : x;
-                x = __shfl(x, r + M * from, 64);
-                float w = __builtin_amdgcn_exp2f(fmaf(x, scale, -base));
-                if constexpr (CODES) w *= side[KB + key];
-                const bool see = seen >> key & 1;
-                // (Four at a time: this path is to cost no registers.)
-                typedef T four __attribute__((ext_vector_type(4)));
-                const char *row = V + key * PITCH;
-                const int swap = C::swap_v(key);
-#pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int g = 0; g < NR / 4; ++g) {
-                        const int at = (M * t + 4 * H * g + 4 * h) * (BYTES ? 1 : (int)sizeof(T));
-                        const char *p = row + ((at >> 4) ^ swap) * 16 + (at & 15);
-                        four v;
-                        if constexpr (BYTES) {
-                            T n[4];
-                            numbers_of(*(const uint32_t *)p, n);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] = n[e];
-                        } else {
-                            v = *(const four *)p;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            o[t][4 * g + e] = see ? fmaf(w, to_f32(v[e]), o[t][4 * g + e]) : o[t][4 * g + e];
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-            }
+        // The keys of a tile that this lane's row sees.
+        const auto seen_of = [&](uint64_t live, int t) -> uint64_t {
+            if (t * KB + KB - 1 <= all_hi && t * KB >= all_lo) return live;   // uniform
+            const int lo = max(0, low - t * KB), hi = min(KB - 1, pos - t * KB);
+            return lo > hi ? 0 : live & (~0ull << lo) & (~0ull >> (63 - hi));
         };
-        const auto tile = [&](const char *K, float *side, uint64_t live, int t, uint64_t bad) {
-            scores_t s[SUB];
+        const auto scaled_scores = [&](const char *K, const float *side, scores_t (&s)[SUB]) {
             scores(K, s);
-            if constexpr (CODES) {
+            if constexpr (CODES)
 #pragma unroll
                 for (int u = 0; u < SUB; ++u)
 #pragma unroll
@@ -888,21 +852,20 @@ self_tiles(SelfArgs a, SelfParts parts) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) s[u][4 * g + e] *= f[e];
                     }
-                if constexpr (F16) {
-                    const int now = uniform(((const int *)side)[2 * KB]);
-                    if (now != my_unit) {   // uniform
-                        const float f = my_unit - now < -126 ? 0.0f : __uint_as_float((uint32_t)(127 + my_unit - now) << 23);
+        };
+        const auto tile = [&](const char *K, const float *side, uint64_t live, int t) {
+            scores_t s[SUB];
+            scaled_scores(K, side, s);
+            if constexpr (CODES && F16) {
+                const int now = uniform(((const int *)side)[3 * KB]);
+                if (now != my_unit) {   // uniform
+                    const float f = my_unit - now < -126 ? 0.0f : __uint_as_float((uint32_t)(127 + my_unit - now) << 23);
 #pragma unroll
-                        for (int t = 0; t < DT; ++t) o[t] *= f;
-                        my_unit = now;
-                    }
+                    for (int t = 0; t < DT; ++t) o[t] *= f;
+                    my_unit = now;
                 }
             }
-            uint64_t seen = live;
-            if (t * KB + KB - 1 > all_hi || t * KB < all_lo) {   // uniform
-                const int lo = max(0, low - t * KB), hi = min(KB - 1, pos - t * KB);
-                seen = lo > hi ? 0 : seen & (~0ull << lo) & (~0ull >> (63 - hi));
-            }
+            const uint64_t seen = seen_of(live, t);
             any |= seen != 0;
             if (__ballot(seen != FULL) != 0) {
 #pragma unroll
@@ -929,33 +892,87 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 for (int u = 0; u < SUB; ++u) s[u] *= scale;
                 scale = 1.0f;
             }
-            if (bad) add_alone(K + BUF, side, s, seen, bad, scale, base);
-            return [=, &l, &add_values](const char *V) {
 #pragma unroll
-                for (int u = 0; u < SUB; ++u) {
-                    float sum = 0.0f;
-                    f32x4 sv[NS / 4];
-                    if constexpr (CODES)
+            for (int u = 0; u < SUB; ++u) {
+                float sum = 0.0f;
+                f32x4 sv[NS / 4];
+                if constexpr (CODES)
 #pragma unroll
-                        for (int g = 0; g < NS / 4; ++g) sv[g] = *(const f32x4 *)(side + KB + 32 * u + 4 * H * g + 4 * h);
-                    add_values(V + 32 * u * PITCH, [&](int i) {
-                        const float w = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
-                        sum += w;
-                        if constexpr (CODES) return w * sv[i >> 2][i & 3];
-                        return w;
-                    });
-                    l += sum;
-                }
-            };
+                    for (int g = 0; g < NS / 4; ++g) sv[g] = *(const f32x4 *)(side + KB + 32 * u + 4 * H * g + 4 * h);
+                add_values(K + BUF + 32 * u * PITCH, [&](int i) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
+                    sum += w;
+                    if constexpr (CODES) return w * sv[i >> 2][i & 3];
+                    return w;
+                });
+                l += sum;
+            }
         };
+        // Values that are no numbers weigh nothing for the rows that do not see
+        // them, but 0 times them is no number: where some row does not see them,
+        // they are 0 for the products, and are added here, once the maxima are
+        // known. (Slowly: this is as good as never.)
+        const auto add_apart = [&](const char *K, const float *side, uint64_t live, int t) {
+            scores_t s[SUB];
+            scaled_scores(K, side, s);
+            const int h = fresh(lane) / M;
+            const uint64_t seen = seen_of(live, t);
+            const float base = m == -INFINITY ? 0.0f : m;
+            float unit = 1.0f;
+            if constexpr (CODES && F16) unit = __builtin_amdgcn_exp2f((float)(((const int *)side)[3 * KB] - my_unit));
+            for (int key = 0; key < KB; ++key) {
+                const bool see = seen >> key & 1;
+                if (__ballot(see) == 0) continue;
+                float extra = 1.0f;
+                if constexpr (CODES) {
+                    extra = side[2 * KB + key];
+                    if (__ballot(extra != 0.0f) == 0) continue;
+                    extra *= unit;
+                }
+                const int i = (key & 31) / (4 * H) * 4 + (key & 3), from = (key >> 2) % H;
+                float x = 0.0f;
+#pragma unroll
+                for (int v = 0; v < SUB; ++v)
+#pragma unroll
+                    for (int n = 0; n < NS; ++n) x = key >> 5 == v && i == n ? s[v][n] : x;
+                x = __shfl(x, r + M * from, 64);
+                const float w = (far ? __builtin_amdgcn_exp2f(x * a.scale - base)
+                                     : __builtin_amdgcn_exp2f(fmaf(x, a.scale, -base))) * extra;
+                typedef T four __attribute__((ext_vector_type(4)));
+                const char *row = K + BUF + key * PITCH;
+                const int swap = C::swap_v(key);
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int g = 0; g < NR / 4; ++g) {
+                        const int at = (M * t + 4 * H * g + 4 * h) * (BYTES ? 1 : (int)sizeof(T));
+                        const char *p = row + ((at >> 4) ^ swap) * 16 + (at & 15);
+                        four v;
+                        if constexpr (BYTES) {
+                            T n[4];
+                            numbers_of(*(const uint32_t *)p, n);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] = n[e];
+                        } else {
+                            v = *(const four *)p;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float f = to_f32(v[e]);
+                            o[t][4 * g + e] = see && (CODES || !(fabsf(f) < INFINITY)) ? fmaf(w, f, o[t][4 * g + e]) : o[t][4 * g + e];
+                        }
+                        __builtin_amdgcn_sched_barrier(0);   // (this path is to cost no registers)
+                    }
+            }
+        };
+        const auto is_partial = [&](int t) { return t * KB + KB - 1 > all_hi || t * KB < all_lo; };   // uniform
 
         for (int t = t0, buf = 0; t < t1; ++t, buf ^= C::BUFS - 1) {
             char *K = smem + buf * 2 * BUF, *V = K + BUF;
-            float *side = (float *)(smem + C::TILES + buf * C::SIDE);
+            const float *side = (const float *)(smem + C::TILES + buf * C::SIDE);
             if constexpr (!STAGED) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
             if constexpr (CODES) put(t, buf);
             const uint64_t live = __ballot(alive);
-            const bool partial = t * KB + KB - 1 > all_hi || t * KB < all_lo;   // uniform: not every row sees all of it
             if (!CODES && live != FULL) {   // uniform
                 // A value that is no state's weighs 0, but not if it is no number.
                 const int lane = fresh(tid & 63);
@@ -963,55 +980,52 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 for (int j = 0; j < NL; ++j)
                     if (!((live >> key_at(j, lane)) & 1)) *(vec *)(V + unit_at(j, lane) * 16) = vec{};
             }
-            uint64_t bad = 0;
-            if (!CODES && partial) {
-                // Keys of this wave's chunks with an infinity or a NaN among their values.
+            if (!CODES && is_partial(t)) {
                 const int lane = fresh(tid & 63);
 #pragma unroll
                 for (int j = 0; j < NL; ++j) {
-                    const vec x = *(const vec *)(V + unit_at(j, lane) * 16);
+                    vec x = *(const vec *)(V + unit_at(j, lane) * 16);
                     float sum = 0.0f;
 #pragma unroll
                     for (int e = 0; e < E; ++e) sum = fmaf(to_f32(x[e]), 0.0f, sum);
-                    uint64_t lanes = __ballot(sum != 0.0f);   // (0 times a number is 0)
-                    for (; lanes; lanes &= lanes - 1)
-                        bad |= 1ull << (((wave * NL + j) * 64 + __ffsll((unsigned long long)lanes) - 1) / CPR);
+                    if (sum != 0.0f) {   // (0 times a number is 0)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) x[e] = fabsf(to_f32(x[e])) < INFINITY ? x[e] : (T)0.0f;
+                        *(vec *)(V + unit_at(j, lane) * 16) = x;
+                        apart = true;
+                    }
                 }
-                if (WAVES > 1 && lane == 0) ((uint64_t *)(smem + C::TILES))[buf * WAVES + wave] = bad;
             }
             __syncthreads();   // the tile is there, and the other one read
-            if (CODES && partial)
-                bad = (uint64_t)(uint32_t)uniform(((const int *)side)[2 * KB + 2]) |
-                      (uint64_t)(uint32_t)uniform(((const int *)side)[2 * KB + 3]) << 32;
-            if (!CODES && WAVES > 1 && partial) {
-                bad = 0;
-#pragma unroll
-                for (int w = 0; w < WAVES; ++w) bad |= ((const uint64_t *)(smem + C::TILES))[buf * WAVES + w];
-                bad = (uint64_t)(uint32_t)uniform((int)bad) | (uint64_t)(uint32_t)uniform((int)(bad >> 32)) << 32;
-            }
             if (t + 1 < t1) {
                 slot = next_slot;
                 load(t + 1, buf ^ 1);
                 next_slot = slot_at(t + 2);
             }
-            const auto zero = [&] {   // (called by all waves: bad is the same for all)
-                __syncthreads();
-                if constexpr (CODES) {
-                    if (tid < KB && (bad >> tid & 1)) side[KB + tid] = 0.0f;
-                } else {
-                    const int lane = fresh(tid & 63);
+            if (work && live != 0) tile(K, side, live, t);
+        }
+        bool again = __ballot(apart) != 0;
+        if constexpr (WAVES > 1) {
+            int *flags = (int *)(smem + C::FLAGS);
+            if (lane == 0) flags[wave] = again;
+            __syncthreads();
+            int sum = 0;
 #pragma unroll
-                    for (int j = 0; j < NL; ++j)
-                        if ((bad >> key_at(j, lane)) & 1) *(vec *)(V + unit_at(j, lane) * 16) = vec{};
-                }
+            for (int w = 0; w < WAVES; ++w) sum |= flags[w];
+            again = uniform(sum) != 0;
+        }
+        if (again) {   // uniform over the workgroup
+            unit = LEAST_UNIT;
+            for (int t = t0; t < t1; ++t) {
+                if (!CODES && !is_partial(t)) continue;
                 __syncthreads();
-            };
-            if (work && live != 0) {
-                const auto add = tile(K, side, live, t, bad);
-                if (bad) zero();
-                add(V);
-            } else if (bad) {
-                zero();
+                slot = slot_at(t);
+                load(t, 0);
+                __builtin_amdgcn_s_waitcnt(0x0f70);
+                if constexpr (CODES) put(t, 0);
+                const uint64_t live = __ballot(alive);
+                __syncthreads();
+                if (work && is_partial(t)) add_apart(smem, (const float *)(smem + C::TILES), live, t);
             }
         }
 
