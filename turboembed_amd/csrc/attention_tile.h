@@ -59,6 +59,36 @@ __device__ __forceinline__ auto below(float w0, float w1) {
     return __builtin_bit_cast(two, __builtin_elementwise_sub_sat(b, bits2{1, 1}));
 }
 
+// LDS reads that transpose, N of them of each of A addresses, the second OFF
+// bytes behind the first, all from AT on, waited for here: for the builtins the
+// compiler waits for every load to LDS that is on its way too, those of the next
+// tile, which these do not read.
+typedef uint32_t words2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) const void *lds_ptr;
+#define TURBO_READS_8(OP)                                                                                              \
+    asm volatile(OP " %0, %8 offset:%12\n\t" OP " %1, %8 offset:%13\n\t" OP " %2, %9 offset:%12\n\t"                  \
+                 OP " %3, %9 offset:%13\n\t" OP " %4, %10 offset:%12\n\t" OP " %5, %10 offset:%13\n\t"                 \
+                 OP " %6, %11 offset:%12\n\t" OP " %7, %11 offset:%13\n\ts_waitcnt lgkmcnt(0)"                        \
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7]) \
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(AT), "n"(AT + OFF)                               \
+                 : "memory")
+#define TURBO_READS_4(OP)                                                                                              \
+    asm volatile(OP " %0, %4 offset:%8\n\t" OP " %1, %5 offset:%8\n\t" OP " %2, %6 offset:%8\n\t" OP                 \
+                    " %3, %7 offset:%8\n\ts_waitcnt lgkmcnt(0)"                                                         \
+                 : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3])                                                   \
+                 : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(AT)                                              \
+                 : "memory")
+// 16-bit elements: two reads of each address, v[2 i] and v[2 i + 1].
+template <int AT, int OFF> __device__ __forceinline__ void read_tr16(words2 (&v)[8], const uint32_t (&at)[4]) {
+    TURBO_READS_8("ds_read_b64_tr_b16");
+}
+// Bytes: one of each.
+template <int AT> __device__ __forceinline__ void read_tr8(words2 (&v)[4], const uint32_t (&at)[4]) {
+    TURBO_READS_4("ds_read_b64_tr_b8");
+}
+#undef TURBO_READS_8
+#undef TURBO_READS_4
+
 // The product whose result has M rows and columns: lane l has column l % M of
 // it, and rows 4 (64 / M) (i / 4) + 4 (l / M) + i % 4 in register i. 16-bit
 // operands: row or column l % M, 8 steps of the inner width from 8 (l / M) on.

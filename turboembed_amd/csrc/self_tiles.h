@@ -726,13 +726,28 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     for (int e = 0; e < E; ++e) part[0][0] = Mul::run(k[x % 3][e], q[x][e], part[0][0]);
                 }
             } else {
-#pragma unroll
-                for (int x = 0; x < NQ; ++x)
+                // (Chunks read two steps ahead of their products: an LDS read takes
+                // longer than the products of one.)
+                constexpr int AHEAD = NQ < 3 ? NQ : 3;
+                vec k[AHEAD][SUB][BLOCKS];
+                const auto ahead = [&](int x) {
 #pragma unroll
                     for (int u = 0; u < SUB; ++u)
 #pragma unroll
                         for (int v = 0; v < BLOCKS; ++v)
-                            part[u][v] = Mul::run(*(const vec *)(row(u, v) + ((H * x + h) ^ swap(v)) * 16), q[x], part[u][v]);
+                            k[x % AHEAD][u][v] = *(const vec *)(row(u, v) + ((H * x + h) ^ swap(v)) * 16);
+                };
+#pragma unroll
+                for (int x = 0; x < AHEAD - 1; ++x) ahead(x);
+#pragma unroll
+                for (int x = 0; x < NQ; ++x) {
+                    if (x + AHEAD - 1 < NQ) ahead(x + AHEAD - 1);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                        for (int v = 0; v < BLOCKS; ++v) part[u][v] = Mul::run(k[x % AHEAD][u][v], q[x], part[u][v]);
+                }
             }
 #pragma unroll
             for (int u = 0; u < SUB; ++u)
@@ -764,11 +779,18 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 // 8 H keys a product: registers 8 j .. 8 j + 7. A group of 16 lanes
                 // reads 4 keys by 16 columns, and a lane gets its column's 4; of
                 // codes 8 keys.
-                typedef short s4 __attribute__((ext_vector_type(4)));
-                typedef int w2 __attribute__((ext_vector_type(2)));
                 const int n = lane & 15, half = r >> 4;    // which 16 of the product's columns
+                // (4 H keys on, and 8 H, the swap is the same.)
+                constexpr int AT = DT < 4 ? DT : DT % 4 == 0 ? 4 : 3;   // results at a time
+                uint32_t place[DT];
 #pragma unroll
-                for (int j = 0; j < NS / 8; ++j) {
+                for (int t = 0; t < DT; ++t) {
+                    const int k = BYTES ? 4 * H * (n >> 3) + 4 * h + ((n >> 1) & 3) : 4 * h + (n >> 2);
+                    const int x = BYTES ? M / 16 * t + half : M / 8 * t + 2 * half + ((n >> 1) & 1);
+                    place[t] = (uint32_t)(uintptr_t)(lds_ptr)(V + k * PITCH + (x ^ C::swap_v(k)) * 16 + (n & 1) * 8);
+                }
+                const auto product = [&](auto jj) {
+                    constexpr int j = decltype(jj)::value;
                     frag f, rest;
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
@@ -781,47 +803,42 @@ self_tiles(SelfArgs a, SelfParts parts) {
                             f[e] = from_f32<T>(w0), f[e + 1] = from_f32<T>(w1);
                         }
                     }
-                    const auto column = [&](int t) {
-                        if constexpr (BYTES) {
-                            const int k = 8 * H * j + 4 * H * (n >> 3) + 4 * h + ((n >> 1) & 3);
-                            const w2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                                (__attribute__((address_space(3))) w2 *)(V + k * PITCH +
-                                                                         ((M / 16 * t + half) ^ C::swap_v(k)) * 16 + (n & 1) * 8));
-                            T y[8];
-                            numbers_of((uint32_t)w[0], y), numbers_of((uint32_t)w[1], y + 4);
-                            frag v;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) v[e] = y[e];
-                            return v;
-                        } else {
-                            const int x = M / 8 * t + 2 * half + ((n >> 1) & 1), key = 8 * H * j + 4 * h + (n >> 2);
-                            const auto place = [&](int k) {
-                                return (__attribute__((address_space(3))) s4 *)(V + k * PITCH + (x ^ C::swap_v(k)) * 16 +
-                                                                                 (n & 1) * 8);
-                            };
-                            struct {
-                                s4 lo, hi;
-                            } v;
-                            v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(key));
-                            v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(place(key + 4 * H));
-                            return __builtin_bit_cast(frag, v);
-                        }
-                    };
-                    // (Four results at a time: the second numbers' products after the first's.)
-                    constexpr int AT = DT < 4 ? DT : DT % 4 == 0 ? 4 : 3;
 #pragma unroll
                     for (int t0 = 0; t0 < DT; t0 += AT) {
-                        frag v[AT];
+                        uint32_t at[4];
 #pragma unroll
-                        for (int t = 0; t < AT; ++t) {
-                            v[t] = column(t0 + t);
-                            o[t0 + t] = Mul::run(v[t], f, o[t0 + t]);
+                        for (int t = 0; t < 4; ++t) at[t] = place[t0 + (t < AT ? t : 0)];
+                        frag v[AT];
+                        if constexpr (BYTES) {
+                            words2 w[4];
+                            read_tr8<8 * H * j * PITCH>(w, at);
+#pragma unroll
+                            for (int t = 0; t < AT; ++t) {
+                                T y[8];
+                                numbers_of(w[t][0], y), numbers_of(w[t][1], y + 4);
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) v[t][e] = y[e];
+                            }
+                        } else {
+                            words2 w[8];
+                            read_tr16<8 * H * j * PITCH, 4 * H * PITCH>(w, at);
+#pragma unroll
+                            for (int t = 0; t < AT; ++t) {
+                                struct {
+                                    words2 lo, hi;
+                                } both{w[2 * t], w[2 * t + 1]};
+                                v[t] = __builtin_bit_cast(frag, both);
+                            }
                         }
+#pragma unroll
+                        for (int t = 0; t < AT; ++t) o[t0 + t] = Mul::run(v[t], f, o[t0 + t]);
                         if constexpr (TWO)
 #pragma unroll
                             for (int t = 0; t < AT; ++t) o[t0 + t] = Mul::run(v[t], rest, o[t0 + t]);
                     }
-                }
+                };
+                product(std::integral_constant<int, 0>());
+                if constexpr (NS / 8 > 1) product(std::integral_constant<int, 1>());
             }
         };
         const auto raise = [&](float mx) {   // m, for scores of up to mx
