@@ -89,6 +89,7 @@ enum class Held : int { Chunks, Loose, Codes, Bytes };
 struct SelfLaunch {
     Held held;
     int rows;            // of a block: 16 or 32 (a wave's), or 128 (four waves')
+    bool split;          // 32 rows are four waves', each with every fourth tile of the keys
     uint32_t groups;     // workgroups: of a prompt, the most blocks that there can be
     int pieces;          // of a call over a cache, each a workgroup of every key head
     int part_rows;       // the most rows of a part

@@ -35,18 +35,29 @@ SelfLaunch self_plan(const SelfArgs &a) {
     const bool chunks = a.c.width * size % 16 == 0 && whole(a.c.k, a.c.ks) && whole(a.c.v, a.c.vs) &&
                         std::max(a.c.ks[0], a.c.vs[0]) < (1u << 31) / 64 / 4;
     f.held = a.i8 ? Held::Codes : chunks ? Held::Chunks : Held::Loose;
-    // Blocks of 128 rows, where sequences have more than a wave's on average and
-    // there are enough of them for every compute unit; of 16, where they have no
-    // more.
+    const bool f32 = a.dt == Dt::F32;
     f.rows = 32;
-    if (f.held != Held::Loose && rows > 32 * seqs && (a.c.paged || a.c.kv * (rows / 128 + seqs) >= 512)) f.rows = 128;
+    if (f.held == Held::Chunks && !a.c.paged) {
+        // Prompts: blocks of 128 rows, where there are enough of them for every
+        // compute unit; else four waves a block of 32. F32, whose products take long:
+        // a wave a block of 32, if those are enough. us, waves of 32 rows, four of 128,
+        // four of 32:
+        //   F32  24 x 20-500 tokens, 12 heads of 64    72   70   82
+        //   F32  3032 tokens, 12 heads of 128          520  519  318
+        //   BF16 2000 tokens, 12 heads of 64           63        28
+        if (!f32 && a.c.kv * (rows / 128 + seqs) >= 512 && rows > 32 * seqs) f.rows = 128;
+        else f.split = !f32 || a.c.kv * (rows / 32 + seqs) < 2048;
+    } else if (f.held != Held::Loose && rows > 32 * seqs) {
+        f.rows = 128;
+    }
     // A wave alone makes numbers of codes as it reads them, four of them once.
     // (F32's slow products leave it no need to.)
-    if (a.i8 && f.rows == 32 && chunks && a.dt != Dt::F32) f.held = Held::Bytes;
-    if (a.c.paged && a.dt != Dt::F32 && rows <= 16 * seqs && (f.held == Held::Bytes || f.held == Held::Chunks)) f.rows = 16;
+    if (a.i8 && f.rows == 32 && chunks && !f32) f.held = Held::Bytes;
+    // Tokens of few heads: blocks of 16 rows.
+    if (a.c.paged && !f32 && rows <= 16 * seqs && (f.held == Held::Bytes || f.held == Held::Chunks)) f.rows = 16;
     const uint64_t blocks = a.c.kv * (rows / f.rows + seqs);   // at most
     if (!a.c.paged) {
-        if (blocks * (f.rows == 128 ? 256 : 64) > 1ull << 31)
+        if (blocks * (f.rows == 128 || f.split ? 256 : 64) > 1ull << 31)
             fail(TURBO_E_CAPACITY, "rocm: a prompt of " + std::to_string(blocks) + " workgroups");
         f.groups = (uint32_t)blocks;
         return f;

@@ -5,13 +5,14 @@
 // The rows of a (sequence, key head) are its tokens' heads that read it, row r
 // token r / share, head kv * share + r % share: its keys and values are read
 // once for all of them. M of them, 32 or 16, are a wave's; a block is one wave's
-// or four waves'. A block's keys pass through LDS in tiles of KB. Scores are
+// or four waves', or the same rows are four waves', each with every fourth tile
+// of the keys. A block's keys pass through LDS in tiles of KB. Scores are
 // computed transposed, S^T = K Q^T, so that a lane holds one row (lane % M) and
-// M / 2 of 32 keys, the others in the lanes M apart; O^T += V^T P^T then takes P as
-// the score registers hold it, against V's columns for the same keys in that
-// order (16-bit values by LDS reads that transpose, F32 values one by one). The softmax is the
-// running one, in base 2 and F32: what it takes for a row's maximum moves only
-// when a score is 2^8 above the one that it was set by.
+// M / 2 of 32 keys, the others in the lanes M apart; O^T += V^T P^T then takes P
+// as the score registers hold it, against V's columns for the same keys in that
+// order (16-bit values by LDS reads that transpose, F32 values one by one). The
+// softmax is the running one, in base 2 and F32: what it takes for a row's
+// maximum moves only when a score is 2^8 above the one that it was set by.
 //
 // Int8 states' codes are numbers of every type, so they go into the products
 // unscaled: a key's scale is a factor of its scores, a value's one of its
@@ -32,21 +33,25 @@ namespace rocm {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-template <typename T, Held HELD, int DP, int WAVES, int M> struct SelfTile {
+template <typename T, Held HELD, int DP, int WAVES, int M, int SPLIT> struct SelfTile {
     static constexpr bool F32 = std::is_same<T, float>::value;
     static constexpr bool BYTES = HELD == Held::Bytes, CODES = HELD == Held::Codes || BYTES;
     static constexpr int ROWS = M * WAVES;
     static constexpr int KB = WAVES == 1 || F32 ? 32 : 64;
     static constexpr int PITCH = DP * (BYTES ? 1 : (int)sizeof(T)), CPR = PITCH / 16;   // a row's bytes and chunks in LDS
     static constexpr int BUF = KB * PITCH;
-    // (A wave alone writes a tile of codes' numbers once it has read the one before.)
-    static constexpr int BUFS = HELD == Held::Codes && WAVES == 1 ? 1 : 2;
+    // (A wave alone writes a tile of codes' numbers once it has read the one before.
+    // While one of F32 or of those that share rows waits for its tile, another of
+    // its SIMD computes: more of them fit.)
+    static constexpr int BUFS = WAVES == 1 && (SPLIT > 1 || F32 || HELD == Held::Codes) ? 1 : 2;
     static constexpr int TILES = BUFS * 2 * BUF;
     // Behind the tiles: of codes, each buffer's scales of K and V, those of V that
     // are added apart, and the exponent of their unit; then a word a wave.
     static constexpr int SIDE = (3 * KB + 4) * 4;
     static constexpr int FLAGS = TILES + (CODES ? BUFS * SIDE : 0);
-    static constexpr int LDS = FLAGS + (WAVES > 1 ? 4 * WAVES : 0);
+    // Of waves that share rows each has an area, where it leaves its results.
+    static constexpr int RESULTS = M * DP * 4 + 1024, AREA = FLAGS > RESULTS ? FLAGS : RESULTS;
+    static constexpr int LDS = SPLIT > 1 ? SPLIT * AREA : FLAGS + (WAVES > 1 ? 4 * WAVES : 0);
     static constexpr int OCC = F32 ? (DP <= (HELD == Held::Chunks ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;
     // LDS serves 256 bytes a cycle, and rows' chunks are swapped so that what it
     // serves at once lies in different banks: 16 keys of one chunk of K; of V what
@@ -358,12 +363,15 @@ __device__ __forceinline__ void two_of(float w0, float w1, T (&hi)[2], T (&lo)[2
     }
 }
 
-template <typename T, Held HELD, bool PAGED, int DP, int WAVES, int M>
-__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(SelfTile<T, HELD, DP, WAVES, M>::OCC)))
+template <typename T, Held HELD, bool PAGED, int DP, int WAVES, int M, int SPLIT>
+__global__ void __launch_bounds__(64 * WAVES * SPLIT)
+__attribute__((amdgpu_waves_per_eu(SelfTile<T, HELD, DP, WAVES, M, SPLIT>::OCC)))
 self_tiles(SelfArgs a, SelfParts parts) {
-    using C = SelfTile<T, HELD, DP, WAVES, M>;
+    using C = SelfTile<T, HELD, DP, WAVES, M, SPLIT>;
+    static_assert(WAVES == 1 || SPLIT == 1, "waves share a tile or rows");
+    constexpr int THREADS = 64 * WAVES * SPLIT;
     using Mul = Product<T, M>;
-    constexpr bool F32 = C::F32, CODES = C::CODES, F16 = std::is_same<T, _Float16>::value, TWO = WAVES == 1 && !F32;
+    constexpr bool F32 = C::F32, CODES = C::CODES, F16 = std::is_same<T, _Float16>::value, TWO = WAVES == 1 && SPLIT == 1 && !F32;
     constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR;
     constexpr int E = Chunk<T>::N, ROWS = C::ROWS;
     // Lanes of a row; a lane's scores of 32 keys; the results of the product with
@@ -383,7 +391,15 @@ self_tiles(SelfArgs a, SelfParts parts) {
     typedef float scores_t __attribute__((ext_vector_type(M / 2)));
     extern __shared__ __attribute__((aligned(1024))) char smem[];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, number = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // Which of the waves that share a tile, or the keys.
+    const int wave = WAVES > 1 ? number : 0, own = SPLIT > 1 ? number : 0;
+    char *const area = smem + (SPLIT > 1 ? own * C::AREA : 0);
+    // What the waves of a tile, or this one alone, wait for each other with.
+    const auto sync = [] {
+        if constexpr (SPLIT > 1) asm volatile("" ::: "memory");
+        else __syncthreads();
+    };
     const int r = lane % M, h = lane / M, d = a.c.width;
     const CacheArgs &c = a.c;
 
@@ -419,7 +435,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
 
     if (HELD == Held::Chunks && d < DP) {   // uniform
         // (Columns past the width keep these zeros.)
-        for (int i = tid; i < C::TILES / 16; i += 64 * WAVES) *(vec *)(smem + i * 16) = vec{};
+        for (int i = tid; i < C::LDS / 16; i += THREADS) *(vec *)(smem + i * 16) = vec{};
     }
 
     Place at{}, end{};
@@ -435,12 +451,12 @@ self_tiles(SelfArgs a, SelfParts parts) {
         else at = end = Place{c.seqs, 0, 0};
         if (!front && tid == 0) parts.marks[unit_id] = SelfMark{};
     } else {
-        const Turn<ROWS, C::TILES / 4> turn(a, blockIdx.x, smem, 64 * WAVES);
+        const Turn<ROWS, C::TILES / 4> turn(a, blockIdx.x, smem, THREADS);
         if (!turn.any) return;
         at = Place{turn.seq, turn.block, 0}, kv = turn.kv;
         if (HELD == Held::Chunks && d < DP && c.seqs > 64) {
             __syncthreads();
-            for (int i = tid; i < C::TILES / 16; i += 64 * WAVES) *(vec *)(smem + i * 16) = vec{};
+            for (int i = tid; i < C::LDS / 16; i += THREADS) *(vec *)(smem + i * 16) = vec{};
         }
     }
     // (A workgroup that begins where it ends, inside of a block, leaves a part
@@ -462,6 +478,9 @@ self_tiles(SelfArgs a, SelfParts parts) {
         // block does.
         const int pos = seq.first() + of_token;
         const int low = a.window > pos ? 0 : pos - a.window + 1;
+        // ...and those that any of this wave's rows does.
+        const int ahead = ROWS == M ? b.last : seq.first() + (b.row0 + min(M * wave + M, b.rows) - 1) / a.share;
+        const int behind = ROWS == M ? 0 : uniform(__builtin_amdgcn_readlane(low, 0));
         const int all_hi = b.at0, all_lo = a.window > b.last ? 0 : b.last - a.window + 1;
         const Kept *K0 = (const Kept *)c.k + b.kv * c.ks[1], *V0 = (const Kept *)c.v + b.kv * c.vs[1];
 
@@ -501,7 +520,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
         };
         // Starts the tile of `slot` on its way; without pages, tile t.
         const auto load = [&](int t, int buf) {
-            char *K = smem + buf * 2 * BUF, *V = K + BUF;
+            char *K = area + buf * 2 * BUF, *V = K + BUF;
             alive = slot >= 0;
             if constexpr (CODES)
                 if (wave == 0) {
@@ -512,12 +531,13 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 // (As buffer loads where a base is common to the lanes: those
                 // take 32-bit offsets.)
                 typedef __attribute__((address_space(3))) void *to;
+                typedef __attribute__((address_space(3))) char *lds;
                 typedef __attribute__((address_space(1))) const void *from;
                 const auto rsrc = [](const Kept *p) {
                     return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, -1, 0x00020000);
                 };
                 const auto send = [&](__amdgpu_buffer_rsrc_t tile, uint32_t at, char *dst) {
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(tile, (to)dst, 16, (int)at, 0, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(tile, (to)((lds)smem + (dst - smem)), 16, (int)at, 0, 0, 0);
                 };
                 const auto base = [&](int j) {
                     // (Without a page: slot 0, whose keys are not looked at.)
@@ -551,10 +571,10 @@ self_tiles(SelfArgs a, SelfParts parts) {
                         const uint64_t s = (uint64_t)max(0, __shfl(slot, key_at(j, lane), 64));
                         const int ck = col_k_at(j, lane), cv = col_v_at(j, lane);
                         if (ck < d)
-                            __builtin_amdgcn_global_load_lds((from)(K0 + s * c.ks[0] + ck), (to)(K + (wave * NL + j) * 1024),
+                            __builtin_amdgcn_global_load_lds((from)(K0 + s * c.ks[0] + ck), (to)((lds)smem + (K - smem) + (wave * NL + j) * 1024),
                                                              16, 0, 0);
                         if (cv < d)
-                            __builtin_amdgcn_global_load_lds((from)(V0 + s * c.vs[0] + cv), (to)(V + (wave * NL + j) * 1024),
+                            __builtin_amdgcn_global_load_lds((from)(V0 + s * c.vs[0] + cv), (to)((lds)smem + (V - smem) + (wave * NL + j) * 1024),
                                                              16, 0, 0);
                     }
                 }
@@ -595,8 +615,8 @@ self_tiles(SelfArgs a, SelfParts parts) {
         // scales of all codes.
         const auto put = [&](int t, int buf) {
             if constexpr (CODES) {
-                char *K = smem + buf * 2 * BUF, *V = K + BUF;
-                float *side = (float *)(smem + C::TILES + buf * C::SIDE);
+                char *K = area + buf * 2 * BUF, *V = K + BUF;
+                float *side = (float *)(area + C::TILES + buf * C::SIDE);
                 const auto spread = [&](const codes_t &q, char *row, int col, int swap) {
 #pragma unroll
                     for (int e0 = 0; e0 < UN; e0 += E) {
@@ -651,10 +671,10 @@ self_tiles(SelfArgs a, SelfParts parts) {
         };
 
         // ---- the tiles
-        if (t0 < t1) {
-            slot = slot_at(t0);
-            load(t0, 0);
-            next_slot = slot_at(t0 + 1);
+        if (t0 + own < t1) {
+            slot = slot_at(t0 + own);
+            load(t0 + own, 0);
+            next_slot = slot_at(t0 + own + SPLIT);
         }
         // This row's q: of each H E columns the lane's E. Of codes as they are, whose
         // chunks are 2 E columns, of each 2 H E the lane's chunk, if they are so many.
@@ -787,7 +807,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 for (int t = 0; t < DT; ++t) {
                     const int k = BYTES ? 4 * H * (n >> 3) + 4 * h + ((n >> 1) & 3) : 4 * h + (n >> 2);
                     const int x = BYTES ? M / 16 * t + half : M / 8 * t + 2 * half + ((n >> 1) & 1);
-                    place[t] = (uint32_t)(uintptr_t)(lds_ptr)(V + k * PITCH + (x ^ C::swap_v(k)) * 16 + (n & 1) * 8);
+                    place[t] = (uint32_t)(uintptr_t)(lds_ptr)smem + (uint32_t)(V - smem) + k * PITCH + (x ^ C::swap_v(k)) * 16 + (n & 1) * 8;
                 }
                 const auto product = [&](auto jj) {
                     constexpr int j = decltype(jj)::value;
@@ -984,9 +1004,9 @@ self_tiles(SelfArgs a, SelfParts parts) {
         };
         const auto is_partial = [&](int t) { return t * KB + KB - 1 > all_hi || t * KB < all_lo; };   // uniform
 
-        for (int t = t0, buf = 0; t < t1; ++t, buf ^= C::BUFS - 1) {
-            char *K = smem + buf * 2 * BUF, *V = K + BUF;
-            const float *side = (const float *)(smem + C::TILES + buf * C::SIDE);
+        for (int t = t0 + own, buf = 0; t < t1; t += SPLIT, buf ^= C::BUFS - 1) {
+            char *K = area + buf * 2 * BUF, *V = K + BUF;
+            const float *side = (const float *)(area + C::TILES + buf * C::SIDE);
             if constexpr (!STAGED) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's loads are in LDS
             if constexpr (CODES) put(t, buf);
             const uint64_t live = __ballot(alive);
@@ -1013,13 +1033,22 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     }
                 }
             }
-            __syncthreads();   // the tile is there, and the other one read
-            if (t + 1 < t1) {
-                slot = next_slot;
-                load(t + 1, buf ^ 1);
-                next_slot = slot_at(t + 2);
+            sync();   // the tile is there, and the other one read
+            const auto next = [&] {
+                if (t + SPLIT < t1) {
+                    slot = next_slot;
+                    load(t + SPLIT, buf ^ (C::BUFS - 1));
+                    next_slot = slot_at(t + 2 * SPLIT);
+                }
+            };
+            // (Into the buffer that is being read, once it has been.)
+            constexpr bool LATE = C::BUFS == 1 && !STAGED;
+            if constexpr (!LATE) next();
+            if (work && live != 0 && t * KB <= ahead && t * KB + KB > behind) tile(K, side, live, t);   // (uniform)
+            if constexpr (LATE) {
+                __builtin_amdgcn_sched_barrier(0);
+                next();
             }
-            if (work && live != 0) tile(K, side, live, t);
         }
         bool again = __ballot(apart) != 0;
         if constexpr (WAVES > 1) {
@@ -1033,16 +1062,16 @@ self_tiles(SelfArgs a, SelfParts parts) {
         }
         if (again) {   // uniform over the workgroup
             unit = LEAST_UNIT;
-            for (int t = t0; t < t1; ++t) {
+            for (int t = t0 + own; t < t1; t += SPLIT) {
                 if (!CODES && !is_partial(t)) continue;
-                __syncthreads();
+                sync();
                 slot = slot_at(t);
                 load(t, 0);
                 __builtin_amdgcn_s_waitcnt(0x0f70);
                 if constexpr (CODES) put(t, 0);
                 const uint64_t live = __ballot(alive);
-                __syncthreads();
-                if (work && is_partial(t)) add_apart(smem, (const float *)(smem + C::TILES), live, t);
+                sync();
+                if (work && is_partial(t)) add_apart(area, (const float *)(area + C::TILES), live, t);
             }
         }
 
@@ -1054,44 +1083,74 @@ self_tiles(SelfArgs a, SelfParts parts) {
 #pragma unroll
                 for (int t = 0; t < DT; ++t) o[t] *= f;
             }
-            if (M * wave + r < b.rows) {
-                if (!PAGED || (!begun && ends)) {
-                    const float inv = any ? 1.0f / l : 0.0f;   // (all scores minus infinity: 0 times infinity)
-                    T *out = (T *)a.out + token * a.os[0] + head * a.os[1];
-                    typedef T loose4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-#pragma unroll
-                    for (int t = 0; t < DT; ++t)
-#pragma unroll
-                        for (int g = 0; g < NR / 4; ++g) {
-                            const int col = M * t + 4 * H * g + 4 * h;
-                            const loose4 y{from_f32<T>(o[t][4 * g] * inv), from_f32<T>(o[t][4 * g + 1] * inv),
-                                           from_f32<T>(o[t][4 * g + 2] * inv), from_f32<T>(o[t][4 * g + 3] * inv)};
-                            if (col + 4 <= d) {
-                                *(loose4 *)(out + col) = y;
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 3; ++e)
-                                    if (col + e < d) out[col + e] = y[e];
-                            }
-                        }
-                } else {
-                    // Four columns of every row, then the next four; then the maxima and sums.
-                    f32x4 *p = (f32x4 *)parts.part(2 * unit_id + (begun ? 0 : 1));
-                    const int at = M * wave + r, groups = (d + 3) / 4;
-#pragma unroll
-                    for (int t = 0; t < DT; ++t)
-#pragma unroll
-                        for (int g = 0; g < NR / 4; ++g) {
-                            const int x = M / 4 * t + H * g + h;
-                            if (x < groups)
-                                p[x * b.rows + at] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
-                        }
-                    if (h == 0) {
-                        float2 *ml = (float2 *)(p + groups * b.rows);
-                        ml[at] = float2{m, any && m == -INFINITY && l == 0.0f ? 1.0f : l};
-                    }
+            // Four of a row's sums, from column col on: divided into the output, or
+            // into a part.
+            const int at = M * wave + r, groups = (d + 3) / 4;
+            const bool there = at < b.rows, direct = !PAGED || (!begun && ends);
+            f32x4 *const part = (f32x4 *)parts.part(2 * unit_id + (begun ? 0 : 1));
+            T *const out = (T *)a.out + token * a.os[0] + head * a.os[1];
+            const auto leave = [&](int col, const f32x4 &v, float inv) {
+                if (!there) return;
+                if (!direct) {
+                    // (Four columns of every row, then the next four.)
+                    if (col / 4 < groups) part[col / 4 * b.rows + at] = v;
+                    return;
                 }
+                typedef T loose4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+                const loose4 y{from_f32<T>(v[0] * inv), from_f32<T>(v[1] * inv), from_f32<T>(v[2] * inv), from_f32<T>(v[3] * inv)};
+                if (col + 4 <= d) {
+                    *(loose4 *)(out + col) = y;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (col + e < d) out[col + e] = y[e];
+                }
+            };
+            if constexpr (SPLIT > 1) {
+                // The waves' results, each from its own maximum, together.
+                f32x4 *const mine = (f32x4 *)area;
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int g = 0; g < NR / 4; ++g)
+                        mine[(t * (NR / 4) + g) * 64 + lane] = f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]};
+                constexpr int LAST = M * DP * 4 / 16;
+                mine[LAST + lane] = f32x4{m, l, any ? 1.0f : 0.0f, 0.0f};
+                __syncthreads();
+                const auto of = [&](int w) { return (const f32x4 *)(smem + w * C::AREA); };
+                f32x4 each[SPLIT];
+                m = -INFINITY, l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < SPLIT; ++w) each[w] = of(w)[LAST + lane], m = fmaxf(m, each[w][0]);
+#pragma unroll
+                for (int w = 0; w < SPLIT; ++w) {
+                    // (Equal: both infinite, of one sign.)
+                    each[w][0] = __builtin_amdgcn_exp2f(each[w][0] == m ? 0.0f : each[w][0] - m);
+                    l = fmaf(each[w][0], each[w][1], l);
+                    any |= each[w][2] != 0.0f;
+                }
+                const float inv = any ? 1.0f / l : 0.0f;
+                for (int x = own; x < DT * (NR / 4); x += SPLIT) {
+                    f32x4 v{};
+#pragma unroll
+                    for (int w = 0; w < SPLIT; ++w) {
+                        const f32x4 u = of(w)[x * 64 + lane];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = fmaf(each[w][0], u[e], v[e]);
+                    }
+                    leave(M * (x / (NR / 4)) + 4 * H * (x % (NR / 4)) + 4 * h, v, inv);
+                }
+            } else {
+                const float inv = any ? 1.0f / l : 0.0f;   // (all scores minus infinity: 0 times infinity)
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int g = 0; g < NR / 4; ++g)
+                        leave(M * t + 4 * H * g + 4 * h, f32x4{o[t][4 * g], o[t][4 * g + 1], o[t][4 * g + 2], o[t][4 * g + 3]}, inv);
             }
+            // ...and behind a part's sums the maxima and sums of weights.
+            if (there && !direct && h == 0 && own == 0)
+                ((float2 *)(part + groups * b.rows))[at] = float2{m, any && m == -INFINITY && l == 0.0f ? 1.0f : l};
         }
         if constexpr (!PAGED) {
             more = false;
@@ -1113,9 +1172,9 @@ self_tiles(SelfArgs a, SelfParts parts) {
     }
 }
 
-// The parts of blocks that were cut: a wave a row, a quarter or less of its
-// lanes a part.
-template <typename T, int DP> __global__ void __launch_bounds__(256) self_join(SelfArgs a, SelfParts parts) {
+// The parts of blocks that were cut: a lane four columns of a row, of every
+// part, or, where there are many, a few lanes, each of some of them.
+template <typename T> __global__ void __launch_bounds__(256) self_join(SelfArgs a, SelfParts parts) {
     const int lane = threadIdx.x & 63, d = a.c.width, kv = a.c.kv;
     int x, head;
     parts.whose(blockIdx.x, kv, x, head);
@@ -1135,47 +1194,49 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) self_join(S
         inside += 64;
     }
     const int n = inside + 2, first = x - inside - 1;
-    const auto part = [&](int p) { return parts.part(2 * ((first + p) * kv + head) + (p == 0)); };
-    constexpr int COLS = DP / 4, AT_ONCE = 64 / COLS;    // lanes of a part (groups of four columns; 96: 24)
-    const int sub = lane / COLS, col = lane % COLS, groups = (d + 3) / 4, rows = mark.rows;
-    for (int i = blockIdx.y * 4 + (threadIdx.x >> 6); i < rows; i += gridDim.y * 4) {
-        // A lane a part: its maximum and sum.
-        const auto ml = [&](int p) { return ((const float2 *)((const f32x4 *)part(p) + groups * rows))[i]; };
-        float m = -INFINITY;
-        for (int p = lane; p < n; p += 64) m = fmaxf(m, ml(p).x);
-#pragma unroll
-        for (int w = 32; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor(m, w, 64));
-        float l = 0.0f;
+    const auto part = [&](int p) { return (const f32x4 *)parts.part(2 * ((first + p) * kv + head) + (p == 0)); };
+    const int groups = (d + 3) / 4, rows = mark.rows;
+    constexpr int AT = 8;     // parts on their way at a time
+    int lanes = 1;            // of four columns: an eighth of the parts, up to 16
+    while (lanes < 16 && lanes * AT < n) lanes *= 2;
+    const int items = 64 / lanes, sub = lane / items;
+    const int waves = (rows * groups + items - 1) / items;
+    for (int w = blockIdx.y * 4 + (threadIdx.x >> 6); w < waves; w += gridDim.y * 4) {
+        const int item = w * items + lane % items, i = min(item / groups, rows - 1), col = item % groups;
+        float m = -INFINITY, l = 0.0f;
         f32x4 o{};
-        for (int p0 = 0; p0 < n; p0 += 64) {
-            const int k = min(64, n - p0);
-            float w = 0.0f;
-            if (lane < k) {
-                const float2 q = ml(p0 + lane);
-                w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(q.x - m);
-                l = fmaf(w, q.y, l);
-            }
-#pragma unroll 4
-            for (int p1 = 0; p1 < k; p1 += AT_ONCE) {   // (every lane, for the shuffle)
-                const int p = p1 + sub;
-                const float wp = __shfl(w, min(p, 63), 64);
-                if (p < k && sub < AT_ONCE && col < groups) {
-                    const f32x4 v = ((const f32x4 *)part(p0 + p))[col * rows + i];
+        for (int p0 = sub; p0 < n; p0 += AT * lanes) {
+            float2 q[AT];
+            f32x4 v[AT];
+            float top = m;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = fmaf(wp, v[e], o[e]);
-                }
+            for (int k = 0; k < AT; ++k) {
+                q[k] = float2{-INFINITY, 0.0f}, v[k] = f32x4{};
+                const int p = p0 + k * lanes;
+                if (p < n) q[k] = ((const float2 *)(part(p) + groups * rows))[i], v[k] = part(p)[col * rows + i];
+            }
+#pragma unroll
+            for (int k = 0; k < AT; ++k) top = fmaxf(top, q[k].x);
+            // (Equal: both infinite, of one sign.)
+            const float f = __builtin_amdgcn_exp2f(m == top ? 0.0f : m - top);
+            l *= f, o *= f, m = top;
+#pragma unroll
+            for (int k = 0; k < AT; ++k) {
+                const float wk = __builtin_amdgcn_exp2f(q[k].x == m ? 0.0f : q[k].x - m);
+                l = fmaf(wk, q[k].y, l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(wk, v[k][e], o[e]);
             }
         }
-        l = wave_sum(l);
-        // The lanes of the same columns. (96: 24 lanes, 2 of them.)
+        for (int s = items; s < 64; s *= 2) {   // the lanes of the same columns
+            const float m2 = __shfl_xor(m, s, 64), l2 = __shfl_xor(l, s, 64), top = fmaxf(m, m2);
+            const float f = __builtin_amdgcn_exp2f(m == top ? 0.0f : m - top), f2 = __builtin_amdgcn_exp2f(m2 == top ? 0.0f : m2 - top);
+            l = fmaf(f, l, f2 * l2);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float total = o[e];
-#pragma unroll
-            for (int s = 1; s < AT_ONCE; ++s) total += __shfl(o[e], col + s * COLS, 64);
-            o[e] = total;
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(f, o[e], f2 * __shfl_xor(o[e], s, 64));
+            m = top;
         }
-        if (lane >= COLS) continue;
+        if (sub != 0 || item >= rows * groups) continue;
         // No maximum: no state (0), or scores of minus infinity alone.
         const float inv = m == -INFINITY ? (l == 0.0f ? 0.0f : __builtin_nanf("")) : 1.0f / l;
         const int row = mark.row0 + i;
@@ -1189,9 +1250,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) self_join(S
 
 // ---- launches --------------------------------------------------------------------------
 
-template <typename T, Held HELD, bool PAGED, int DP, int WAVES, int M = 32>
+template <typename T, Held HELD, bool PAGED, int DP, int WAVES, int M = 32, int SPLIT = 1>
 static hipError_t launch_tiles(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
-    using C = SelfTile<T, HELD, DP, WAVES, M>;
+    using C = SelfTile<T, HELD, DP, WAVES, M, SPLIT>;
     SelfParts parts{};
     if (PAGED) {
         parts.marks = (SelfMark *)a.ws;
@@ -1200,10 +1261,11 @@ static hipError_t launch_tiles(hipStream_t s, const SelfArgs &a, const SelfLaunc
         parts.pieces = f.pieces;
         parts.least = (uint64_t)a.share * 4 * C::KB;
     }
-    const hipError_t e = enqueue(self_tiles<T, HELD, PAGED, DP, WAVES, M>, dim3(f.groups), dim3(64 * WAVES), C::LDS, s, a, parts);
+    const hipError_t e = enqueue(self_tiles<T, HELD, PAGED, DP, WAVES, M, SPLIT>, dim3(f.groups), dim3(64 * WAVES * SPLIT),
+                                 C::LDS, s, a, parts);
     // (Blocks of one tile are not cut.)
     if (e != hipSuccess || !PAGED || room(a.c) <= C::KB) return e;
-    return enqueue(self_join<T, DP>, dim3(f.groups, (f.part_rows + 15) / 16), dim3(256), 0, s, a, parts);
+    return enqueue(self_join<T>, dim3(f.groups, f.part_rows <= 16 ? 2 : (f.part_rows * DP / 4 + 511) / 512), dim3(256), 0, s, a, parts);
 }
 
 template <typename T, bool PAGED, int DP> static hipError_t launch_held(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
@@ -1221,8 +1283,14 @@ template <typename T, bool PAGED, int DP> static hipError_t launch_held(hipStrea
             return f.rows == 32 ? launch_tiles<T, Held::Codes, true, DP, 1>(s, a, f)
                                 : launch_tiles<T, Held::Codes, true, DP, 4>(s, a, f);
     if (f.held == Held::Loose) return launch_tiles<T, Held::Loose, PAGED, DP, 1>(s, a, f);
-    return f.rows == 32 ? launch_tiles<T, Held::Chunks, PAGED, DP, 1>(s, a, f)
-                        : launch_tiles<T, Held::Chunks, PAGED, DP, 4>(s, a, f);
+    // (A wave alone has F32 prompts and a cache's tokens, four share the rows of
+    // prompts alone, or, but for F32 prompts, a tile.)
+    if constexpr (!PAGED)
+        if (f.split) return launch_tiles<T, Held::Chunks, false, DP, 1, 32, 4>(s, a, f);
+    if constexpr (PAGED || F32)
+        if (f.rows == 32) return launch_tiles<T, Held::Chunks, PAGED, DP, 1>(s, a, f);
+    if constexpr (PAGED || !F32) return launch_tiles<T, Held::Chunks, PAGED, DP, 4>(s, a, f);
+    return hipErrorInvalidValue;
 }
 
 template <typename T> static hipError_t launch_self(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
