@@ -1,8 +1,10 @@
 // Rows into the pages of a cache, as they are or as int8 codes, and back.
 //
 // A few lanes hold a head's row, eight values each, so a wave moves several
-// rows of K and of V at once. A wave looks for its first row's sequence 64
-// sequences a step, the lanes go on from there.
+// rows of K and of V at once, and of long calls four times as many: what does
+// not depend on where a row goes is on its way before that is known. A wave
+// looks for its first row's sequence 64 sequences a step, the lanes go on from
+// there.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -24,31 +26,57 @@ template <typename T> struct Eight {
     typedef T loose __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
-// Eight elements from one place to another, n of them there.
-template <typename T> __device__ __forceinline__ void copy8(T *to, const T *from, int n) {
-    typedef typename Eight<T>::loose loose;
-    if (n >= 8) {
-        *(loose *)to = *(const loose *)from;
-    } else {
+// Eight elements, n of them there.
+template <typename T> struct Group {
+    typename Eight<T>::loose v;
+    __device__ __forceinline__ void read(const T *from, int n) {
+        if (n >= 8) {
+            v = *(const typename Eight<T>::loose *)from;
+        } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < n) to[k] = from[k];
+            for (int k = 0; k < 8; ++k) v[k] = k < n ? from[k] : (T)0;
+        }
     }
+    __device__ __forceinline__ void write(T *to, int n) const {
+        if (n >= 8) {
+            *(typename Eight<T>::loose *)to = v;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < n) to[k] = v[k];
+        }
+    }
+};
+
+// The largest of LANES lanes' numbers that share a row, as each of them has it.
+template <int LANES> __device__ __forceinline__ uint32_t row_max(uint32_t v) {
+    const auto with = [&](int other) { v = max(v, (uint32_t)other); };
+    if constexpr (LANES == 16) {
+        with(__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));   // 8 lanes on, of 16
+        with(__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));   // 4
+        with(__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));
+        with(__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
+    } else {
+        if constexpr (LANES == 8) with(__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));   // 7 - lane, of 8
+        with(__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true));    // lane ^ 1
+        with(__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true));    // lane ^ 2
+    }
+    return v;
 }
 
-// The codes of eight of a head's values into its slot, and its scale.
+// The codes of eight of a head's values, and its scale.
 template <typename T, int LANES>
-__device__ __forceinline__ void write_codes(const T *from, int n, bool there, int8_t *to, float *scale) {
-    float v[8], top = 0.0f, bad = 0.0f;   // bad is not 0: an infinity or a NaN among the values
+__device__ __forceinline__ void write_codes(const Group<T> &x, int n, bool there, int8_t *to, float *scale) {
+    // (The bits of numbers of 0 or more are in their order, an infinity's and a
+    // NaN's behind them all.)
+    float v[8];
+    uint32_t most = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-    if (there && n > 0) read8(from, n, v);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k])), bad = fmaf(v[k], 0.0f, bad);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64)), bad += __shfl_xor(bad, o, 64);
+    for (int k = 0; k < 8; ++k) v[k] = to_f32(x.v[k]), most = max(most, __float_as_uint(v[k]) & 0x7fffffffu);
+    most = row_max<LANES>(most);
+    const float top = __uint_as_float(most);
     if (!there) return;
-    const bool fine = bad == 0.0f;
+    const bool fine = most < 0x7f800000u;
     if (n > 0) {
         uint32_t q[2];
         codes_of8(v, top, fine, q);
@@ -61,86 +89,113 @@ __device__ __forceinline__ void write_codes(const T *from, int n, bool there, in
                 if (k < n) to[k] = (int8_t)(q[k >> 2] >> (8 * (k & 3)));
         }
     }
-    if (threadIdx.x % LANES == 0) *scale = fine ? (float)((double)top / 127.0) : __builtin_nanf("");
+    if (threadIdx.x % LANES == 0) {
+        // top / 127 rounded to F32: a quotient corrected by its exact remainder.
+        constexpr float INV = 1.0f / 127.0f;
+        const float near = top * INV, s = top < 1e-30f ? __fdiv_rn(top, 127.0f) : fmaf(fmaf(-127.0f, near, top), INV, near);
+        *scale = fine ? s : __builtin_nanf("");
+    }
 }
 
 // Eight codes times their scale, rounded once to T.
-template <typename T> __device__ __forceinline__ void read_codes(const int8_t *from, float scale, int n, T *to) {
-    uint32_t q[2] = {0, 0};
-    if (n >= 8) {
-        typedef uint32_t loose2 __attribute__((ext_vector_type(2), aligned(1)));
-        const loose2 x = *(const loose2 *)from;
-        q[0] = x[0], q[1] = x[1];
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (k < n) q[k >> 2] |= (uint32_t)(uint8_t)from[k] << (8 * (k & 3));
-    }
+template <typename T> __device__ __forceinline__ void write_values(const Group<int8_t> &q, float scale, int n, T *to) {
     float v[8];
-    bool tie = false;
+    // (A product that F32 has rounded onto the border of two 16-bit numbers would
+    // be rounded a second time, from there; among F16's smallest the borders are
+    // elsewhere.)
+    bool tie = std::is_same<T, _Float16>::value && fabsf(scale) < 6.103515625e-5f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        v[k] = (float)(int8_t)(q[k >> 2] >> (8 * (k & 3))) * scale;
-        // (A product that F32 has rounded onto the border of two 16-bit numbers
-        // would be rounded a second time, from there.)
+        v[k] = (float)q.v[k] * scale;
         const uint32_t u = __float_as_uint(v[k]);
         if (std::is_same<T, __bf16>::value) tie |= (u & 0xffffu) == 0x8000u;
-        if (std::is_same<T, _Float16>::value) tie |= (u & 0x1fffu) == 0x1000u || (u & 0x7fffffffu) < 0x38800000u;
+        if (std::is_same<T, _Float16>::value) tie |= (u & 0x1fffu) == 0x1000u;
     }
     if (!std::is_same<T, float>::value && tie)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = odd_f32((double)(int8_t)(q[k >> 2] >> (8 * (k & 3))) * scale);
+        for (int k = 0; k < 8; ++k) v[k] = odd_f32((double)q.v[k] * scale);
     write8(to, n, v);
 }
 
-// LANES lanes a head's row. WRITE: the call's rows into the cache, else back.
-template <typename T, bool I8, bool WRITE, int LANES> __global__ void __launch_bounds__(256) cache_rows(RowsArgs a) {
+// LANES lanes a head's row, U rows each. WRITE: the call's rows into the cache,
+// else back.
+template <typename T, bool I8, bool WRITE, int LANES, int U> __global__ void __launch_bounds__(256) cache_rows(RowsArgs a) {
     typedef typename std::conditional<I8, int8_t, T>::type H;   // as the cache holds them
+    typedef typename std::conditional<WRITE, T, H>::type From;
     constexpr int PER = 64 / LANES;
     const CacheArgs &c = a.c;
     const int lane = threadIdx.x & 63, col = 8 * (lane % LANES), n = c.width - col;
     const uint32_t rows = (uint32_t)c.tokens * (uint32_t)c.kv;   // (below 2^31)
-    const uint32_t stride = gridDim.x * 4 * PER;
-    for (uint32_t r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * PER; r0 < rows; r0 += stride) {
+    const uint32_t stride = gridDim.x * 4 * PER * U;
+    for (uint32_t r0 = (blockIdx.x * 4 + (threadIdx.x >> 6)) * PER * U; r0 < rows; r0 += stride) {
+        int t[U], slot[U];
+        uint32_t head[U];
+        bool own[U];
+        Group<From> k[U], v[U];
+        float sk[U], sv[U];
+        const auto row = [&](void *p, const uint64_t (&s)[2], int u) { return (T *)p + t[u] * s[0] + head[u] * s[1] + col; };
+        const auto state = [&](void *p, const uint64_t (&s)[2], int u) {
+            return (H *)p + (uint64_t)max(0, slot[u]) * s[0] + head[u] * s[1] + col;
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // (Rows past the last: the last one, for which nothing is done.)
+            const uint32_t r = min(r0 + u * PER + lane / LANES, rows - 1);
+            own[u] = r == r0 + u * PER + lane / LANES;
+            t[u] = (int)(r / (uint32_t)c.kv), head[u] = r - (uint32_t)t[u] * (uint32_t)c.kv;
+            if constexpr (WRITE) k[u].read(row(a.k, a.ks, u), n), v[u].read(row(a.v, a.vs, u), n);
+        }
         int seq = seq_before(c, (int)(r0 / (uint32_t)c.kv));
-        const uint32_t r = r0 + lane / LANES;
-        const int t = (int)(r / (uint32_t)c.kv);
-        const uint64_t head = r - (uint32_t)t * (uint32_t)c.kv;
-        // (Rows past the last belong to no sequence: a call's tokens end before them.)
-        const int p = r < rows ? position_of(c, t, seq) : -1;
-        const bool own = r < rows && seq >= 0 && seq < c.seqs && t >= within(c.starts[seq], 0, c.tokens);
-        const int slot = p >= 0 ? slot_of(c, seq, p) : -1;
-        T *k = (T *)a.k + t * a.ks[0] + head * a.ks[1] + col, *v = (T *)a.v + t * a.vs[0] + head * a.vs[1] + col;
-        const uint64_t at = slot < 0 ? 0 : slot;
-        H *hk = (H *)c.k + at * c.ks[0] + head * c.ks[1] + col, *hv = (H *)c.v + at * c.vs[0] + head * c.vs[1] + col;
-        float *sk = c.k_scales + at * c.kss + head, *sv = c.v_scales + at * c.vss + head;
-        if constexpr (WRITE && I8) {
-            write_codes<T, LANES>(k, n, slot >= 0, hk, sk);
-            write_codes<T, LANES>(v, n, slot >= 0, hv, sv);
-        } else if constexpr (WRITE) {
-            if (slot >= 0 && n > 0) copy8(hk, k, n), copy8(hv, v, n);
-        } else if (own && n > 0) {
-            if (slot < 0) {
-                const float zero[8] = {};
-                write8(k, n, zero), write8(v, n, zero);
-            } else if constexpr (I8) {
-                read_codes(hk, *sk, n, k), read_codes(hv, *sv, n, v);
-            } else {
-                copy8(k, hk, n), copy8(v, hv, n);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int p = position_of(c, t[u], seq);
+            own[u] = own[u] && seq >= 0 && seq < c.seqs && t[u] >= within(c.starts[seq], 0, c.tokens);
+            slot[u] = own[u] && p >= 0 ? slot_of(c, seq, p) : -1;
+        }
+        if constexpr (!WRITE)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (slot[u] >= 0) {
+                    k[u].read(state(c.k, c.ks, u), n), v[u].read(state(c.v, c.vs, u), n);
+                    if constexpr (I8)
+                        sk[u] = c.k_scales[(uint64_t)slot[u] * c.kss + head[u]], sv[u] = c.v_scales[(uint64_t)slot[u] * c.vss + head[u]];
+                }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if constexpr (WRITE && I8) {
+                const uint64_t at = (uint64_t)max(0, slot[u]);
+                write_codes<T, LANES>(k[u], n, slot[u] >= 0, state(c.k, c.ks, u), c.k_scales + at * c.kss + head[u]);
+                write_codes<T, LANES>(v[u], n, slot[u] >= 0, state(c.v, c.vs, u), c.v_scales + at * c.vss + head[u]);
+            } else if constexpr (WRITE) {
+                if (slot[u] >= 0) k[u].write(state(c.k, c.ks, u), n), v[u].write(state(c.v, c.vs, u), n);
+            } else if (own[u]) {
+                if (slot[u] < 0) {
+                    const float zero[8] = {};
+                    write8(row(a.k, a.ks, u), n, zero), write8(row(a.v, a.vs, u), n, zero);
+                } else if constexpr (I8) {
+                    write_values(k[u], sk[u], n, row(a.k, a.ks, u)), write_values(v[u], sv[u], n, row(a.v, a.vs, u));
+                } else {
+                    k[u].write(row(a.k, a.ks, u), n), v[u].write(row(a.v, a.vs, u), n);
+                }
             }
         }
     }
 }
 
 template <typename T, bool I8, bool WRITE> static hipError_t launch_rows(hipStream_t s, const RowsArgs &a) {
-    const auto go = [&](auto kernel, int lanes) {
-        const uint64_t rows = (uint64_t)a.c.tokens * a.c.kv, per = 4 * (64 / lanes);
+    // Four rows a lane where that leaves a workgroup for every compute unit.
+    const uint64_t rows = (uint64_t)a.c.tokens * a.c.kv;
+    const auto go = [&](auto kernel, int per) {
         const uint64_t blocks = std::min<uint64_t>((rows + per - 1) / per, 1 << 20);
         return enqueue(kernel, dim3((uint32_t)blocks), dim3(256), 0, s, a);
     };
-    if (a.c.width <= 32) return go(cache_rows<T, I8, WRITE, 4>, 4);
-    if (a.c.width <= 64) return go(cache_rows<T, I8, WRITE, 8>, 8);
-    return go(cache_rows<T, I8, WRITE, 16>, 16);
+#define ROWS(L)                                                                          \
+    if (rows >= 256 * 4 * (256 / L)) return go(cache_rows<T, I8, WRITE, L, 4>, 4 * (256 / L)); \
+    return go(cache_rows<T, I8, WRITE, L, 1>, 256 / L)
+    if (a.c.width <= 32) { ROWS(4); }
+    if (a.c.width <= 64) { ROWS(8); }
+    ROWS(16);
+#undef ROWS
 }
 
 template <bool WRITE> static hipError_t rows_of(hipStream_t s, const RowsArgs &a, Dt t, bool i8) {

@@ -55,32 +55,46 @@ __device__ __forceinline__ int nearest_code(double c, double top, double low) {
     return (int)(d > 0.0 ? low + 1.0 : d < 0.0 ? low : 2.0 * rint(0.5 * half));
 }
 
+// The same in F32, where nothing of it over- or underflows: (127 c - half top) is
+// decided by the rounded products' difference, which is exact as they lie within
+// a factor of 2, and their errors'.
+__device__ __forceinline__ float nearest_code_f32(float c, float top, float low) {
+#pragma clang fp contract(off)
+    const float half = low + 0.5f, a = 127.0f * c, b = half * top;
+    const float d = (a - b) + (fmaf(127.0f, c, -a) - fmaf(half, top, -b));
+    return d > 0.0f ? low + 1.0f : d < 0.0f ? low : 2.0f * rintf(0.5f * half);
+}
+
 // The codes of eight of a row's values, top the largest magnitude of the row
-// (finite and not 0, but where `fine` is not set: then they are 0): those of
-// nearest_code, by an F32 quotient where no border is nearer than its error.
+// (finite, but where `fine` is not set: then they are 0): those of nearest_code,
+// by an F32 quotient where no border is nearer than its error, 4 2^-24 of 127.
+// (Of 16-bit rows a third has a value that is half of its largest: 63.5.)
 __device__ __forceinline__ void codes_of8(const float (&v)[8], float top, bool fine, uint32_t (&q)[2]) {
-    const double k127 = fine && top > 0.0f ? 127.0 / top : 0.0;
-    const float factor = (float)k127;
-    // (Rows so large or small that F32 does not hold the steps.)
-    const bool far = k127 > 1e30 || (k127 > 0.0 && k127 < 1e-30);
-    float near = 0.0f;   // the largest distance from a whole number
-    int code[8];
-    float t[8];
+    const float factor = top > 0.0f ? 127.0f * __builtin_amdgcn_rcpf(top) : 0.0f;
+    // 1.5 2^23 and a small number: the whole number next to it, its lowest byte the code.
+    constexpr float SHIFT = 12582912.0f, NEAR = 0.5f - 3.5e-5f;
+    float near = 0.0f, t[8], off[8];   // the distances from a whole number
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        t[k] = v[k] * factor;
-        const float whole = rintf(t[k]);
-        near = fmaxf(near, fabsf(t[k] - whole));
-        code[k] = fine ? (int)whole : 0;
+        t[k] = fmaf(v[k], factor, SHIFT);
+        off[k] = fmaf(v[k], factor, SHIFT - t[k]);
+        near = fmaxf(near, fabsf(off[k]));
     }
-    if (fine && (near > 0.5f - 2.5e-5f || far)) {
+    // (Rows so large or small that F32 does not hold the steps.)
+    if (fine && top > 0.0f && (top > 1e30f || top < 1e-28f)) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = SHIFT + (float)nearest_code(v[k], top, floor(127.0 * v[k] / top));
+    } else if (fine && near > NEAR) {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-            code[k] = nearest_code(v[k], top, far ? floor(127.0 * v[k] / top) : (double)floorf(t[k]));
+            if (fabsf(off[k]) > NEAR) t[k] = SHIFT + nearest_code_f32(v[k], top, floorf(v[k] * factor));
     }
-    q[0] = q[1] = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) q[k >> 2] |= (uint32_t)(uint8_t)(int8_t)code[k] << (8 * (k & 3));
+    for (int w = 0; w < 2; ++w) {
+        const auto bits = [&](int k) { return __float_as_uint(t[4 * w + k]); };
+        const uint32_t lo = __builtin_amdgcn_perm(bits(1), bits(0), 0x0c0c0400u), hi = __builtin_amdgcn_perm(bits(3), bits(2), 0x0c0c0400u);
+        q[w] = fine ? lo | hi << 16 : 0;
+    }
 }
 
 }  // namespace rocm
