@@ -574,3 +574,58 @@ def test_a_stream_that_is_not_the_current_one(context):
     s.synchronize()
     check(cache, q, out)
     assert math.isfinite(out.float().sum().item())
+
+
+def _check_single(out, v):
+    # One state's probability is 1, off by 2^-21 against its sum and by half a step of its type; the output is rounded once.
+    half, tiny = torch.finfo(out.dtype).eps / 2, torch.finfo(out.dtype).tiny
+    want = v.double().repeat_interleave(out.shape[1] // v.shape[1], 1)
+    assert ((out.double() - want).abs() <= (2 * half + 2.0 ** -20) * want.abs().clamp_min(tiny)).all()
+
+
+@pytest.mark.parametrize("n, share", [(65, 3), (200, 1), (100, 40), (4097, 1), (9000, 2), (9000, 40)])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_prompts_of_many_sequences(context, n, share, t):
+    """Single tokens, a sequence without any, and some longer ones between them."""
+    rows, kv, d = [1] * n, 4 if n == 100 else 1, 32
+    if n == 100:
+        rows = [20] * n
+    rows[n // 2], rows[n // 3], rows[63], rows[-1] = 0, 150, 40, 33
+    m = sum(rows)
+    q, k, v = _rows(n, m, share * kv, d, t), _rows(n + 1, m, kv, d, t), _rows(n + 2, m, kv, d, t)
+    out = torch.full_like(q, 3.0)
+    context.prompt_attention(q, k, v, starts_of(rows), out, stream=stream())
+    at, single = 0, []
+    for r in rows:
+        if r == 1:
+            single.append(at)
+        else:
+            check_rows(out[at:at + r], q[at:at + r], 0, k[at:at + r].double(), v[at:at + r].double())
+        at += r
+    if single:
+        single = torch.tensor(single, device="cuda")
+        _check_single(out[single], v[single])
+
+
+@pytest.mark.parametrize("n", [64, 65, 129, 5000])
+@pytest.mark.parametrize("rows_each, share", [(1, 2), (1, 32), (3, 64)])
+@pytest.mark.parametrize("t, held", [("f32", "same"), ("bf16", "same"), ("f16", "i8")])
+def test_caches_of_many_sequences(context, n, rows_each, share, t, held):
+    rows, lengths = [rows_each] * n, [rows_each] * n
+    for i, m, s in ((n // 2, 0, 9), (n // 3, 1, 700), (63, 30, 90), (n - 1, 2, 2000)):
+        rows[i], lengths[i] = m, s
+    cache = Cache(n, rows, lengths, 1, 32, t, held, 16)
+    q = _rows(n, sum(rows), share, 32, t)
+    out = _attend(context, cache, q)
+    at, single, slots = 0, [], []
+    for i, (m, s) in enumerate(zip(rows, lengths)):
+        if s == 1:
+            single.append(at)
+            slots.append(cache.at(i, 0, 1))
+        elif s > rows_each or i % 50 == 0:
+            where = cache.at(i, 0, s)
+            check_rows(out[at:at + m], q[at:at + m], s - m, cache.values(0, where), cache.values(1, where),
+                       coded=cache.scales[1][where] if held == "i8" else None)
+        at += m
+    if single:
+        _check_single(out[torch.tensor(single, device="cuda")], cache.values(1, torch.cat(slots)))

@@ -86,12 +86,13 @@ enum class Held : int { Chunks, Loose, Codes, Bytes };
 
 // How a call is launched, from what the host knows of it: its rows and
 // sequences, not their lengths.
+constexpr int MOST_ALONE = 3072, MOST_TILED = 768;   // workgroups of a call over a cache, of a wave and of four
 struct SelfLaunch {
     Held held;
     int rows;            // of a block: 16 or 32 (a wave's), or 128 (four waves')
     bool split;          // 32 rows are four waves', each with every fourth tile of the keys
-    uint32_t groups;     // workgroups: of a prompt, the most blocks that there can be
-    int pieces;          // of a call over a cache, each a workgroup of every key head
+    uint32_t groups;     // of a prompt: workgroups, the most blocks that there can be
+    int pieces;          // of a call over a cache, at most, each a workgroup of every key head
     int part_rows;       // the most rows of a part
 };
 SelfLaunch self_plan(const SelfArgs &a);

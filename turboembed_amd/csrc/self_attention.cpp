@@ -10,11 +10,9 @@ namespace rocm {
 
 namespace {
 
-// Pieces of a call over a cache, by its blocks' rows: workgroups enough for a
-// card, and no more.
+// The most pieces of a call over a cache, by its blocks' rows.
 uint64_t most_pieces(int rows, int kv) {
-    uint64_t groups = rows == 128 ? 512 : 3072;
-    return std::max<uint64_t>(1, groups / kv);
+    return std::max<uint64_t>(1, (rows == 128 ? MOST_TILED : MOST_ALONE) / kv);
 }
 
 uint64_t parts_bytes(int rows, uint64_t all_rows, int kv, int width) {
@@ -65,7 +63,6 @@ SelfLaunch self_plan(const SelfArgs &a) {
     // (No more than there can be tiles.)
     const uint64_t tiles = blocks / a.c.kv * std::max<uint64_t>(1, ((uint64_t)room(a.c) + 31) / 32);
     f.pieces = (int)std::min<uint64_t>(most_pieces(f.rows, a.c.kv), std::max<uint64_t>(1, tiles));
-    f.groups = (uint32_t)(f.pieces + 7) / 8 * 8 * a.c.kv;
     f.part_rows = (int)std::min<uint64_t>(f.rows, rows);
     return f;
 }

@@ -53,6 +53,17 @@ template <typename T, Held HELD, int DP, int WAVES, int M, int SPLIT> struct Sel
     static constexpr int RESULTS = M * DP * 4 + 1024, AREA = FLAGS > RESULTS ? FLAGS : RESULTS;
     static constexpr int LDS = SPLIT > 1 ? SPLIT * AREA : FLAGS + (WAVES > 1 ? 4 * WAVES : 0);
     static constexpr int OCC = F32 ? (DP <= (HELD == Held::Chunks ? 96 : 64) || WAVES == 4 ? 2 : 1) : DP <= 64 ? 3 : 2;
+    // Workgroups of a call over a cache: as many as the card's 256 compute units
+    // hold at once, of 160 KiB of LDS each, given in steps of 1280 bytes: their
+    // work is equal, and a second turn would be a short one. us at 0.75, 1, 1.34
+    // and 2 times as many:
+    //   256 tokens over 256 BF16 states each, 4 heads of 64                     33  33  40  41
+    //   64 tokens over 200-8192 BF16 states, 32 heads over 8 of 128             263 241 279 245
+    //   96 F16 tokens over 100-6000 int8 states, 12 heads of 64                 154 149 166 150
+    //   8 x 512 tokens over 1024-8192 int8 states, 32 heads over 8 of 128       589 481 586 484
+    static constexpr int BY_LDS = 163840 / ((LDS + 1279) / 1280 * 1280), BY_WAVES = OCC * 4 / WAVES;
+    static constexpr int GROUPS = 256 * (BY_LDS < BY_WAVES ? BY_LDS : BY_WAVES);
+    static_assert(GROUPS <= (WAVES > 1 ? MOST_TILED : MOST_ALONE), "a workspace holds their parts");
     // LDS serves 256 bytes a cycle, and rows' chunks are swapped so that what it
     // serves at once lies in different banks: 16 keys of one chunk of K; of V what
     // 32 lanes read, 8 bytes each, to transpose.
@@ -172,19 +183,19 @@ template <int ROWS, int KB> struct Cuts {
     bool any;
     __device__ __forceinline__ Cuts(const SelfArgs &a, int g, int pieces, uint64_t least) {
         const int lane = threadIdx.x & 63, n = a.c.seqs;
-        uint64_t total = 0, cost = 0;
-        Blocks mine{};
-        Seq seq{};
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            cost = 0;
-            if (i0 + lane < n) {
-                seq = seq_of(a.c, i0 + lane);
-                mine = cost_of(a, seq, ROWS);
-                cost = cost_to(mine, mine.n);
-            }
-            cost = prefix_sum(cost);
-            total += lane_of(cost, 63);
-        }
+        const auto cost = [&](int i) {
+            const Blocks b = cost_of(a, seq_of(a.c, i), ROWS);
+            return cost_to(b, b.n);
+        };
+        // Lane l adds up sequences l * per and on: one sum over the wave, however
+        // many sequences there are.
+        const int per = (n + 63) / 64;
+        uint64_t upto = 0;
+#pragma unroll 4
+        for (int j = 0; j < per; ++j)
+            if (lane * per + j < n) upto += cost(lane * per + j);
+        upto = prefix_sum(upto);
+        const uint64_t total = lane_of(upto, 63);
         // (No more pieces than their least work makes worth while.)
         const uint64_t worth = quotient(total + least - 1, least);
         if (worth < (uint64_t)pieces) pieces = max(1, (int)worth);
@@ -196,26 +207,27 @@ template <int ROWS, int KB> struct Cuts {
         const uint64_t f = cut((uint64_t)g + (lane & 1));
         const uint64_t f0 = lane_of(f, 0), f1 = lane_of(f, 1);
         // The sequences of both, and their costs' start.
-        int at = n;
-        uint64_t before = total, seen = 0;
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            if (n > 64) {
-                cost = 0;
-                if (i0 + lane < n) {
-                    const Seq s = seq_of(a.c, i0 + lane);
-                    const Blocks m = cost_of(a, s, ROWS);
-                    cost = cost_to(m, m.n);
-                }
-                cost = prefix_sum(cost);
+        int at0 = n, at1 = n;
+        uint64_t before0 = total, before1 = total;
+        const auto find = [&](uint64_t f, int &at, uint64_t &before) {
+            const uint64_t past = __ballot(upto > f);
+            if (past == 0) return;
+            const int l = __ffsll((unsigned long long)past) - 1;
+            at = l * per;
+            before = l ? lane_of(upto, l - 1) : 0;
+            for (int j = 0; per > 1 && j < per; j += 64) {
+                const uint64_t sum = prefix_sum(j + lane < per && at + lane < n ? cost(at + lane) : 0);
+                const uint64_t here = __ballot(before + sum > f);
+                const int k = here ? __ffsll((unsigned long long)here) - 1 : 64;
+                at += k;
+                before += k ? lane_of(sum, k - 1) : 0;
+                if (here) return;
             }
-            const uint64_t past0 = __ballot(seen + cost > f0), past1 = __ballot(seen + cost > f1);
-            const uint64_t past = lane & 1 ? past1 : past0;
-            const int first = past ? __ffsll((unsigned long long)past) - 1 : 64;
-            uint32_t lo = (uint32_t)__shfl((int)(uint32_t)cost, (first + 63) & 63, 64);
-            uint32_t hi = (uint32_t)__shfl((int)(cost >> 32), (first + 63) & 63, 64);
-            if (at == n && past) at = i0 + first, before = seen + (first ? (uint64_t)hi << 32 | lo : 0);
-            seen += lane_of(cost, 63);
-        }
+        };
+        find(f0, at0, before0);
+        find(f1, at1, before1);
+        const int at = lane & 1 ? at1 : at0;
+        const uint64_t before = lane & 1 ? before1 : before0;
         Place p{at, 0, 0};
         if (at < n) {
             const Seq s = seq_of(a.c, at);
@@ -1254,18 +1266,20 @@ template <typename T, Held HELD, bool PAGED, int DP, int WAVES, int M = 32, int 
 static hipError_t launch_tiles(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
     using C = SelfTile<T, HELD, DP, WAVES, M, SPLIT>;
     SelfParts parts{};
+    uint32_t groups = f.groups;
     if (PAGED) {
+        parts.pieces = std::min(f.pieces, std::max(1, C::GROUPS / a.c.kv));
+        groups = (uint32_t)(parts.pieces + 7) / 8 * 8 * a.c.kv;
         parts.marks = (SelfMark *)a.ws;
-        parts.parts = (float *)(parts.marks + (uint64_t)f.pieces * a.c.kv);
+        parts.parts = (float *)(parts.marks + (uint64_t)parts.pieces * a.c.kv);
         parts.pitch = self_part_floats(f.part_rows, a.c.width);
-        parts.pieces = f.pieces;
         parts.least = (uint64_t)a.share * 4 * C::KB;
     }
-    const hipError_t e = enqueue(self_tiles<T, HELD, PAGED, DP, WAVES, M, SPLIT>, dim3(f.groups), dim3(64 * WAVES * SPLIT),
+    const hipError_t e = enqueue(self_tiles<T, HELD, PAGED, DP, WAVES, M, SPLIT>, dim3(groups), dim3(64 * WAVES * SPLIT),
                                  C::LDS, s, a, parts);
     // (Blocks of one tile are not cut.)
     if (e != hipSuccess || !PAGED || room(a.c) <= C::KB) return e;
-    return enqueue(self_join<T>, dim3(f.groups, f.part_rows <= 16 ? 2 : (f.part_rows * DP / 4 + 511) / 512), dim3(256), 0, s, a, parts);
+    return enqueue(self_join<T>, dim3(groups, f.part_rows <= 16 ? 2 : (f.part_rows * DP / 4 + 511) / 512), dim3(256), 0, s, a, parts);
 }
 
 template <typename T, bool PAGED, int DP> static hipError_t launch_held(hipStream_t s, const SelfArgs &a, const SelfLaunch &f) {
