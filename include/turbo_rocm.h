@@ -358,7 +358,9 @@ int32_t turbo_rocm_cache_read(void *ctx, const turbo_rocm_cache_rows_call *call,
  * no state is zeros. What a state that a row does not see holds, its scale with
  * it, changes nothing of that row, an infinity or a NaN included. Numerics,
  * infinities and NaN are those of cross attention; int8 states are used
- * unrounded (a probability times its value's scale is what is rounded).
+ * unrounded (a probability times its value's scale is what is rounded, in F16
+ * against the sequence's scales: values 2^-24 of the largest may weigh nothing;
+ * an infinite scale that a row sees may make its row NaN). At most 2^20 key heads.
  *
  * workspace: 16-byte aligned memory of the context's device, of the bytes that
  * turbo_rocm_cache_workspace gives for at least as many tokens and sequences,
@@ -387,7 +389,9 @@ int32_t turbo_rocm_cache_workspace(uint64_t tokens, uint64_t sequences, uint32_t
  * state came before them: token t of a sequence attends to the sequence's rows
  * of k and v [tokens, kv_heads, width] up to its own, the last `window` of them
  * (0: all). q and out [tokens, heads, width], all of one type; starts as above.
- * out may not overlap an input. */
+ * out may not overlap an input. A call of more than 2^31 threads (four waves for
+ * each 32 or 128 tokens' heads of a key head, and for what is left of each
+ * sequence's) is refused (TURBO_E_CAPACITY). */
 typedef struct turbo_rocm_prompt_attention_call {
     uint32_t struct_size;
     uint32_t flags;

@@ -233,3 +233,17 @@ def test_numbers_are_not_cut_to_32_bits():
             _attend(window=bad)
         with pytest.raises(ValueError):
             _cache(page=bad)
+
+
+def test_calls_of_too_many_workgroups_are_refused():
+    # 2^23 sequences of a token each, four waves a workgroup: 2^31 threads and those of a block more.
+    n = 1 << 23
+    one = dict(q=Fake(1 * GB, (n, 1, 8), F16), k=Fake(2 * GB, (n, 1, 8), F16), v=Fake(3 * GB, (n, 1, 8), F16), out=Fake(4 * GB, (n, 1, 8), F16))
+    assert _status(lambda: _prompt(**one, starts=Fake(20 * GB, (n + 1,), I32))) == (CAPACITY, 0)
+    assert _status(lambda: _prompt(**one, starts=Fake(20 * GB, (n // 2 + 1,), I32))) == NO_CONTEXT
+    # 2^20 key heads: eight workgroups of each, of 256 threads, are 2^31.
+    for k, want in ((1 << 20, NO_CONTEXT), ((1 << 20) + 1, (CAPACITY, 0))):
+        need = O.cache_workspace(1, N, k, k, 8, F16)
+        rows = dict(q=Fake(40 * GB, (1, k, 8), F16), out=Fake(41 * GB, (1, k, 8), F16), workspace=Fake(50 * GB, (need,), I8))
+        cache = _cache(k=Fake(10 * GB, (P * PAGE, k, 8), F16), v=Fake(30 * GB, (P * PAGE, k, 8), F16))
+        assert _status(lambda: _attend(cache, **rows)) == want

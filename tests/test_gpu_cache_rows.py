@@ -275,3 +275,17 @@ def test_captured_with_arrays_that_change(context, held):
             assert _same(cache.states[0][slots], nk) and _same(cache.states[1][slots], nv)
         else:
             assert np.array_equal(cache.states[1][slots].cpu().numpy(), _codes(nv)[0])
+
+
+@pytest.mark.parametrize("n", [70, 5000])
+@pytest.mark.parametrize("held", ["same", "i8"])
+def test_many_empty_sequences_between_the_tokens(context, n, held):
+    rows, lengths = [0] * n, [0] * n
+    for i, m in ((0, 1), (1, 2), (n // 2, 1), (n // 2 + 17, 3), (n - 4, 90), (n - 2, 1)):
+        rows[i], lengths[i] = m, m + 20
+    cache = Cache(1, rows, lengths, 3, 64, "bf16", held, 16)
+    k, v = _new(2, rows, 3, 64, "bf16")
+    slots = cache.new_slots()
+    _written(context, cache, k, v, slots)
+    for x, y in zip(_read(context, cache, torch.bfloat16), (0, 1)):
+        assert torch.equal(x, cache.values(y, slots).to(torch.bfloat16))

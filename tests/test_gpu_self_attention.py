@@ -583,7 +583,7 @@ def _check_single(out, v):
     assert ((out.double() - want).abs() <= (2 * half + 2.0 ** -20) * want.abs().clamp_min(tiny)).all()
 
 
-@pytest.mark.parametrize("n, share", [(65, 3), (200, 1), (100, 40), (4097, 1), (9000, 2), (9000, 40)])
+@pytest.mark.parametrize("n, share", [(65, 3), (200, 1), (100, 40), (2048, 1), (2049, 1), (4097, 1), (9000, 2), (9000, 40)])
 @pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
 def test_prompts_of_many_sequences(context, n, share, t):
     """Single tokens, a sequence without any, and some longer ones between them."""
@@ -629,3 +629,18 @@ def test_caches_of_many_sequences(context, n, rows_each, share, t, held):
         at += m
     if single:
         _check_single(out[torch.tensor(single, device="cuda")], cache.values(1, torch.cat(slots)))
+
+
+@pytest.mark.parametrize("share", [1, 3])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_prompts_of_many_empty_sequences(context, share, t):
+    """A few tokens among 5000 sequences, whose starts begin behind rows of nobody."""
+    rows = [0] * 5000
+    for i, m in ((3, 1), (4, 200), (2500, 33), (4990, 64), (4998, 1)):
+        rows[i] = m
+    m = sum(rows)
+    q, k, v = _rows(1, m + 50, share, 32, t), _rows(2, m + 50, 1, 32, t), _rows(3, m + 50, 1, 32, t)
+    out = torch.full_like(q, 3.0)
+    context.prompt_attention(q, k, v, starts_of(rows) + 40, out, stream=stream())
+    _check_prompt(out[40:40 + m], q[40:40 + m], k[40:40 + m], v[40:40 + m], rows)
+    assert (out[:40] == 3).all() and (out[40 + m:] == 3).all()

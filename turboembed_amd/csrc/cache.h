@@ -86,6 +86,7 @@ enum class Held : int { Chunks, Loose, Codes, Bytes };
 
 // How a call is launched, from what the host knows of it: its rows and
 // sequences, not their lengths.
+constexpr int MOST_COUNTED = 2048;   // sequences of a prompt whose blocks are ordered
 constexpr int MOST_ALONE = 3072, MOST_TILED = 768;   // workgroups of a call over a cache, of a wave and of four
 struct SelfLaunch {
     Held held;

@@ -26,7 +26,12 @@ __device__ __forceinline__ int seq_before(const CacheArgs &a, int t) {
 // The position of token t of sequence i, from seq_before(t' <= t) on; i is
 // moved to t's own sequence. Below 0: it has none, or no state.
 __device__ __forceinline__ int position_of(const CacheArgs &a, int t, int &i) {
-    while (i < a.seqs && a.starts[i + 1] <= t) ++i;
+    // (Doubled steps: the sequences between two tokens may be many empty ones.)
+    const auto past = [&](uint32_t n) { return n <= (uint32_t)(a.seqs - i) && a.starts[i + (int)n] <= t; };
+    uint32_t step = 1;
+    for (; past(step); step *= 2) i += (int)step;
+    while ((step /= 2) > 0)
+        if (past(step)) i += (int)step;
     if (i < 0 || i >= a.seqs) return -1;
     const Seq s = seq_of(a, i);
     return t < s.row0 ? -1 : s.first() + (t - s.row0);

@@ -10,6 +10,8 @@ namespace rocm {
 
 namespace {
 
+constexpr uint64_t MOST_THREADS = 1ull << 31;   // of a launch
+
 // The most pieces of a call over a cache, by its blocks' rows.
 uint64_t most_pieces(int rows, int kv) {
     return std::max<uint64_t>(1, (rows == 128 ? MOST_TILED : MOST_ALONE) / kv);
@@ -53,9 +55,10 @@ SelfLaunch self_plan(const SelfArgs &a) {
     if (a.i8 && f.rows == 32 && chunks && !f32) f.held = Held::Bytes;
     // Tokens of few heads: blocks of 16 rows.
     if (a.c.paged && !f32 && rows <= 16 * seqs && (f.held == Held::Bytes || f.held == Held::Chunks)) f.rows = 16;
-    const uint64_t blocks = a.c.kv * (rows / f.rows + seqs);   // at most
+    // At most. (Of many sequences, an empty one has a place too.)
+    const uint64_t blocks = a.c.kv * (rows / f.rows + (!a.c.paged && a.c.seqs > MOST_COUNTED ? a.c.seqs : seqs));
     if (!a.c.paged) {
-        if (blocks * (f.rows == 128 || f.split ? 256 : 64) > 1ull << 31)
+        if (blocks * (f.rows == 128 || f.split ? 256 : 64) > MOST_THREADS)
             fail(TURBO_E_CAPACITY, "rocm: a prompt of " + std::to_string(blocks) + " workgroups");
         f.groups = (uint32_t)blocks;
         return f;
@@ -63,6 +66,9 @@ SelfLaunch self_plan(const SelfArgs &a) {
     // (No more than there can be tiles.)
     const uint64_t tiles = blocks / a.c.kv * std::max<uint64_t>(1, ((uint64_t)room(a.c) + 31) / 32);
     f.pieces = (int)std::min<uint64_t>(most_pieces(f.rows, a.c.kv), std::max<uint64_t>(1, tiles));
+    // (Eight pieces of each key head at least, of 256 threads where they are joined.)
+    if ((uint64_t)(f.pieces + 7) / 8 * 8 * a.c.kv * 256 > MOST_THREADS)
+        fail(TURBO_E_CAPACITY, "rocm: cache attention of " + std::to_string(a.c.kv) + " key heads");
     f.part_rows = (int)std::min<uint64_t>(f.rows, rows);
     return f;
 }

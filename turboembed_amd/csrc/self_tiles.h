@@ -266,8 +266,8 @@ template <int ROWS, int KB> struct Cuts {
 // Workgroup x's (sequence, key head, block) of a prompt: the blocks with the
 // most keys first, over all sequences, so that the last to run are short; of one
 // number, the key heads next to each other (8 of them go to as many XCDs). Of
-// more than HELD sequences, whose numbers LDS does not hold: one after another.
-template <int ROWS, int HELD> struct Turn {
+// more than MOST_COUNTED sequences: one after another.
+template <int ROWS> struct Turn {
     int seq, kv, block;
     bool any;
     __device__ __forceinline__ Turn(const SelfArgs &a, uint32_t x, char *lds, int threads) {
@@ -277,20 +277,25 @@ template <int ROWS, int HELD> struct Turn {
         any = false;
         const int item = (int)(x / (uint32_t)kv_heads);
         kv = (int)(x - (uint32_t)item * (uint32_t)kv_heads);
-        if (n > HELD) {
-            int seen = 0;
-            for (int i0 = 0; i0 < n; i0 += 64) {
-                const int b = blocks(i0 + lane), sum = (int)prefix_sum((uint64_t)b);
-                const uint64_t past = __ballot(seen + sum > item);
-                if (past) {
-                    const int l = __ffsll((unsigned long long)past) - 1;
-                    seq = i0 + l;
-                    block = item - seen - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(b, l));
-                    any = true;
-                    return;
-                }
-                seen += __builtin_amdgcn_readlane(sum, 63);
+        if (n > MOST_COUNTED) {
+            // (Sequence i's blocks from place i + its first row / ROWS on: they end
+            // before the next one's, and a search finds whose a place is.)
+            const auto place = [&](int i) {
+                return (uint32_t)within(a.c.starts[i], 0, a.c.tokens) * (uint32_t)a.share / ROWS + (uint32_t)i;
+            };
+            int lo = 0, count = n;
+            for (;;) {
+                const int step = (count + 63) / 64, at = lane * step;
+                const int hits = __popcll(__ballot(at < count && place(lo + at) <= (uint32_t)item));
+                if (hits == 0) return;
+                const int found = (hits - 1) * step;
+                lo += found, count = min(step, count - found);
+                if (step == 1) break;
             }
+            seq = lo;
+            const uint32_t at = (uint32_t)item - place(lo);
+            any = at < (uint32_t)blocks(lo);
+            block = (int)at;
             return;
         }
         int own = 0;    // the first 64 sequences' in registers
@@ -386,6 +391,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
     constexpr bool F32 = C::F32, CODES = C::CODES, F16 = std::is_same<T, _Float16>::value, TWO = WAVES == 1 && SPLIT == 1 && !F32;
     constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR;
     constexpr int E = Chunk<T>::N, ROWS = C::ROWS;
+    static_assert(PAGED || C::LDS >= 4 * MOST_COUNTED, "LDS holds the sequences' numbers of blocks");
     // Lanes of a row; a lane's scores of 32 keys; the results of the product with
     // V, and a lane's registers of one. Register i: key or column 4 H (i / 4) + 4 h
     // + i % 4 (h: which of the row's lanes).
@@ -463,7 +469,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
         else at = end = Place{c.seqs, 0, 0};
         if (!front && tid == 0) parts.marks[unit_id] = SelfMark{};
     } else {
-        const Turn<ROWS, C::TILES / 4> turn(a, blockIdx.x, smem, THREADS);
+        const Turn<ROWS> turn(a, blockIdx.x, smem, THREADS);
         if (!turn.any) return;
         at = Place{turn.seq, turn.block, 0}, kv = turn.kv;
         if (HELD == Held::Chunks && d < DP && c.seqs > 64) {
