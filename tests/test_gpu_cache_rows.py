@@ -86,6 +86,38 @@ def test_rows_there_and_back(context, rows, lengths, kv, d, page, t, held):
             assert torch.equal(got.double(), want)
 
 
+@pytest.mark.parametrize("kv, d", [(13, 32), (13, 20), (7, 64), (9, 43), (5, 128), (5, 101)])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("held", ["same", "i8"])
+def test_long_calls(context, kv, d, t, held):
+    """Rows enough for every kernel of long calls, a number that no workgroup divides, some of them nobody's and some
+    without a place."""
+    rows = (3001, 1, 0, 2500, 77)
+    cache = Cache(1, rows, (3300, 1, 5, 2500, 100), kv, d, t, held, 16)
+    k, v = _new(2, (sum(rows) + 11,), kv, d, t)
+    slots = cache.new_slots()
+    cache.starts += 6
+    cache.pages[3, 40:50] = -1                                # tokens 640 to 799 of sequence 3
+    there = torch.ones(sum(rows), dtype=torch.bool, device="cuda")
+    there[3002 + 640:3002 + 800] = False
+    context.cache_write(k, v, cache.operand(T), *cache.arrays(), stream=stream())
+    for out_type in [TYPES[t]] if held == "same" else TYPES.values():
+        got = [torch.full((len(k), kv, d), 7.0, dtype=out_type, device="cuda") for _ in "kv"]
+        context.cache_read(cache.operand(T), *cache.arrays(), *got, stream=stream())
+        for i, (g, x) in enumerate(zip(got, (k, v))):
+            assert (g[:6] == 7).all() and (g[-5:] == 7).all()
+            mine, x = g[6:-5], x[6:-5]
+            assert (mine[~there] == 0).all()
+            if held == "same":
+                assert _same(mine[there], x[there]) and _same(cache.states[i][slots[there]], x[there])
+                continue
+            codes, scales = _codes(x[there])
+            assert np.array_equal(cache.states[i][slots[there]].cpu().numpy(), codes)
+            assert np.array_equal(cache.scales[i][slots[there]].cpu().numpy(), scales)
+            want = _once(codes.astype(np.float64) * scales.astype(np.float64)[..., None], out_type)
+            assert np.array_equal(mine[there].double().cpu().numpy(), want)
+
+
 def _once(x, t):
     """64-bit numbers to the nearest of type t, ties to even, as 64-bit numbers."""
     f = torch.finfo(t)

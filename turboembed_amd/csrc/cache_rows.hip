@@ -1,12 +1,12 @@
 // Rows into the pages of a cache, as they are or as int8 codes, and back.
 //
 // A few lanes hold a head's row, eight values each, so a wave moves several
-// rows of K and of V at once, and of long calls four times as many: what does
-// not depend on where a row goes is on its way before that is known. A wave
+// rows of K and of V at once: what does not depend on where a row goes is on its
+// way before that is known. A wave
 // looks for its first row's sequence 64 sequences a step, the lanes go on from
 // there. Bytes bound long calls: 8 x 4096 BF16 tokens of 8 heads of 128 into int8
-// pages take 63 us (3.2 TB/s), 8 x 2048-4096 of 16 heads of 64 out
-// of them as F16 41 us (3.7); short ones a launch and four reads in turn (4 us).
+// pages take 60 us (3.4 TB/s), 8 x 2048-4096 of 16 heads of 64 out of them as
+// F16 36 us (4.2); short ones a launch and four reads in turn (4 us).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -39,9 +39,10 @@ template <typename T> struct Group {
             for (int k = 0; k < 8; ++k) v[k] = k < n ? from[k] : (T)0;
         }
     }
-    __device__ __forceinline__ void write(T *to, int n) const {
+    template <bool PAST = false> __device__ __forceinline__ void write(T *to, int n) const {
         if (n >= 8) {
-            *(typename Eight<T>::loose *)to = v;
+            if constexpr (PAST) __builtin_nontemporal_store(v, (typename Eight<T>::loose *)to);
+            else *(typename Eight<T>::loose *)to = v;
         } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
@@ -100,7 +101,7 @@ __device__ __forceinline__ void write_codes(const Group<T> &x, int n, bool there
 }
 
 // Eight codes times their scale, rounded once to T.
-template <typename T> __device__ __forceinline__ void write_values(const Group<int8_t> &q, float scale, int n, T *to) {
+template <typename T> __device__ __forceinline__ Group<T> values_of(const Group<int8_t> &q, float scale) {
     float v[8];
     // (A product that F32 has rounded onto the border of two 16-bit numbers would
     // be rounded a second time, from there; among F16's smallest the borders are
@@ -116,12 +117,15 @@ template <typename T> __device__ __forceinline__ void write_values(const Group<i
     if (!std::is_same<T, float>::value && tie)
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = odd_f32((double)q.v[k] * scale);
-    write8(to, n, v);
+    Group<T> g;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) g.v[k] = from_f32<T>(v[k]);
+    return g;
 }
 
 // LANES lanes a head's row, U rows each. WRITE: the call's rows into the cache,
-// else back.
-template <typename T, bool I8, bool WRITE, int LANES, int U> __global__ void __launch_bounds__(256) cache_rows(RowsArgs a) {
+// else back; PAST: the rows go past the caches, which keep states instead.
+template <typename T, bool I8, bool WRITE, int LANES, int U, bool PAST> __global__ void __launch_bounds__(256) cache_rows(RowsArgs a) {
     typedef typename std::conditional<I8, int8_t, T>::type H;   // as the cache holds them
     typedef typename std::conditional<WRITE, T, H>::type From;
     constexpr int PER = 64 / LANES;
@@ -172,12 +176,13 @@ template <typename T, bool I8, bool WRITE, int LANES, int U> __global__ void __l
                 if (slot[u] >= 0) k[u].write(state(c.k, c.ks, u), n), v[u].write(state(c.v, c.vs, u), n);
             } else if (own[u]) {
                 if (slot[u] < 0) {
-                    const float zero[8] = {};
-                    write8(row(a.k, a.ks, u), n, zero), write8(row(a.v, a.vs, u), n, zero);
+                    const Group<T> zero{};
+                    zero.write(row(a.k, a.ks, u), n), zero.write(row(a.v, a.vs, u), n);
                 } else if constexpr (I8) {
-                    write_values(k[u], sk[u], n, row(a.k, a.ks, u)), write_values(v[u], sv[u], n, row(a.v, a.vs, u));
+                    values_of<T>(k[u], sk[u]).template write<PAST>(row(a.k, a.ks, u), n);
+                    values_of<T>(v[u], sv[u]).template write<PAST>(row(a.v, a.vs, u), n);
                 } else {
-                    k[u].write(row(a.k, a.ks, u), n), v[u].write(row(a.v, a.vs, u), n);
+                    k[u].template write<PAST>(row(a.k, a.ks, u), n), v[u].template write<PAST>(row(a.v, a.vs, u), n);
                 }
             }
         }
@@ -185,15 +190,23 @@ template <typename T, bool I8, bool WRITE, int LANES, int U> __global__ void __l
 }
 
 template <typename T, bool I8, bool WRITE> static hipError_t launch_rows(hipStream_t s, const RowsArgs &a) {
-    // Four rows a lane where that leaves a workgroup for every compute unit.
+    // Reads, where they leave two workgroups for every compute unit: two rows a
+    // lane of codes, and stores past the caches. (8 x 2048-4096 tokens of 16 heads
+    // of 64, codes as F16, states that no cache holds: 68 us with four rows a lane
+    // and plain stores, 45 with one row, 40 so; 8 x 4096 BF16 tokens of 8 heads of 128, copied,
+    // 71, and 61 with one row. Writes of these 64 us with four rows a lane, 59 with
+    // one; their stores stay in the caches, where the attention will look.)
     const uint64_t rows = (uint64_t)a.c.tokens * a.c.kv;
     const auto go = [&](auto kernel, int per) {
         const uint64_t blocks = std::min<uint64_t>((rows + per - 1) / per, 1 << 20);
         return enqueue(kernel, dim3((uint32_t)blocks), dim3(256), 0, s, a);
     };
-#define ROWS(L)                                                                          \
-    if (rows >= 256 * 4 * (256 / L)) return go(cache_rows<T, I8, WRITE, L, 4>, 4 * (256 / L)); \
-    return go(cache_rows<T, I8, WRITE, L, 1>, 256 / L)
+    constexpr int LONG = I8 && !WRITE ? 2 : 1;
+#define ROWS(L)                                                                                 \
+    if constexpr (!WRITE)                                                                       \
+        if (rows >= 256 * 2 * LONG * (256 / L))                                                 \
+            return go(cache_rows<T, I8, WRITE, L, LONG, true>, LONG * (256 / L));               \
+    return go(cache_rows<T, I8, WRITE, L, 1, false>, 256 / L)
     if (a.c.width <= 32) { ROWS(4); }
     if (a.c.width <= 64) { ROWS(8); }
     ROWS(16);
