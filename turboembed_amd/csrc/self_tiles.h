@@ -436,6 +436,11 @@ self_tiles(SelfArgs a, SelfParts parts) {
     constexpr int UN = STAGED ? C::unit() : 16 / (int)sizeof(Kept), UPR = DP / UN;
     constexpr int NL = KB * UPR / 64 / WAVES;
     static_assert(NL * 64 * WAVES == KB * UPR, "whole loads a wave");
+    // A wave alone reads a cache's states once, where their rows are whole lines of
+    // 128 bytes: past the caches (nt), which have nobody to keep them for. (64 tokens
+    // over 200-8192 BF16 states, 32 heads over 8 of 128: 235 us, 212 so; over int8
+    // heads of 64, two of which share a line, 149 and 168.)
+    constexpr int ONCE = PAGED && WAVES == 1 && PITCH % 128 == 0 ? 2 : 0;
     constexpr int GROUP = 16;                 // keys that lie in one page, where pages are whole groups
     const auto group_at = [&](int j) { return (wave * NL + j) * 64 / CPR / GROUP * GROUP; };
     const auto unit_at = [&](int j, int l) { return (wave * NL + j) * 64 + l; };
@@ -562,7 +567,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     return __builtin_amdgcn_make_buffer_rsrc((void *)p, (short)0, -1, 0x00020000);
                 };
                 const auto send = [&](__amdgpu_buffer_rsrc_t tile, uint32_t at, char *dst) {
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(tile, (to)((lds)smem + (dst - smem)), 16, (int)at, 0, 0, 0);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(tile, (to)((lds)smem + (dst - smem)), 16, (int)at, 0, 0, ONCE);
                 };
                 const auto base = [&](int j) {
                     // (Without a page: slot 0, whose keys are not looked at.)
@@ -597,10 +602,10 @@ self_tiles(SelfArgs a, SelfParts parts) {
                         const int ck = col_k_at(j, lane), cv = col_v_at(j, lane);
                         if (ck < d)
                             __builtin_amdgcn_global_load_lds((from)(K0 + s * c.ks[0] + ck), (to)((lds)smem + (K - smem) + (wave * NL + j) * 1024),
-                                                             16, 0, 0);
+                                                             16, 0, ONCE);
                         if (cv < d)
                             __builtin_amdgcn_global_load_lds((from)(V0 + s * c.vs[0] + cv), (to)((lds)smem + (V - smem) + (wave * NL + j) * 1024),
-                                                             16, 0, 0);
+                                                             16, 0, ONCE);
                     }
                 }
             } else if constexpr (HELD == Held::Loose) {
