@@ -20,8 +20,8 @@
 // into LDS; a wave alone has the codes themselves in LDS.
 //
 // What it reaches, and what bounds it: single tokens the states' bytes (64 over
-// 200-8192 BF16 states, 32 heads over 8 of 128: 210 us, 5.3 TB/s; 96 over 100-6000
-// int8 states, 12 heads of 64: 124 us, 3.9 TB/s); long 16-bit prompts the
+// 200-8192 BF16 states, 32 heads over 8 of 128: 194 us, 5.7 TB/s; 96 over 100-6000
+// int8 states, 12 heads of 64: 125 us, 3.8 TB/s); long 16-bit prompts the
 // softmax's vector instructions beside the products (8 x 2048-8192 tokens, 32
 // heads over 8 of 128: 2.05 ms, 965 TFLOP/s); F32 the slow products (24 x 20-500
 // tokens, 12 heads of 64: 65-70 us, 50 TFLOP/s).
@@ -65,7 +65,7 @@ template <typename T, Held HELD, int DP, int WAVES, int M, int SPLIT> struct Sel
     // work is equal, and a second turn would be a short one. us at 0.75, 1, 1.34
     // and 2 times as many:
     //   256 tokens over 256 BF16 states each, 4 heads of 64                     33  33  40  41
-    //   64 tokens over 200-8192 BF16 states, 32 heads over 8 of 128             263 241 279 245
+    //   64 tokens over 200-8192 BF16 states, 32 heads over 8 of 128 (no nt)     263 241 279 245
     //   96 F16 tokens over 100-6000 int8 states, 12 heads of 64                 154 149 166 150
     //   8 x 512 tokens over 1024-8192 int8 states, 32 heads over 8 of 128       589 481 586 484
     static constexpr int BY_LDS = 163840 / ((LDS + 1279) / 1280 * 1280), BY_WAVES = OCC * 4 / WAVES;
