@@ -644,3 +644,20 @@ def test_prompts_of_many_empty_sequences(context, share, t):
     context.prompt_attention(q, k, v, starts_of(rows) + 40, out, stream=stream())
     _check_prompt(out[40:40 + m], q[40:40 + m], k[40:40 + m], v[40:40 + m], rows)
     assert (out[:40] == 3).all() and (out[40 + m:] == 3).all()
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("held", ["same", "i8"])
+def test_sequences_that_share_pages(context, t, held):
+    """A common prefix in the same pages, and one sequence twice."""
+    for rows in ((1, 1, 1, 1), (20, 3, 40, 40)):
+        cache = Cache(4, rows, (200, 170, 90, 90), 2, 64, t, held, 16)
+        cache.pages[1, :8] = cache.pages[0, :8]
+        cache.pages[3] = cache.pages[2]
+        q = _rows(5, sum(rows), 8, 64, t)
+        q[-rows[3]:] = q[-rows[3] - rows[2]:-rows[3]]
+        out = _attend(context, cache, q)
+        check(cache, q, out)
+        k, v = (torch.full((sum(rows), 2, 64), 7.0, dtype=TYPES[t], device="cuda") for _ in "kv")
+        context.cache_read(cache.operand(T), *cache.arrays(), k, v, stream=stream())
+        assert torch.equal(k[-rows[3]:], k[-rows[3] - rows[2]:-rows[3]]) and torch.isfinite(v).all()
