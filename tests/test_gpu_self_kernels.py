@@ -1,0 +1,87 @@
+"""The kernels of a prompt's attention and of attention over a cache, one by one, on an MI355X against 64-bit arithmetic:
+what each holds its weights in, at every padded width, with windows, values that are no numbers, strides and replays."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from paged import TYPES, starts_of, stream  # noqa: E402
+
+# A weight's error against itself. F32: none of its own. Rounded once: half a step. As the sum of two numbers: the first is
+# less than two steps below the weight, the second what is left, rounded once: half a step of two steps.
+ONCE = {"f32": 0.0, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+TWO = {"f32": 0.0, "f16": 2.0 ** -11 * 2.0 ** -9, "bf16": 2.0 ** -8 * 2.0 ** -6}
+
+
+def rows_of(seed, n, heads, d, t, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(n, heads, d, generator=g) * spread).to(TYPES[t]).cuda()
+
+
+def check(out, q, first, k, v, kept, window=0, scale=None, weightless=0.0):
+    """out is the attention of q's rows at positions first .. to the states k and v [n, kv, d] (64 bits).
+
+    A score is a sum of d F32 products times one or two factors, less a maximum: off by at most e = (d + 6) 2^-24 A + 2^-22 S, A
+    the largest sum of |q_c k_c| scale and S the largest |score| of the row. A weight is off by a factor of 1 +- (2 e + 2^-21)
+    against its row's sum and by `kept` of itself, and, in F16, by half the smallest number, 2^-25 of the row's largest (times
+    `weightless`, the largest size of a value's scale, where those are part of it). Sums of n products are off by n 2^-24 each,
+    and the output is rounded once."""
+    m, heads, d = q.shape
+    n, kv = k.shape[0], k.shape[1]
+    if m == 0:
+        return
+    scale = d ** -0.5 if scale is None else scale
+    half, tiny = torch.finfo(out.dtype).eps / 2, torch.finfo(out.dtype).tiny
+    at, p = first + torch.arange(m, device="cuda"), torch.arange(n, device="cuda")
+    live = p[None] <= at[:, None]
+    if window:
+        live &= p[None] > at[:, None] - window
+    seen = live.any(0)[:, None, None]
+    none = ~live.any(1)
+    assert (out[none] == 0).all()
+    if none.all():
+        return
+    # (States that no row sees may hold anything.)
+    k, v = torch.where(seen, k, 0.0), torch.where(seen, v, 0.0)
+    for h0 in range(0, heads, heads // kv):       # (the heads of one key head: little memory)
+        kk, vv = k[:, h0 * kv // heads], v[:, h0 * kv // heads]
+        qs, o = q[:, h0:h0 + heads // kv].double().transpose(0, 1), out[:, h0:h0 + heads // kv].double().transpose(0, 1)
+        s = (torch.matmul(qs, kk.t().contiguous()) * scale).masked_fill(~live, -float("inf"))
+        pr = torch.softmax(s, -1).nan_to_num(0.0)
+        want = torch.matmul(pr, vv)
+        a = torch.matmul(qs.abs(), kk.abs().t().contiguous()).masked_fill(~live, 0).amax(-1, keepdim=True)
+        big = s.abs().masked_fill(~live, 0).amax(-1, keepdim=True)
+        off = 2 * ((d + 6) * 2.0 ** -24 * a * abs(scale) + 2.0 ** -22 * big) + 2.0 ** -21 + n * 2.0 ** -23 + kept
+        weight = torch.matmul(pr * off, vv.abs())
+        if out.dtype == torch.float16:
+            each = vv.abs().sum(0) if not weightless else 127.0 * n * weightless
+            weight = weight + 2.0 ** -25 * pr.amax(-1, keepdim=True) * each
+        tol = weight * 1.01 + want.abs().clamp_min(tiny) * half * 1.01
+        o, want, tol = o[:, ~none], want[:, ~none], tol[:, ~none]
+        assert torch.isfinite(o).all()
+        worst = ((o - want).abs() / tol).max().item()
+        assert worst <= 1, (m, n, h0, worst)
+
+
+def check_prompt(out, q, k, v, rows, kept, window=0, scale=None):
+    at = 0
+    for m in rows:
+        check(out[at:at + m], q[at:at + m], 0, k[at:at + m].double(), v[at:at + m].double(), kept, window, scale)
+        at += m
+
+
+def prompt(context, q, k, v, rows, kept, window=0, scale=None, out=None):
+    out = torch.full_like(q, 3.0) if out is None else out
+    context.prompt_attention(q, k, v, starts_of(rows), out, window=window, scale=scale, stream=stream())
+    check_prompt(out, q, k, v, rows, kept, window, scale)
+    return out
+
+
+@pytest.mark.parametrize("rows", [(1,), (23,), (33,), (5, 0, 90), (300, 7)], ids=lambda x: "-".join(map(str, x)))
+@pytest.mark.parametrize("heads, kv, d", [(12, 12, 64), (4, 1, 32), (3, 3, 80), (8, 2, 128)])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_prompts_of_few_rows_carry_weights_as_two_numbers(context, rows, heads, kv, d, t):
+    n = sum(rows)
+    q, k, v = rows_of(n, n, heads, d, t), rows_of(n + 1, n, kv, d, t), rows_of(n + 2, n, kv, d, t)
+    for window in (0, 40):
+        prompt(context, q, k, v, rows, TWO[t], window)

@@ -395,7 +395,14 @@ self_tiles(SelfArgs a, SelfParts parts) {
     static_assert(WAVES == 1 || SPLIT == 1, "waves share a tile or rows");
     constexpr int THREADS = 64 * WAVES * SPLIT;
     using Mul = Product<T, M>;
-    constexpr bool F32 = C::F32, CODES = C::CODES, F16 = std::is_same<T, _Float16>::value, TWO = WAVES == 1 && SPLIT == 1 && !F32;
+    constexpr bool F32 = C::F32, CODES = C::CODES, F16 = std::is_same<T, _Float16>::value;
+    // 16-bit weights for the products with V: the sum of two numbers, so that the
+    // output's rounding alone shows; but rounded once where four waves share a tile:
+    // the matrix cores bound those calls, and a second product with V takes 31% longer
+    // (8 x 2048-8192 tokens, 32 heads over 8 of 128: 2.11 to 2.78 ms; 8 x 512 over
+    // int8 states: 490 to 600 us). Waves that share rows wait for what comes before:
+    // 2000 tokens, 12 heads of 64, 26.5 us with one, 28.6 with two.
+    constexpr bool TWO = WAVES == 1 && !F32;
     constexpr int KB = C::KB, SUB = KB / 32, PITCH = C::PITCH, BUF = C::BUF, CPR = C::CPR;
     constexpr int E = Chunk<T>::N, ROWS = C::ROWS;
     static_assert(PAGED || C::LDS >= 4 * MOST_COUNTED, "LDS holds the sequences' numbers of blocks");
@@ -947,7 +954,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
             // the one before runs, and two of its weights are made behind each of that
             // one's instructions (8 x 2048-8192 tokens, 32 heads over 8 of 128: 2068 to
             // 2021 us).
-            constexpr bool EARLY = !TWO && !F32 && !CODES;
+            constexpr bool EARLY = !F32 && !CODES && (WAVES > 1 || SPLIT > 1);
             constexpr int STEP = 8 * H, STEPS = KB / STEP;   // keys of a product
             frag v[2][EARLY ? DT : 1];
             const auto fetch = [&](int x) {
@@ -990,16 +997,22 @@ self_tiles(SelfArgs a, SelfParts parts) {
             if constexpr (EARLY) {
                 // Two weights of the next product behind each of this one's.
                 float sum[2] = {};
-                const auto pair = [&](int x, int e, frag &f) {
+                const auto pair = [&](int x, int e, frag &f, frag &rest) {
                     const int u = x * STEP / 32, i = x * STEP % 32 / STEP * 8 + e;
                     const float w0 = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
                     const float w1 = __builtin_amdgcn_exp2f(fmaf(s[u][i + 1], scale, -base));
                     sum[0] += w0, sum[1] += w1;
-                    f[e] = from_f32<T>(w0), f[e + 1] = from_f32<T>(w1);
+                    if constexpr (TWO) {
+                        T hi[2], lo[2];
+                        two_of<T>(w0, w1, hi, lo, true);
+                        f[e] = hi[0], f[e + 1] = hi[1], rest[e] = lo[0], rest[e + 1] = lo[1];
+                    } else {
+                        f[e] = from_f32<T>(w0), f[e + 1] = from_f32<T>(w1);
+                    }
                 };
-                frag f, g;
+                frag f, rest, f2, rest2;
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) pair(0, e, f);
+                for (int e = 0; e < 8; e += 2) pair(0, e, f, rest);
 #pragma unroll
                 for (int x = 0; x < STEPS; ++x) {
                     __builtin_amdgcn_sched_barrier(0);
@@ -1009,10 +1022,14 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     for (int t = 0; t < (DT > 4 ? DT : 4); ++t) {
                         if (t < DT) o[t] = Mul::run(v[x % 2][t], f, o[t]);
                         __builtin_amdgcn_sched_barrier(0);
-                        if (x + 1 < STEPS && t < 4) pair(x + 1, 2 * t, g);
+                        if (x + 1 < STEPS && t < 4) pair(x + 1, 2 * t, f2, rest2);
                         __builtin_amdgcn_sched_barrier(0);
                     }
-                    f = g;
+                    if constexpr (TWO)
+#pragma unroll
+                        for (int t = 0; t < DT; ++t) o[t] = Mul::run(v[x % 2][t], rest, o[t]);
+                    f = f2;
+                    if constexpr (TWO) rest = rest2;
                 }
                 l += sum[0] + sum[1];
                 return;
