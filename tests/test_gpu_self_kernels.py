@@ -85,3 +85,24 @@ def test_prompts_of_few_rows_carry_weights_as_two_numbers(context, rows, heads, 
     q, k, v = rows_of(n, n, heads, d, t), rows_of(n + 1, n, kv, d, t), rows_of(n + 2, n, kv, d, t)
     for window in (0, 40):
         prompt(context, q, k, v, rows, TWO[t], window)
+
+
+@pytest.mark.parametrize("n", [65, 300, 2048])
+@pytest.mark.parametrize("heads, kv, d", [(1, 1, 80), (3, 3, 40), (2, 1, 24), (8, 4, 112)])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_padded_heads_of_more_sequences_than_a_wave(context, n, heads, kv, d, t):
+    """Columns past the width are cleared in the bytes where such a prompt's blocks are counted: no count may be lost."""
+    rows = [1 + 7 * i % 5 for i in range(n)]
+    rows[3], rows[n // 2], rows[-1] = 0, 150, 70
+    m = sum(rows)
+    q, k, v = rows_of(n, m, heads, d, t), rows_of(n + 1, m, kv, d, t), rows_of(n + 2, m, kv, d, t)
+    outs = [torch.full_like(q, float("nan")) for _ in range(4)]
+    for out in outs:
+        context.prompt_attention(q, k, v, starts_of(rows), out, stream=stream())
+    same = all(torch.equal(outs[0], out) for out in outs)
+    assert same
+    ends = torch.tensor(rows).cumsum(0).tolist()
+    for i in sorted({0, 1, 2, 3, 4, 63, 64, n // 2 - 1, n // 2, n // 2 + 1, n - 2, n - 1} | set(range(0, n, n // 30))):
+        a, b = ends[i] - rows[i], ends[i]
+        check(outs[0][a:b], q[a:b], 0, k[a:b].double(), v[a:b].double(), ONCE[t])
+    assert torch.isfinite(outs[0]).all()

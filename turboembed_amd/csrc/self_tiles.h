@@ -470,10 +470,12 @@ self_tiles(SelfArgs a, SelfParts parts) {
     // (uniform; where a load has keys of two groups, a lane takes its own)
     const bool groups_whole = PAGED && GROUP * CPR % 64 == 0 && c.page_tokens % GROUP == 0;
 
-    if (HELD == Held::Chunks && d < DP) {   // uniform
-        // (Columns past the width keep these zeros.)
-        for (int i = tid; i < C::LDS / 16; i += THREADS) *(vec *)(smem + i * 16) = vec{};
-    }
+    // (Columns past the width keep these zeros. Behind Turn, whose last barrier
+    // follows its last look at what it counts in the same bytes.)
+    const auto clear = [&] {
+        if (HELD == Held::Chunks && d < DP)   // uniform
+            for (int i = tid; i < C::LDS / 16; i += THREADS) *(vec *)(smem + i * 16) = vec{};
+    };
 
     Place at{}, end{};
     bool front = false;    // this workgroup starts inside of a block
@@ -491,11 +493,8 @@ self_tiles(SelfArgs a, SelfParts parts) {
         const Turn<ROWS> turn(a, blockIdx.x, smem, THREADS);
         if (!turn.any) return;
         at = Place{turn.seq, turn.block, 0}, kv = turn.kv;
-        if (HELD == Held::Chunks && d < DP && c.seqs > 64) {
-            __syncthreads();
-            for (int i = tid; i < C::LDS / 16; i += THREADS) *(vec *)(smem + i * 16) = vec{};
-        }
     }
+    clear();
     // (A workgroup that begins where it ends, inside of a block, leaves a part
     // without keys.)
     bool more = !PAGED || !(at == end) || front;
