@@ -2,10 +2,12 @@
 what each holds its weights in, at every padded width, with windows, values that are no numbers, strides and replays."""
 import pytest
 
+import turboembed_amd as T
+
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from paged import TYPES, starts_of, stream  # noqa: E402
+from paged import TYPES, Cache, starts_of, stream  # noqa: E402
 
 # A weight's error against itself. F32: none of its own. Rounded once: half a step. As the sum of two numbers: the first is
 # less than two steps below the weight, the second what is left, rounded once: half a step of two steps.
@@ -18,14 +20,14 @@ def rows_of(seed, n, heads, d, t, spread=1.0):
     return (torch.randn(n, heads, d, generator=g) * spread).to(TYPES[t]).cuda()
 
 
-def check(out, q, first, k, v, kept, window=0, scale=None, weightless=0.0):
+def check(out, q, first, k, v, kept, window=0, scale=None, unit=None):
     """out is the attention of q's rows at positions first .. to the states k and v [n, kv, d] (64 bits).
 
     A score is a sum of d F32 products times one or two factors, less a maximum: off by at most e = (d + 6) 2^-24 A + 2^-22 S, A
     the largest sum of |q_c k_c| scale and S the largest |score| of the row. A weight is off by a factor of 1 +- (2 e + 2^-21)
-    against its row's sum and by `kept` of itself, and, in F16, by half the smallest number, 2^-25 of the row's largest (times
-    `weightless`, the largest size of a value's scale, where those are part of it). Sums of n products are off by n 2^-24 each,
-    and the output is rounded once."""
+    against its row's sum and by `kept` of itself, and, in F16, by half the smallest number, 2^-25 of the row's largest. Of int8
+    values the scale is part of it, against a unit of at most 4 times the largest that the row sees: `unit` [m, 1], for each
+    of n codes. Sums of n products are off by n 2^-24 each, and the output is rounded once."""
     m, heads, d = q.shape
     n, kv = k.shape[0], k.shape[1]
     if m == 0:
@@ -54,7 +56,7 @@ def check(out, q, first, k, v, kept, window=0, scale=None, weightless=0.0):
         off = 2 * ((d + 6) * 2.0 ** -24 * a * abs(scale) + 2.0 ** -22 * big) + 2.0 ** -21 + n * 2.0 ** -23 + kept
         weight = torch.matmul(pr * off, vv.abs())
         if out.dtype == torch.float16:
-            each = vv.abs().sum(0) if not weightless else 127.0 * n * weightless
+            each = vv.abs().sum(0) if unit is None else 127.0 * n * unit
             weight = weight + 2.0 ** -25 * pr.amax(-1, keepdim=True) * each
         tol = weight * 1.01 + want.abs().clamp_min(tiny) * half * 1.01
         o, want, tol = o[:, ~none], want[:, ~none], tol[:, ~none]
@@ -106,3 +108,92 @@ def test_padded_heads_of_more_sequences_than_a_wave(context, n, heads, kv, d, t)
         a, b = ends[i] - rows[i], ends[i]
         check(outs[0][a:b], q[a:b], 0, k[a:b].double(), v[a:b].double(), ONCE[t])
     assert torch.isfinite(outs[0]).all()
+
+
+def attend(context, cache, q, window=0, scale=None, out=None):
+    out = torch.full_like(q, 3.0) if out is None else out
+    need = context.cache_workspace(len(q), len(cache.rows), q.shape[1], cache.kv, cache.d, cache.dtype)
+    ws = torch.full((need,), 0xff, dtype=torch.uint8, device="cuda")
+    context.cache_attention(q, cache.operand(T), *cache.arrays(), out, window=window, scale=scale, workspace=ws, stream=stream())
+    return out
+
+
+# Calls of 16, 32 and 128 rows a block.
+CHUNKS = [((1,), (700,)), ((12,), (90,)), ((20,), (90,)), ((40,), (40,)), ((300,), (300,)), ((300,), (1500,))]
+
+
+@pytest.mark.parametrize("rows, lengths", CHUNKS, ids=lambda x: "-".join(map(str, x)))
+@pytest.mark.parametrize("window", [0, 9, 200])
+@pytest.mark.parametrize("way", ["up", "down", "first"])
+@pytest.mark.parametrize("d", [64, 40])
+def test_f16_rows_over_int8_values_of_sizes_that_change(context, rows, lengths, window, way, d):
+    """Every row against the largest scale that it sees itself."""
+    (m,), (n,) = rows, lengths
+    cache = Cache(m, rows, lengths, 2, d, "f16", "i8", 16)
+    p, at = torch.arange(n, device="cuda"), cache.at(0, 0, n)
+    size = {"up": torch.exp2(p * 12.0 / n - 13), "down": torch.exp2(-p * 12.0 / n - 1),
+            "first": torch.where(p == 0, 2.0 ** -30, 0.02)}[way]
+    cache.scales[1][at] = size[:, None].expand(n, 2).contiguous()
+    q = rows_of(m, m, 4, d, "f16")
+    out = attend(context, cache, q, window)
+    pos = n - m + torch.arange(m, device="cuda")
+    live = (p[None] <= pos[:, None]) & (p[None] > pos[:, None] - (window or n))
+    unit = 4 * torch.where(live, size[None], 0.0).amax(1, keepdim=True).double()
+    # (Two heads of a key head: more than 32 rows of a sequence are four waves', whose weights are rounded once.)
+    kept = ONCE["f16"] if 2 * m > 32 else TWO["f16"]
+    check(out, q, n - m, cache.values(0, at), cache.values(1, at), kept, window, unit=unit)
+
+
+@pytest.mark.parametrize("m, n", [(20, 30), (40, 40), (300, 300)])
+def test_a_value_that_is_large_and_weighs_nothing(context, m, n):
+    """A finite scale of 2^100 whose weight is 0 leaves the rows that see it finite, and the others' bits as they are."""
+    cache = Cache(1, (m,), (n,), 1, 64, "f16", "i8", 16)
+    q = rows_of(2, m, 2, 64, "f16")
+    q[:, :, 0] = 1.0
+    at = n - m // 2
+    slot = cache.at(0, at, at + 1)
+    cache.scales[1][cache.at(0, 0, 1)] = 0.0
+    before = attend(context, cache, q, scale=1.0)
+    cache.states[0][slot] = 0
+    cache.states[0][slot, 0, 0] = -127
+    cache.scales[0][slot] = 4.0                # (a score of -508)
+    cache.scales[1][slot] = 2.0 ** 100
+    out = attend(context, cache, q, scale=1.0)
+    fine = torch.isfinite(out).all()
+    assert fine
+    same = torch.equal(out[:at - (n - m)], before[:at - (n - m)])
+    assert same
+
+
+def _time(f):
+    f()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        f()
+    times = []
+    for _ in range(7):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        graph.replay()
+        a.record()
+        for _ in range(5):
+            graph.replay()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return min(times)
+
+
+@pytest.mark.parametrize("window, first", [(64, 1.0), (1024, 1.0), (0, 2.0 ** -12)])
+def test_f16_rows_over_int8_values_take_bf16_s_time(context, window, first):
+    """Windows, and a first value that is small, cost F16 rows no more than others: half as much again at most."""
+    took = {}
+    rows, lengths = (512,) * 4, (512,) * 4 if first < 1 else (1024, 3000, 5000, 8192)
+    for t in ("f16", "bf16"):
+        cache = Cache(1, rows, lengths, 8, 64, t, "i8", 32)
+        for i in range(4):
+            cache.scales[1][cache.at(i, 0, 1)] *= first
+        q = rows_of(2, 2048, 8, 64, t)
+        ws = torch.empty(context.cache_workspace(2048, 4, 8, 8, 64, TYPES[t]), dtype=torch.uint8, device="cuda")
+        operand, arrays, out = cache.operand(T), cache.arrays(), torch.empty_like(q)
+        took[t] = _time(lambda: context.cache_attention(q, operand, *arrays, out, window=window, workspace=ws, stream=stream()))
+    assert took["f16"] <= 1.5 * took["bf16"], took

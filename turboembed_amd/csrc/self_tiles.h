@@ -53,7 +53,7 @@ template <typename T, Held HELD, int DP, int WAVES, int M, int SPLIT> struct Sel
     static constexpr int BUFS = WAVES == 1 && (SPLIT > 1 || F32 || HELD == Held::Codes) ? 1 : 2;
     static constexpr int TILES = BUFS * 2 * BUF;
     // Behind the tiles: of codes, each buffer's scales of K and V, those of V that
-    // are added apart, and the exponent of their unit; then a word a wave.
+    // are added apart, and the largest of V's; then a word a wave.
     static constexpr int SIDE = (3 * KB + 4) * 4;
     static constexpr int FLAGS = TILES + (CODES ? BUFS * SIDE : 0);
     // Of waves that share rows each has an area, where it leaves its results.
@@ -368,6 +368,19 @@ struct SelfParts {
 
 // ---- the kernel ------------------------------------------------------------------------
 
+// The largest of a wave's numbers of 0 or more.
+__device__ __forceinline__ float wave_max(float v) {
+    const auto with = [&](int other) { v = fmaxf(v, __uint_as_float((uint32_t)other)); };
+    with(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x128, 0xf, 0xf, true));   // 8 lanes on, of 16
+    with(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x124, 0xf, 0xf, true));
+    with(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x122, 0xf, 0xf, true));
+    with(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), 0x121, 0xf, 0xf, true));
+    return four_max(v);
+}
+
+// 1 / v of a power of 2 from 2^-126 to 2^126.
+__device__ __forceinline__ float inverse(float v) { return __uint_as_float((254u << 23) - __float_as_uint(v)); }
+
 // v, as one that the compiler knows nothing of: what is made of it in a path
 // that is rarely taken is made there, and no register holds it meanwhile.
 __device__ __forceinline__ int fresh(int v) {
@@ -416,7 +429,6 @@ self_tiles(SelfArgs a, SelfParts parts) {
     // and its weights have no range to give away: there they reach 2^LAG.
     constexpr float LAG = 8.0f, LEAD = F16 ? 0.0f : LAG;
     constexpr uint64_t FULL = KB == 64 ? ~0ull : 0xffffffffull;
-    constexpr int LEAST_UNIT = -40;   // (127 times half of that is nothing in F16)
     typedef typename Chunk<T>::vec vec;
     typedef typename Mul::frag frag;
     typedef typename Mul::acc acc;
@@ -532,7 +544,6 @@ self_tiles(SelfArgs a, SelfParts parts) {
         typedef uint32_t codes_t __attribute__((ext_vector_type(UN >= 16 ? 4 : UN >= 8 ? 2 : 1), aligned(1)));
         codes_t kq[STAGED ? NL : 1], vq[STAGED ? NL : 1];
         float sk = 0.0f, sv = 0.0f;
-        int unit = LEAST_UNIT;          // the exponent of the weights' unit (F16 codes)
         bool apart = false;             // some values are to be added apart
 
         // n of a unit's codes, a word at a time.
@@ -678,30 +689,17 @@ self_tiles(SelfArgs a, SelfParts parts) {
                     // Values that some rows do not see, and that those cannot have
                     // next to theirs, are added apart.
                     const bool common = t * KB + lane <= all_hi && t * KB + lane >= all_lo;
-                    bool alone = lane < KB && !common && !(fabsf(sv) < INFINITY);
-                    if constexpr (F16) {
-                        // F16 weights have no range for a scale's: they are of its
-                        // size against a power of 2 that is twice to four times the
-                        // largest so far. One that not every row sees has no say in
-                        // that; a larger one is apart.
-                        const auto past = [&] { return fabsf(sv) > __uint_as_float((uint32_t)(127 + unit) << 23); };
-                        const bool counts = lane < KB && common && fabsf(sv) < INFINITY;
-                        if (__ballot(counts && past()) != 0) {
-                            float top = counts ? fabsf(sv) : 0.0f;
-#pragma unroll
-                            for (int o = KB / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-                            unit = uniform(min(126, (int)(__float_as_uint(top) >> 23) - 127 + 2));
-                        }
-                        alone |= lane < KB && !common && past();
-                    }
+                    const bool alone = lane < KB && !common && !(fabsf(sv) < INFINITY);
                     apart |= alone;
                     if (lane < KB) {
-                        const float v = F16 ? sv * __uint_as_float((uint32_t)(127 - unit) << 23) : sv;
                         side[lane] = sk;
-                        side[KB + lane] = alone ? 0.0f : v;
-                        side[2 * KB + lane] = alone ? v : 0.0f;
+                        side[KB + lane] = alone ? 0.0f : sv;
+                        side[2 * KB + lane] = alone ? sv : 0.0f;
                     }
-                    if (lane == 0) ((int *)side)[3 * KB] = unit;
+                    if constexpr (F16) {
+                        const float top = wave_max(alone ? 0.0f : fabsf(sv));
+                        if (lane == 0) side[3 * KB] = top;
+                    }
                 }
             }
         };
@@ -737,7 +735,12 @@ self_tiles(SelfArgs a, SelfParts parts) {
         for (int t = 0; t < DT; ++t) o[t] = acc{};
         float m = -INFINITY, l = 0.0f;
         bool any = false, far = false;   // this row has seen a state; a maximum past 2^24
-        int my_unit = LEAST_UNIT;        // of o's sums
+        // Weights of F16 have no range for a value's scale beside their own: they are
+        // of its size against a power of 2 that is at least this row's largest so far,
+        // and twice to four times it when that sets it (from 2^-40 on, of which 127
+        // halves are nothing in F16). Those of rows that see other states differ, and
+        // nothing of a row depends on what it does not see.
+        float unit = __uint_as_float((127 - 40) << 23);
 
         // S^T of the tile's keys, 32 of them a scores_t.
         const int kr = r * PITCH, ks = C::swap_k(r);
@@ -926,18 +929,29 @@ self_tiles(SelfArgs a, SelfParts parts) {
                         for (int e = 0; e < 4; ++e) s[u][4 * g + e] *= f[e];
                     }
         };
+        // `unit`, for a tile with a value's scale above it. (Rarely: in a loop, before
+        // there are scores, for the registers.)
+        const auto raise_unit = [&](const float *side, uint64_t live, int t) {
+            if (__ballot(side[3 * KB] > unit) == 0) return;
+            const uint64_t seen = seen_of(live, t);
+            float top = 0.0f;
+#pragma nounroll
+            for (int key = 4 * (fresh(lane) / M); key < KB; key += 4 * H) {
+                const f32x4 v = *(const f32x4 *)(side + KB + key);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, seen >> (key + e) & 1 ? fabsf(v[e]) : 0.0f);
+            }
+            top = M == 32 ? both_max(top) : four_max(top);
+            const uint32_t e = min(253u, (__float_as_uint(top) >> 23) + 2);
+            const float now = top > unit ? __uint_as_float(e << 23) : unit, f = unit * inverse(now);
+#pragma unroll
+            for (int t = 0; t < DT; ++t) o[t] *= f;
+            unit = now;
+        };
         const auto tile = [&](const char *K, const float *side, uint64_t live, int t) {
+            if constexpr (CODES && F16) raise_unit(side, live, t);
             scores_t s[SUB];
             scaled_scores(K, side, s);
-            if constexpr (CODES && F16) {
-                const int now = uniform(((const int *)side)[3 * KB]);
-                if (now != my_unit) {   // uniform
-                    const float f = my_unit - now < -126 ? 0.0f : __uint_as_float((uint32_t)(127 + my_unit - now) << 23);
-#pragma unroll
-                    for (int t = 0; t < DT; ++t) o[t] *= f;
-                    my_unit = now;
-                }
-            }
             const uint64_t seen = seen_of(live, t);
             any |= seen != 0;
             if (__ballot(seen != FULL) != 0) {
@@ -1040,9 +1054,11 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 if constexpr (CODES)
 #pragma unroll
                     for (int g = 0; g < NS / 4; ++g) sv[g] = *(const f32x4 *)(side + KB + 32 * u + 4 * H * g + 4 * h);
+                const float inv = inverse(unit);
                 add_values(K + BUF + 32 * u * PITCH, [&](int i) {
                     const float w = __builtin_amdgcn_exp2f(fmaf(s[u][i], scale, -base));
                     sum += w;
+                    if constexpr (CODES && F16) return w * inv * sv[i >> 2][i & 3];
                     if constexpr (CODES) return w * sv[i >> 2][i & 3];
                     return w;
                 });
@@ -1059,8 +1075,6 @@ self_tiles(SelfArgs a, SelfParts parts) {
             const int h = fresh(lane) / M;
             const uint64_t seen = seen_of(live, t);
             const float base = m == -INFINITY ? 0.0f : m;
-            float unit = 1.0f;
-            if constexpr (CODES && F16) unit = __builtin_amdgcn_exp2f((float)(((const int *)side)[3 * KB] - my_unit));
             for (int key = 0; key < KB; ++key) {
                 const bool see = seen >> key & 1;
                 if (__ballot(see) == 0) continue;
@@ -1068,7 +1082,6 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 if constexpr (CODES) {
                     extra = side[2 * KB + key];
                     if (__ballot(extra != 0.0f) == 0) continue;
-                    extra *= unit;
                 }
                 const int i = (key & 31) / (4 * H) * 4 + (key & 3), from = (key >> 2) % H;
                 float x = 0.0f;
@@ -1165,9 +1178,8 @@ self_tiles(SelfArgs a, SelfParts parts) {
             again = uniform(sum) != 0;
         }
         if (again) {   // uniform over the workgroup
-            unit = LEAST_UNIT;
             for (int t = t0 + own; t < t1; t += SPLIT) {
-                if (!CODES && !is_partial(t)) continue;
+                if (!is_partial(t)) continue;
                 sync();
                 slot = slot_at(t);
                 load(t, 0);
@@ -1175,18 +1187,16 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 if constexpr (CODES) put(t, 0);
                 const uint64_t live = __ballot(alive);
                 sync();
-                if (work && is_partial(t)) add_apart(area, (const float *)(area + C::TILES), live, t);
+                if (work) add_apart(area, (const float *)(area + C::TILES), live, t);
             }
         }
 
         if (work) {
             const int h = fresh(lane) / M;
             l = M == 32 ? both_sum(l) : four_sum(l);
-            if constexpr (CODES && F16) {
-                const float f = __uint_as_float((uint32_t)(127 + my_unit) << 23);
+            if constexpr (CODES && F16)
 #pragma unroll
-                for (int t = 0; t < DT; ++t) o[t] *= f;
-            }
+                for (int t = 0; t < DT; ++t) o[t] *= unit;
             // Four of a row's sums, from column col on: divided into the output, or
             // into a part.
             const int at = M * wave + r, groups = (d + 3) / 4;
