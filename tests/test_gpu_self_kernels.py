@@ -197,3 +197,38 @@ def test_f16_rows_over_int8_values_take_bf16_s_time(context, window, first):
         operand, arrays, out = cache.operand(T), cache.arrays(), torch.empty_like(q)
         took[t] = _time(lambda: context.cache_attention(q, operand, *arrays, out, window=window, workspace=ws, stream=stream()))
     assert took["f16"] <= 1.5 * took["bf16"], took
+
+
+def _among(n, live):
+    """n sequences of which a few have a token, or more."""
+    rows, lengths = [0] * n, [0] * n
+    for i, m, s in live:
+        rows[i], lengths[i] = m, s
+    return rows, lengths
+
+
+@pytest.mark.parametrize("t, held", [("f32", "same"), ("bf16", "same"), ("f16", "i8")])
+@pytest.mark.parametrize("many", [0, 40])
+def test_a_few_tokens_among_many_idle_sequences(context, t, held, many):
+    rows, lengths = _among(5000, ((0, 1, 400), (1, 1, 30), (64, 1, 90), (700, many, 900), (701, 1, 64), (2900, 1, 3000), (4998, 2, 5)))
+    cache = Cache(1, rows, lengths, 2, 64, t, held, 16)
+    q = rows_of(2, sum(rows), 4, 64, t)
+    out, at = attend(context, cache, q), 0
+    for i, (m, s) in enumerate(zip(rows, lengths)):
+        if m:
+            where = cache.at(i, 0, s)
+            unit = 4 * cache.scales[1][where].amax().double() * torch.ones(m, 1, device="cuda") if held == "i8" else None
+            check(out[at:at + m], q[at:at + m], s - m, cache.values(0, where), cache.values(1, where), ONCE[t], unit=unit)
+            at += m
+
+
+def test_idle_sequences_between_two_take_no_time_each(context):
+    """Two live sequences behind 20,000 idle ones, and one of them before those: four times the time at most."""
+    n, took = 20002, []
+    for first in (n - 2, 0):
+        rows, lengths = _among(n, ((first, 1, 200), (n - 1, 1, 200)))
+        cache = Cache(1, rows, lengths, 1, 64, "bf16", "same", 16)
+        q, ws = rows_of(2, 2, 4, 64, "bf16"), torch.empty(context.cache_workspace(2, n, 4, 1, 64, torch.bfloat16), dtype=torch.uint8, device="cuda")
+        operand, arrays, out = cache.operand(T), cache.arrays(), torch.empty_like(q)
+        took.append(_time(lambda: context.cache_attention(q, operand, *arrays, out, workspace=ws, stream=stream())))
+    assert took[1] <= 4 * took[0], took

@@ -179,6 +179,17 @@ struct Place {
     __device__ bool operator==(const Place &o) const { return seq == o.seq && block == o.block && tile == o.tile; }
 };
 
+// The first sequence from i on that has rows, or how many there are: found by a
+// wave, 64 a step, as idle ones may be many.
+__device__ __forceinline__ int with_rows(const CacheArgs &a, int i) {
+    const int lane = threadIdx.x & 63;
+    for (; i < a.seqs; i += 64) {
+        const uint64_t has = __ballot(i + lane < a.seqs && seq_of(a, i + lane).rows > 0);
+        if (has) return i + __ffsll((unsigned long long)has) - 1;
+    }
+    return a.seqs;
+}
+
 // A call over a cache is cut into pieces of equal cost, wherever the cuts fall:
 // its lengths are on the device, and one token's sequences may be as different
 // as they like. A piece is a workgroup of each key head: those go to one XCD, at
@@ -263,10 +274,7 @@ template <int ROWS, int KB> struct Cuts {
         from = Place{one(p.seq, 0), one(p.block, 0), one(p.tile, 0)};
         to = Place{one(p.seq, 1), one(p.block, 1), one(p.tile, 1)};
         // (A sequence without rows has no place.)
-        const auto settle = [&](Place &q) {
-            while (q.seq < n && seq_of(a.c, q.seq).rows == 0) ++q.seq;
-        };
-        settle(from), settle(to);
+        from.seq = with_rows(a.c, from.seq), to.seq = with_rows(a.c, to.seq);
     }
 };
 
@@ -1277,8 +1285,7 @@ self_tiles(SelfArgs a, SelfParts parts) {
                 at.tile = 0;
                 if (++at.block == blocks_of(seq, a.share, ROWS)) {
                     at.block = 0;
-                    do ++at.seq;
-                    while (at.seq < c.seqs && seq_of(c, at.seq).rows == 0);
+                    at.seq = with_rows(c, at.seq + 1);
                 }
                 more = at.seq < c.seqs && !(at == end);
             }
