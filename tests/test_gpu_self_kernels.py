@@ -232,3 +232,30 @@ def test_idle_sequences_between_two_take_no_time_each(context):
         operand, arrays, out = cache.operand(T), cache.arrays(), torch.empty_like(q)
         took.append(_time(lambda: context.cache_attention(q, operand, *arrays, out, workspace=ws, stream=stream())))
     assert took[1] <= 4 * took[0], took
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("held", ["same", "i8"])
+def test_keys_and_values_next_to_each_other(context, t, held):
+    """Head by head in a slot, in a head, and in a head's plane: written, read back and attended to as apart."""
+    rows, lengths, kv, d = (5, 40), (50, 40), 3, 40
+    plain = Cache(9, rows, lengths, kv, d, t, held, 8)
+    k, v, q = (rows_of(s, 45, h, d, t) for s, h in ((1, kv), (2, kv), (3, 6)))
+
+    def step(cache):
+        out = [torch.empty_like(k), torch.empty_like(v)]
+        context.cache_write(k, v, cache.operand(T), *cache.arrays(), stream=stream())
+        context.cache_read(cache.operand(T), *cache.arrays(), *out, stream=stream())
+        return [*out, attend(context, cache, q), *(x[cache.new_slots()].clone() for x in cache.states)]
+    n, dtype = plain.slots, plain.states[0].dtype
+    before = [x.clone() for x in plain.states]
+    want = step(plain)
+    for shape, axes in (((n, kv, 2, d), (0, 1, 2)), ((kv, n, 2, d), (1, 0, 2)), ((kv, 2, n, d), (2, 0, 1))):
+        both = torch.empty(shape, dtype=dtype, device="cuda").permute(*axes, 3)
+        cache = Cache(9, rows, lengths, kv, d, t, held, 8)
+        cache.states = [both[:, :, 0], both[:, :, 1]]
+        for x, y in zip(cache.states, before):
+            x.copy_(y)
+        for got, w in zip(step(cache), want):
+            same = torch.equal(got, w)
+            assert same

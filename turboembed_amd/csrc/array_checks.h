@@ -94,24 +94,55 @@ inline void check_apart(const Arg &a) {
     }
 }
 
-// Whether two arrays share a byte: their extents meet, unless both step rows
-// of one length and lie in different columns of them.
+// t's bytes modulo `step`, where they are one run behind its first: of axes of
+// multiples of it, and of `axes` shorter steps, `inner` the last. length 0: they
+// are not.
+struct Run {
+    u128 length, inner = 0;
+    int axes = 0;
+};
+inline Run run_within(const Tensor &t, u128 step) {
+    Run r{t.shape[t.ndim - 1] * (u128)element(t.dtype)};
+    for (uint32_t i = 0; i + 1 < t.ndim; ++i) {
+        if (t.shape[i] == 1) continue;
+        const u128 s = (u128)t.stride[i] * element(t.dtype);
+        if (s >= step && s % step) return Run{0};
+        if (s < step) r.length += (t.shape[i] - 1) * s, r.inner = s, ++r.axes;
+    }
+    return r.length <= step ? r : Run{0};
+}
+
+// Whether two arrays share a byte: their extents meet, unless they lie in
+// different columns of rows of one length, which is a step of either, or of the
+// rows within such a row (K and V side by side in a token's row, in a head's, or
+// in a head's plane).
 inline bool meet(const Tensor &a, const Tensor &b) {
+    typedef __int128 i128;
     if (a.ndim == 0 || b.ndim == 0 || empty(a) || empty(b)) return false;
     const u128 a0 = reinterpret_cast<uintptr_t>(a.data), b0 = reinterpret_cast<uintptr_t>(b.data);
     const u128 a1 = a0 + span(a) * element(a.dtype), b1 = b0 + span(b) * element(b.dtype);
     if (a1 <= b0 || b1 <= a0) return false;
-    if (a.ndim < 2 || b.ndim < 2) return true;
-    const u128 step = (u128)a.stride[0] * element(a.dtype);
-    if (step == 0 || step != (u128)b.stride[0] * element(b.dtype)) return true;
-    auto width = [](const Tensor &t) {
-        return ((t.ndim == 3 ? (u128)(t.shape[1] - 1) * t.stride[1] : 0) + t.shape[t.ndim - 1]) * element(t.dtype);
+    const i128 wa = (i128)a.shape[a.ndim - 1] * element(a.dtype), wb = (i128)b.shape[b.ndim - 1] * element(b.dtype);
+    // off: b's place in a's rows.
+    const auto columns = [](i128 off, i128 step, i128 wa, i128 wb) {
+        const i128 at = (off % step + step) % step;
+        return at >= wa && at + wb <= step;
     };
-    const u128 wa = width(a), wb = width(b);
-    if (wa > step || wb > step) return true;
-    // The later start's place in the other's row.
-    const u128 off = a0 <= b0 ? (b0 - a0) % step : (a0 - b0) % step;
-    return a0 <= b0 ? off < wa || off + wb > step : off < wb || off + wa > step;
+    for (const Tensor *t : {&a, &b})
+        for (uint32_t i = 0; i + 1 < t->ndim; ++i) {
+            const i128 step = (i128)t->stride[i] * element(t->dtype);
+            if (t->shape[i] == 1 || step == 0) continue;
+            const Run ra = run_within(a, step), rb = run_within(b, step);
+            if (!ra.length || !rb.length) continue;
+            const i128 off = (((i128)b0 - (i128)a0) % step + step) % step, inner = ra.inner ? ra.inner : rb.inner;
+            const auto clear = [&](i128 off) {   // of a's run, b's at off
+                if (off >= (i128)ra.length || off + (i128)rb.length <= 0) return true;
+                return inner && ra.axes < 2 && rb.axes < 2 && (!ra.axes || !rb.axes || ra.inner == rb.inner) &&
+                       columns(off, inner, wa, wb);
+            };
+            if (clear(off) && clear(off - step)) return false;
+        }
+    return true;
 }
 
 inline bool same(const Tensor &a, const Tensor &b) {
