@@ -360,7 +360,9 @@ int32_t turbo_rocm_cache_read(void *ctx, const turbo_rocm_cache_rows_call *call,
  * infinities and NaN are those of cross attention; int8 states are used
  * unrounded (a probability times its value's scale is what is rounded, in F16
  * against the largest scale that the row sees: values 2^-24 of it may weigh
- * nothing; an infinite scale that a row sees may make its row NaN). At most 2^20 key heads.
+ * nothing; an infinite scale that a row sees may make its row NaN). At most 2^20
+ * key heads; a key head's rows (tokens times its heads) times its heads times a
+ * sequence's positions past 2^52 may be refused (TURBO_E_CAPACITY).
  *
  * workspace: 16-byte aligned memory of the context's device, of the bytes that
  * turbo_rocm_cache_workspace gives for at least as many tokens and sequences,
