@@ -259,3 +259,30 @@ def test_keys_and_values_next_to_each_other(context, t, held):
         for got, w in zip(step(cache), want):
             same = torch.equal(got, w)
             assert same
+
+
+@pytest.mark.parametrize("heads, d", [(8, 64), (40, 64), (8, 40)])
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+def test_weights_over_int8_values_are_the_sum_of_their_numbers(context, heads, d, t):
+    """Few states a row and many rows: tens of thousands of weights times scales, some of them next to the border of two
+    numbers, where the first number and what it leaves have to be of the same product."""
+    n = 500
+    cache = Cache(d, (1,) * n, (8,) * n, 2, d, t, "i8", 8)
+    q = rows_of(1, n, heads, d, t)
+    out = attend(context, cache, q)
+    k, v, sv = (torch.stack([f(cache.at(i, 0, 8)) for i in range(n)]) for f in
+                (lambda at: cache.values(0, at), lambda at: cache.values(1, at), lambda at: cache.scales[1][at].double()))
+    # (A sequence's rows see all of its states: heads as rows of one product.)
+    qs = q.double().view(n, 2, heads // 2, d)
+    kk, vv = k.permute(0, 2, 3, 1).contiguous(), v.transpose(1, 2).contiguous()
+    s = torch.matmul(qs, kk) * d ** -0.5
+    pr = torch.softmax(s, -1)
+    want = torch.matmul(pr, vv)
+    a = torch.matmul(qs.abs(), kk.abs()).amax(-1, keepdim=True) * d ** -0.5
+    off = 2 * ((d + 6) * 2.0 ** -24 * a + 2.0 ** -22 * s.abs().amax(-1, keepdim=True)) + 2.0 ** -21 + 8 * 2.0 ** -23 + TWO[t]
+    half, tiny = torch.finfo(q.dtype).eps / 2, torch.finfo(q.dtype).tiny
+    tol = torch.matmul(pr * off, vv.abs()) * 1.01 + want.abs().clamp_min(tiny) * half * 1.01
+    if t == "f16":
+        tol = tol + 1.01 * 2.0 ** -25 * pr.amax(-1, keepdim=True) * 127 * 8 * 4 * sv.amax(1)[:, :, None, None]
+    worst = ((out.double().view_as(want) - want).abs() / tol).max().item()
+    assert worst <= 1, worst

@@ -403,6 +403,9 @@ __device__ __forceinline__ void two_of(float w0, float w1, T (&hi)[2], T (&lo)[2
         hi[0] = b[0], hi[1] = b[1];
         lo[0] = from_f32<T>(w0 - to_f32(hi[0])), lo[1] = from_f32<T>(w1 - to_f32(hi[1]));
     } else {
+        // (Of w0 and w1 as they are in F32: made of a product's exact value, the first
+        // number may be another one than that which is taken off.)
+        asm("" : "+v"(w0), "+v"(w1));
         hi[0] = from_f32<T>(w0), hi[1] = from_f32<T>(w1);
         lo[0] = from_f32<T>(w0 - to_f32(hi[0])), lo[1] = from_f32<T>(w1 - to_f32(hi[1]));
     }
