@@ -430,6 +430,17 @@ int32_t turbo_rocm_linear_i8_kernel(uint32_t m, uint32_t n, uint32_t k, uint32_t
  * 128, and the most states; a sequence of more states is joined from parts. */
 int32_t turbo_rocm_cross_cut(const turbo_rocm_cross_desc *desc, uint32_t *rows, uint64_t *states, turbo_error *err);
 
+/* Which kernel attention of a call's own tokens runs, without a device. states:
+ * 0 for a prompt, 1 for a cache of q's type, 2 for one of I8. aligned: the
+ * states' addresses and strides are multiples of 16 bytes. rows: the most rows
+ * (tokens' heads that read one key head) of a block, 16, 32 or 128. waves: 1 of
+ * its own, or 4, which share a block of 128's tiles or a block of 32's keys.
+ * held: how states reach LDS: 0 whole chunks, 1 through registers; I8 states'
+ * codes 2 as numbers, 3 as they are. */
+int32_t turbo_rocm_self_kernel(uint64_t tokens, uint64_t sequences, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                               uint32_t dtype, uint32_t states, uint32_t aligned, uint32_t *rows, uint32_t *waves,
+                               uint32_t *held, turbo_error *err);
+
 /* The last run's packing, read back from the device: each row's first packed
  * token and length ([batch] each), each packed token's r * seq + p ([tokens]),
  * and the packed token count. */

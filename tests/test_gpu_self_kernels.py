@@ -3,11 +3,13 @@ what each holds its weights in, at every padded width, with windows, values that
 import pytest
 
 import turboembed_amd as T
+from turboembed_amd import operators as O
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from paged import TYPES, Cache, starts_of, stream  # noqa: E402
+from paged import TYPES, Cache, ints, starts_of, stream  # noqa: E402
+from test_self_kernels import BYTES, CHUNKS as WHOLE, CODES, INT8, LOOSE, PROMPT, SAME  # noqa: E402
 
 # A weight's error against itself. F32: none of its own. Rounded once: half a step. As the sum of two numbers: the first is
 # less than two steps below the weight, the second what is left, rounded once: half a step of two steps.
@@ -45,21 +47,24 @@ def check(out, q, first, k, v, kept, window=0, scale=None, unit=None):
         return
     # (States that no row sees may hold anything.)
     k, v = torch.where(seen, k, 0.0), torch.where(seen, v, 0.0)
-    for h0 in range(0, heads, heads // kv):       # (the heads of one key head: little memory)
-        kk, vv = k[:, h0 * kv // heads], v[:, h0 * kv // heads]
-        qs, o = q[:, h0:h0 + heads // kv].double().transpose(0, 1), out[:, h0:h0 + heads // kv].double().transpose(0, 1)
-        s = (torch.matmul(qs, kk.t().contiguous()) * scale).masked_fill(~live, -float("inf"))
-        pr = torch.softmax(s, -1).nan_to_num(0.0)
-        want = torch.matmul(pr, vv)
-        a = torch.matmul(qs.abs(), kk.abs().t().contiguous()).masked_fill(~live, 0).amax(-1, keepdim=True)
-        big = s.abs().masked_fill(~live, 0).amax(-1, keepdim=True)
+    share, step = heads // kv, max(1, (1 << 24) // (m * n * (heads // kv)))
+    for h0 in range(0, kv, step):                 # (some key heads at a time)
+        h1 = min(kv, h0 + step)
+        one = lambda x: x[:, h0 * share:h1 * share].double().unflatten(1, (h1 - h0, share)).permute(1, 2, 0, 3)  # noqa: E731
+        qs, o = one(q).flatten(1, 2).contiguous(), one(out)
+        kk, vv = k[:, h0:h1].permute(1, 2, 0).contiguous(), v[:, h0:h1].transpose(0, 1).contiguous()
+        s = torch.matmul(qs, kk).mul_(scale).unflatten(1, (share, m)).masked_fill_(~live, -float("inf"))
+        pr = torch.softmax(s, -1).nan_to_num_(0.0)
+        want = torch.matmul(pr.flatten(1, 2), vv).unflatten(1, (share, m))
+        a = torch.matmul(qs.abs(), kk.abs()).unflatten(1, (share, m)).masked_fill_(~live, 0).amax(-1, keepdim=True)
+        big = s.abs().masked_fill_(~live, 0).amax(-1, keepdim=True)
         off = 2 * ((d + 6) * 2.0 ** -24 * a * abs(scale) + 2.0 ** -22 * big) + 2.0 ** -21 + n * 2.0 ** -23 + kept
-        weight = torch.matmul(pr * off, vv.abs())
+        weight = torch.matmul((pr * off).flatten(1, 2), vv.abs()).unflatten(1, (share, m))
         if out.dtype == torch.float16:
-            each = vv.abs().sum(0) if unit is None else 127.0 * n * unit
+            each = vv.abs().sum(1)[:, None, None] if unit is None else 127.0 * n * unit
             weight = weight + 2.0 ** -25 * pr.amax(-1, keepdim=True) * each
         tol = weight * 1.01 + want.abs().clamp_min(tiny) * half * 1.01
-        o, want, tol = o[:, ~none], want[:, ~none], tol[:, ~none]
+        o, want, tol = o[:, :, ~none], want[:, :, ~none], tol[:, :, ~none]
         assert torch.isfinite(o).all()
         worst = ((o - want).abs() / tol).max().item()
         assert worst <= 1, (m, n, h0, worst)
@@ -259,6 +264,160 @@ def test_keys_and_values_next_to_each_other(context, t, held):
         for got, w in zip(step(cache), want):
             same = torch.equal(got, w)
             assert same
+
+
+# ---- the kernels of long prompts -----------------------------------------------------------
+
+# 70 sequences of 40 to 120 tokens, and a few long ones, of so many key heads that blocks of 128 rows (F32: of 32, a wave
+# each) fill the card.
+MANY, LONG = (tuple(40 + 80 * i // 69 for i in range(70)), 8), ((300, 900, 65, 128, 513, 0, 700, 641), 16)
+
+
+def _long(rows, heads, kv, d, t):
+    n = sum(rows)
+    assert O.self_kernel(n, len(rows), heads, kv, d, TYPES[t]) == ((32, 1, WHOLE) if t == "f32" else (128, 4, WHOLE))
+    return rows_of(n, n, heads, d, t), rows_of(n + 1, n, kv, d, t), rows_of(n + 2, n, kv, d, t)
+
+
+@pytest.mark.parametrize("d", [24, 32, 40, 64, 80, 96, 112, 128])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_long_prompts_of_every_padded_width(context, d, t):
+    for (rows, kv), share in ((MANY, 4), (LONG, 2)):
+        q, k, v = _long(rows, share * kv, kv, d, t)
+        for window in (0, 1, 50, 300):
+            prompt(context, q, k, v, rows, ONCE[t], window)
+
+
+JUNK = (float("nan"), float("inf"), -float("inf"), 1e30)
+
+
+@pytest.mark.parametrize("rows, kv", [MANY, LONG], ids=["many", "long"])
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_long_prompts_do_not_see_later_tokens_whatever_they_hold(context, rows, kv, d, t):
+    """One token in each sequence's middle holds no numbers: the rows before it, and those past its window, are the formula's."""
+    q, k0, v0 = _long(rows, 2 * kv, kv, d, t)
+    for junk, window in zip(JUNK + JUNK, (0, 9, 70, 0, 130, 0, 9, 9)):
+        k, v, at = k0.clone(), v0.clone(), 0
+        for m in rows:
+            if m:
+                v[at + m // 2], k[at + m // 2, :, 3] = junk, junk
+            at += m
+        out = torch.full_like(q, 3.0)
+        context.prompt_attention(q, k, v, starts_of(rows), out, window=window, stream=stream())
+        at = 0
+        for m in rows:
+            j = m // 2
+            check(out[at:at + j], q[at:at + j], 0, k[at:at + j].double(), v[at:at + j].double(), ONCE[t], window)
+            if window and j + window < m:
+                a, b = at + j + 1, at + m        # (the states from behind it on)
+                past = at + j + window
+                check(out[past:b], q[past:b], window - 1, k[a:b].double(), v[a:b].double(), ONCE[t], window)
+            at += m
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.5, 1.0, 1e-30])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_long_prompts_scales(context, scale, t):
+    for (rows, kv), d in ((MANY, 64), (LONG, 80)):
+        q, k, v = _long(rows, 2 * kv, kv, d, t)
+        prompt(context, q, k, v, rows, ONCE[t], scale=scale)
+
+
+@pytest.mark.parametrize("d", [32, 64, 80, 128])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_long_prompts_layouts(context, d, t):
+    """Every layout gives the same bits."""
+    rows, kv = MANY
+    heads, n = 2 * kv, sum(rows)
+    q, k, v = _long(rows, heads, kv, d, t)
+    want = prompt(context, q, k, v, rows, ONCE[t], 70)
+
+    def head_major(x):
+        return x.transpose(0, 1).contiguous().transpose(0, 1)
+
+    def wider(x, off, by):      # rows of more columns, of which x has some
+        y = torch.full((n, x.shape[1] * d + by), 2.0, dtype=x.dtype, device="cuda")[:, off:off + x.shape[1] * d].unflatten(1, (x.shape[1], d))
+        y.copy_(x)
+        return y
+    side = torch.cat([q, k, v], 1).split([heads, kv, kv], 1)
+    between = torch.stack([k, v], 2)
+    for a, b, c in ((head_major(q), head_major(k), head_major(v)), side, (wider(q, 1, 7), wider(k, 16, 32), wider(v, 8, 8)),
+                    (q, between[:, :, 0], between[:, :, 1])):
+        for out in (torch.empty_like(q), wider(q, 5, 11), head_major(q).clone()):
+            out.fill_(3.0)
+            context.prompt_attention(a, b, c, starts_of(rows), out, window=70, stream=stream())
+            same = torch.equal(out, want)
+            assert same
+    # One key head for all, and rows of the call that are nobody's.
+    k1, v1 = (x[:, :1].expand(n, kv, d) for x in (k, v))
+    prompt(context, q, k1, v1, rows, ONCE[t])
+    fewer, out = rows[:-1], torch.full_like(q, 3.0)
+    context.prompt_attention(q, k, v, starts_of(fewer), out, window=70, stream=stream())
+    same = torch.equal(out[:sum(fewer)], want[:sum(fewer)]) and bool((out[sum(fewer):] == 3).all())
+    assert same
+
+
+@pytest.mark.parametrize("d", [64, 80])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_long_prompts_captured_with_starts_that_change(context, d, t):
+    rows, kv = MANY
+    q, k, v = _long(rows, 2 * kv, kv, d, t)
+    n, starts, out = sum(rows), starts_of(rows), torch.empty_like(q)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        context.prompt_attention(q, k, v, starts, out, window=200, stream=stream())
+    for again in range(4):
+        now = rows[again:] + rows[:again] if again < 3 else (1,) * 69 + (n - 69,)
+        starts.copy_(starts_of(now))
+        q.copy_(rows_of(50 + again, n, 2 * kv, d, t))
+        out.fill_(3.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check_prompt(out, q, k, v, now, ONCE[t], 200)
+        first = out.clone()
+        context.prompt_attention(q, k, v, starts, out, window=200, stream=stream())
+        same = torch.equal(first, out)
+        assert same
+
+
+# ---- every kernel of a call over a cache ---------------------------------------------------
+
+def check_cache(cache, q, out, kept, window=0):
+    at = 0
+    for i, (m, n) in enumerate(zip(cache.rows, cache.lens)):
+        where, unit = cache.at(i, 0, n), None
+        if cache.held == "i8":
+            p, pos = torch.arange(n, device="cuda"), n - m + torch.arange(m, device="cuda")
+            live = (p[None] <= pos[:, None]) & (p[None] > pos[:, None] - (window or n))
+            unit = 4 * torch.where(live, cache.scales[1][where].amax(1)[None].double(), 0.0).amax(1, keepdim=True)
+        check(out[at:at + m], q[at:at + m], n - m, cache.values(0, where), cache.values(1, where), kept, window, unit=unit)
+        at += m
+
+
+OVER = [(t, states, rows) for t in ("f32", "f16", "bf16") for states in (SAME, INT8) for rows in (16, 32, 128) if (t, rows) != ("f32", 16)]
+
+
+@pytest.mark.parametrize("d", [24, 32, 33, 48, 64, 80, 91, 96, 112, 127, 128])
+@pytest.mark.parametrize("t, states, rows", OVER)
+def test_every_kernel_of_a_call_over_a_cache(context, t, states, rows, d):
+    """One token, a few and many, two heads to a key head; pages that a tile divides, that divide it, and of one slot."""
+    new, lengths = {16: ((1, 1, 1), (700, 33, 1)), 32: ((12, 3, 17), (300, 64, 17)), 128: ((150, 40, 1), (700, 40, 90))}[rows]
+    whole = d * (1 if states == INT8 else torch.finfo(TYPES[t]).bits // 8) % 16 == 0
+    if states == SAME:
+        kernel = ((32 if t == "f32" and rows < 128 else rows), 1 if rows < 128 else 4, WHOLE) if whole else (32, 1, LOOSE)
+    elif rows == 128:
+        kernel = (128, 4, CODES)
+    else:
+        kernel = (rows, 1, BYTES) if whole and t != "f32" else (32, 1, CODES)
+    assert O.self_kernel(sum(new), 3, 4, 2, d, TYPES[t], states, whole) == kernel
+    kept = ONCE[t] if kernel[1] == 4 else TWO[t]
+    q = rows_of(d, sum(new), 4, d, t)
+    for page in (16, 64, 24, 1):
+        cache = Cache(d + page, new, lengths, 2, d, t, "same" if states == SAME else "i8", page)
+        for window in (0, 5, 70):
+            check_cache(cache, q, attend(context, cache, q, window), kept, window)
 
 
 @pytest.mark.parametrize("heads, d", [(8, 64), (40, 64), (8, 40)])

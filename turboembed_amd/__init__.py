@@ -85,6 +85,8 @@ def library():
         "turbo_rocm_cache_workspace": [C.c_uint64, C.c_uint64, u32, u32, u32, u32, C.POINTER(C.c_uint64), E],
         "turbo_rocm_linear_i8_kernel": [u32, u32, u32, u32, C.POINTER(u32), E],
         "turbo_rocm_cross_cut": [C.POINTER(S.turbo_rocm_cross_desc), C.POINTER(u32), C.POINTER(C.c_uint64), E],
+        "turbo_rocm_self_kernel": [C.c_uint64, C.c_uint64, u32, u32, u32, u32, u32, u32, C.POINTER(u32), C.POINTER(u32),
+                                   C.POINTER(u32), E],
         "turbo_rocm_cross_check": [C.POINTER(S.turbo_rocm_cross_desc), C.c_char_p, E],
     }
     for name, args in protos.items():

@@ -253,4 +253,27 @@ int32_t turbo_rocm_cache_workspace(uint64_t tokens, uint64_t sequences, uint32_t
     });
 }
 
+int32_t turbo_rocm_self_kernel(uint64_t tokens, uint64_t sequences, uint32_t heads, uint32_t kv_heads, uint32_t width,
+                               uint32_t dtype, uint32_t states, uint32_t aligned, uint32_t *rows, uint32_t *waves,
+                               uint32_t *held, turbo_error *err) {
+    return guarded(err, [&] {
+        if (!rows || !waves || !held) refuse(0, "nowhere to leave the kernel");
+        if (!(bit(dtype) & FLOATS)) fail(TURBO_E_INVALID_ENUM, "rocm: attention of type " + std::to_string(dtype));
+        if (states > 2) refuse(0, "states " + std::to_string(states));
+        if (tokens == 0 || sequences == 0 || sequences > (uint64_t)INT32_MAX)
+            misshapen(0, std::to_string(tokens) + " tokens of " + std::to_string(sequences) + " sequences");
+        Tensor q{};
+        q.shape[0] = tokens;
+        check_heads(Arg{&q, "q", 0}, heads, kv_heads, width);
+        SelfArgs a{};
+        a.c.k = a.c.v = reinterpret_cast<void *>((uintptr_t)(aligned ? 16 : 4));
+        a.c.seqs = (int)sequences, a.c.tokens = (int)tokens, a.c.kv = (int)kv_heads, a.c.width = (int)width;
+        a.c.paged = states != 0, a.c.columns = a.c.page_tokens = 1;
+        a.i8 = states == 2, a.dt = dt_of(dtype), a.share = (int)(heads / kv_heads);
+        const SelfLaunch f = self_plan(a);
+        *rows = (uint32_t)f.rows, *waves = f.rows == 128 || f.split ? 4 : 1, *held = (uint32_t)f.held;
+        return TURBO_OK;
+    });
+}
+
 }  // extern "C"

@@ -231,6 +231,17 @@ def linear_i8_kernel(m, n, k, aligned):
     return kernel.value
 
 
+def self_kernel(tokens, sequences, heads, kv_heads, width, dtype, states=0, aligned=True):
+    """(rows, waves, held) of the kernel that attention of a call's own tokens
+    runs (turbo_rocm_self_kernel); a test hook."""
+    from . import _ok
+    rows, waves, held, err = C.c_uint32(), C.c_uint32(), C.c_uint32(), S.new_error()
+    _ok(_lib().turbo_rocm_self_kernel(tokens, sequences, *_u32((heads, kv_heads, width), "heads or a width"), dtype_code(dtype),
+                                      states, 1 if aligned else 0, C.byref(rows), C.byref(waves), C.byref(held), C.byref(err)),
+        err)
+    return rows.value, waves.value, held.value
+
+
 class CrossPlan:
     """Cross attention of sequences of these lengths (turbo_rocm_cross_plan_create)."""
 
