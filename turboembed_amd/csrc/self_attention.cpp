@@ -40,11 +40,18 @@ SelfLaunch self_plan(const SelfArgs &a) {
     if (f.held == Held::Chunks && !a.c.paged) {
         // Prompts: blocks of 128 rows, where there are enough of them for every
         // compute unit; else four waves a block of 32. F32, whose products take long:
-        // a wave a block of 32, if those are enough. us, waves of 32 rows, four of 128,
-        // four of 32:
-        //   F32  24 x 20-500 tokens, 12 heads of 64    72   70   82
-        //   F32  3032 tokens, 12 heads of 128          520  519  318
-        //   BF16 2000 tokens, 12 heads of 64           63        28
+        // a wave a block of 32, if those are enough. us of 12 heads of 64, by how many
+        // blocks there are of that size:
+        //   F32, waves of 32 rows, and four of 32    2184  20 x 20-500 tokens    63   74
+        //                                            1752  16 x 20-500           59   60
+        //                                             984  8 x 100-500           54   38
+        //                                            1128  3000                 262  148
+        //   BF16, four of 128, and four of 32         636  16 x 100-500          21   32
+        //                                             516  5400                 101  116
+        //                                             384  4000                  78   74
+        //                                             192  2000                  43   30
+        // (Not in order: a long sequence's last blocks run alone. 6000 F32 tokens, of
+        // 2256 blocks, would take 486 for 650, 12 x 100-500 BF16, of 480, 21 for 25.)
         if (!f32 && a.c.kv * (rows / 128 + seqs) >= 512 && rows > 32 * seqs) f.rows = 128;
         else f.split = !f32 || a.c.kv * (rows / 32 + seqs) < 2048;
     } else if (f.held != Held::Loose && rows > 32 * seqs) {

@@ -23,8 +23,9 @@
 // 200-8192 BF16 states, 32 heads over 8 of 128: 194 us, 5.7 TB/s; 96 over 100-6000
 // int8 states, 12 heads of 64: 125 us, 3.8 TB/s); long 16-bit prompts the
 // softmax's vector instructions beside the products (8 x 2048-8192 tokens, 32
-// heads over 8 of 128: 2.05 ms, 965 TFLOP/s); F32 the slow products (24 x 20-500
-// tokens, 12 heads of 64: 65-70 us, 50 TFLOP/s).
+// heads over 8 of 128: 2.11-2.15 ms, 920-940 TFLOP/s); F32 prompts how evenly
+// blocks of one to 16 tiles fall on the SIMDs (24 x 20-500 tokens, 12 heads of 64:
+// 65-71 us, in which matrix instructions, 64 cycles each, are busy a third).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -37,8 +38,6 @@
 #include "launch.h"
 
 namespace rocm {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T, Held HELD, int DP, int WAVES, int M, int SPLIT> struct SelfTile {
     static constexpr bool F32 = std::is_same<T, float>::value;
@@ -466,10 +465,12 @@ self_tiles(SelfArgs a, SelfParts parts) {
     constexpr int UN = STAGED ? C::unit() : 16 / (int)sizeof(Kept), UPR = DP / UN;
     constexpr int NL = KB * UPR / 64 / WAVES;
     static_assert(NL * 64 * WAVES == KB * UPR, "whole loads a wave");
-    // A wave alone reads a cache's states once, where their rows are whole lines of
-    // 128 bytes: past the caches (nt), which have nobody to keep them for. (64 tokens
-    // over 200-8192 BF16 states, 32 heads over 8 of 128: 235 us, 212 so; over int8
-    // heads of 64, two of which share a line, 149 and 168.)
+    // A wave alone reads the states of a sequence of one block once: where their rows
+    // are whole lines of 128 bytes, past the caches (nt), which have nobody to keep them
+    // for. (64 tokens over 200-8192 BF16 states, 32 heads over 8 of 128: 235 us, 212 so;
+    // over int8 heads of 64, two of which share a line, 149 and 168. A chunk among
+    // many single tokens has more such blocks, each of which reads them again: 200
+    // tokens 645 us, 512 of one sequence 133, both in one call 1390.)
     constexpr int ONCE = PAGED && WAVES == 1 && PITCH % 128 == 0 ? 2 : 0;
     constexpr int GROUP = 16;                 // keys that lie in one page, where pages are whole groups
     const auto group_at = [&](int j) { return (wave * NL + j) * 64 / CPR / GROUP * GROUP; };
