@@ -76,8 +76,9 @@ SelfLaunch self_plan(const SelfArgs &a) {
     // (Eight pieces of each key head at least, of 256 threads where they are joined.)
     if ((uint64_t)(f.pieces + 7) / 8 * 8 * a.c.kv * 256 > MOST_THREADS)
         fail(TURBO_E_CAPACITY, "rocm: cache attention of " + std::to_string(a.c.kv) + " key heads");
-    // (The device adds up the blocks' costs in 64 bits and shares them out in F64,
-    // so a piece's has to stay below 2^52; of fewer pieces than these, 16 times less.)
+    // (The device adds up the blocks' costs in 64 bits and shares them out in F64: a
+    // piece's has to stay below 2^52, 2^48 for these, of which a kernel may run a
+    // sixteenth.)
     const u128 cost = (u128)(blocks / a.c.kv) * ((u128)a.share * ((uint64_t)room(a.c) + 96) + rows + 128);
     if (cost >> 48 >= (uint64_t)f.pieces)
         fail(TURBO_E_CAPACITY, "rocm: cache attention of " + std::to_string(a.share) + " heads to a key head over " +
